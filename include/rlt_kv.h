@@ -490,6 +490,113 @@ int rlt_expand_prefill(const int64_t* positions, const int64_t* sequences,
                        int64_t page_size, int64_t* blocks, int64_t* offsets, int64_t n,
                        void* stream);
 
+/*
+ * 8-bit KV cache.  Key and value caches of e4m3 codes (one byte each, four bits
+ * of exponent, three of mantissa, no infinity) and, for every (token, head), one
+ * power-of-two scale as its e8m0 byte b: a cached value is code * 2^(b - 127),
+ * NaN for b = 255.  Caches are [num_blocks, num_layers, page_size, num_kv_heads,
+ * head_dim] (a layer slice without num_layers), scales the same without head_dim;
+ * strides in elements, shared by K and V.  The scale that the appends store is the
+ * smallest with amax <= 448 * scale over the finite values of the row (at least
+ * 2^-127); codes are rounded to nearest even, and values that are not finite
+ * become NaN.
+ */
+
+/*
+ * Quantising KV append of one layer: rlt_kv_append to an 8-bit cache.  `dtype` is
+ * the type of k and v.  Slots outside the pool are skipped.
+ */
+int rlt_kv_append_fp8(void* key_cache, void* value_cache, const int64_t* cache_strides, void* key_scales,
+                      void* value_scales, const int64_t* scale_strides, const void* k, const int64_t* k_strides,
+                      const void* v, const int64_t* v_strides, const int64_t* write_blocks,
+                      const int64_t* write_offsets, int64_t n_rows, int64_t layer, int64_t num_layers,
+                      int64_t num_blocks, int64_t page_size, int64_t num_kv_heads, int64_t head_dim, int dtype,
+                      void* stream);
+
+/*
+ * Rotary embedding by positions of one to four axes (time, height, width, ...)
+ * fused with the KV append of one layer.  Frequency j < half of a head turns the
+ * dims j and j + half by the position of axis axis_of[j]:
+ *   (c, s) = table[positions[row][axis_of[j]]][j]
+ *   out[j] = x[j] c - x[j + half] s;  out[j + half] = x[j + half] c + x[j] s
+ * in fp32, each product and the sum rounded, then once to the stored type; dims
+ * past 2 * half pass through.  q_out[i] for i < n_rows (q_out may be q); rotated k
+ * and v go to slot i for i < n_write: quantised into an 8-bit cache when key_scales
+ * is given, into a cache of `dtype` when key_scales and value_scales are NULL.  A
+ * row with a position outside [0, max_position) gets q_out = 0 and no append.
+ *   positions: device int64, position_strides[2]: row, axis.
+ *   table: device fp32 [max_position, half, 2] (cos, sin), contiguous.
+ *   axis_of: HOST bytes [half], each below axes.
+ */
+int rlt_rope_axes_kv_append(void* key_cache, void* value_cache, const int64_t* cache_strides, void* key_scales,
+                            void* value_scales, const int64_t* scale_strides, const void* q,
+                            const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                            const int64_t* v_strides, void* q_out, const int64_t* q_out_strides,
+                            const int64_t* positions, const int64_t* position_strides, int64_t axes,
+                            const float* table, int64_t max_position, const uint8_t* axis_of, int64_t half,
+                            const int64_t* write_blocks, const int64_t* write_offsets, int64_t n_rows,
+                            int64_t n_write, int64_t layer, int64_t num_layers, int64_t num_blocks,
+                            int64_t page_size, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                            int dtype, void* stream);
+
+/*
+ * rlt_paged_decode over a layer slice of an 8-bit cache; q and out are of `dtype`.
+ * A row of length 0 (or less) is written as zeros; lengths are clamped to what the
+ * table covers.  A row's output bits depend on its own q, pages and length only.
+ * The workspace (rlt_paged_decode_fp8_workspace_bytes, a function of the shape)
+ * holds the partials of cut rows; calls that overlap need one each.
+ */
+int64_t rlt_paged_decode_fp8_workspace_bytes(int64_t n_rows, int64_t max_table_width, int64_t num_q_heads,
+                                             int64_t num_kv_heads, int64_t head_dim, int64_t page_size);
+int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, const void* key_cache, const void* value_cache,
+                         const int64_t* kv_strides, const void* key_scales, const void* value_scales,
+                         const int64_t* scale_strides, const int32_t* block_tables, int64_t table_row_stride,
+                         int64_t max_table_width, const int32_t* context_lengths, void* out,
+                         const int64_t* out_strides, int64_t n_rows, int64_t num_q_heads, int64_t num_kv_heads,
+                         int64_t head_dim, int64_t page_size, int64_t num_blocks, float scale, int dtype,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * rlt_paged_prefill over a layer slice of an 8-bit cache: packed chunks, bottom-
+ * right causal.  Query row i of sequence s's n_q sees keys 0 .. context_lengths[s]
+ * - n_q + i; one that sees none is written as zeros.  Rows of no sequence (at or
+ * past cu_seqlens_q[num_seqs]) are left as they were.
+ */
+int64_t rlt_paged_prefill_fp8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
+                                              int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t page_size);
+int rlt_paged_prefill_fp8(const void* q, const int64_t* q_strides, const void* key_cache, const void* value_cache,
+                          const int64_t* kv_strides, const void* key_scales, const void* value_scales,
+                          const int64_t* scale_strides, const int32_t* block_tables, int64_t table_row_stride,
+                          int64_t max_table_width, const int32_t* context_lengths, const int32_t* cu_seqlens_q,
+                          int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, void* out,
+                          const int64_t* out_strides, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                          int64_t page_size, int64_t num_blocks, float scale, int dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/*
+ * Slot maps and block tables of a packed batch of chunks, from the requests'
+ * lengths alone: what rlt_stage_prefill and rlt_expand_prefill build from
+ * per-token arrays that the host writes, in one launch from one (slot, depth,
+ * start, tokens) descriptor a sequence (device or pinned host memory).  Sequence i
+ * takes `tokens` new tokens at positions start, start + 1, ... of
+ * tables[slot, depth] (plane 0 when planes is 1):
+ *   cu_seqlens [size + 1]  int32, running token counts
+ *   lengths [size]         int32, start + tokens
+ *   positions, sequences, blocks, offsets [capacity]  int64, per token
+ *   out_tables [size, out_width]  int32
+ * Sequences count .. size - 1 are padding: no tokens, length 0, a table row of 0.
+ * Tokens behind the last sequence get position 0, sequence -1, block -1 (an append
+ * skips them).  A descriptor outside the tables keeps its tokens in the packing but
+ * gets length 0, a table row of 0 and block -1, position 0; tokens past `capacity`
+ * are dropped from the end, in cu_seqlens as well.
+ */
+int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t count, int64_t size, const int32_t* tables,
+                             int64_t num_slots, int64_t table_width, int64_t planes, int64_t page_size,
+                             int32_t* cu_seqlens, int32_t* lengths, int64_t* positions, int64_t* sequences,
+                             int64_t* blocks, int64_t* offsets, int64_t capacity, int32_t* out_tables,
+                             int64_t out_table_stride, int64_t out_width, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

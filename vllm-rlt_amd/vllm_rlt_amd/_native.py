@@ -140,6 +140,41 @@ SIGNATURES = {
         c_int,
         [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
     ),
+    "rlt_kv_append_fp8": (
+        c_int,
+        [c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, _i64p, c_void_p, _i64p, c_void_p, c_void_p]
+        + [c_int64] * 7
+        + [c_int, c_void_p],
+    ),
+    "rlt_rope_axes_kv_append": (
+        c_int,
+        [c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, _i64p, c_void_p, _i64p, c_void_p, _i64p]
+        + [c_void_p, _i64p, c_void_p, _i64p, c_int64, c_void_p, c_int64, c_char_p, c_int64, c_void_p, c_void_p]
+        + [c_int64] * 9
+        + [c_int, c_void_p],
+    ),
+    "rlt_paged_decode_fp8_workspace_bytes": (c_int64, [c_int64] * 6),
+    "rlt_paged_decode_fp8": (
+        c_int,
+        [c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_int64, c_int64, c_void_p]
+        + [c_void_p, _i64p]
+        + [c_int64] * 6
+        + [c_float, c_int, c_void_p, c_int64, c_void_p],
+    ),
+    "rlt_paged_prefill_fp8_workspace_bytes": (c_int64, [c_int64] * 7),
+    "rlt_paged_prefill_fp8": (
+        c_int,
+        [c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_int64, c_int64, c_void_p]
+        + [c_void_p] + [c_int64] * 3
+        + [c_void_p, _i64p]
+        + [c_int64] * 5
+        + [c_float, c_int, c_void_p, c_int64, c_void_p],
+    ),
+    "rlt_build_chunk_metadata": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p] + [c_int64] * 4 + [c_void_p] * 6
+        + [c_int64, c_void_p, c_int64, c_int64, c_void_p],
+    ),
 }
 
 _lib = None

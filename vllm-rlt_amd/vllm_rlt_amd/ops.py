@@ -8,6 +8,7 @@ the CPU and nothing falls back to another implementation.
 
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass
 
@@ -956,3 +957,366 @@ def expand_prefill(
         ),
         "rlt_expand_prefill",
     )
+
+
+def build_chunk_metadata(
+    descriptors: torch.Tensor,
+    count: int,
+    size: int,
+    tables: torch.Tensor,
+    page_size: int,
+    cu_seqlens: torch.Tensor,
+    lengths: torch.Tensor,
+    positions: torch.Tensor,
+    sequences: torch.Tensor,
+    blocks: torch.Tensor,
+    offsets: torch.Tensor,
+    out_tables: torch.Tensor,
+    out_width: int,
+) -> None:
+    """Slot maps and block tables of a packed batch of chunks, on the device (rlt_build_chunk_metadata).
+
+    descriptors: int64 [>= count, 4] of (slot, depth, start, tokens), on the device
+    or in pinned host memory; tables: the resident int32 [slots, planes, width].
+    Writes int32 cu_seqlens [size + 1], lengths [size] (start + tokens) and
+    out_tables [size, out_width], and int64 positions, sequences, blocks and offsets
+    of every token.  The token buffers share one length, the capacity: tokens
+    behind the last sequence get position 0, sequence -1, block -1 and offset 0, so
+    an append of the whole buffer skips them; tokens past it are dropped from the
+    end.  Sequences from count on are padding: no tokens, length 0.
+    """
+    device = _require_rocm(tables, cu_seqlens, lengths, positions, sequences, blocks, offsets, out_tables)
+    if tables.dtype != torch.int32 or tables.ndim != 3 or not tables.is_contiguous():
+        raise ValueError("tables must be contiguous int32 [slots, planes, width]")
+    if descriptors.dtype != torch.int64 or descriptors.ndim != 2 or descriptors.shape[1] != 4:
+        raise ValueError("descriptors must be int64 [n, 4]")
+    if not descriptors.is_contiguous():
+        raise ValueError("descriptors must be contiguous")
+    if descriptors.device.type == "cpu":
+        if not descriptors.is_pinned():
+            raise ValueError("host descriptors must be pinned")
+    elif descriptors.device != device:
+        raise ValueError("descriptors must be pinned host memory or on the tables' device")
+    if out_tables.dtype != torch.int32 or out_tables.ndim != 2 or out_tables.stride(1) != 1:
+        raise ValueError("out_tables must be int32 [rows, width] with contiguous rows")
+    _require_int(cu_seqlens, torch.int32, "cu_seqlens")
+    _require_int(lengths, torch.int32, "lengths")
+    capacity = positions.numel()
+    for t, name in ((positions, "positions"), (sequences, "sequences"), (blocks, "blocks"), (offsets, "offsets")):
+        _require_int(t, torch.int64, name)
+        if t.numel() != capacity:
+            raise ValueError("positions, sequences, blocks and offsets must share a length")
+    if not 0 <= count <= min(size, descriptors.shape[0]):
+        raise ValueError("count must be in [0, size] and covered by descriptors")
+    if min(cu_seqlens.numel() - 1, lengths.numel(), out_tables.shape[0]) < size:
+        raise ValueError("output buffers are smaller than size")
+    if not 0 <= out_width <= min(tables.shape[2], out_tables.shape[1]):
+        raise ValueError("out_width exceeds the tables")
+    with _current(device):
+        rc = _native.load().rlt_build_chunk_metadata(
+            descriptors.data_ptr(), count, size, tables.data_ptr(), tables.shape[0], tables.shape[2], tables.shape[1],
+            page_size, cu_seqlens.data_ptr(), lengths.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
+            blocks.data_ptr(), offsets.data_ptr(), capacity, out_tables.data_ptr(), max(out_tables.stride(0), out_width),
+            out_width, stream_handle(device),
+        )
+    check(rc, "rlt_build_chunk_metadata")
+
+
+# ------------------------------------------------------------- 8-bit KV cache
+_HERE = contextlib.nullcontext()
+
+
+def _current(device: torch.device):
+    """A context in which `device` is the current one: nothing to do where it is already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _require_fp8(key_cache, value_cache, key_scales, value_scales, ndim: int):
+    """Checks an 8-bit cache: e4m3 codes with ndim dims and e8m0 scales of the same shape without the last."""
+    if key_cache.dtype != torch.float8_e4m3fn or value_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError("an 8-bit cache holds torch.float8_e4m3fn codes")
+    if key_scales.dtype != torch.float8_e8m0fnu or value_scales.dtype != torch.float8_e8m0fnu:
+        raise ValueError("key_scales and value_scales must be torch.float8_e8m0fnu")
+    if key_cache.ndim != ndim:
+        layers = "layers, " if ndim == 5 else ""
+        raise ValueError(f"caches must be [blocks, {layers}page, kv_heads, head_dim]")
+    if key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride():
+        raise ValueError("key_cache and value_cache must share shape and strides")
+    for t in (key_scales, value_scales):
+        if t.shape != key_cache.shape[:-1] or t.stride() != key_scales.stride():
+            raise ValueError("scales must have the caches' shape without head_dim, and equal strides")
+
+
+def kv_append_fp8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    write_blocks: torch.Tensor,
+    write_offsets: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    n_rows: int | None = None,
+) -> None:
+    """kv_append to an 8-bit cache: k[i] and v[i] quantised into slot i for i < n_rows (rlt_kv_append_fp8).
+
+    Caches are torch.float8_e4m3fn [blocks, layers, page, kv_heads, head_dim], scales
+    torch.float8_e8m0fnu [blocks, layers, page, kv_heads]: a cached value is its
+    code times the scale of its (token, head) row, the smallest power of two with
+    amax <= 448 * scale over the row's finite values.  Values that are not finite are
+    stored as NaN.  k and v are float32, float16 or bfloat16.
+    """
+    device = _require_rocm(key_cache, value_cache, key_scales, value_scales, write_blocks, write_offsets, k, v)
+    _require_fp8(key_cache, value_cache, key_scales, value_scales, 5)
+    nb, nl, page, hkv, d = key_cache.shape
+    for t, name in ((k, "k"), (v, "v")):
+        if t.ndim != 3 or t.shape[1:] != (hkv, d):
+            raise ValueError(f"{name} must have shape [batch, {hkv}, {d}]")
+    if k.dtype != v.dtype:
+        raise ValueError("k and v must share a dtype")
+    _require_int(write_blocks, torch.int64, "write_blocks")
+    _require_int(write_offsets, torch.int64, "write_offsets")
+    n = len(write_blocks) if n_rows is None else n_rows
+    if n > min(len(write_blocks), len(write_offsets), k.shape[0], v.shape[0]):
+        raise ValueError("n_rows exceeds the provided rows")
+    with _current(device):
+        rc = _native.load().rlt_kv_append_fp8(
+            key_cache.data_ptr(), value_cache.data_ptr(), int64_array(key_cache.stride()), key_scales.data_ptr(),
+            value_scales.data_ptr(), int64_array(key_scales.stride()), k.data_ptr(), int64_array(k.stride()),
+            v.data_ptr(), int64_array(v.stride()), write_blocks.data_ptr(), write_offsets.data_ptr(), n, layer, nl, nb,
+            page, hkv, d, dtype_code(k.dtype), stream_handle(device),
+        )
+    check(rc, "rlt_kv_append_fp8")
+
+
+def rope_axes_kv_append(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    layer: int,
+    write_blocks: torch.Tensor,
+    write_offsets: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    axes,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    n_rows: int | None = None,
+) -> torch.Tensor:
+    """Rotate q and k by positions of one to four axes, append rotated k and v; returns rotated q (rlt_rope_axes_kv_append).
+
+    positions: int64 [batch, axes] (any strides), a token's place on every axis
+    (time, height, width; one axis for text).  table: contiguous float32
+    [max_position, half, 2] of (cos, sin), computed once from the angles
+    position * inv_freq in float64.  axes: for each of the `half` frequencies the
+    axis whose position turns it, e.g. (0,) * 24 + (1,) * 20 + (2,) * 20, or
+    interleaved.  Frequency j turns the dims j and j + half of a head; dims past
+    2 * half pass through.  Products and sums are rounded to float32, results once to
+    the type they are stored in (rope_kv_append rounds to the storage type after
+    each step).
+
+    The cache is one of q's dtype, or an 8-bit one when its scales are given
+    (kv_append_fp8).  Rows below n_rows (default: all of write_blocks) are written; q
+    is rotated for every row.  A row with a position outside the table gets zeros
+    and is not written.  `out` may be q itself.
+    """
+    device = _require_rocm(key_cache, value_cache, write_blocks, write_offsets, q, k, v, positions, table)
+    if (key_scales is None) != (value_scales is None):
+        raise ValueError("key_scales and value_scales go together")
+    if key_scales is not None:
+        _require_rocm(q, key_scales, value_scales)
+        _require_fp8(key_cache, value_cache, key_scales, value_scales, 5)
+    elif key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride():
+        raise ValueError("key_cache and value_cache must share shape and strides")
+    elif key_cache.ndim != 5:
+        raise ValueError("caches must be [blocks, layers, page, kv_heads, head_dim]")
+    elif key_cache.dtype != q.dtype or value_cache.dtype != q.dtype:
+        raise ValueError(f"the caches must use q's dtype {q.dtype}, or 8 bits with their scales")
+    nb, nl, page, hkv, d = key_cache.shape
+    rows = q.shape[0]
+    if q.ndim != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % hkv:
+        raise ValueError(f"q must have shape [batch, heads, {d}] with heads a positive multiple of {hkv}")
+    for t, name in ((k, "k"), (v, "v")):
+        if t.shape != (rows, hkv, d):
+            raise ValueError(f"{name} must have shape [{rows}, {hkv}, {d}]")
+        if t.dtype != q.dtype:
+            raise ValueError(f"{name} must use dtype {q.dtype}")
+    if positions.dtype != torch.int64 or positions.ndim != 2 or positions.shape[0] != rows:
+        raise ValueError(f"positions must be int64 [{rows}, axes]")
+    if table.dtype != torch.float32 or table.ndim != 3 or table.shape[2] != 2 or not table.is_contiguous():
+        raise ValueError("table must be contiguous float32 [max_position, half, 2]")
+    half = table.shape[1]
+    if len(axes) != half or 2 * half > d:
+        raise ValueError("axes must name one axis for each of the table's frequencies, at most head_dim / 2")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must match q")
+    _require_int(write_blocks, torch.int64, "write_blocks")
+    _require_int(write_offsets, torch.int64, "write_offsets")
+    n = len(write_blocks) if n_rows is None else n_rows
+    if n > min(len(write_blocks), len(write_offsets), rows):
+        raise ValueError("n_rows exceeds the provided rows")
+    with _current(device):
+        rc = _native.load().rlt_rope_axes_kv_append(
+            key_cache.data_ptr(), value_cache.data_ptr(), int64_array(key_cache.stride()),
+            None if key_scales is None else key_scales.data_ptr(),
+            None if key_scales is None else value_scales.data_ptr(),
+            None if key_scales is None else int64_array(key_scales.stride()),
+            q.data_ptr(), int64_array(q.stride()), k.data_ptr(), int64_array(k.stride()), v.data_ptr(),
+            int64_array(v.stride()), out.data_ptr(), int64_array(out.stride()), positions.data_ptr(),
+            int64_array(positions.stride()), positions.shape[1], table.data_ptr(), table.shape[0], bytes(axes), half,
+            write_blocks.data_ptr(), write_offsets.data_ptr(), rows, n, layer, nl, nb, page, q.shape[1], hkv, d,
+            dtype_code(q.dtype), stream_handle(device),
+        )
+    check(rc, "rlt_rope_axes_kv_append")
+    return out
+
+
+def _fp8_attention_inputs(q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out):
+    """Validated arguments that decode and prefill over an 8-bit cache share, and the output."""
+    device = _require_rocm(q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths)
+    _require_fp8(key_cache, value_cache, key_scales, value_scales, 4)
+    dtype_code(q.dtype)
+    hkv, d = key_cache.shape[2:]
+    if q.ndim != 3 or q.shape[2] != d:
+        raise ValueError(f"q must have shape [rows, heads, {d}]")
+    if q.shape[1] == 0 or q.shape[1] % hkv:
+        raise ValueError("query heads must be a positive multiple of KV heads")
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.stride(1) != 1:
+        raise ValueError("block_tables must be int32 [sequences, width] with contiguous rows")
+    _require_int(context_lengths, torch.int32, "context_lengths")
+    if context_lengths.shape[0] != block_tables.shape[0]:
+        raise ValueError("block_tables and context_lengths must have one entry per sequence")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device:
+        raise ValueError("out must match q")
+    return device, out
+
+
+def _workspace_of(need: int, workspace, device):
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.numel() * workspace.element_size() < need or workspace.device != device:
+        raise ValueError(f"workspace must hold {need} bytes on {device}")
+    return workspace
+
+
+def decode_fp8_workspace_bytes(
+    n_rows: int, table_width: int, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int
+) -> int:
+    """Bytes of partials rlt_paged_decode_fp8 needs (shape only)."""
+    return int(
+        _native.load().rlt_paged_decode_fp8_workspace_bytes(
+            n_rows, table_width, num_q_heads, num_kv_heads, head_dim, page_size
+        )
+    )
+
+
+def paged_decode_fp8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lengths: torch.Tensor,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """paged_decode over layer slices of an 8-bit cache (rlt_paged_decode_fp8).
+
+    Codes torch.float8_e4m3fn [blocks, page, kv_heads, head_dim], scales
+    torch.float8_e8m0fnu [blocks, page, kv_heads] (kv_append_fp8); q float32, float16
+    or bfloat16.  Returns a new tensor like q unless out is given; a row of length 0
+    is zeros.  `workspace` (decode_fp8_workspace_bytes) holds the partials of long
+    rows and is allocated here unless given.  A row's output bits depend on its own
+    q, pages and length only.
+    """
+    device, out = _fp8_attention_inputs(
+        q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
+    )
+    rows, hq, d = q.shape
+    nb, page, hkv, _ = key_cache.shape
+    if block_tables.shape[0] != rows:
+        raise ValueError("block_tables and context_lengths must have one entry per row")
+    if rows == 0:
+        return out
+    width = block_tables.shape[1]
+    workspace = _workspace_of(decode_fp8_workspace_bytes(rows, width, hq, hkv, d, page), workspace, device)
+    with _current(device):
+        rc = _native.load().rlt_paged_decode_fp8(
+            q.data_ptr(), int64_array(q.stride()), key_cache.data_ptr(), value_cache.data_ptr(),
+            int64_array(key_cache.stride()), key_scales.data_ptr(), value_scales.data_ptr(),
+            int64_array(key_scales.stride()), block_tables.data_ptr(), block_tables.stride(0), width,
+            context_lengths.data_ptr(), out.data_ptr(), int64_array(out.stride()), rows, hq, hkv, d, page, nb,
+            1.0 / math.sqrt(d) if scale is None else scale, dtype_code(q.dtype), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), stream_handle(device),
+        )
+    check(rc, "rlt_paged_decode_fp8")
+    return out
+
+
+def prefill_fp8_workspace_bytes(
+    total_q: int, num_seqs: int, table_width: int, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int
+) -> int:
+    """Bytes rlt_paged_prefill_fp8 needs (shape only)."""
+    return int(
+        _native.load().rlt_paged_prefill_fp8_workspace_bytes(
+            total_q, num_seqs, table_width, num_q_heads, num_kv_heads, head_dim, page_size
+        )
+    )
+
+
+def paged_prefill_fp8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lengths: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_seqlen_q: int,
+    out: torch.Tensor | None = None,
+    scale: float | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """paged_prefill over layer slices of an 8-bit cache: packed chunks, bottom-right causal (rlt_paged_prefill_fp8).
+
+    The cache is paged_decode_fp8's; the new tokens' keys are in it already.  Query row
+    i of a sequence's n sees its keys up to context_length - n + i; one that sees
+    none is zeros.  Rows of no sequence (from cu_seqlens_q[-1] on) are left as they
+    are in `out`.  max_seqlen_q is at least the longest chunk.
+    """
+    device, out = _fp8_attention_inputs(
+        q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
+    )
+    _require_rocm(q, cu_seqlens_q)
+    _require_int(cu_seqlens_q, torch.int32, "cu_seqlens_q")
+    total, hq, d = q.shape
+    nb, page, hkv, _ = key_cache.shape
+    nseq, width = block_tables.shape
+    if cu_seqlens_q.shape != (nseq + 1,):
+        raise ValueError("context_lengths and cu_seqlens_q must describe one entry per sequence")
+    if total == 0 or nseq == 0:
+        return out
+    workspace = _workspace_of(prefill_fp8_workspace_bytes(total, nseq, width, hq, hkv, d, page), workspace, device)
+    with _current(device):
+        rc = _native.load().rlt_paged_prefill_fp8(
+            q.data_ptr(), int64_array(q.stride()), key_cache.data_ptr(), value_cache.data_ptr(),
+            int64_array(key_cache.stride()), key_scales.data_ptr(), value_scales.data_ptr(),
+            int64_array(key_scales.stride()), block_tables.data_ptr(), block_tables.stride(0), width,
+            context_lengths.data_ptr(), cu_seqlens_q.data_ptr(), nseq, total, max_seqlen_q, out.data_ptr(),
+            int64_array(out.stride()), hq, hkv, d, page, nb, 1.0 / math.sqrt(d) if scale is None else scale,
+            dtype_code(q.dtype), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            stream_handle(device),
+        )
+    check(rc, "rlt_paged_prefill_fp8")
+    return out
