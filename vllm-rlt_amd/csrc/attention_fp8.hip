@@ -3,6 +3,7 @@
 // over a sequence's keys, for one new token a sequence (decode) and for packed
 // chunks, bottom-right causal (prefill).  Scores, softmax sums and outputs are
 // fp32; the scales multiply the score and the probability of their token.
+#include "decode_fp8.hpp"
 #include "fp8.hpp"
 
 namespace rlt {
@@ -163,7 +164,10 @@ using namespace rlt;
 
 extern "C" int64_t rlt_paged_decode_fp8_workspace_bytes(int64_t n_rows, int64_t max_table_width, int64_t num_q_heads,
                                                         int64_t num_kv_heads, int64_t head_dim, int64_t page_size) {
-  return 0;
+  if (n_rows <= 0 || max_table_width <= 0 || !decode8_shape(num_q_heads, num_kv_heads, head_dim, page_size) ||
+      max_table_width > 0x7fffffff / page_size)
+    return 0;
+  return decode8_workspace(n_rows, max_table_width * page_size, num_q_heads, head_dim);
 }
 
 extern "C" int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, const void* key_cache,
@@ -180,7 +184,11 @@ extern "C" int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, con
                               page_size, num_blocks, scale, dtype, &a))
     return rc;
   if (n_rows == 0) return RLT_OK;
-  return launch_attn8_generic(a, dtype, as_stream(stream), "rlt_paged_decode_fp8");
+  const int64_t need = rlt_paged_decode_fp8_workspace_bytes(n_rows, max_table_width, num_q_heads, num_kv_heads, head_dim, page_size);
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8))
+    return fail(RLT_EWORKSPACE, "rlt_paged_decode_fp8: workspace must be %lld bytes on 8", (long long)need);
+  if (!decode8_layout(a)) return launch_attn8_generic(a, dtype, as_stream(stream), "rlt_paged_decode_fp8");
+  return launch_decode8(a, dtype, workspace, as_stream(stream), "rlt_paged_decode_fp8");
 }
 
 extern "C" int64_t rlt_paged_prefill_fp8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
