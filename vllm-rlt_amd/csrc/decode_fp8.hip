@@ -1,30 +1,37 @@
 // Decode over the 8-bit KV cache: one new token a sequence, split over the
 // cache's length and joined.
 //
-// A row's keys are cut into splits of kSplit tokens (longer ones, doubled, where
-// kMaxSplits would not cover the row), a function of the row's length alone, so a
-// row's bits never depend on its batch.  One workgroup of four waves takes one (row,
-// KV head, split): wave w the w-th quarter of its tokens, so a short row's keys are
-// all in flight at once.  Rows of one split are written at once; the others leave
-// (max, sum, acc) in the workspace for a merge kernel.
+// A row's keys are cut into splits (longer ones, doubled, where kMaxSplits would
+// not cover the row) and a split into kParts parts of consecutive tokens, a
+// function of the row's length alone.  A part of one head is worked by D/16 lanes in
+// order, with a running maximum and sum of its own; the parts of a split and then
+// the splits are joined in order.  So a row's bits depend neither on its batch nor
+// on how parts are spread over waves.
 //
-// Bytes bound it: 2 (D + 1) of them a (token, KV head) against 4 D G flops.  D
-// 64/128/256 on the vector units (one or two query heads a KV head): a lane owns 16
-// dims of a token (one 16-byte load) and D/16 lanes a token, so one load instruction
-// moves 1 KiB of 64 D/16 tokens; codes become fp32 two an instruction.
+// Bytes bound it: 2 (D + 1) of them a (token, KV head) against 4 D G flops.  A lane
+// owns 16 dims of a (token, head), LPT = D/16 lanes hold one.  A wave works on HPW
+// neighbouring heads of PPI parts at once: a load instruction moves HPW * D
+// contiguous bytes of PPI tokens.  After LPT instructions (a tile, 64 (token, head)
+// rows) a reduce-scatter leaves one row's score in every lane, which does one row's
+// softmax.  Wide waves read longest runs of memory; narrow ones, of more parts,
+// give a small launch more waves.
+#include <type_traits>
+
 #include "decode_fp8.hpp"
 
 namespace rlt {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kSplit = 512;
+constexpr int kParts = 16;
+constexpr int kUnit = 16;  // tokens of a page looked up at once (pages hold whole units), and of the shortest part
 constexpr int kMaxSplits = 64;
 constexpr int kXcds = 8;
+constexpr int kCus = 256;
 constexpr int64_t kMaxGrid = 32768;
 
 __host__ __device__ inline void split_plan(int64_t len, int* split_len, int* nsplit) {
-  int64_t per = kSplit;
+  int64_t per = kParts * kUnit;
   while (per * kMaxSplits < len) per <<= 1;
   *split_len = static_cast<int>(per);
   *nsplit = static_cast<int>(len > 0 ? (len + per - 1) / per : 1);
@@ -36,7 +43,8 @@ struct Decode8Args {
   float2* ws_ml;   // [rows][hkv][splits][G], max in log2 units and sum
   int splits;      // splits a row of the tables' width has
   int split_slots; // split-dimension workgroups launched; each walks every split_slots-th split
-  int xcd;         // workgroups of one (split, head) of all rows share an XCD
+  int hpw;         // heads a wave
+  int xcd;         // workgroups of one (split, head block) of all rows share an XCD
   int q_vec;       // q rows are 16-byte aligned, dims together
 };
 
@@ -54,198 +62,262 @@ __device__ __forceinline__ void unpack_codes(const u32x4 w, float* x) {
   }
 }
 
-__device__ __forceinline__ int64_t readlane64(int64_t x, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(x)), lane);
-  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint64_t>(x) >> 32), lane);
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+// Sum over the LPT lanes of a group of LPT values at once: lane s of the group ends
+// with the sum of value s.  Every step halves the values a lane still carries.
+template <int LPT>
+__device__ __forceinline__ float reduce_scatter(float (&x)[LPT], int s) {
+  if constexpr (LPT >= 16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool up = s & 8;
+      const float keep = up ? x[i + 8] : x[i], send = up ? x[i] : x[i + 8];
+      x[i] = keep + __shfl_xor(send, 8, 64);
+    }
+  }
+  if constexpr (LPT >= 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool up = s & 4;
+      const float keep = up ? x[i + 4] : x[i], send = up ? x[i] : x[i + 4];
+      x[i] = keep + __shfl_xor(send, 4, 64);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool up = s & 2;
+    const float keep = up ? x[i + 2] : x[i], send = up ? x[i] : x[i + 2];
+    x[i] = keep + dpp<kDppXor2>(send);
+  }
+  const bool up = s & 1;
+  const float keep = up ? x[1] : x[0], send = up ? x[0] : x[1];
+  return keep + dpp<kDppXor1>(send);
 }
 
-#ifndef WPE
-#define WPE 2
-#endif
-template <typename T, int D, int G>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(WPE))) void decode8_split_kernel(Decode8Args p) {
-  constexpr int LPT = D / 16;      // lanes a token
-  constexpr int TPI = 64 / LPT;    // tokens a load instruction
-  constexpr int IPU = 16 / TPI;    // load instructions a unit of 16 tokens
-  constexpr int TILE = D == 256 ? 32 : 64;
-  constexpr int NI = TILE / TPI;   // loads a tile
-  constexpr int UPT = TILE / 16;   // units a tile
-  constexpr int PARTS = kWaves * TPI;
-  __shared__ __align__(16) float part[PARTS][D];
-  __shared__ float2 part_ml[G][PARTS];
+template <typename T, int D, int G, int HPW, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void decode8_split_kernel(Decode8Args p) {
+  constexpr int LPT = D / 16;              // lanes a (token, head), and tokens (load instructions) a tile
+  constexpr int PPI = 64 / (LPT * HPW);    // parts a wave works on at once
+  constexpr int PPW = kParts / (W * PPI);  // parts a group of lanes works through
+  constexpr int TPU = kUnit / LPT;         // tiles a unit
+  static_assert(LPT * HPW * PPI == 64 && PPW * W * PPI == kParts && TPU * LPT == kUnit, "whole groups, parts and tiles");
+  __shared__ __align__(16) float part[kParts][HPW][G][D];
+  __shared__ float2 part_ml[kParts][HPW][G];
 
   const Attn8Args& a = p.a;
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
-  const uint32_t groups = static_cast<uint32_t>(a.hkv) * p.split_slots;
+  const uint32_t rows = static_cast<uint32_t>(a.rows), x = blockIdx.x % kXcds, t = blockIdx.x / kXcds;
+  const uint32_t blocks = a.hkv / HPW, groups = blocks * p.split_slots;
   uint32_t gi, r;
-  if (p.xcd) {  // workgroup b runs on XCD b % 8: the rows of one (split, head) on one XCD, back to back
-    const uint32_t t = blockIdx.x / kXcds, rows = static_cast<uint32_t>(a.rows);
-    gi = t / rows * kXcds + blockIdx.x % kXcds;
+  if (p.xcd) {  // workgroup b runs on XCD b % 8: all rows of a (split, head block) on one XCD, back to back
+    gi = t / rows * kXcds + x;
     r = t % rows;
   } else {
     gi = blockIdx.x % groups;
     r = blockIdx.x / groups;
   }
   gi = uniform(gi), r = uniform(r);
-  const int h = gi % a.hkv;
+  const int h0 = gi % blocks * HPW;
   const int len = sequence_length(a, r);
   int split_len, ns;
   split_plan(len, &split_len, &ns);
-  const int g = lane / LPT, s = lane % LPT;
+  const int s = lane % LPT, gh = lane / LPT % HPW, gp = lane / (LPT * HPW), group0 = lane & ~(LPT - 1);
+  const int part_len = split_len / kParts;
+  const uint32_t units = static_cast<uint32_t>(part_len) / kUnit;  // a part, a power of two
+  const int unit_shift = 31 - __builtin_clz(units);
 
   T* orow = static_cast<T*>(a.out) + r * a.o_row;
   const int32_t* trow = a.tables + r * a.table_stride;
-  const uint8_t* kh = a.k + h * a.kv_head + 16 * s;
-  const uint8_t* vh = a.v + h * a.kv_head + 16 * s;
-  const uint8_t* ksh = a.ks + h * a.s_head;
-  const uint8_t* vsh = a.vs + h * a.s_head;
+  const uint8_t* kh = a.k + h0 * a.kv_head;
+  const uint8_t* vh = a.v + h0 * a.kv_head;
+  const uint8_t* ksh = a.ks + (h0 + gh) * a.s_head;
+  const uint8_t* vsh = a.vs + (h0 + gh) * a.s_head;
+  const uint32_t token_bytes = static_cast<uint32_t>(a.kv_token);
+  const int64_t lane_off = gh * a.kv_head + 16 * s;
 
-  for (int sp = gi / a.hkv; sp < ns; sp += p.split_slots) {
-    // The wave's tokens [t0, t0 + n).
-    const int quarter = split_len / kWaves;
-    const int t0 = sp * split_len + wave * quarter;
-    const int n = min(max(len - t0, 0), quarter);
+  for (int sp = gi / blocks; sp < ns; sp += p.split_slots) {
+    const int n_split = min(len - sp * split_len, split_len);
+    // Steps of this wave: unit u of its k-th parts, as far as its first group has tokens.
+    const int wave_tok = wave * (PPW * PPI) * part_len;
+    const int rel = n_split - wave_tok;
+    uint32_t tiles = 0;
+    if (rel > 0) {
+      const int round = PPI * part_len;  // tokens from one part of a group to its next
+      const int k = min(rel / round, PPW), rem = k < PPW ? rel - k * round : 0;
+      tiles = k * (units * TPU) + (min(rem, part_len) + LPT - 1) / LPT;
+    }
+    // The first token of a step's unit in this lane's group.
+    auto unit_token = [&](uint32_t step) __attribute__((always_inline)) {
+      return sp * split_len + wave_tok + static_cast<int>((step >> unit_shift) * PPI + gp) * part_len +
+             static_cast<int>(step & (units - 1)) * kUnit;
+    };
     float q[G][16], acc[G][16], m[G], l[G];
+    if (!p.q_vec) {  // any strides: through LDS, a few elements a thread
+#pragma unroll 1
+      for (int o = threadIdx.x; o < HPW * G * D; o += 64 * W)
+        (&part[0][0][0][0])[o] = load_elem(static_cast<const T*>(a.q) + r * a.q_row + (h0 * G + o / D) * a.q_head + o % D * a.q_dim);
+      __syncthreads();
+    }
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-      const T* qrow = static_cast<const T*>(a.q) + r * a.q_row + (h * G + j) * a.q_head;
       if (p.q_vec) {
+        const T* qrow = static_cast<const T*>(a.q) + r * a.q_row + ((h0 + gh) * G + j) * a.q_head + 16 * s;
         constexpr int N = Packet<T>::N;
 #pragma unroll
-        for (int c = 0; c < 16 / N; ++c) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + 16 * s + c * N), &q[j][c * N]);
+        for (int c = 0; c < 16 / N; ++c) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + c * N), &q[j][c * N]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) q[j][e] = load_elem(qrow + (16 * s + e) * a.q_dim);
+        for (int e = 0; e < 16; ++e) q[j][e] = part[0][0][0][(gh * G + j) * D + 16 * s + e];
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) q[j][e] *= a.qscale, acc[j][e] = 0.f;
       m[j] = -INFINITY, l[j] = 0.f;
     }
-    for (int c0 = 0; c0 < n; c0 += 1024) {  // 64 units, one a lane
-      const int left = min(n - c0, 1024);
-      const int units = (left + 15) / 16;
-      // This lane's unit: where its 16 tokens begin (pages hold whole units).
-      const int tok = t0 + c0 + 16 * min(lane, units - 1);
-      const int page = tok / a.page, slot = tok - page * a.page;
-      const int64_t blk = block_of(a, trow[page]);
-      const int64_t unit_kv = blk * a.kv_block + slot * a.kv_token;
-      const int64_t unit_s = blk * a.s_block + slot * a.s_token;
-      const int last_unit = units - 1, last_tok = left - 1 - 16 * last_unit;
-      u32x4 k[NI], v[NI];
-      uint32_t kb = 0, vb = 0;
-      // Tokens past the end re-read the last one: in bounds, and masked below.
-      auto issue = [&](int tile, const uint8_t* base, u32x4 (&x)[NI]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int u = min(tile * UPT + i / IPU, last_unit);
-          const int t = min((i % IPU) * TPI + g, u == last_unit ? last_tok : 15);
-          x[i] = load_codes(base + readlane64(unit_kv, u) + static_cast<int32_t>(t * static_cast<int32_t>(a.kv_token)));
-        }
+    if (!p.q_vec) __syncthreads();
+
+    if (tiles > 0) {
+      const int last_unit = (len - 1) / kUnit * kUnit;
+      int64_t entry_kv, entry_s;  // lane s of a group: where the group's unit of step chunk * LPT + s begins
+      int64_t off, off_s;         // where this lane's unit of the tile being loaded begins
+      int lim;                    // its last token
+      uint32_t kb, vb;
+      u32x4 k[LPT], v[LPT];
+      // A unit past the row's end is replaced by the row's last, and a token past it by
+      // its last token: in bounds, and masked below.
+      auto load_entries = [&](uint32_t chunk) __attribute__((always_inline)) {
+        const int tok = min(unit_token(chunk * LPT + s), last_unit);
+        const int page = tok / a.page, slot = tok - page * a.page;
+        const int64_t blk = block_of(a, trow[page]);
+        entry_kv = blk * a.kv_block + slot * a.kv_token;
+        entry_s = blk * a.s_block + slot * a.s_token;
       };
-      auto issue_scales = [&](int tile) __attribute__((always_inline)) {
-        const int t = min(tile * TILE + (lane & (TILE - 1)), left - 1);
-        const int64_t at = __shfl(unit_s, t >> 4, 64) + (t & 15) * a.s_token;
+      auto find_unit = [&](uint32_t step) __attribute__((always_inline)) {
+        if (step % LPT == 0) load_entries(step / LPT);
+        const int from = group0 + static_cast<int>(step % LPT);
+        off = __shfl(entry_kv, from, 64) + lane_off;
+        off_s = __shfl(entry_s, from, 64);
+        lim = min(len - 1 - min(unit_token(step), last_unit), kUnit - 1);
+      };
+      auto issue = [&](uint32_t tile, const uint8_t* base, u32x4 (&y)[LPT]) __attribute__((always_inline)) {
+        const uint32_t first = tile % TPU * LPT;
+#pragma unroll
+        for (uint32_t i = 0; i < LPT; ++i)
+          y[i] = load_codes(base + (off + __umul24(min(first + i, static_cast<uint32_t>(lim)), token_bytes)));
+      };
+      // This lane's row of a tile: token s, head gh.
+      auto issue_scales = [&](uint32_t tile) __attribute__((always_inline)) {
+        const int64_t at = off_s + min(static_cast<int>(tile % TPU * LPT) + s, lim) * a.s_token;
         kb = ksh[at];
         vb = vsh[at];
       };
-      const int tiles = (left + TILE - 1) / TILE;
+      auto step = [&](uint32_t tile, auto more) __attribute__((always_inline)) {
+        constexpr bool MORE = decltype(more)::value;  // another tile follows
+        float score[G][LPT];
+#pragma unroll
+        for (int i = 0; i < LPT; ++i) {
+          float y[16];
+          unpack_codes(k[i], y);
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+            float dot = q[j][0] * y[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) dot = fmaf(q[j][e], y[e], dot);
+            score[j][i] = dot;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const float sk = scale_value(kb), sv = scale_value(vb), bias = value_bias(vb);
+        const bool in = unit_token(tile / TPU) + static_cast<int>(tile % TPU * LPT) + s < len;
+        if constexpr (MORE) {
+          if ((tile + 1) % TPU == 0) find_unit((tile + 1) / TPU);
+          issue_scales(tile + 1);
+          issue(tile + 1, kh, k);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        float pv[G];  // this lane's row: its probability times its V scale
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          const float sum = reduce_scatter<LPT>(score[j], s) * sk;
+          const float dot = in ? sum : -INFINITY;
+          const float top = fmaxf(m[j], group_max<LPT>(dot + bias));
+          const float base = top == -INFINITY ? 0.f : top;  // only -inf scores so far: they weigh 0
+          const float corr = fast_exp2(m[j] - base);
+          const float w = fast_exp2(dot - base);
+          m[j] = top;
+          l[j] = fmaf(l[j], corr, w);
+          pv[j] = w * sv;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
+        }
+#pragma unroll
+        for (int i = 0; i < LPT; ++i) {
+          float y[16];
+          unpack_codes(v[i], y);
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+            const float w = __shfl(pv[j], group0 + i, 64);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(w, y[e], acc[j][e]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (MORE) {
+          issue(tile + 1, vh, v);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // The end of a part: its state to LDS.
+        if (!MORE || (tile + 1) % (units * TPU) == 0) {
+          const int pt = (wave * PPW + static_cast<int>(tile / TPU >> unit_shift)) * PPI + gp;
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+            const float sum = group_sum<LPT>(l[j]);
+            if (s == 0) part_ml[pt][gh][j] = make_float2(m[j], sum);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              u32x4 y;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(acc[j][4 * c + e]), acc[j][4 * c + e] = 0.f;
+              *reinterpret_cast<u32x4*>(&part[pt][gh][j][16 * s + 4 * c]) = y;
+            }
+            m[j] = -INFINITY, l[j] = 0.f;
+          }
+        }
+      };
+      find_unit(0);
       issue_scales(0);
       issue(0, kh, k);
       issue(0, vh, v);
-      for (int tile = 0; tile < tiles; ++tile) {
-        const float sk = scale_value(kb), sv = scale_value(vb), bias = value_bias(vb);
-        if (tile + 1 < tiles) issue_scales(tile + 1);
-        float score[G][NI];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          float x[16];
-          unpack_codes(k[i], x);
-          const float scale = __shfl(sk, i * TPI + g, 64);
-          const bool in = tile * TILE + i * TPI + g < left;
-#pragma unroll
-          for (int j = 0; j < G; ++j) {
-            float dot = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dot = fmaf(q[j][e], x[e], dot);
-            dot = group_sum<LPT>(dot) * scale;
-            score[j][i] = in ? dot : -INFINITY;
-          }
-        }
-        if (tile + 1 < tiles) issue(tile + 1, kh, k);
-        float w[NI], b[NI];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          w[i] = __shfl(sv, i * TPI + g, 64);
-          b[i] = __shfl(bias, i * TPI + g, 64);
-        }
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-          float top = m[j];
-#pragma unroll
-          for (int i = 0; i < NI; ++i) top = fmaxf(top, score[j][i] + b[i]);
-          const float off = top == -INFINITY ? 0.f : top;  // only -inf scores so far: they weigh 0
-          const float corr = fast_exp2(m[j] - off);
-          m[j] = top;
-          l[j] *= corr;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
-#pragma unroll
-          for (int i = 0; i < NI; ++i) {
-            score[j][i] = fast_exp2(score[j][i] - off);
-            l[j] += score[j][i];
-            score[j][i] *= w[i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          float x[16];
-          unpack_codes(v[i], x);
-#pragma unroll
-          for (int j = 0; j < G; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(score[j][i], x[e], acc[j][e]);
-        }
-        if (tile + 1 < tiles) issue(tile + 1, vh, v);
-      }
+#pragma unroll 1
+      for (uint32_t tile = 0; tile + 1 < tiles; ++tile) step(tile, std::true_type{});
+      step(tiles - 1, std::false_type{});
     }
-    // Join the waves' token groups, in a fixed order.
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-      if (s == 0) part_ml[j][wave * TPI + g] = make_float2(m[j], l[j]);
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      if (j) __syncthreads();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        u32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __float_as_uint(acc[j][4 * c + e]);
-        *reinterpret_cast<u32x4*>(&part[wave * TPI + g][16 * s + 4 * c]) = x;
-      }
-      __syncthreads();
+    __syncthreads();
+    // Join the parts that have tokens, in order.
+    const int live = (n_split + part_len - 1) / part_len;
+#pragma unroll 1
+    for (int o = threadIdx.x; o < HPW * G * D; o += 64 * W) {
+      const int hd = o / (G * D), j = o / D % G, d = o % D;
       float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < PARTS; ++i) top = fmaxf(top, part_ml[j][i].x);
-      const float off = top == -INFINITY ? 0.f : top;
-      const int d = threadIdx.x;
-      if (d < D) {
-        float sum = 0.f, x = 0.f;
+      for (int i = 0; i < kParts; ++i)
+        if (i < live) top = fmaxf(top, part_ml[i][hd][j].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, y = 0.f;
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
-          const float2 ml = part_ml[j][i];
-          const float w = fast_exp2(ml.x - off);
-          sum = fmaf(ml.y, w, sum);
-          x = fmaf(part[i][d], w, x);
-        }
-        if (ns == 1) {
-          store_elem(orow + (h * G + j) * a.o_head + d * a.o_dim, len > 0 ? x * (1.f / sum) : 0.f);
-        } else {
-          const int64_t at = ((static_cast<int64_t>(r) * a.hkv + h) * p.splits + sp) * G + j;
-          p.ws_acc[at * D + d] = x;
-          if (d == 0) p.ws_ml[at] = make_float2(top, sum);
-        }
+      for (int i = 0; i < kParts; ++i) {
+        if (i >= live) break;
+        const float2 ml = part_ml[i][hd][j];
+        const float w = fast_exp2(ml.x - base);
+        sum = fmaf(ml.y, w, sum);
+        y = fmaf(part[i][hd][j][d], w, y);
+      }
+      const int h = h0 + hd;
+      if (ns == 1) {
+        store_elem(orow + (h * G + j) * a.o_head + d * a.o_dim, len > 0 ? y * (1.f / sum) : 0.f);
+      } else {
+        const int64_t at = ((static_cast<int64_t>(r) * a.hkv + h) * p.splits + sp) * G + j;
+        p.ws_acc[at * D + d] = y;
+        if (d == 0) p.ws_ml[at] = make_float2(top, sum);
       }
     }
     __syncthreads();
@@ -293,33 +365,65 @@ __global__ __launch_bounds__(64 * kWaves) void decode8_merge_kernel(Decode8Args 
   for (int e = 0; e < E; ++e) store_elem(orow + (lane + 64 * e) * a.o_dim, acc[e] * inv);
 }
 
-template <typename T, int D>
-void launch_shape(const Decode8Args& p, int G, unsigned grid, hipStream_t stream) {
-  const dim3 block(64 * kWaves);
-  switch (G) {
-    case 1: hipLaunchKernelGGL((decode8_split_kernel<T, D, 1>), dim3(grid), block, 0, stream, p); break;
-    default: hipLaunchKernelGGL((decode8_split_kernel<T, D, 2>), dim3(grid), block, 0, stream, p); break;
-  }
-  if (p.splits > 1) {
-    const unsigned merge = static_cast<unsigned>((p.a.rows * p.a.hq + kWaves - 1) / kWaves);
-    hipLaunchKernelGGL((decode8_merge_kernel<T, D>), dim3(merge), block, 0, stream, p);
+template <typename T, int D, int G, int HPW>
+void launch_split(const Decode8Args& p, unsigned grid, hipStream_t stream) {
+  constexpr int PPI = 1024 / (D * HPW);
+  if constexpr (PPI > 0 && HPW * G * D <= 1024) {
+    constexpr int W = PPI * 4 <= kParts ? 4 : kParts / PPI;
+    hipLaunchKernelGGL((decode8_split_kernel<T, D, G, HPW, W>), dim3(grid), dim3(64 * W), 0, stream, p);
   }
 }
 
-template <typename T>
-void launch_type(const Decode8Args& p, int G, unsigned grid, hipStream_t stream) {
-  switch (p.a.d) {
-    case 64: launch_shape<T, 64>(p, G, grid, stream); break;
-    case 128: launch_shape<T, 128>(p, G, grid, stream); break;
-    default: launch_shape<T, 256>(p, G, grid, stream); break;
+template <typename T, int D, int G>
+void launch_shape(const Decode8Args& p, unsigned grid, hipStream_t stream) {
+  switch (p.hpw) {
+    case 8: launch_split<T, D, G, 8>(p, grid, stream); break;
+    case 4: launch_split<T, D, G, 4>(p, grid, stream); break;
+    case 2: launch_split<T, D, G, 2>(p, grid, stream); break;
+    default: launch_split<T, D, G, 1>(p, grid, stream); break;
   }
+  if (p.splits > 1) {
+    const unsigned merge = static_cast<unsigned>((p.a.rows * p.a.hq + kWaves - 1) / kWaves);
+    hipLaunchKernelGGL((decode8_merge_kernel<T, D>), dim3(merge), dim3(64 * kWaves), 0, stream, p);
+  }
+}
+
+template <typename T, int D>
+void launch_group(const Decode8Args& p, unsigned grid, hipStream_t stream) {
+  if (p.a.hq == p.a.hkv) launch_shape<T, D, 1>(p, grid, stream);
+  else launch_shape<T, D, 2>(p, grid, stream);
+}
+
+template <typename T>
+void launch_type(const Decode8Args& p, unsigned grid, hipStream_t stream) {
+  switch (p.a.d) {
+    case 64: launch_group<T, 64>(p, grid, stream); break;
+    case 128: launch_group<T, 128>(p, grid, stream); break;
+    default: launch_group<T, 256>(p, grid, stream); break;
+  }
+}
+
+// Heads a wave: as many neighbours as divide the heads, fit a load instruction and
+// the LDS of two workgroups a CU, and leave a workgroup for three CUs in four.  Measured, us
+// (16 heads x 128, bf16, 1 / 2 / 4 / 8 heads a wave): 4 rows of up to 256 tokens 6.7
+// / 7.1 / 12.3 / 20.4, 16 of up to 512 13.8 / 12.2 / 16.8 / 25.2, 1 of 8000 16.5 /
+// 14.6 / 19.4 / 26.5, 256 of up to 256 45.2 / 42.7 / 46.6 / 41.5, 64 of 512-4096 143
+// / 134 / 143 / 126, 256 of 1024-8192 1055 / 1000 / 1020 / 867, 2 of 16384-32768
+// (244 workgroups at 8) 55.9 / 51.6 / 53.1 / 47.5.
+int heads_a_wave(const Attn8Args& a, int64_t splits) {
+  const int G = a.hq / a.hkv;
+  int hpw = 1;
+  while (hpw < 8 && a.hkv % (2 * hpw) == 0 && 2 * hpw * G * a.d <= 1024 &&
+         a.rows * (a.hkv / (2 * hpw)) * splits >= kCus * 3 / 4)
+    hpw *= 2;
+  return hpw;
 }
 
 }  // namespace
 
 bool decode8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page) {
   const int64_t G = hkv > 0 ? hq / hkv : 0;
-  return (d == 64 || d == 128 || d == 256) && page % 16 == 0 && (G == 1 || G == 2);
+  return (d == 64 || d == 128 || d == 256) && page % kUnit == 0 && (G == 1 || G == 2);
 }
 
 int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t d) {
@@ -331,7 +435,7 @@ int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t d) 
 bool decode8_layout(const Attn8Args& a) {
   auto rows16 = [](const void* x) { return aligned16(x); };
   return decode8_shape(a.hq, a.hkv, a.d, a.page) && a.kv_dim == 1 && rows16(a.k) && rows16(a.v) && a.kv_head % 16 == 0 &&
-         a.kv_token % 16 == 0 && a.kv_block % 16 == 0 && a.kv_token < (int64_t(1) << 27);
+         a.kv_token % 16 == 0 && a.kv_block % 16 == 0 && a.kv_token < (int64_t(1) << 24) && a.kv_head < (int64_t(1) << 24);
 }
 
 int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, const char* name) {
@@ -339,19 +443,20 @@ int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, 
   p.a = a;
   int per;
   split_plan(a.max_len, &per, &p.splits);
-  const int64_t items = a.rows * a.hkv;
+  p.hpw = heads_a_wave(a, p.splits);
+  const int64_t items = a.rows * (a.hkv / p.hpw);
   p.split_slots = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.splits, kMaxGrid / items)));
-  p.xcd = a.hkv * p.split_slots % kXcds == 0;
+  p.xcd = a.hkv / p.hpw * p.split_slots % kXcds == 0;
   const int es = dtype_size(dtype);
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
   p.ws_acc = static_cast<float*>(ws);
   p.ws_ml = reinterpret_cast<float2*>(p.ws_acc + a.rows * p.splits * a.hq * a.d);
   const unsigned grid = static_cast<unsigned>(items * p.split_slots);
-  const int G = a.hq / a.hkv;
+
   switch (dtype) {
-    case RLT_BFLOAT16: launch_type<bf16>(p, G, grid, stream); break;
-    case RLT_FLOAT16: launch_type<f16>(p, G, grid, stream); break;
-    default: launch_type<float>(p, G, grid, stream); break;
+    case RLT_BFLOAT16: launch_type<bf16>(p, grid, stream); break;
+    case RLT_FLOAT16: launch_type<f16>(p, grid, stream); break;
+    default: launch_type<float>(p, grid, stream); break;
   }
   return check_launch(name);
 }
