@@ -5,6 +5,7 @@
 // fp32; the scales multiply the score and the probability of their token.
 #include "decode_fp8.hpp"
 #include "fp8.hpp"
+#include "prefill_fp8.hpp"
 
 namespace rlt {
 namespace {
@@ -216,5 +217,6 @@ extern "C" int rlt_paged_prefill_fp8(const void* q, const int64_t* q_strides, co
   if (total_q == 0 || num_seqs == 0) return RLT_OK;
   if (!cu_seqlens_q) return fail(RLT_EINVAL, "rlt_paged_prefill_fp8: NULL pointer argument");
   a.cu = cu_seqlens_q;
+  if (prefill8_layout(a)) return launch_prefill8(a, dtype, as_stream(stream), "rlt_paged_prefill_fp8");
   return launch_attn8_generic(a, dtype, as_stream(stream), "rlt_paged_prefill_fp8");
 }

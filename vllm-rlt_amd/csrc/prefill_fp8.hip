@@ -1,0 +1,461 @@
+// Packed chunked prefill over the 8-bit KV cache, bottom-right causal, on the
+// matrix cores (head_dim 64 / 128, pages of a power of two of at least 16 tokens).
+//
+// A workgroup of 4 waves takes 128 query rows of one (sequence, query head) over a
+// segment of its keys, a wave 32 rows, 64 keys a tile:
+// - S^T = K Q^T on the scaled 8-bit MFMA (32x32x64): K's codes go from LDS into it as
+//   they are, and its scale operand takes a key's e8m0 byte, so nothing of K is
+//   converted.  q becomes rows of codes, each the rest of the one before with a scale 16
+//   times smaller: 4 significant bits each, so two hold a bf16 and three an fp16 (the
+//   last bits of values 2^13 below their row's largest aside).  The 8-bit MFMA has twice
+//   the rate of the 16-bit one: two parts cost what a bf16 q would.  Its sums carry about
+//   18 bits, too few for an fp32 q, which is split in three bf16 parts for the bf16
+//   MFMA against K converted with its scale (exact: a code has 4 bits).
+// - O^T += V^T P^T on the bf16 MFMA (32x32x16).  V becomes bf16, its scale included
+//   (exact: a code has 4 bits), once a workgroup, on its way into LDS; V^T comes from
+//   transposing LDS reads, P from the registers S^T left it in.  P is rounded to bf16
+//   (its sum is taken over the rounded values) for bf16 outputs, and split in two or three
+//   bf16 parts for fp16 and fp32 ones.
+// The running maximum moves only when a tile's exceeds it by 2^kRescale.
+#include "prefill_fp8.hpp"
+
+#include "mfma.hpp"
+
+namespace rlt {
+namespace {
+
+constexpr int kBM = 128;  // query rows a workgroup
+constexpr int kBN = 64;   // keys a tile
+constexpr float kRescale = 8.f;
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Parts;
+template <> struct Parts<bf16> { static constexpr int Q = 2, P = 1; };
+template <> struct Parts<f16> { static constexpr int Q = 3, P = 2; };
+template <> struct Parts<float> { static constexpr int Q = 3, P = 3; };
+
+struct Prefill8Args {
+  Attn8Args a;
+  int page_shift;
+  int out_vec;  // 4 elements of an out row can be stored at once
+  int q_vec;    // q rows are 16-byte aligned, dims together
+};
+
+// Rows [row0, row0 + nq) of sequence s, inside [0, rows) whatever cu holds.
+__device__ __forceinline__ void seq_rows(const Attn8Args& a, int s, int& row0, int& nq) {
+  const int rows = static_cast<int>(a.rows);
+  row0 = min(max(a.cu[s], 0), rows);
+  nq = min(max(a.cu[s + 1], row0), rows) - row0;
+}
+
+// Query tile `unit` of the packed batch: its sequence, found by the wave 64 at a time.
+__device__ __forceinline__ bool find_tile(const Attn8Args& a, int unit, int* seq, int* tile) {
+  const int lane = threadIdx.x & 63;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+    int row0 = 0, nq = 0;
+    if (s0 + lane < a.num_seqs) seq_rows(a, s0 + lane, row0, nq);
+    const int tiles = (nq + kBM - 1) / kBM;
+    int upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += y;
+    }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(unit >= upto - tiles && unit < upto);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      *seq = s0 + at;
+      *tile = unit - __builtin_amdgcn_readlane(upto - tiles, at);
+      return true;
+    }
+    unit -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) { return MfmaOps<bf16>::pack2(x, y); }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void prefill8_kernel(Prefill8Args p) {
+  using Ops = MfmaOps<bf16>;
+  constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P;
+  constexpr int KS = D / 64;       // MFMA steps over the dims
+  constexpr int DT = D / 32;       // output tiles of 32 dims
+  constexpr int CH = D / 16;       // 16-byte chunks of a code row
+  constexpr int TPP = 256 / CH;    // tokens a staging pass
+  constexpr int PASSES = kBN / TPP;
+  // Padded rows: 8 lanes' 16-byte reads of 8 K rows fall into distinct bank groups
+  // (the stride is an odd multiple of 16 bytes modulo 128), and so do the
+  // transposing V reads (64 modulo 256).
+  constexpr int KROW = D + 16, VROW = D + 32;  // bytes, bf16 elements
+  __shared__ __align__(16) uint8_t k_lds[2][kBN * KROW];
+  __shared__ __align__(16) uint16_t v_lds[2][kBN * VROW];
+  __shared__ uint8_t ks_lds[2][kBN];
+  __shared__ __align__(16) float bias_lds[2][4];  // of each wave's staged V scales (value_bias)
+  __shared__ __align__(16) int nan_lds[2][4];     // whether the wave staged a V that is NaN
+
+  const Attn8Args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  int seq, qt;
+  const int h = blockIdx.x % a.hq;
+  if (!find_tile(a, blockIdx.x / a.hq, &seq, &qt)) return;
+  seq = uniform(seq);
+  int row0, nq;
+  seq_rows(a, seq, row0, nq);
+  row0 = uniform(row0), nq = uniform(nq);
+  qt = uniform((nq + kBM - 1) / kBM - 1 - qt);  // the last rows, which see most keys, first
+  const int len = uniform(sequence_length(a, seq));
+  const int prefix = len - nq;  // query row i sees keys up to prefix + i
+  const int qt0 = qt * kBM;
+  const int kvh = h / (a.hq / a.hkv);
+  const int wg_keys = min(prefix + min(qt0 + kBM, nq), len);
+  const int ntiles = (max(wg_keys, 0) + kBN - 1) / kBN;
+
+  const int half = lane >> 5, col = lane & 31;
+  const int wave_row0 = qt0 + wave * 32;
+  const int my_row = wave_row0 + col;
+  const bool row_valid = my_row < nq;
+  const int limit = row_valid ? prefix + my_row : -1;  // last key this lane's query sees
+  const int wave_last = prefix + min(wave_row0 + 31, nq - 1);
+  const bool wave_live = wave_row0 < nq;
+
+  // q's parts, B operands.  8-bit: lane (col, half) holds dims [64c + 32 half, + 32) of
+  // row col; bf16: of the 32 dims of a pair of k-steps, [16 half, + 8) for the first and
+  // the next 8 for the second.
+  constexpr bool WIDE = sizeof(T) == 4;
+  i32x8 qb[NQ][KS];
+  u32x4 qw[NQ][2 * DT];
+  int q_scale[NQ];
+  {
+    const T* qrow = static_cast<const T*>(a.q) + (row0 + min(my_row, nq - 1)) * a.q_row + h * a.q_head;
+    constexpr int RUN = WIDE ? 16 : 32, RUNS = D / 2 / RUN;  // a lane's dims: RUNS runs of RUN
+    float x[RUNS][RUN];
+    float amax = 0.f;
+#pragma unroll
+    for (int c = 0; c < RUNS; ++c) {
+      const int d0 = 2 * RUN * c + RUN * half;
+      if (p.q_vec) {
+        constexpr int N = Packet<T>::N;
+#pragma unroll
+        for (int i = 0; i < RUN / N; ++i) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + d0 + i * N), &x[c][i * N]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) x[c][i] = load_elem(qrow + (d0 + i) * a.q_dim);
+      }
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) amax = fmaxf(amax, finite_abs(x[c][i]));
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int c = 0; c < RUNS; ++c)
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            // The top 16 bits: the rest is exact, and the third part holds all of it.
+            const uint32_t lo = __float_as_uint(x[c][2 * w]), hi = __float_as_uint(x[c][2 * w + 1]);
+            qw[n][2 * c + w / 4][w % 4] = lo >> 16 | (hi & 0xffff0000u);
+            x[c][2 * w] -= __uint_as_float(lo & 0xffff0000u);
+            x[c][2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
+          }
+    } else {
+      amax = max_across_halves(amax);
+      const uint32_t b = max(scale_byte(amax), 4u * NQ);
+      const float inv = inverse_scale(b);
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          x[c][i] = (__float_as_uint(x[c][i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : x[c][i] * inv;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        q_scale[n] = static_cast<int>(b) - 4 * n;
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            float* y = &x[c][4 * w];
+            int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+            word = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], word, true);
+            qb[n][c][w] = word;
+            if (n + 1 < NQ) {
+              const f32x2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
+              y[0] = (y[0] - lo[0]) * 16.f, y[1] = (y[1] - lo[1]) * 16.f;
+              y[2] = (y[2] - hi[0]) * 16.f, y[3] = (y[3] - hi[1]) * 16.f;
+            }
+          }
+      }
+    }
+  }
+
+  // Staging: thread (token, chunk), PASSES tokens TPP apart.  Tokens past the last key
+  // re-read it (in bounds; they are masked).
+  const int32_t* trow = a.tables + seq * a.table_stride;
+  const int st = tid / CH, sc = tid % CH;
+  const uint8_t* kbase = a.k + kvh * a.kv_head + sc * 16;
+  const uint8_t* vbase = a.v + kvh * a.kv_head + sc * 16;
+  const uint8_t* ksbase = a.ks + kvh * a.s_head;
+  const uint8_t* vsbase = a.vs + kvh * a.s_head;
+  const int page_mask = a.page - 1;
+  int32_t ids[PASSES], ks_id;
+  u32x4 kreg[PASSES], vreg[PASSES];
+  uint32_t vsreg[PASSES], ksreg;
+  auto token = [&](int tile, int t) { return min(tile * kBN + t, wg_keys - 1); };
+  auto load_ids = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
+    ks_id = trow[token(tile, lane) >> p.page_shift];
+  };
+  auto load_tile = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int slot = token(tile, i * TPP + st) & page_mask;
+      const int64_t blk = block_of(a, ids[i]);
+      const int64_t at = blk * a.kv_block + slot * a.kv_token;
+      kreg[i] = *reinterpret_cast<const u32x4*>(kbase + at);
+      vreg[i] = *reinterpret_cast<const u32x4*>(vbase + at);
+      vsreg[i] = vsbase[blk * a.s_block + slot * a.s_token];
+    }
+    ksreg = ksbase[block_of(a, ks_id) * a.s_block + (token(tile, lane) & page_mask) * a.s_token];
+  };
+  auto store_tile = [&](int buf, bool masked) __attribute__((always_inline)) {
+    float bias = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int t = i * TPP + st;
+      *reinterpret_cast<u32x4*>(&k_lds[buf][t * KROW + sc * 16]) = kreg[i];
+      // The scale operand is the exponent of an fp32: byte 0 and 255 as in the e8m0 type.
+      const float sv = scale_value(vsreg[i]);
+      bias = fmaxf(bias, value_bias(vsreg[i] == 255u ? 0u : vsreg[i]));
+      u32x4 lo, hi;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const f32x2v x0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(vreg[i][w]), false);
+        const f32x2v x1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(vreg[i][w]), true);
+        const uint32_t u = bf16_pair(x0[0] * sv, x0[1] * sv), v = bf16_pair(x1[0] * sv, x1[1] * sv);
+        if (w < 2) lo[2 * w] = u, lo[2 * w + 1] = v;
+        else hi[2 * w - 4] = u, hi[2 * w - 3] = v;
+        if (masked) nan |= (((vreg[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0 || vsreg[i] == 255u;
+      }
+      uint16_t* dst = &v_lds[buf][t * VROW + sc * 16];
+      *reinterpret_cast<u32x4*>(dst) = lo;
+      *reinterpret_cast<u32x4*>(dst + 8) = hi;
+    }
+    if (wave == 0) ks_lds[buf][lane] = static_cast<uint8_t>(ksreg);
+    const float wave_bias = __builtin_amdgcn_ballot_w64(bias > 0.f) ? group_max<64>(bias) : 0.f;
+    const int wave_nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    if (lane == 0) {
+      bias_lds[buf][wave] = wave_bias;
+      nan_lds[buf][wave] = wave_nan;
+    }
+  };
+  // Whether some row of the workgroup does not see all of a tile's keys.
+  auto tile_masked = [&](int tile) { return tile * kBN + kBN - 1 > prefix + qt0; };
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int c = 0; c < DT; ++c) acc[c] = f32x16{};
+  float m = -INFINITY, lsum = 0.f;
+
+  // V^T operands: in each 16-lane group lane L addresses key row L / 4 of its four and 4
+  // dims; k-step ks, element e of half hf holds key 16 ks + 8 (e / 4) + 4 hf + e % 4.
+  const int grp = lane >> 4, gl = lane & 15;
+  const int tr_off = (4 * (grp >> 1) + (gl >> 2)) * VROW + 16 * (grp & 1) + 4 * (gl & 3);
+
+  if (ntiles > 0) {
+    load_ids(0);
+    load_tile(0);
+    load_ids(1);
+    store_tile(0, tile_masked(0));
+  }
+  __syncthreads();
+  for (int j = 0; j < ntiles; ++j) {
+    const int buf = j & 1;
+    if (j + 1 < ntiles) {
+      load_tile(j + 1);
+      load_ids(j + 2);
+    }
+    if (wave_live && j * kBN <= wave_last) {
+      f32x16 s[2] = {{}, {}};
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int ksc = ks_lds[buf][hh * 32 + col];
+        const uint8_t* row = &k_lds[buf][(hh * 32 + col) * KROW];
+        if constexpr (WIDE) {
+          const float kscale = scale_value(static_cast<uint32_t>(ksc));
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            const u32x4 codes = *reinterpret_cast<const u32x4*>(row + 32 * c + 16 * half);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              u32x4 ka;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int w = static_cast<int>(codes[2 * u + e / 2]);
+                const f32x2v y = e % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+                ka[e] = bf16_pair(y[0] * kscale, y[1] * kscale);
+              }
+#pragma unroll
+              for (int n = 0; n < NQ; ++n) s[hh] = Ops::mma(as_v8<bf16x8>(ka), as_v8<bf16x8>(qw[n][2 * c + u]), s[hh]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < KS; ++c) {
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(row + 64 * c + 32 * half);
+            const u32x4 hi = *reinterpret_cast<const u32x4*>(row + 64 * c + 32 * half + 16);
+            i32x8 ka;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ka[e] = static_cast<int>(lo[e]), ka[4 + e] = static_cast<int>(hi[e]);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+              s[hh] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka, qb[n][c], s[hh], 0, 0, 0, ksc, 0, q_scale[n]);
+          }
+        }
+      }
+      // Element r of half hh is key key0 + 32 hh + 8 (r / 4) + 4 half + r % 4.
+      const int key0 = j * kBN;
+      float tmax = -INFINITY;
+      const bool masked = uniform(key0 + kBN - 1 > prefix + wave_row0 || wave_row0 + 31 >= nq);
+      if (masked) {
+        const int lim = limit - key0 - 4 * half;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[hh][r] = hh * 32 + (r / 4) * 8 + r % 4 > lim ? -INFINITY : s[hh][r] * a.qscale;
+      } else {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[hh][r] *= a.qscale;
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
+      const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias_lds[buf]);
+      tmax = max_across_halves(tmax) + fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+      if (__builtin_amdgcn_ballot_w64(tmax > m + kRescale) != 0) {
+        const float mn = fmaxf(m, tmax);
+        const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+        m = mn;
+        lsum *= corr;
+#pragma unroll
+        for (int c = 0; c < DT; ++c)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
+      }
+      const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[hh][r] = fast_exp2(s[hh][r] - mb);
+      const int4 n4 = *reinterpret_cast<const int4*>(nan_lds[buf]);
+      const bool nan_tile = masked && uniform(n4.x | n4.y | n4.z | n4.w) != 0;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        u32x4 pb[NP];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = s[ks / 2][(ks % 2) * 8 + 2 * e], y = s[ks / 2][(ks % 2) * 8 + 2 * e + 1];
+          if constexpr (NP > 1) lsum += x + y;
+#pragma unroll
+          for (int n = 0; n < NP; ++n) {
+            pb[n][e] = bf16_pair(x, y);
+            x -= bf16_lo(pb[n][e]), y -= bf16_hi(pb[n][e]);
+          }
+          if constexpr (NP == 1) lsum = Ops::sum2(pb[0][e], lsum);
+        }
+#pragma unroll
+        for (int c = 0; c < DT; ++c) {
+          const uint16_t* vlo = &v_lds[buf][tr_off + ks * 16 * VROW + c * 32];
+          const u32x2 lo = lds_read_tr(vlo), hi = lds_read_tr(vlo + 8 * VROW);
+          const u32x4 va = {lo[0], lo[1], hi[0], hi[1]};
+          if (!nan_tile) {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(va), as_v8<bf16x8>(pb[n]), acc[c]);
+          } else {
+            // A NaN in V that some row does not see: products without it, and a NaN where a
+            // row sees one (counted by a product of indicators).
+            u32x4 clean, is_nan, seen;
+            const int lim = limit - key0 - 4 * half - 16 * ks;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool n0 = (va[e] & 0x7fffu) > 0x7f80u, n1 = (va[e] & 0x7fff0000u) > 0x7f800000u;
+              clean[e] = (n0 ? 0u : va[e] & 0xffffu) | (n1 ? 0u : va[e] & 0xffff0000u);
+              is_nan[e] = (n0 ? 0x3f80u : 0u) | (n1 ? 0x3f800000u : 0u);
+              const int key = (e / 2) * 8 + (2 * e) % 4;
+              seen[e] = (key <= lim ? 0x3f80u : 0u) | (key + 1 <= lim ? 0x3f800000u : 0u);
+            }
+#pragma unroll
+            for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(clean), as_v8<bf16x8>(pb[n]), acc[c]);
+            const f32x16 count = Ops::mma(as_v8<bf16x8>(is_nan), as_v8<bf16x8>(seen), f32x16{});
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[c][r] = count[r] > 0.f ? __uint_as_float(0x7fc00000u) : acc[c][r];
+          }
+        }
+      }
+    }
+    if (j + 1 < ntiles) store_tile(buf ^ 1, tile_masked(j + 1));
+    __syncthreads();
+  }
+
+  if (!row_valid) return;
+  lsum += __shfl_xor(lsum, 32, 64);
+  // A row that sees no key is zeros.
+  const float inv = limit < 0 ? 0.f : 1.f / lsum;
+  T* orow = static_cast<T*>(a.out) + (row0 + my_row) * a.o_row + h * a.o_head;
+#pragma unroll
+  for (int c = 0; c < DT; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * c + 8 * g + 4 * half;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = limit < 0 ? 0.f : acc[c][4 * g + e] * inv;
+      if (p.out_vec) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(orow + d) = f32x4{x[0], x[1], x[2], x[3]};
+        else *reinterpret_cast<u32x2*>(orow + d) = u32x2{MfmaOps<T>::pack2(x[0], x[1]), MfmaOps<T>::pack2(x[2], x[3])};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) store_elem(orow + (d + e) * a.o_dim, x[e]);
+      }
+    }
+}
+
+}  // namespace
+
+bool prefill8_shape(int64_t d, int64_t page) { return (d == 64 || d == 128) && page >= 16 && (page & (page - 1)) == 0; }
+
+bool prefill8_layout(const Attn8Args& a) {
+  return prefill8_shape(a.d, a.page) && a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && a.kv_head % 16 == 0 &&
+         a.kv_token % 16 == 0 && a.kv_block % 16 == 0;
+}
+
+int launch_prefill8(const Attn8Args& a, int dtype, hipStream_t stream, const char* name) {
+  Prefill8Args p{};
+  p.a = a;
+  p.page_shift = __builtin_ctz(a.page);
+  const int es = dtype_size(dtype);
+  p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
+  p.out_vec = a.o_dim == 1 && aligned16(a.out) && a.o_row * es % 16 == 0 && a.o_head * es % 16 == 0;
+  const int64_t tiles = a.rows / kBM + std::min<int64_t>(a.num_seqs, a.rows);
+  if (tiles * a.hq > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  const dim3 grid(static_cast<unsigned>(tiles * a.hq)), block(256);
+#define LAUNCH(T)                                                                                        \
+  do {                                                                                                   \
+    if (a.d == 64) hipLaunchKernelGGL((prefill8_kernel<T, 64>), grid, block, 0, stream, p);              \
+    else hipLaunchKernelGGL((prefill8_kernel<T, 128>), grid, block, 0, stream, p);                       \
+  } while (0)
+  switch (dtype) {
+    case RLT_BFLOAT16: LAUNCH(bf16); break;
+    case RLT_FLOAT16: LAUNCH(f16); break;
+    default: LAUNCH(float); break;
+  }
+#undef LAUNCH
+  return check_launch(name);
+}
+
+}  // namespace rlt
