@@ -377,3 +377,28 @@ def test_refusals():
         prefill(longest=-1)
     assert decode(q=c.q[:0], tables=c.tables[:0], lens=c.lens[:0]).shape == (0, 4, 64)
     assert prefill(q=c.q[:0]).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_scale_bytes_of_every_size_and_a_negative_softmax_scale_in_prefill(dtype, d):
+    from vllm_rlt_amd import ops
+
+    # One key a sequence: its value comes back, whatever its K and softmax scales are.
+    kc = torch.full((4, 16, 1, d), 0x3C, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)  # 1.5
+    bytes_ = [0, 1, 60, 127, 130, 252] if dtype != torch.float16 else [113, 120, 127, 130, 140, 141]
+    q = queries(6, 2, d, dtype, 1).cuda()
+    lens, cu = torch.ones(6, dtype=torch.int32, device="cuda"), torch.arange(7, dtype=torch.int32, device="cuda")
+    tables = torch.arange(6, dtype=torch.int32, device="cuda")[:, None] % 4
+    for byte in bytes_:
+        ks = torch.full((4, 16, 1), 254 - byte if byte < 250 else 3, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+        vs = torch.full((4, 16, 1), byte, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+        out = ops.paged_prefill_fp8(q, kc, kc, ks, vs, tables, lens, cu, 1, scale=-2.0**-20)
+        want = torch.full(out.shape, 1.5 * 2.0 ** (byte - 127), dtype=torch.float64).to(dtype)
+        assert torch.equal(out.cpu(), want), byte
+    c = Case([150, 300], 4, 2, d, dtype=dtype, seed=8, chunks=[100, 290])
+    c.scale = -c.scale
+    c.check(c.prefill())
+    c.q = c.q[:2]
+    c.chunks = None
+    c.check(c.decode())

@@ -19,6 +19,8 @@
 // The running maximum moves only when a tile's exceeds it by 2^kRescale.
 #include "prefill_fp8.hpp"
 
+#include <cmath>
+
 #include "mfma.hpp"
 
 namespace rlt {
@@ -27,6 +29,7 @@ namespace {
 constexpr int kBM = 128;  // query rows a workgroup
 constexpr int kBN = 64;   // keys a tile
 constexpr float kRescale = 8.f;
+constexpr int kMaxQExp = 24;
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -38,6 +41,11 @@ template <> struct Parts<float> { static constexpr int Q = 3, P = 3; };
 struct Prefill8Args {
   Attn8Args a;
   int page_shift;
+  // |softmax scale| * log2(e) = qscale * 2^q_exp: the power of two goes into q, so that
+  // a score overflows only where the scaled one does.
+  float qscale;
+  int q_exp;
+  uint32_t q_sign;  // 0x80000000 negates q (a negative scale), else 0
   int out_vec;  // 4 elements of an out row can be stored at once
   int q_vec;    // q rows are 16-byte aligned, dims together
 };
@@ -75,6 +83,16 @@ __device__ __forceinline__ bool find_tile(const Attn8Args& a, int unit, int* seq
 }
 
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) { return MfmaOps<bf16>::pack2(x, y); }
+
+// Two codes of a word (its low or high half) times the scale of byte b, as bf16.
+// The instruction takes the scale as an fp32's exponent, with the byte's meaning: 0
+// is 2^-127, 255 NaN.
+__device__ __forceinline__ uint32_t scaled_bf16(uint32_t word, uint32_t b, bool high) {
+  const float s = __uint_as_float(b << 23);
+  const bf16x2 r = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(word), s, true)
+                        : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(word), s, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void prefill8_kernel(Prefill8Args p) {
@@ -144,9 +162,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         for (int i = 0; i < RUN; ++i) x[c][i] = load_elem(qrow + (d0 + i) * a.q_dim);
       }
 #pragma unroll
-      for (int i = 0; i < RUN; ++i) amax = fmaxf(amax, finite_abs(x[c][i]));
+      for (int i = 0; i < RUN; ++i) {
+        x[c][i] = __uint_as_float(__float_as_uint(x[c][i]) ^ p.q_sign);
+        amax = fmaxf(amax, finite_abs(x[c][i]));
+      }
     }
     if constexpr (WIDE) {
+      const float power = __uint_as_float(static_cast<uint32_t>(127 + p.q_exp) << 23);
+#pragma unroll
+      for (int c = 0; c < RUNS; ++c)
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) x[c][i] *= power;
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -161,7 +187,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
           }
     } else {
       amax = max_across_halves(amax);
-      const uint32_t b = max(scale_byte(amax), 4u * NQ);
+      const uint32_t b = max(scale_byte(amax), 4u * NQ + kMaxQExp);
       const float inv = inverse_scale(b);
 #pragma unroll
       for (int c = 0; c < KS; ++c)
@@ -170,7 +196,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
           x[c][i] = (__float_as_uint(x[c][i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : x[c][i] * inv;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        q_scale[n] = static_cast<int>(b) - 4 * n;
+        q_scale[n] = min(static_cast<int>(b) + p.q_exp, 254) - 4 * n;
 #pragma unroll
         for (int c = 0; c < KS; ++c)
 #pragma unroll
@@ -197,11 +223,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const uint8_t* vbase = a.v + kvh * a.kv_head + sc * 16;
   const uint8_t* ksbase = a.ks + kvh * a.s_head;
   const uint8_t* vsbase = a.vs + kvh * a.s_head;
-  const int page_mask = a.page - 1;
-  int32_t ids[PASSES], ks_id;
+  const uint32_t block_bytes = static_cast<uint32_t>(a.kv_block), token_bytes = static_cast<uint32_t>(a.kv_token);
+  const uint32_t s_block = static_cast<uint32_t>(a.s_block), s_token = static_cast<uint32_t>(a.s_token);
+  const uint32_t page_mask = a.page - 1, last_key = max(wg_keys, 1) - 1, num_blocks = static_cast<uint32_t>(a.num_blocks);
+  uint32_t ids[PASSES], ks_id;
   u32x4 kreg[PASSES], vreg[PASSES];
   uint32_t vsreg[PASSES], ksreg;
-  auto token = [&](int tile, int t) { return min(tile * kBN + t, wg_keys - 1); };
+  auto token = [&](int tile, int t) { return min(static_cast<uint32_t>(tile * kBN + t), last_key); };
+  auto offset = [](uint32_t id, uint32_t block, uint32_t slot, uint32_t token) {
+    return static_cast<uint64_t>(id) * block + slot * token;
+  };
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
@@ -210,44 +241,40 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   auto load_tile = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const int slot = token(tile, i * TPP + st) & page_mask;
-      const int64_t blk = block_of(a, ids[i]);
-      const int64_t at = blk * a.kv_block + slot * a.kv_token;
+      const uint32_t slot = token(tile, i * TPP + st) & page_mask, id = ids[i] < num_blocks ? ids[i] : 0;
+      const uint64_t at = offset(id, block_bytes, slot, token_bytes);
       kreg[i] = *reinterpret_cast<const u32x4*>(kbase + at);
       vreg[i] = *reinterpret_cast<const u32x4*>(vbase + at);
-      vsreg[i] = vsbase[blk * a.s_block + slot * a.s_token];
+      vsreg[i] = vsbase[offset(id, s_block, slot, s_token)];
     }
-    ksreg = ksbase[block_of(a, ks_id) * a.s_block + (token(tile, lane) & page_mask) * a.s_token];
+    if (wave == 0) ksreg = ksbase[offset(ks_id < num_blocks ? ks_id : 0, s_block, token(tile, lane) & page_mask, s_token)];
   };
   auto store_tile = [&](int buf, bool masked) __attribute__((always_inline)) {
-    float bias = 0.f;
+    uint32_t top = 0;  // largest V scale
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int t = i * TPP + st;
       *reinterpret_cast<u32x4*>(&k_lds[buf][t * KROW + sc * 16]) = kreg[i];
-      // The scale operand is the exponent of an fp32: byte 0 and 255 as in the e8m0 type.
-      const float sv = scale_value(vsreg[i]);
-      bias = fmaxf(bias, value_bias(vsreg[i] == 255u ? 0u : vsreg[i]));
-      u32x4 lo, hi;
+      u32x4 w[2];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const f32x2v x0 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(vreg[i][w]), false);
-        const f32x2v x1 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(vreg[i][w]), true);
-        const uint32_t u = bf16_pair(x0[0] * sv, x0[1] * sv), v = bf16_pair(x1[0] * sv, x1[1] * sv);
-        if (w < 2) lo[2 * w] = u, lo[2 * w + 1] = v;
-        else hi[2 * w - 4] = u, hi[2 * w - 3] = v;
-        if (masked) nan |= (((vreg[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0 || vsreg[i] == 255u;
-      }
+      for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = scaled_bf16(vreg[i][e / 2], vsreg[i], e % 2);
       uint16_t* dst = &v_lds[buf][t * VROW + sc * 16];
-      *reinterpret_cast<u32x4*>(dst) = lo;
-      *reinterpret_cast<u32x4*>(dst + 8) = hi;
+      *reinterpret_cast<u32x4*>(dst) = w[0];
+      *reinterpret_cast<u32x4*>(dst + 8) = w[1];
+      top = max(top, vsreg[i]);
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nan |= (((vreg[i][e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+        nan |= vsreg[i] == 255u;
+      }
     }
     if (wave == 0) ks_lds[buf][lane] = static_cast<uint8_t>(ksreg);
-    const float wave_bias = __builtin_amdgcn_ballot_w64(bias > 0.f) ? group_max<64>(bias) : 0.f;
-    const int wave_nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    float bias = 0.f;
+    if (__builtin_amdgcn_ballot_w64(top > 191u)) bias = group_max<64>(value_bias(top == 255u ? 0u : top));
+    const int wave_nan = masked && __builtin_amdgcn_ballot_w64(nan) != 0;
     if (lane == 0) {
-      bias_lds[buf][wave] = wave_bias;
+      bias_lds[buf][wave] = bias;
       nan_lds[buf][wave] = wave_nan;
     }
   };
@@ -279,64 +306,59 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     }
     if (wave_live && j * kBN <= wave_last) {
       f32x16 s[2] = {{}, {}};
+      if constexpr (WIDE) {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int ksc = ks_lds[buf][hh * 32 + col];
-        const uint8_t* row = &k_lds[buf][(hh * 32 + col) * KROW];
-        if constexpr (WIDE) {
-          const float kscale = scale_value(static_cast<uint32_t>(ksc));
+        for (int hh = 0; hh < 2; ++hh) {
+          const uint32_t ksc = ks_lds[buf][hh * 32 + col];
 #pragma unroll
           for (int c = 0; c < DT; ++c) {
-            const u32x4 codes = *reinterpret_cast<const u32x4*>(row + 32 * c + 16 * half);
+            const u32x4 codes = *reinterpret_cast<const u32x4*>(&k_lds[buf][(hh * 32 + col) * KROW + 32 * c + 16 * half]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               u32x4 ka;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int w = static_cast<int>(codes[2 * u + e / 2]);
-                const f32x2v y = e % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
-                ka[e] = bf16_pair(y[0] * kscale, y[1] * kscale);
-              }
+              for (int e = 0; e < 4; ++e) ka[e] = scaled_bf16(codes[2 * u + e / 2], ksc, e % 2);
 #pragma unroll
               for (int n = 0; n < NQ; ++n) s[hh] = Ops::mma(as_v8<bf16x8>(ka), as_v8<bf16x8>(qw[n][2 * c + u]), s[hh]);
             }
           }
-        } else {
+        }
+      } else {
+        const int ksc[2] = {ks_lds[buf][col], ks_lds[buf][32 + col]};
 #pragma unroll
-          for (int c = 0; c < KS; ++c) {
-            const u32x4 lo = *reinterpret_cast<const u32x4*>(row + 64 * c + 32 * half);
-            const u32x4 hi = *reinterpret_cast<const u32x4*>(row + 64 * c + 32 * half + 16);
-            i32x8 ka;
+        for (int c = 0; c < KS; ++c) {
+          i32x8 ka[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) ka[e] = static_cast<int>(lo[e]), ka[4 + e] = static_cast<int>(hi[e]);
+          for (int hh = 0; hh < 2; ++hh) {
+            const uint8_t* row = &k_lds[buf][(hh * 32 + col) * KROW + 64 * c + 32 * half];
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(row), hi = *reinterpret_cast<const u32x4*>(row + 16);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
-              s[hh] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka, qb[n][c], s[hh], 0, 0, 0, ksc, 0, q_scale[n]);
+            for (int e = 0; e < 4; ++e) ka[hh][e] = static_cast<int>(lo[e]), ka[hh][4 + e] = static_cast<int>(hi[e]);
           }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+              s[hh] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[hh], qb[n][c], s[hh], 0, 0, 0, ksc[hh], 0, q_scale[n]);
         }
       }
       // Element r of half hh is key key0 + 32 hh + 8 (r / 4) + 4 half + r % 4.
       const int key0 = j * kBN;
-      float tmax = -INFINITY;
       const bool masked = uniform(key0 + kBN - 1 > prefix + wave_row0 || wave_row0 + 31 >= nq);
       if (masked) {
         const int lim = limit - key0 - 4 * half;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[hh][r] = hh * 32 + (r / 4) * 8 + r % 4 > lim ? -INFINITY : s[hh][r] * a.qscale;
-      } else {
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[hh][r] *= a.qscale;
+          for (int r = 0; r < 16; ++r) s[hh][r] = hh * 32 + (r / 4) * 8 + r % 4 > lim ? -INFINITY : s[hh][r];
       }
+      float tmax = -INFINITY;
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
         for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
       const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias_lds[buf]);
-      tmax = max_across_halves(tmax) + fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+      tmax = max_across_halves(tmax) * p.qscale + fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
       if (__builtin_amdgcn_ballot_w64(tmax > m + kRescale) != 0) {
         const float mn = fmaxf(m, tmax);
         const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
@@ -348,18 +370,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
           for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
       }
       const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
+      // exp2(s * qscale - m) in one rounding, unless m's own is no longer small.
+      float qs = p.qscale;
+      if (__builtin_amdgcn_ballot_w64(fabsf(mb) > 4096.f) != 0) {
+        qs = 1.f;
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
+        for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[hh][r] = fast_exp2(s[hh][r] - mb);
-      const int4 n4 = *reinterpret_cast<const int4*>(nan_lds[buf]);
-      const bool nan_tile = masked && uniform(n4.x | n4.y | n4.z | n4.w) != 0;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        u32x4 pb[NP];
+          for (int r = 0; r < 16; ++r) s[hh][r] *= p.qscale;
+      }
+      // P of k-step ks, in parts; its sum is taken over what the products see.
+      auto weights = [&](int ks, u32x4 (&pb)[NP]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = s[ks / 2][(ks % 2) * 8 + 2 * e], y = s[ks / 2][(ks % 2) * 8 + 2 * e + 1];
+          const int r = (ks % 2) * 8 + 2 * e;
+          float x = fast_exp2(fmaf(s[ks / 2][r], qs, -mb)), y = fast_exp2(fmaf(s[ks / 2][r + 1], qs, -mb));
           if constexpr (NP > 1) lsum += x + y;
 #pragma unroll
           for (int n = 0; n < NP; ++n) {
@@ -368,32 +393,53 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
           }
           if constexpr (NP == 1) lsum = Ops::sum2(pb[0][e], lsum);
         }
+      };
+      auto values = [&](int ks, int c) __attribute__((always_inline)) {
+        const uint16_t* vlo = &v_lds[buf][tr_off + ks * 16 * VROW + c * 32];
+        const u32x2 lo = lds_read_tr(vlo), hi = lds_read_tr(vlo + 8 * VROW);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      };
+      const int4 n4 = *reinterpret_cast<const int4*>(nan_lds[buf]);
+      if (masked && uniform(n4.x | n4.y | n4.z | n4.w) != 0) {
+        // A NaN in V that some row may not see: products without it, and a NaN where a row
+        // sees one (counted by a product of indicators).
 #pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          const uint16_t* vlo = &v_lds[buf][tr_off + ks * 16 * VROW + c * 32];
-          const u32x2 lo = lds_read_tr(vlo), hi = lds_read_tr(vlo + 8 * VROW);
-          const u32x4 va = {lo[0], lo[1], hi[0], hi[1]};
-          if (!nan_tile) {
+        for (int ks = 0; ks < 4; ++ks) {
+          u32x4 pb[NP], seen;
+          weights(ks, pb);
+          const int lim = limit - key0 - 4 * half - 16 * ks;
 #pragma unroll
-            for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(va), as_v8<bf16x8>(pb[n]), acc[c]);
-          } else {
-            // A NaN in V that some row does not see: products without it, and a NaN where a
-            // row sees one (counted by a product of indicators).
-            u32x4 clean, is_nan, seen;
-            const int lim = limit - key0 - 4 * half - 16 * ks;
+          for (int e = 0; e < 4; ++e) {
+            const int key = (e / 2) * 8 + (2 * e) % 4;
+            seen[e] = (key <= lim ? 0x3f80u : 0u) | (key + 1 <= lim ? 0x3f800000u : 0u);
+          }
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            const u32x4 va = values(ks, c);
+            u32x4 clean, is_nan;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const bool n0 = (va[e] & 0x7fffu) > 0x7f80u, n1 = (va[e] & 0x7fff0000u) > 0x7f800000u;
               clean[e] = (n0 ? 0u : va[e] & 0xffffu) | (n1 ? 0u : va[e] & 0xffff0000u);
               is_nan[e] = (n0 ? 0x3f80u : 0u) | (n1 ? 0x3f800000u : 0u);
-              const int key = (e / 2) * 8 + (2 * e) % 4;
-              seen[e] = (key <= lim ? 0x3f80u : 0u) | (key + 1 <= lim ? 0x3f800000u : 0u);
             }
 #pragma unroll
             for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(clean), as_v8<bf16x8>(pb[n]), acc[c]);
             const f32x16 count = Ops::mma(as_v8<bf16x8>(is_nan), as_v8<bf16x8>(seen), f32x16{});
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[c][r] = count[r] > 0.f ? __uint_as_float(0x7fc00000u) : acc[c][r];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          u32x4 pb[NP];
+          weights(ks, pb);
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            const u32x4 va = values(ks, c);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(va), as_v8<bf16x8>(pb[n]), acc[c]);
           }
         }
       }
@@ -430,14 +476,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 bool prefill8_shape(int64_t d, int64_t page) { return (d == 64 || d == 128) && page >= 16 && (page & (page - 1)) == 0; }
 
 bool prefill8_layout(const Attn8Args& a) {
+  auto small = [](int64_t x) { return x >= 0 && x < (int64_t(1) << 32); };
   return prefill8_shape(a.d, a.page) && a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && a.kv_head % 16 == 0 &&
-         a.kv_token % 16 == 0 && a.kv_block % 16 == 0;
+         a.kv_token % 16 == 0 && a.kv_block % 16 == 0 && small(a.kv_block) && small(a.kv_token * a.page) &&
+         small(a.s_block) && small(a.s_token * a.page);
 }
 
 int launch_prefill8(const Attn8Args& a, int dtype, hipStream_t stream, const char* name) {
   Prefill8Args p{};
   p.a = a;
   p.page_shift = __builtin_ctz(a.page);
+  p.qscale = std::fabs(a.qscale);
+  p.q_exp = std::isnormal(p.qscale) ? std::min(std::max(std::ilogb(p.qscale), -kMaxQExp), kMaxQExp) : 0;
+  p.qscale = std::ldexp(p.qscale, -p.q_exp);
+  p.q_sign = a.qscale < 0.f ? 0x80000000u : 0u;
   const int es = dtype_size(dtype);
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
   p.out_vec = a.o_dim == 1 && aligned16(a.out) && a.o_row * es % 16 == 0 && a.o_head * es % 16 == 0;
