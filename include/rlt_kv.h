@@ -560,7 +560,11 @@ int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, const void* ke
  * rlt_paged_prefill over a layer slice of an 8-bit cache: packed chunks, bottom-
  * right causal.  Query row i of sequence s's n_q sees keys 0 .. context_lengths[s]
  * - n_q + i; one that sees none is written as zeros.  Rows of no sequence (at or
- * past cu_seqlens_q[num_seqs]) are left as they were.
+ * past cu_seqlens_q[num_seqs]) are left as they were.  The workspace
+ * (rlt_paged_prefill_fp8_workspace_bytes, on 16 bytes; calls that overlap need one
+ * each) holds the partials of long sequences, whose keys are cut by the launch's
+ * shapes: a row's last bits may depend on what shares its launch.  With a NULL
+ * workspace none is cut, and they depend on its own sequence only.
  */
 int64_t rlt_paged_prefill_fp8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
                                               int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,

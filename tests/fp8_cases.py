@@ -102,7 +102,9 @@ def attention(q, cache, table, limits, scale, p_unit):
     v_seen = torch.nan_to_num(v, nan=0.0)
     out, spread = p @ v_seen, p @ v_seen.abs()
     unit = torch.finfo(q.dtype).eps / 2
-    bound = unit * out.abs() + (2 * (d + 8) * 2.0**-24 * size + 2.0**-20 + p_unit) * spread
+    # Below the smallest normal number the type's step no longer shrinks: half of it is
+    # smallest_normal * eps / 2 (fp16 2^-25), whatever the value.
+    bound = unit * out.abs().clamp(min=torch.finfo(q.dtype).smallest_normal) + (2 * (d + 8) * 2.0**-24 * size + 2.0**-20 + p_unit) * spread
     return out.transpose(0, 1), bound.transpose(0, 1) + 1e-30
 
 

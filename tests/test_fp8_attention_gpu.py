@@ -402,3 +402,29 @@ def test_scale_bytes_of_every_size_and_a_negative_softmax_scale_in_prefill(dtype
     c.q = c.q[:2]
     c.chunks = None
     c.check(c.decode())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prefixes,chunks", [([3000, 5, 0], [70, 140, 260]), ([0], [2100]), ([8191, 511, 512, 513], [1, 1, 129, 128]), ([30, 2000], [400, 0])])
+def test_prefill_of_cut_keys_and_the_batch_invariant_form(dtype, prefixes, chunks):
+    lengths = [p + n for p, n in zip(prefixes, chunks)]
+    c = Case(lengths, 8, 8, 128, dtype=dtype, seed=len(chunks), chunks=chunks)
+    c.check(c.prefill())
+    whole = c.prefill(batch_invariant=True)
+    c.check(whole)
+    at = 0
+    for s, n in enumerate(chunks):  # a sequence alone gives the batch's bits
+        if n:
+            from vllm_rlt_amd import ops
+
+            alone = ops.paged_prefill_fp8(c.q[at : at + n], *c.cache, c.tables[s : s + 1], c.lens[s : s + 1],
+                                          torch.tensor([0, n], dtype=torch.int32, device="cuda"), n, scale=c.scale, batch_invariant=True)
+            assert torch.equal(alone, whole[at : at + n])
+        at += n
+
+
+def test_prefill_of_a_row_before_the_keys_of_cut_sequences():
+    # Chunks longer than their context: the first query tiles see no key of the first segment either.
+    c = Case([1500, 40], 8, 8, 128, seed=2, chunks=[2000, 300])
+    c.check(c.prefill())
+    assert (c.prefill()[:500] == 0).all()

@@ -195,7 +195,10 @@ extern "C" int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, con
 extern "C" int64_t rlt_paged_prefill_fp8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
                                                          int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
                                                          int64_t page_size) {
-  return 0;
+  if (total_q <= 0 || num_seqs <= 0 || max_table_width <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      !prefill8_shape(head_dim, page_size) || max_table_width > 0x7fffffff / page_size)
+    return 0;
+  return prefill8_workspace(total_q, num_seqs, max_table_width * page_size, num_q_heads, head_dim);
 }
 
 extern "C" int rlt_paged_prefill_fp8(const void* q, const int64_t* q_strides, const void* key_cache,
@@ -217,6 +220,10 @@ extern "C" int rlt_paged_prefill_fp8(const void* q, const int64_t* q_strides, co
   if (total_q == 0 || num_seqs == 0) return RLT_OK;
   if (!cu_seqlens_q) return fail(RLT_EINVAL, "rlt_paged_prefill_fp8: NULL pointer argument");
   a.cu = cu_seqlens_q;
-  if (prefill8_layout(a)) return launch_prefill8(a, dtype, as_stream(stream), "rlt_paged_prefill_fp8");
+  const int64_t need = rlt_paged_prefill_fp8_workspace_bytes(total_q, num_seqs, max_table_width, num_q_heads, num_kv_heads,
+                                                             head_dim, page_size);
+  if (workspace && need > 0 && (workspace_bytes < need || !aligned16(workspace)))
+    return fail(RLT_EWORKSPACE, "rlt_paged_prefill_fp8: workspace must be %lld bytes on 16", (long long)need);
+  if (prefill8_layout(a)) return launch_prefill8(a, dtype, workspace, as_stream(stream), "rlt_paged_prefill_fp8");
   return launch_attn8_generic(a, dtype, as_stream(stream), "rlt_paged_prefill_fp8");
 }

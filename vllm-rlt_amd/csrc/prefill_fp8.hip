@@ -17,6 +17,13 @@
 //   (its sum is taken over the rounded values) for bf16 outputs, and split in two or three
 //   bf16 parts for fp16 and fp32 ones.
 // The running maximum moves only when a tile's exceeds it by 2^kRescale.
+//
+// Key segments.  Items of one launch differ by two orders of magnitude (a new prompt's
+// 128 rows beside a chunk at the end of 16000 keys), and a launch of few rows has too
+// few of them.  So the keys of long sequences are cut into segments of about the
+// launch's work over kTargetItems, and a merge kernel joins them; the items go out
+// longest first, the heads of a sequence over the XCDs so that its query tiles share an
+// L2.  Every wave works the plan out for itself from the lengths.
 #include "prefill_fp8.hpp"
 
 #include <cmath>
@@ -30,6 +37,16 @@ constexpr int kBM = 128;  // query rows a workgroup
 constexpr int kBN = 64;   // keys a tile
 constexpr float kRescale = 8.f;
 constexpr int kMaxQExp = 24;
+constexpr int kXcds = 8;
+#ifndef TARGET
+#define TARGET 1024
+#endif
+#ifndef MINSEG
+#define MINSEG 8
+#endif
+constexpr int kTargetItems = TARGET;  // two workgroups a CU, two rounds of them
+constexpr int kMinSegTiles = MINSEG;
+constexpr int kPlanSeqs = 64;      // sequences ranked and cut: one a lane
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -46,6 +63,9 @@ struct Prefill8Args {
   float qscale;
   int q_exp;
   uint32_t q_sign;  // 0x80000000 negates q (a negative scale), else 0
+  // Key segments: partials of cut sequences, row slots x heads (null: none is cut).
+  float* part_acc;    // [slots][hq][D]
+  float2* part_ml;    // [slots][hq], max in log2 units and sum
   int out_vec;  // 4 elements of an out row can be stored at once
   int q_vec;    // q rows are 16-byte aligned, dims together
 };
@@ -57,27 +77,105 @@ __device__ __forceinline__ void seq_rows(const Attn8Args& a, int s, int& row0, i
   nq = min(max(a.cu[s + 1], row0), rows) - row0;
 }
 
-// Query tile `unit` of the packed batch: its sequence, found by the wave 64 at a time.
-__device__ __forceinline__ bool find_tile(const Attn8Args& a, int unit, int* seq, int* tile) {
+__device__ __forceinline__ int wave_prefix(int x, int lane) {  // sum of the lanes before
+  int upto = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += y;
+  }
+  return upto - x;
+}
+
+// One sequence a lane: its rows, keys and cut.
+struct SeqPlan {
+  int row0, nq, len;
+  int tiles;      // query tiles
+  int segs;       // key segments
+  int seg_tiles;  // key tiles of a segment
+  int slot0;      // first partial row of a cut sequence: row i of segment g is slot0 + g * nq + i
+};
+__device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
+  SeqPlan s{};
+  if (lane < p.a.num_seqs) {
+    seq_rows(p.a, lane, s.row0, s.nq);
+    s.len = sequence_length(p.a, lane);
+  }
+  s.tiles = (s.nq + kBM - 1) / kBM;
+  const int keys = (s.len + kBN - 1) / kBN;
+  s.segs = 1;
+  s.seg_tiles = keys;
+  if (p.part_acc) {
+    // Work in (query tile, key tile) pairs of all heads; 64-bit for one long sequence of many rows.
+    int64_t work = static_cast<int64_t>(s.tiles) * keys;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
+    const int target = max(kMinSegTiles, static_cast<int>(min<int64_t>((work * p.a.hq + kTargetItems - 1) / kTargetItems, 1 << 30)));
+    s.segs = max(1, (keys + target - 1) / target);
+    s.seg_tiles = (keys + s.segs - 1) / s.segs;
+    s.slot0 = wave_prefix(s.segs > 1 ? s.nq * s.segs : 0, lane);
+  }
+  return s;
+}
+
+struct Item {
+  int seq, head, tile, seg;
+  int row0, nq, len, segs, seg_tiles, slot0;
+};
+
+// Work item blockIdx.x, worked out by every wave alike; false past the last.
+__device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
+  const Attn8Args& a = p.a;
   const int lane = threadIdx.x & 63;
+  // Workgroup b runs on XCD b % 8, which serves the heads h == b (mod 8).
+  const int groups = a.hq % kXcds == 0 ? kXcds : 1, heads = a.hq / groups;
+  const int x = blockIdx.x % groups;
+  int pos = blockIdx.x / groups;
+  int unit;
+  if (a.num_seqs <= kPlanSeqs) {
+    const SeqPlan s = plan_of(p, lane);
+    const int units = s.tiles * s.segs, cost = s.seg_tiles;
+    int before = 0;  // units of sequences with longer items (equal ones in order)
+    for (int q = 0; q < a.num_seqs; ++q) {
+      const int c = __builtin_amdgcn_readlane(cost, q), u = __builtin_amdgcn_readlane(units, q);
+      before += c > cost || (c == cost && q < lane) ? u : 0;
+    }
+    const int64_t first = static_cast<int64_t>(before) * heads, end = first + static_cast<int64_t>(units) * heads;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < a.num_seqs && pos >= first && pos < end);
+    if (!hit) return false;
+    const int at = __builtin_ctzll(hit);
+    it->seq = at;
+    pos -= __builtin_amdgcn_readlane(before, at) * heads;
+    it->row0 = __builtin_amdgcn_readlane(s.row0, at), it->nq = __builtin_amdgcn_readlane(s.nq, at);
+    it->len = __builtin_amdgcn_readlane(s.len, at), it->segs = __builtin_amdgcn_readlane(s.segs, at);
+    it->seg_tiles = __builtin_amdgcn_readlane(s.seg_tiles, at), it->slot0 = __builtin_amdgcn_readlane(s.slot0, at);
+    const int tiles = __builtin_amdgcn_readlane(s.tiles, at), of_head = tiles * it->segs;
+    it->head = x + groups * (pos / of_head);
+    unit = pos % of_head;
+    it->seg = unit / tiles;
+    unit -= it->seg * tiles;
+    it->tile = tiles - 1 - unit;  // the last rows, which see most keys, first
+    return true;
+  }
+  // More sequences: in order and uncut, found 64 at a time.
+  it->head = x + groups * (pos % heads);
+  unit = pos / heads;
   for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
     int row0 = 0, nq = 0;
     if (s0 + lane < a.num_seqs) seq_rows(a, s0 + lane, row0, nq);
-    const int tiles = (nq + kBM - 1) / kBM;
-    int upto = tiles;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += y;
-    }
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(unit >= upto - tiles && unit < upto);
+    const int tiles = (nq + kBM - 1) / kBM, before = wave_prefix(tiles, lane);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(unit >= before && unit < before + tiles);
     if (hit) {
       const int at = __builtin_ctzll(hit);
-      *seq = s0 + at;
-      *tile = unit - __builtin_amdgcn_readlane(upto - tiles, at);
+      it->seq = s0 + at;
+      it->row0 = __builtin_amdgcn_readlane(row0, at), it->nq = __builtin_amdgcn_readlane(nq, at);
+      it->len = uniform(sequence_length(a, it->seq));
+      it->segs = 1, it->seg = 0, it->slot0 = 0;
+      it->seg_tiles = (it->len + kBN - 1) / kBN;
+      it->tile = __builtin_amdgcn_readlane(tiles, at) - 1 - (unit - __builtin_amdgcn_readlane(before, at));
       return true;
     }
-    unit -= __builtin_amdgcn_readlane(upto, 63);
+    unit -= __builtin_amdgcn_readlane(before + tiles, 63);
   }
   return false;
 }
@@ -115,20 +213,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 
   const Attn8Args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  int seq, qt;
-  const int h = blockIdx.x % a.hq;
-  if (!find_tile(a, blockIdx.x / a.hq, &seq, &qt)) return;
-  seq = uniform(seq);
-  int row0, nq;
-  seq_rows(a, seq, row0, nq);
-  row0 = uniform(row0), nq = uniform(nq);
-  qt = uniform((nq + kBM - 1) / kBM - 1 - qt);  // the last rows, which see most keys, first
-  const int len = uniform(sequence_length(a, seq));
+  Item it;
+  if (!find_item(p, &it)) return;
+  const int seq = uniform(it.seq), h = uniform(it.head), row0 = uniform(it.row0), nq = uniform(it.nq);
+  const int len = uniform(it.len);
   const int prefix = len - nq;  // query row i sees keys up to prefix + i
-  const int qt0 = qt * kBM;
+  const int qt0 = uniform(it.tile) * kBM;
   const int kvh = h / (a.hq / a.hkv);
-  const int wg_keys = min(prefix + min(qt0 + kBM, nq), len);
-  const int ntiles = (max(wg_keys, 0) + kBN - 1) / kBN;
+  const int wg_keys = min(prefix + min(qt0 + kBM, nq), len);  // keys that some row of the workgroup sees
+  const int first_tile = uniform(it.seg * it.seg_tiles);
+  const int ntiles = min(first_tile + uniform(it.seg_tiles), (max(wg_keys, 0) + kBN - 1) / kBN);
+  if (it.segs > 1 && it.seg > 0 && ntiles <= first_tile) return;  // the merge skips such a segment
 
   const int half = lane >> 5, col = lane & 31;
   const int wave_row0 = qt0 + wave * 32;
@@ -291,14 +386,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const int grp = lane >> 4, gl = lane & 15;
   const int tr_off = (4 * (grp >> 1) + (gl >> 2)) * VROW + 16 * (grp & 1) + 4 * (gl & 3);
 
-  if (ntiles > 0) {
-    load_ids(0);
-    load_tile(0);
-    load_ids(1);
-    store_tile(0, tile_masked(0));
+  if (ntiles > first_tile) {
+    load_ids(first_tile);
+    load_tile(first_tile);
+    load_ids(first_tile + 1);
+    store_tile(first_tile & 1, tile_masked(first_tile));
   }
   __syncthreads();
-  for (int j = 0; j < ntiles; ++j) {
+  for (int j = first_tile; j < ntiles; ++j) {
     const int buf = j & 1;
     if (j + 1 < ntiles) {
       load_tile(j + 1);
@@ -448,8 +543,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     __syncthreads();
   }
 
-  if (!row_valid) return;
   lsum += __shfl_xor(lsum, 32, 64);
+  if (!row_valid) return;
+  if (uniform(it.segs) > 1) {
+    const int64_t slot = (static_cast<int64_t>(it.slot0) + static_cast<int64_t>(it.seg) * nq + my_row) * a.hq + h;
+    float* dst = p.part_acc + slot * D + 4 * half;
+#pragma unroll
+    for (int c = 0; c < DT; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(dst + 32 * c + 8 * g) = f32x4{acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
+    if (half == 0) p.part_ml[slot] = make_float2(m, lsum);
+    return;
+  }
   // A row that sees no key is zeros.
   const float inv = limit < 0 ? 0.f : 1.f / lsum;
   T* orow = static_cast<T*>(a.out) + (row0 + my_row) * a.o_row + h * a.o_head;
@@ -471,6 +577,57 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     }
 }
 
+// Joins the segments of cut sequences, in order: a wave kMergeRows rows of one head.
+constexpr int kMergeRows = 4;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefill8_merge_kernel(Prefill8Args p) {
+  const Attn8Args& a = p.a;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int h = blockIdx.x % a.hq;
+  const int first = (blockIdx.x / a.hq * 4 + wave) * kMergeRows;
+  const SeqPlan s = plan_of(p, lane);
+  for (int row = first; row < min(first + kMergeRows, static_cast<int>(a.rows)); ++row) {
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(row >= s.row0 && row < s.row0 + s.nq);
+    if (!hit) continue;
+    const int at = __builtin_ctzll(hit);
+    const int segs = __builtin_amdgcn_readlane(s.segs, at);
+    if (segs < 2) continue;
+    const int nq = __builtin_amdgcn_readlane(s.nq, at), len = __builtin_amdgcn_readlane(s.len, at);
+    const int i = row - __builtin_amdgcn_readlane(s.row0, at);
+    // Segments past the last key of the row's query tile were not computed.
+    const int keys = max(len - nq + min(i / kBM * kBM + kBM, nq), 0);
+    const int seg_keys = __builtin_amdgcn_readlane(s.seg_tiles, at) * kBN;
+    const int live = min(segs, max(1, (keys + seg_keys - 1) / seg_keys));
+    const int64_t step = static_cast<int64_t>(nq) * a.hq;  // slots from one segment to the next
+    const int64_t base = (static_cast<int64_t>(__builtin_amdgcn_readlane(s.slot0, at)) + i) * a.hq + h;
+    float top = -INFINITY;
+    for (int g = 0; g < live; ++g) top = fmaxf(top, p.part_ml[base + g * step].x);
+    const float off = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc[D / 64] = {};
+    for (int g = 0; g < live; ++g) {
+      const float2 ml = p.part_ml[base + g * step];
+      const float w = fast_exp2(ml.x - off);
+      sum = fmaf(ml.y, w, sum);
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(p.part_acc[(base + g * step) * D + lane + 64 * e], w, acc[e]);
+    }
+    const bool blind = len - nq + i < 0;  // a row that sees no key
+    const float inv = 1.f / sum;
+    T* orow = static_cast<T*>(a.out) + row * a.o_row + h * a.o_head;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) store_elem(orow + (lane + 64 * e) * a.o_dim, blind ? 0.f : acc[e] * inv);
+  }
+}
+
+// Partial rows that a launch can need: a sequence's rows once a segment.  Segments
+// are at least (all work) / kTargetItems, so those past each sequence's first cover at
+// most 128 kTargetItems / hq rows; and no sequence has more than its table's keys.
+int64_t partial_slots(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq) {
+  const int64_t most = ((max_len + kBN - 1) / kBN + kMinSegTiles - 1) / kMinSegTiles;
+  if (num_seqs > kPlanSeqs || most < 2) return 0;
+  return std::min(rows * most, rows + (kBM * kTargetItems + hq - 1) / hq);
+}
+
 }  // namespace
 
 bool prefill8_shape(int64_t d, int64_t page) { return (d == 64 || d == 128) && page >= 16 && (page & (page - 1)) == 0; }
@@ -482,9 +639,19 @@ bool prefill8_layout(const Attn8Args& a) {
          small(a.s_block) && small(a.s_token * a.page);
 }
 
-int launch_prefill8(const Attn8Args& a, int dtype, hipStream_t stream, const char* name) {
+int64_t prefill8_workspace(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq, int64_t d) {
+  return partial_slots(rows, num_seqs, max_len, hq) * hq * (d * 4 + 8);
+}
+
+int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, const char* name) {
   Prefill8Args p{};
   p.a = a;
+  const int64_t slots = ws ? partial_slots(a.rows, a.num_seqs, a.max_len, a.hq) : 0;
+  if (slots > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  if (slots) {
+    p.part_acc = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(p.part_acc + slots * a.hq * a.d);
+  }
   p.page_shift = __builtin_ctz(a.page);
   p.qscale = std::fabs(a.qscale);
   p.q_exp = std::isnormal(p.qscale) ? std::min(std::max(std::ilogb(p.qscale), -kMaxQExp), kMaxQExp) : 0;
@@ -493,13 +660,20 @@ int launch_prefill8(const Attn8Args& a, int dtype, hipStream_t stream, const cha
   const int es = dtype_size(dtype);
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
   p.out_vec = a.o_dim == 1 && aligned16(a.out) && a.o_row * es % 16 == 0 && a.o_head * es % 16 == 0;
-  const int64_t tiles = a.rows / kBM + std::min<int64_t>(a.num_seqs, a.rows);
-  if (tiles * a.hq > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
-  const dim3 grid(static_cast<unsigned>(tiles * a.hq)), block(256);
-#define LAUNCH(T)                                                                                        \
+  // Query tiles, and the segments past the first (as many items as partial_slots() has such rows).
+  const int64_t tiles = a.rows / kBM + std::min<int64_t>(a.num_seqs, a.rows) + (slots ? (kTargetItems + a.hq - 1) / a.hq : 0);
+  const int64_t merge_rows = (a.rows + 4 * kMergeRows - 1) / (4 * kMergeRows);
+  if (tiles * a.hq > 0x7fffffff || merge_rows * a.hq > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  const dim3 grid(static_cast<unsigned>(tiles * a.hq)), merge(static_cast<unsigned>(merge_rows * a.hq)), block(256);
+#define LAUNCH_D(T, D)                                                                                   \
   do {                                                                                                   \
-    if (a.d == 64) hipLaunchKernelGGL((prefill8_kernel<T, 64>), grid, block, 0, stream, p);              \
-    else hipLaunchKernelGGL((prefill8_kernel<T, 128>), grid, block, 0, stream, p);                       \
+    hipLaunchKernelGGL((prefill8_kernel<T, D>), grid, block, 0, stream, p);                              \
+    if (slots) hipLaunchKernelGGL((prefill8_merge_kernel<T, D>), merge, block, 0, stream, p);            \
+  } while (0)
+#define LAUNCH(T)                       \
+  do {                                  \
+    if (a.d == 64) LAUNCH_D(T, 64);     \
+    else LAUNCH_D(T, 128);              \
   } while (0)
   switch (dtype) {
     case RLT_BFLOAT16: LAUNCH(bf16); break;
@@ -507,6 +681,7 @@ int launch_prefill8(const Attn8Args& a, int dtype, hipStream_t stream, const cha
     default: LAUNCH(float); break;
   }
 #undef LAUNCH
+#undef LAUNCH_D
   return check_launch(name);
 }
 

@@ -1287,6 +1287,7 @@ def paged_prefill_fp8(
     out: torch.Tensor | None = None,
     scale: float | None = None,
     workspace: torch.Tensor | None = None,
+    batch_invariant: bool = False,
 ) -> torch.Tensor:
     """paged_prefill over layer slices of an 8-bit cache: packed chunks, bottom-right causal (rlt_paged_prefill_fp8).
 
@@ -1294,6 +1295,10 @@ def paged_prefill_fp8(
     i of a sequence's n sees its keys up to context_length - n + i; one that sees
     none is zeros.  Rows of no sequence (from cu_seqlens_q[-1] on) are left as they
     are in `out`.  max_seqlen_q is at least the longest chunk.
+
+    `workspace` (prefill_fp8_workspace_bytes) holds the partials of sequences whose keys
+    are cut, by the launch's shapes, and is allocated here unless given.  With
+    `batch_invariant` none is cut: a row's bits depend on its own sequence only.
     """
     device, out = _fp8_attention_inputs(
         q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
@@ -1307,7 +1312,8 @@ def paged_prefill_fp8(
         raise ValueError("context_lengths and cu_seqlens_q must describe one entry per sequence")
     if total == 0 or nseq == 0:
         return out
-    workspace = _workspace_of(prefill_fp8_workspace_bytes(total, nseq, width, hq, hkv, d, page), workspace, device)
+    need = 0 if batch_invariant else prefill_fp8_workspace_bytes(total, nseq, width, hq, hkv, d, page)
+    workspace = _workspace_of(need, workspace, device)
     with _current(device):
         rc = _native.load().rlt_paged_prefill_fp8(
             q.data_ptr(), int64_array(q.stride()), key_cache.data_ptr(), value_cache.data_ptr(),
@@ -1315,8 +1321,8 @@ def paged_prefill_fp8(
             int64_array(key_scales.stride()), block_tables.data_ptr(), block_tables.stride(0), width,
             context_lengths.data_ptr(), cu_seqlens_q.data_ptr(), nseq, total, max_seqlen_q, out.data_ptr(),
             int64_array(out.stride()), hq, hkv, d, page, nb, 1.0 / math.sqrt(d) if scale is None else scale,
-            dtype_code(q.dtype), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-            stream_handle(device),
+            dtype_code(q.dtype), workspace.data_ptr() if need else None,
+            workspace.numel() * workspace.element_size(), stream_handle(device),
         )
     check(rc, "rlt_paged_prefill_fp8")
     return out
