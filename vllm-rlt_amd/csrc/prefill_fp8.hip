@@ -27,6 +27,7 @@
 #include "prefill_fp8.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 #include "mfma.hpp"
 
@@ -39,12 +40,13 @@ constexpr float kRescale = 8.f;
 constexpr int kMaxQExp = 24;
 constexpr int kXcds = 8;
 #ifndef TARGET
-#define TARGET 1024
+#define TARGET 768
 #endif
 #ifndef MINSEG
-#define MINSEG 8
+#define MINSEG 4
 #endif
-constexpr int kTargetItems = TARGET;  // two workgroups a CU, two rounds of them
+constexpr int kTargetItems = TARGET;
+constexpr int kSlots = 512;  // workgroups that run at once: two a CU
 constexpr int kMinSegTiles = MINSEG;
 constexpr int kPlanSeqs = 64;      // sequences ranked and cut: one a lane
 
@@ -55,6 +57,14 @@ template <> struct Parts<bf16> { static constexpr int Q = 2, P = 1; };
 template <> struct Parts<f16> { static constexpr int Q = 3, P = 2; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 3; };
 
+// One sequence a lane: its rows, keys and cut.
+struct SeqPlan {
+  int row0, nq, len;
+  int tiles;      // query tiles
+  int segs;       // key segments
+  int seg_tiles;  // key tiles of a segment
+  int slot0;      // first partial row of a cut sequence: row i of segment g is slot0 + g * nq + i
+};
 struct Prefill8Args {
   Attn8Args a;
   int page_shift;
@@ -66,6 +76,7 @@ struct Prefill8Args {
   // Key segments: partials of cut sequences, row slots x heads (null: none is cut).
   float* part_acc;    // [slots][hq][D]
   float2* part_ml;    // [slots][hq], max in log2 units and sum
+  SeqPlan* plan;      // [kPlanSeqs], for the merge kernel
   int out_vec;  // 4 elements of an out row can be stored at once
   int q_vec;    // q rows are 16-byte aligned, dims together
 };
@@ -77,24 +88,25 @@ __device__ __forceinline__ void seq_rows(const Attn8Args& a, int s, int& row0, i
   nq = min(max(a.cu[s + 1], row0), rows) - row0;
 }
 
-__device__ __forceinline__ int wave_prefix(int x, int lane) {  // sum of the lanes before
-  int upto = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += y;
-  }
-  return upto - x;
+// Inclusive scans over the wave's lanes by DPP (a shuffle each would cost 1.3 us an item):
+// row_shr 1, 2, 4, 8 within 16 lanes, then the rows' last lanes into the rows after.
+template <typename X, typename F>
+__device__ __forceinline__ X wave_scan(X x, F join) {
+  auto take = [&](auto ctrl, auto rows) {
+    return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                             decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  x = join(x, take(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{}));
+  x = join(x, take(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{}));
+  x = join(x, take(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{}));
+  x = join(x, take(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{}));
+  x = join(x, take(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{}));
+  x = join(x, take(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{}));
+  return x;
 }
+__device__ __forceinline__ int scan_sum(int x) { return wave_scan(x, [](int a, int b) { return a + b; }); }
 
-// One sequence a lane: its rows, keys and cut.
-struct SeqPlan {
-  int row0, nq, len;
-  int tiles;      // query tiles
-  int segs;       // key segments
-  int seg_tiles;  // key tiles of a segment
-  int slot0;      // first partial row of a cut sequence: row i of segment g is slot0 + g * nq + i
-};
 __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
   SeqPlan s{};
   if (lane < p.a.num_seqs) {
@@ -106,14 +118,29 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
   s.segs = 1;
   s.seg_tiles = keys;
   if (p.part_acc) {
-    // Work in (query tile, key tile) pairs of all heads; 64-bit for one long sequence of many rows.
-    int64_t work = static_cast<int64_t>(s.tiles) * keys;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
-    const int target = max(kMinSegTiles, static_cast<int>(min<int64_t>((work * p.a.hq + kTargetItems - 1) / kTargetItems, 1 << 30)));
-    s.segs = max(1, (keys + target - 1) / target);
-    s.seg_tiles = (keys + s.segs - 1) / s.segs;
-    s.slot0 = wave_prefix(s.segs > 1 ? s.nq * s.segs : 0, lane);
+    // In (query tile, key tile) pairs.  The sum's rounding is inside the slack of
+    // partial_slots() and of the grid.
+    const float work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(
+        static_cast<float>(s.tiles) * static_cast<float>(keys), [](float a, float b) { return a + b; })), 63)) * p.a.hq;
+    const int longest = __builtin_amdgcn_readlane(wave_scan(keys, [](int a, int b) { return max(a, b); }), 63);
+    // Cut where the longest item would outlast the others by half: 24 chunks of 100-170 rows
+    // over up to 1000 keys (768 items of up to 18 tiles) took 66 us whole, 90 cut.
+    if (longest * (2.f * kSlots) > 3.f * work) {
+      // Few items: cut into one round of workgroups.  Many, of different lengths: into half as
+      // many again, so that the short ones fill the gaps (eight chunks 444 us in 512, 392
+      // in 768, 431 in 1024; one chunk of 64 items 112, 134, 129).
+      const bool few = __builtin_amdgcn_readlane(scan_sum(s.tiles), 63) * p.a.hq <= kSlots / 2;
+      int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few ? kSlots : kTargetItems)), 1e9f)));
+      for (int i = 0; few && i < 4; ++i) {  // as rounding up makes more items, towards the round
+        const int items = __builtin_amdgcn_readlane(scan_sum(s.tiles * max(1, (keys + target - 1) / target)), 63) * p.a.hq;
+        if (items <= kSlots) break;
+        target = max(target + 1, static_cast<int>(static_cast<float>(target) * items * (1.f / kSlots)));
+      }
+      s.segs = max(1, (keys + target - 1) / target);
+      s.seg_tiles = (keys + s.segs - 1) / s.segs;
+      const int slots = s.segs > 1 ? s.nq * s.segs : 0;
+      s.slot0 = scan_sum(slots) - slots;
+    }
   }
   return s;
 }
@@ -134,6 +161,7 @@ __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
   int unit;
   if (a.num_seqs <= kPlanSeqs) {
     const SeqPlan s = plan_of(p, lane);
+    if (p.part_acc && blockIdx.x == 0 && threadIdx.x < a.num_seqs) p.plan[lane] = s;
     const int units = s.tiles * s.segs, cost = s.seg_tiles;
     int before = 0;  // units of sequences with longer items (equal ones in order)
     for (int q = 0; q < a.num_seqs; ++q) {
@@ -163,7 +191,7 @@ __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
   for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
     int row0 = 0, nq = 0;
     if (s0 + lane < a.num_seqs) seq_rows(a, s0 + lane, row0, nq);
-    const int tiles = (nq + kBM - 1) / kBM, before = wave_prefix(tiles, lane);
+    const int tiles = (nq + kBM - 1) / kBM, before = scan_sum(tiles) - tiles;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(unit >= before && unit < before + tiles);
     if (hit) {
       const int at = __builtin_ctzll(hit);
@@ -577,46 +605,66 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     }
 }
 
-// Joins the segments of cut sequences, in order: a wave kMergeRows rows of one head.
-constexpr int kMergeRows = 4;
+// Joins the segments of cut sequences: a wave a (row, head).  Lane g holds segment g's
+// (max, sum) of a batch of 64; a load instruction reads SPI whole accumulators, and a
+// lane adds its segments in order before the SPI lanes of a chunk are added.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefill8_merge_kernel(Prefill8Args p) {
+  constexpr int CH = D / 4, SPI = 64 / CH, BATCH = 4;
   const Attn8Args& a = p.a;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int h = blockIdx.x % a.hq;
-  const int first = (blockIdx.x / a.hq * 4 + wave) * kMergeRows;
-  const SeqPlan s = plan_of(p, lane);
-  for (int row = first; row < min(first + kMergeRows, static_cast<int>(a.rows)); ++row) {
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(row >= s.row0 && row < s.row0 + s.nq);
-    if (!hit) continue;
-    const int at = __builtin_ctzll(hit);
-    const int segs = __builtin_amdgcn_readlane(s.segs, at);
-    if (segs < 2) continue;
-    const int nq = __builtin_amdgcn_readlane(s.nq, at), len = __builtin_amdgcn_readlane(s.len, at);
-    const int i = row - __builtin_amdgcn_readlane(s.row0, at);
-    // Segments past the last key of the row's query tile were not computed.
-    const int keys = max(len - nq + min(i / kBM * kBM + kBM, nq), 0);
-    const int seg_keys = __builtin_amdgcn_readlane(s.seg_tiles, at) * kBN;
-    const int live = min(segs, max(1, (keys + seg_keys - 1) / seg_keys));
-    const int64_t step = static_cast<int64_t>(nq) * a.hq;  // slots from one segment to the next
-    const int64_t base = (static_cast<int64_t>(__builtin_amdgcn_readlane(s.slot0, at)) + i) * a.hq + h;
-    float top = -INFINITY;
-    for (int g = 0; g < live; ++g) top = fmaxf(top, p.part_ml[base + g * step].x);
+  const int row = blockIdx.x / a.hq * 4 + wave;
+  SeqPlan s{};
+  if (lane < a.num_seqs) s = p.plan[lane];
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(row >= s.row0 && row < s.row0 + s.nq);
+  if (!hit) return;
+  const int at = __builtin_ctzll(hit);
+  const int segs = __builtin_amdgcn_readlane(s.segs, at);
+  if (segs < 2) return;
+  const int nq = __builtin_amdgcn_readlane(s.nq, at), len = __builtin_amdgcn_readlane(s.len, at);
+  const int i = row - __builtin_amdgcn_readlane(s.row0, at);
+  // Segments past the last key of the row's query tile were not computed.
+  const int keys = max(len - nq + min(i / kBM * kBM + kBM, nq), 0);
+  const int seg_keys = __builtin_amdgcn_readlane(s.seg_tiles, at) * kBN;
+  const int live = min(segs, max(1, (keys + seg_keys - 1) / seg_keys));
+  const int64_t step = static_cast<int64_t>(nq) * a.hq;  // slots from one segment to the next
+  const int64_t base = (static_cast<int64_t>(__builtin_amdgcn_readlane(s.slot0, at)) + i) * a.hq + h;
+  const int c = lane % CH, q = lane / CH;
+  float m = -INFINITY, sum = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int g0 = 0; g0 < live; g0 += 64) {
+    const int n = min(live - g0, 64);
+    const float2 ml = lane < n ? p.part_ml[base + (g0 + lane) * step] : make_float2(-INFINITY, 0.f);
+    const float top = fmaxf(m, group_max<64>(ml.x));
     const float off = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[D / 64] = {};
-    for (int g = 0; g < live; ++g) {
-      const float2 ml = p.part_ml[base + g * step];
-      const float w = fast_exp2(ml.x - off);
-      sum = fmaf(ml.y, w, sum);
+    const float corr = fast_exp2(m - off);
+    const float w = lane < n ? fast_exp2(ml.x - off) : 0.f;
+    m = top;
+    sum = fmaf(sum, corr, group_sum<64>(ml.y * w));
+    acc *= corr;
+    for (int u0 = 0; u0 < n; u0 += BATCH * SPI) {
+      f32x4 x[BATCH];
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(p.part_acc[(base + g * step) * D + lane + 64 * e], w, acc[e]);
+      for (int u = 0; u < BATCH; ++u)
+        x[u] = *reinterpret_cast<const f32x4*>(p.part_acc + (base + min(g0 + u0 + u * SPI + q, live - 1) * step) * D + 4 * c);
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int g = u0 + u * SPI + q;
+        const float wg = __shfl(w, g & 63, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = g < n ? fmaf(x[u][e], wg, acc[e]) : acc[e];
+      }
     }
-    const bool blind = len - nq + i < 0;  // a row that sees no key
-    const float inv = 1.f / sum;
-    T* orow = static_cast<T*>(a.out) + row * a.o_row + h * a.o_head;
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) store_elem(orow + (lane + 64 * e) * a.o_dim, blind ? 0.f : acc[e] * inv);
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = strided_sum<CH>(acc[e]);
+  if (q) return;
+  const bool blind = len - nq + i < 0;  // a row that sees no key
+  const float inv = 1.f / sum;
+  T* orow = static_cast<T*>(a.out) + row * a.o_row + h * a.o_head;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) store_elem(orow + (4 * c + e) * a.o_dim, blind ? 0.f : acc[e] * inv);
 }
 
 // Partial rows that a launch can need: a sequence's rows once a segment.  Segments
@@ -625,7 +673,7 @@ __global__ __launch_bounds__(256) void prefill8_merge_kernel(Prefill8Args p) {
 int64_t partial_slots(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq) {
   const int64_t most = ((max_len + kBN - 1) / kBN + kMinSegTiles - 1) / kMinSegTiles;
   if (num_seqs > kPlanSeqs || most < 2) return 0;
-  return std::min(rows * most, rows + (kBM * kTargetItems + hq - 1) / hq);
+  return std::min(rows * most, rows + (kBM * kTargetItems + hq - 1) / hq + 64);
 }
 
 }  // namespace
@@ -640,7 +688,8 @@ bool prefill8_layout(const Attn8Args& a) {
 }
 
 int64_t prefill8_workspace(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq, int64_t d) {
-  return partial_slots(rows, num_seqs, max_len, hq) * hq * (d * 4 + 8);
+  const int64_t slots = partial_slots(rows, num_seqs, max_len, hq);
+  return slots ? slots * hq * (d * 4 + 8) + kPlanSeqs * static_cast<int64_t>(sizeof(SeqPlan)) : 0;
 }
 
 int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, const char* name) {
@@ -651,6 +700,7 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   if (slots) {
     p.part_acc = static_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float2*>(p.part_acc + slots * a.hq * a.d);
+    p.plan = reinterpret_cast<SeqPlan*>(p.part_ml + slots * a.hq);
   }
   p.page_shift = __builtin_ctz(a.page);
   p.qscale = std::fabs(a.qscale);
@@ -661,8 +711,8 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
   p.out_vec = a.o_dim == 1 && aligned16(a.out) && a.o_row * es % 16 == 0 && a.o_head * es % 16 == 0;
   // Query tiles, and the segments past the first (as many items as partial_slots() has such rows).
-  const int64_t tiles = a.rows / kBM + std::min<int64_t>(a.num_seqs, a.rows) + (slots ? (kTargetItems + a.hq - 1) / a.hq : 0);
-  const int64_t merge_rows = (a.rows + 4 * kMergeRows - 1) / (4 * kMergeRows);
+  const int64_t tiles = a.rows / kBM + std::min<int64_t>(a.num_seqs, a.rows) + (slots ? (kTargetItems + a.hq - 1) / a.hq + 2 : 0);
+  const int64_t merge_rows = (a.rows + 3) / 4;
   if (tiles * a.hq > 0x7fffffff || merge_rows * a.hq > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const dim3 grid(static_cast<unsigned>(tiles * a.hq)), merge(static_cast<unsigned>(merge_rows * a.hq)), block(256);
 #define LAUNCH_D(T, D)                                                                                   \
