@@ -210,6 +210,9 @@ __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
 
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) { return MfmaOps<bf16>::pack2(x, y); }
 
+// The top bit of every byte of a word of codes that is NaN (all bits of its magnitude set).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // Two codes of a word (its low or high half) times the scale of byte b, as bf16.
 // The instruction takes the scale as an fp32's exponent, with the byte's meaning: 0
 // is 2^-127, 255 NaN.
@@ -237,7 +240,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   __shared__ __align__(16) uint16_t v_lds[2][kBN * VROW];
   __shared__ uint8_t ks_lds[2][kBN];
   __shared__ __align__(16) float bias_lds[2][4];  // of each wave's staged V scales (value_bias)
-  __shared__ __align__(16) int nan_lds[2][4];     // whether the wave staged a V that is NaN
 
   const Attn8Args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -353,32 +355,47 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   u32x4 kreg[PASSES], vreg[PASSES];
   uint32_t vsreg[PASSES], ksreg;
   auto token = [&](int tile, int t) { return min(static_cast<uint32_t>(tile * kBN + t), last_key); };
-  auto offset = [](uint32_t id, uint32_t block, uint32_t slot, uint32_t token) {
-    return static_cast<uint64_t>(id) * block + slot * token;
-  };
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
-    ks_id = trow[token(tile, lane) >> p.page_shift];
+    if (wave == 0) ks_id = trow[token(tile, lane) >> p.page_shift];
   };
   auto load_tile = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const uint32_t slot = token(tile, i * TPP + st) & page_mask, id = ids[i] < num_blocks ? ids[i] : 0;
-      const uint64_t at = offset(id, block_bytes, slot, token_bytes);
+      const uint32_t slot = token(tile, i * TPP + st) & page_mask;
+      const uint64_t id = ids[i] < num_blocks ? ids[i] : 0;
+      const uint64_t at = id * block_bytes + __umul24(slot, token_bytes);
       kreg[i] = *reinterpret_cast<const u32x4*>(kbase + at);
       vreg[i] = *reinterpret_cast<const u32x4*>(vbase + at);
-      vsreg[i] = vsbase[offset(id, s_block, slot, s_token)];
+      vsreg[i] = vsbase[id * s_block + __umul24(slot, s_token)];
     }
-    if (wave == 0) ksreg = ksbase[offset(ks_id < num_blocks ? ks_id : 0, s_block, token(tile, lane) & page_mask, s_token)];
+    if (wave == 0)
+      ksreg = ksbase[static_cast<uint64_t>(ks_id < num_blocks ? ks_id : 0) * s_block + __umul24(token(tile, lane) & page_mask, s_token)];
   };
+  // A V that is NaN must not reach the rows that do not see it through a product with 0:
+  // in tiles that some row sees part of, it is stored as 0, and noted (see the end).
+  bool nan = false;
   auto store_tile = [&](int buf, bool masked) __attribute__((always_inline)) {
     uint32_t top = 0;  // largest V scale
-    bool nan = false;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int t = i * TPP + st;
       *reinterpret_cast<u32x4*>(&k_lds[buf][t * KROW + sc * 16]) = kreg[i];
+      if (masked) {
+        bool here = vsreg[i] == 255u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) here |= nan_codes(vreg[i][e]) != 0;
+        if (here) {
+          nan = true;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t bad = vsreg[i] == 255u ? 0x80808080u : nan_codes(vreg[i][e]);
+            vreg[i][e] &= ~((bad >> 7) * 0xffu);
+          }
+          vsreg[i] = vsreg[i] == 255u ? 127u : vsreg[i];
+        }
+      }
       u32x4 w[2];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = scaled_bf16(vreg[i][e / 2], vsreg[i], e % 2);
@@ -386,20 +403,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
       *reinterpret_cast<u32x4*>(dst) = w[0];
       *reinterpret_cast<u32x4*>(dst + 8) = w[1];
       top = max(top, vsreg[i]);
-      if (masked) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) nan |= (((vreg[i][e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
-        nan |= vsreg[i] == 255u;
-      }
     }
     if (wave == 0) ks_lds[buf][lane] = static_cast<uint8_t>(ksreg);
     float bias = 0.f;
     if (__builtin_amdgcn_ballot_w64(top > 191u)) bias = group_max<64>(value_bias(top == 255u ? 0u : top));
-    const int wave_nan = masked && __builtin_amdgcn_ballot_w64(nan) != 0;
-    if (lane == 0) {
-      bias_lds[buf][wave] = bias;
-      nan_lds[buf][wave] = wave_nan;
-    }
+    if (lane == 0) bias_lds[buf][wave] = bias;
   };
   // Whether some row of the workgroup does not see all of a tile's keys.
   auto tile_masked = [&](int tile) { return tile * kBN + kBN - 1 > prefix + qt0; };
@@ -482,15 +490,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
       const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias_lds[buf]);
       tmax = max_across_halves(tmax) * p.qscale + fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
-      if (__builtin_amdgcn_ballot_w64(tmax > m + kRescale) != 0) {
+      const bool rescale = __builtin_amdgcn_ballot_w64(tmax > m + kRescale) != 0;
+      float corr = 1.f;
+      if (rescale) {
         const float mn = fmaxf(m, tmax);
-        const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+        corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
         m = mn;
         lsum *= corr;
-#pragma unroll
-        for (int c = 0; c < DT; ++c)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
       }
       const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
       // exp2(s * qscale - m) in one rounding, unless m's own is no longer small.
@@ -522,48 +528,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         const u32x2 lo = lds_read_tr(vlo), hi = lds_read_tr(vlo + 8 * VROW);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
-      const int4 n4 = *reinterpret_cast<const int4*>(nan_lds[buf]);
-      if (masked && uniform(n4.x | n4.y | n4.z | n4.w) != 0) {
-        // A NaN in V that some row may not see: products without it, and a NaN where a row
-        // sees one (counted by a product of indicators).
+      // One site for all products: accumulators changed on two paths get two register sets.
+      if (rescale) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          u32x4 pb[NP], seen;
-          weights(ks, pb);
-          const int lim = limit - key0 - 4 * half - 16 * ks;
+        for (int c = 0; c < DT; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = (e / 2) * 8 + (2 * e) % 4;
-            seen[e] = (key <= lim ? 0x3f80u : 0u) | (key + 1 <= lim ? 0x3f800000u : 0u);
-          }
+          for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
+      }
 #pragma unroll
-          for (int c = 0; c < DT; ++c) {
-            const u32x4 va = values(ks, c);
-            u32x4 clean, is_nan;
+      for (int ks = 0; ks < 4; ++ks) {
+        u32x4 pb[NP];
+        weights(ks, pb);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const bool n0 = (va[e] & 0x7fffu) > 0x7f80u, n1 = (va[e] & 0x7fff0000u) > 0x7f800000u;
-              clean[e] = (n0 ? 0u : va[e] & 0xffffu) | (n1 ? 0u : va[e] & 0xffff0000u);
-              is_nan[e] = (n0 ? 0x3f80u : 0u) | (n1 ? 0x3f800000u : 0u);
-            }
+        for (int c = 0; c < DT; ++c) {
+          const u32x4 va = values(ks, c);
 #pragma unroll
-            for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(clean), as_v8<bf16x8>(pb[n]), acc[c]);
-            const f32x16 count = Ops::mma(as_v8<bf16x8>(is_nan), as_v8<bf16x8>(seen), f32x16{});
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[c][r] = count[r] > 0.f ? __uint_as_float(0x7fc00000u) : acc[c][r];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          u32x4 pb[NP];
-          weights(ks, pb);
-#pragma unroll
-          for (int c = 0; c < DT; ++c) {
-            const u32x4 va = values(ks, c);
-#pragma unroll
-            for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(va), as_v8<bf16x8>(pb[n]), acc[c]);
-          }
+          for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(va), as_v8<bf16x8>(pb[n]), acc[c]);
         }
       }
     }
@@ -571,6 +551,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     __syncthreads();
   }
 
+  // V that was NaN in tiles that some row sees part of: it is NaN in the rows that see it.
+  if (__syncthreads_or(nan)) {
+    for (int j = max(first_tile, max(prefix + qt0 + 1, 0) / kBN); j < ntiles; ++j) {
+#pragma unroll 1
+      for (int t = j * kBN; t < min(j * kBN + kBN, wg_keys); ++t) {
+        const uint32_t id = trow[t >> p.page_shift], slot = t & page_mask;
+        const uint64_t blk = id < num_blocks ? id : 0;
+        const uint8_t* row = a.v + kvh * a.kv_head + blk * block_bytes + slot * token_bytes + 4 * half;
+        const bool all = vsbase[blk * s_block + slot * s_token] == 255u;
+#pragma unroll
+        for (int c = 0; c < DT; ++c)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t bad = all ? 0x80808080u : nan_codes(*reinterpret_cast<const uint32_t*>(row + 32 * c + 8 * g));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t <= limit && (bad >> (8 * e + 7) & 1)) acc[c][4 * g + e] = __uint_as_float(0x7fc00000u);
+          }
+      }
+    }
+  }
   lsum += __shfl_xor(lsum, 32, 64);
   if (!row_valid) return;
   if (uniform(it.segs) > 1) {
@@ -681,10 +682,11 @@ int64_t partial_slots(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t h
 bool prefill8_shape(int64_t d, int64_t page) { return (d == 64 || d == 128) && page >= 16 && (page & (page - 1)) == 0; }
 
 bool prefill8_layout(const Attn8Args& a) {
+  auto near = [](int64_t x) { return x >= 0 && x < (int64_t(1) << 24); };
   auto small = [](int64_t x) { return x >= 0 && x < (int64_t(1) << 32); };
   return prefill8_shape(a.d, a.page) && a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && a.kv_head % 16 == 0 &&
-         a.kv_token % 16 == 0 && a.kv_block % 16 == 0 && small(a.kv_block) && small(a.kv_token * a.page) &&
-         small(a.s_block) && small(a.s_token * a.page);
+         a.kv_token % 16 == 0 && a.kv_block % 16 == 0 && small(a.kv_block) && small(a.s_block) &&
+         near(a.kv_token) && near(a.s_token) && near(a.page) && small(a.kv_token * a.page) && small(a.s_token * a.page);
 }
 
 int64_t prefill8_workspace(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq, int64_t d) {
