@@ -9,6 +9,8 @@
 //   out[j] = x[j] c - x[j + half] s,   out[j + half] = x[j + half] c + x[j] s
 // each product and the sum rounded to fp32 on its own, the result rounded once to
 // the type it is stored in.  Dims past 2 * half pass through.
+#include <algorithm>
+
 #include "fp8.hpp"
 
 namespace rlt {
@@ -16,6 +18,7 @@ namespace {
 
 constexpr int kMaxAxes = 4;
 constexpr int kMaxHalf = 256;  // frequencies of a head
+constexpr int kFewWaves = 4096;
 
 struct AppendRow {
   const void* x;
@@ -149,6 +152,134 @@ __global__ __launch_bounds__(64) void rope_axes_generic_kernel(RopeAxesArgs a) {
   }
 }
 
+// Aligned rows of 16-bit or fp32 heads that turn as a whole (2 half == d, or half 0: no
+// rotation): a wave takes a row, LPH lanes a head.  Lane i of a head holds the 16-byte packets
+// i of its two halves, so both dims of its pairs, and its cosines and sines serve all
+// heads of the row.  Bytes bound it: 4096 rows of 16 + 16 + 16 heads x 128 move 84 MB.
+template <typename T, bool ROT, bool FP8, int LPH, int U>
+__global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a, int64_t n_rows, int parts) {
+  using PK = Packet<T>;
+  constexpr int N = PK::N, HALF = LPH * N, NG = 64 / LPH;  // dims of a half, heads at a time (U times, of q, k and v each)
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + uniform(threadIdx.x >> 6);
+  const int64_t row = parts == 1 ? item : item / parts;
+  if (row >= n_rows) return;
+  const int lane = threadIdx.x & 63, i = lane % LPH, g = lane / LPH;
+  const int first = static_cast<int>(item - row * parts) * NG + g, stride = parts * NG;
+  const bool listed = row < a.n_write;
+  auto load = [&](int which, int head, u32x4 (&x)[2]) __attribute__((always_inline)) {
+    const T* src = static_cast<const T*>(a.in[which].x) + row * a.in[which].row + head * a.in[which].head + i * N;
+    x[0] = *reinterpret_cast<const u32x4*>(src);
+    x[1] = *reinterpret_cast<const u32x4*>(src + HALF);
+  };
+  u32x4 q[U][2] = {}, k[U][2] = {}, v[U][2] = {};
+  auto load_heads = [&](int h0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * stride;
+      if (ROT && h < a.hq) load(0, h, q[u]);
+      if (listed && h < a.hkv) {
+        load(1, h, k[u]);
+        load(2, h, v[u]);
+      }
+    }
+  };
+  load_heads(first);
+  int64_t block = -1, offset = -1;
+  if (listed) {
+    block = a.blocks[row];
+    offset = a.offsets[row];
+  }
+  bool write = block >= 0 && block < a.num_blocks && offset >= 0 && offset < a.page;
+  bool inside = true;
+  float cs[N], sn[N];
+  if constexpr (ROT) {
+    const int64_t* pos = a.positions + row * a.p_row;
+    const int64_t p0 = pos[0], p1 = a.axes > 1 ? pos[a.p_axis] : 0, p2 = a.axes > 2 ? pos[2 * a.p_axis] : 0;
+    const int64_t p3 = a.axes > 3 ? pos[3 * a.p_axis] : 0;
+    const uint64_t most = static_cast<uint64_t>(a.max_position);
+    inside = static_cast<uint64_t>(p0) < most && static_cast<uint64_t>(p1) < most && static_cast<uint64_t>(p2) < most &&
+             static_cast<uint64_t>(p3) < most;
+    write &= inside;
+    uint32_t words = 0;  // the axes of this lane's frequencies, 2 bits each
+#pragma unroll
+    for (int w = 0; w < (HALF + 15) / 16; ++w)
+      if (i * N / 16 == w) words = a.axis_of[w] >> (2 * (i * N % 16));
+    // 32-bit byte offsets into the table (the host checks its size).
+    const uint32_t r0 = static_cast<uint32_t>(p0), r1 = static_cast<uint32_t>(p1), r2 = static_cast<uint32_t>(p2), r3 = static_cast<uint32_t>(p3);
+    const char* base = reinterpret_cast<const char*>(a.table);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const uint32_t x = words >> (2 * e) & 3;
+      const uint32_t at = x & 2 ? (x & 1 ? r3 : r2) : (x & 1 ? r1 : r0);
+      const float2 t = *reinterpret_cast<const float2*>(base + (inside ? at * (8u * HALF) : 0u) + 8u * (i * N + e));
+      cs[e] = t.x, sn[e] = t.y;
+    }
+  }
+  auto turned = [&](const u32x4 (&x)[2], bool rotate, float (&lo)[N], float (&hi)[N]) __attribute__((always_inline)) {
+    PK::unpack(x[0], lo);
+    PK::unpack(x[1], hi);
+    if (rotate) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float l = lo[e], h = hi[e];
+        turn(l, h, cs[e], sn[e], &lo[e], &hi[e]);
+      }
+    }
+  };
+  auto store = [&](int which, int head, const u32x4 (&x)[2], bool rotate) __attribute__((always_inline)) {
+    float lo[N], hi[N];
+    turned(x, rotate, lo, hi);
+    const int64_t slot = block * a.c_block + a.layer * a.c_layer + offset * a.c_token + head * a.c_head;
+    if constexpr (FP8) {
+      float amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) amax = fmaxf(amax, fmaxf(finite_abs(lo[e]), finite_abs(hi[e])));
+      const uint32_t b = scale_byte(group_max<LPH>(amax));
+      const float inv = inverse_scale(b);
+      uint8_t* codes = static_cast<uint8_t*>(a.cache[which]) + slot + i * N;
+      uint32_t w[2][N / 4];
+#pragma unroll
+      for (int e = 0; e < N / 4; ++e) {
+        w[0][e] = codes2(lo[4 * e], lo[4 * e + 1], inv) | codes2(lo[4 * e + 2], lo[4 * e + 3], inv) << 16;
+        w[1][e] = codes2(hi[4 * e], hi[4 * e + 1], inv) | codes2(hi[4 * e + 2], hi[4 * e + 3], inv) << 16;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(codes + u * HALF) = make_uint2(w[u][0], w[u][1]);
+        else *reinterpret_cast<uint32_t*>(codes + u * HALF) = w[u][0];
+      }
+      if (i == 0)
+        a.scales[which][block * a.s_block + a.layer * a.s_layer + offset * a.s_token + head * a.s_head] = static_cast<uint8_t>(b);
+    } else {
+      T* dst = static_cast<T*>(a.cache[which]) + slot + i * N;
+      *reinterpret_cast<u32x4*>(dst) = rotate ? PK::pack(lo) : x[0];
+      *reinterpret_cast<u32x4*>(dst + HALF) = rotate ? PK::pack(hi) : x[1];
+    }
+  };
+  for (int h0 = first; h0 < max(a.hq, write ? a.hkv : 0); h0 += U * stride) {
+    if (h0 != first) load_heads(h0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * stride;
+      if (ROT && h < a.hq) {
+        float lo[N], hi[N];
+        turned(q[u], true, lo, hi);
+        T* dst = static_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head + i * N;
+        *reinterpret_cast<u32x4*>(dst) = inside ? PK::pack(lo) : u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(dst + HALF) = inside ? PK::pack(hi) : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * stride;
+      if (write && h < a.hkv) {
+        store(0, h, k[u], ROT);
+        store(1, h, v[u], false);
+      }
+    }
+  }
+}
+
 // Checks of both entry points; fills everything but q, the rotation and the rows.
 int append_args(const char* name, void* key_cache, void* value_cache, const int64_t* cache_strides, void* key_scales,
                 void* value_scales, const int64_t* scale_strides, const void* k, const int64_t* k_strides,
@@ -193,12 +324,65 @@ int append_args(const char* name, void* key_cache, void* value_cache, const int6
   return RLT_OK;
 }
 
-int launch(const RopeAxesArgs& a, int64_t n_rows, int dtype, hipStream_t stream, const char* name) {
+// Whether rope_axes_kernel covers the call.
+bool rows16(const RopeAxesArgs& a, int es) {
+  auto packets = [&](const void* x, int64_t s0, int64_t s1, int64_t dim) {
+    return dim == 1 && aligned16(x) && s0 * es % 16 == 0 && s1 * es % 16 == 0;
+  };
+  if (a.half && 2 * a.half != a.d) return false;
+  for (int w = a.half ? 0 : 1; w < 3; ++w)
+    if (!packets(a.in[w].x, a.in[w].row, a.in[w].head, a.in[w].dim)) return false;
+  if (a.half && !packets(a.q_out, a.qo_row, a.qo_head, a.qo_dim)) return false;
+  if (a.half && ((reinterpret_cast<uintptr_t>(a.table) & 7u) || a.max_position > (int64_t(1) << 32) / (8 * a.half))) return false;
+  const int ce = a.scales[0] ? 1 : es, unit = a.scales[0] ? 16 / es : 16;  // bytes a lane stores at once
+  for (int w = 0; w < 2; ++w)
+    if (reinterpret_cast<uintptr_t>(a.cache[w]) % unit) return false;
+  return a.c_dim == 1 && a.c_block * ce % unit == 0 && a.c_layer * ce % unit == 0 && a.c_token * ce % unit == 0 &&
+         a.c_head * ce % unit == 0;
+}
+
+template <typename T, bool ROT, bool FP8>
+bool launch_rows(const RopeAxesArgs& a, int64_t n_rows, hipStream_t stream) {
+  const int lanes = a.d % (2 * Packet<T>::N) == 0 ? a.d / 2 / Packet<T>::N : 0;  // of a head
+  // A wave a row, or a few waves where rows are few (us, one against several): 8 rows of 16 +
+  // 16 heads x 128 into a bf16 cache 5.5 / 4.0, 512 of 32 + 8 into an 8-bit one 8.2 / 6.1, 1500
+  // of 16 + 16 12.4 / 11.1.
+  int parts = 1;
+  while (lanes && n_rows * parts < kFewWaves && parts * (64 / lanes) < std::max(a.hq, a.hkv)) parts *= 2;
+  const bool once = lanes && parts * (64 / lanes) >= std::max(a.hq, a.hkv);  // a wave has all its heads at once
+  const int64_t waves = n_rows * parts;
+  const dim3 grid(static_cast<unsigned>((waves + 3) / 4)), block(256);
+#define LAUNCH(L)                                                                                                      \
+  do {                                                                                                                 \
+    if (once) hipLaunchKernelGGL((rope_axes_kernel<T, ROT, FP8, L, 1>), grid, block, 0, stream, a, n_rows, parts);     \
+    else hipLaunchKernelGGL((rope_axes_kernel<T, ROT, FP8, L, 2>), grid, block, 0, stream, a, n_rows, parts);          \
+  } while (0)
+  switch (lanes) {
+    case 4: LAUNCH(4); return true;
+    case 8: LAUNCH(8); return true;
+    case 16: LAUNCH(16); return true;
+    case 32: LAUNCH(32); return true;
+    default: return false;
+  }
+#undef LAUNCH
+}
+
+template <typename T>
+void launch_type(const RopeAxesArgs& a, int64_t n_rows, hipStream_t stream) {
+  if (rows16(a, sizeof(T))) {
+    if (a.half ? (a.scales[0] ? launch_rows<T, true, true>(a, n_rows, stream) : launch_rows<T, true, false>(a, n_rows, stream))
+               : launch_rows<T, false, true>(a, n_rows, stream))
+      return;
+  }
   const dim3 grid(static_cast<unsigned>(n_rows), static_cast<unsigned>(a.hq + 2 * a.hkv));
+  hipLaunchKernelGGL((rope_axes_generic_kernel<T>), grid, dim3(64), 0, stream, a);
+}
+
+int launch(const RopeAxesArgs& a, int64_t n_rows, int dtype, hipStream_t stream, const char* name) {
   switch (dtype) {
-    case RLT_BFLOAT16: hipLaunchKernelGGL((rope_axes_generic_kernel<bf16>), grid, dim3(64), 0, stream, a); break;
-    case RLT_FLOAT16: hipLaunchKernelGGL((rope_axes_generic_kernel<f16>), grid, dim3(64), 0, stream, a); break;
-    default: hipLaunchKernelGGL((rope_axes_generic_kernel<float>), grid, dim3(64), 0, stream, a); break;
+    case RLT_BFLOAT16: launch_type<bf16>(a, n_rows, stream); break;
+    case RLT_FLOAT16: launch_type<f16>(a, n_rows, stream); break;
+    default: launch_type<float>(a, n_rows, stream); break;
   }
   return check_launch(name);
 }
