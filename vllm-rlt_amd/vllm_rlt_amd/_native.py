@@ -192,6 +192,13 @@ HOST_CALLED = (
     "rlt_paged_prefill_split",
     "rlt_paged_prefill_split_workspace_bytes",
     "rlt_rope_kv_append",
+    "rlt_paged_decode_fp8",
+    "rlt_paged_decode_fp8_workspace_bytes",
+    "rlt_paged_prefill_fp8",
+    "rlt_paged_prefill_fp8_workspace_bytes",
+    "rlt_kv_append_fp8",
+    "rlt_rope_axes_kv_append",
+    "rlt_build_chunk_metadata",
 )
 
 

@@ -42,6 +42,13 @@ def _host_calls(t: torch.Tensor):
     return _native.host, stream_handle(t.device)
 
 
+def _host_calls_here(t: torch.Tensor):
+    """_host_calls for launches on the current device; (None, 0) where t is on another."""
+    if not t.is_cuda or torch.cuda.current_device() != t.device.index:
+        return None, 0
+    return _host_calls(t)
+
+
 def _finish(result, name: str) -> torch.Tensor:
     if type(result) is int:
         check(result, name)
@@ -985,6 +992,14 @@ def build_chunk_metadata(
     an append of the whole buffer skips them; tokens past it are dropped from the
     end.  Sequences from count on are padding: no tokens, length 0.
     """
+    host, stream = _host_calls_here(tables)
+    if host is not None:
+        result = host.chunk_metadata(
+            descriptors, count, size, tables, page_size, cu_seqlens, lengths, positions, sequences, blocks, offsets,
+            out_tables, out_width, stream,
+        )
+        if result is not None:
+            return check(result, "rlt_build_chunk_metadata")
     device = _require_rocm(tables, cu_seqlens, lengths, positions, sequences, blocks, offsets, out_tables)
     if tables.dtype != torch.int32 or tables.ndim != 3 or not tables.is_contiguous():
         raise ValueError("tables must be contiguous int32 [slots, planes, width]")
@@ -1067,6 +1082,13 @@ def kv_append_fp8(
     amax <= 448 * scale over the row's finite values.  Values that are not finite are
     stored as NaN.  k and v are float32, float16 or bfloat16.
     """
+    host, stream = _host_calls_here(key_cache)
+    if host is not None:
+        result = host.append8(
+            key_cache, value_cache, key_scales, value_scales, layer, write_blocks, write_offsets, k, v, n_rows, stream
+        )
+        if result is not None:
+            return check(result, "rlt_kv_append_fp8")
     device = _require_rocm(key_cache, value_cache, key_scales, value_scales, write_blocks, write_offsets, k, v)
     _require_fp8(key_cache, value_cache, key_scales, value_scales, 5)
     nb, nl, page, hkv, d = key_cache.shape
@@ -1124,6 +1146,14 @@ def rope_axes_kv_append(
     is rotated for every row.  A row with a position outside the table gets zeros
     and is not written.  `out` may be q itself.
     """
+    host, stream = _host_calls_here(q)
+    if host is not None:
+        result = host.rope_axes(
+            key_cache, value_cache, layer, write_blocks, write_offsets, q, k, v, positions, table, axes, key_scales,
+            value_scales, out, n_rows, stream,
+        )
+        if result is not None:
+            return _finish(result, "rlt_rope_axes_kv_append")
     device = _require_rocm(key_cache, value_cache, write_blocks, write_offsets, q, k, v, positions, table)
     if (key_scales is None) != (value_scales is None):
         raise ValueError("key_scales and value_scales go together")
@@ -1239,6 +1269,13 @@ def paged_decode_fp8(
     rows and is allocated here unless given.  A row's output bits depend on its own
     q, pages and length only.
     """
+    host, stream = _host_calls_here(q)
+    if host is not None:
+        result = host.decode8(
+            q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out, workspace, scale, stream
+        )
+        if result is not None:
+            return _finish(result, "rlt_paged_decode_fp8")
     device, out = _fp8_attention_inputs(
         q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
     )
@@ -1300,6 +1337,14 @@ def paged_prefill_fp8(
     are cut, by the launch's shapes, and is allocated here unless given.  With
     `batch_invariant` none is cut: a row's bits depend on its own sequence only.
     """
+    host, stream = _host_calls_here(q)
+    if host is not None:
+        result = host.prefill8(
+            q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, cu_seqlens_q, max_seqlen_q,
+            out, workspace, scale, batch_invariant, stream,
+        )
+        if result is not None:
+            return _finish(result, "rlt_paged_prefill_fp8")
     device, out = _fp8_attention_inputs(
         q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
     )
