@@ -168,7 +168,7 @@ extern "C" int64_t rlt_paged_decode_fp8_workspace_bytes(int64_t n_rows, int64_t 
   if (n_rows <= 0 || max_table_width <= 0 || !decode8_shape(num_q_heads, num_kv_heads, head_dim, page_size) ||
       max_table_width > 0x7fffffff / page_size)
     return 0;
-  return decode8_workspace(n_rows, max_table_width * page_size, num_q_heads, head_dim);
+  return decode8_workspace(n_rows, max_table_width * page_size, num_q_heads, num_kv_heads, head_dim);
 }
 
 extern "C" int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, const void* key_cache,

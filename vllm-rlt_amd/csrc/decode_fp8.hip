@@ -1,8 +1,7 @@
 // Decode over the 8-bit KV cache: one new token a sequence, split over the
 // cache's length and joined.
 //
-// A row's keys are cut into splits (longer ones, doubled, where kMaxSplits would
-// not cover the row) and a split into kParts parts of consecutive tokens, a
+// A row's keys are cut into splits (decode8_split_plan) and a split into kParts parts of consecutive tokens, a
 // function of the row's length alone.  A part of one head is worked by D/16 lanes in
 // order, with a running maximum and sum of its own; the parts of a split and then
 // the splits are joined in order.  So a row's bits depend neither on its batch nor
@@ -25,28 +24,9 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kParts = 16;
 constexpr int kUnit = 16;  // tokens of a page looked up at once (pages hold whole units), and of the shortest part
-constexpr int kMaxSplits = 64;
 constexpr int kXcds = 8;
 constexpr int kCus = 256;
 constexpr int64_t kMaxGrid = 32768;
-
-__host__ __device__ inline void split_plan(int64_t len, int* split_len, int* nsplit) {
-  int64_t per = kParts * kUnit;
-  while (per * kMaxSplits < len) per <<= 1;
-  *split_len = static_cast<int>(per);
-  *nsplit = static_cast<int>(len > 0 ? (len + per - 1) / per : 1);
-}
-
-struct Decode8Args {
-  Attn8Args a;
-  float* ws_acc;   // [rows][hkv][splits][G][D]
-  float2* ws_ml;   // [rows][hkv][splits][G], max in log2 units and sum
-  int splits;      // splits a row of the tables' width has
-  int split_slots; // split-dimension workgroups launched; each walks every split_slots-th split
-  int hpw;         // heads a wave
-  int xcd;         // workgroups of one (split, head block) of all rows share an XCD
-  int q_vec;       // q rows are 16-byte aligned, dims together
-};
 
 __device__ __forceinline__ u32x4 load_codes(const uint8_t* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
@@ -120,7 +100,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
   const int h0 = gi % blocks * HPW;
   const int len = sequence_length(a, r);
   int split_len, ns;
-  split_plan(len, &split_len, &ns);
+  decode8_split_plan(len, kParts * kUnit, &split_len, &ns);
   const int s = lane % LPT, gh = lane / LPT % HPW, gp = lane / (LPT * HPW), group0 = lane & ~(LPT - 1);
   const int part_len = split_len / kParts;
   const uint32_t units = static_cast<uint32_t>(part_len) / kUnit;  // a part, a power of two
@@ -335,7 +315,7 @@ __global__ __launch_bounds__(64 * kWaves) void decode8_merge_kernel(Decode8Args 
   const int r = static_cast<int>(item / a.hq), hq = static_cast<int>(item - static_cast<int64_t>(r) * a.hq);
   const int G = a.hq / a.hkv, h = hq / G, j = hq - h * G;
   int split_len, ns;
-  split_plan(sequence_length(a, r), &split_len, &ns);
+  decode8_split_plan(sequence_length(a, r), p.base, &split_len, &ns);
   if (ns < 2) return;
   const int64_t base = (static_cast<int64_t>(r) * a.hkv + h) * p.splits * G + j;
   const float2 ml = lane < ns ? p.ws_ml[base + static_cast<int64_t>(lane) * G] : make_float2(-INFINITY, 0.f);
@@ -382,16 +362,16 @@ void launch_shape(const Decode8Args& p, unsigned grid, hipStream_t stream) {
     case 2: launch_split<T, D, G, 2>(p, grid, stream); break;
     default: launch_split<T, D, G, 1>(p, grid, stream); break;
   }
-  if (p.splits > 1) {
-    const unsigned merge = static_cast<unsigned>((p.a.rows * p.a.hq + kWaves - 1) / kWaves);
-    hipLaunchKernelGGL((decode8_merge_kernel<T, D>), dim3(merge), dim3(64 * kWaves), 0, stream, p);
-  }
 }
 
 template <typename T, int D>
 void launch_group(const Decode8Args& p, unsigned grid, hipStream_t stream) {
   if (p.a.hq == p.a.hkv) launch_shape<T, D, 1>(p, grid, stream);
-  else launch_shape<T, D, 2>(p, grid, stream);
+  else if (p.a.hq == 2 * p.a.hkv) launch_shape<T, D, 2>(p, grid, stream);
+  if (p.splits > 1) {
+    const unsigned merge = static_cast<unsigned>((p.a.rows * p.a.hq + kWaves - 1) / kWaves);
+    hipLaunchKernelGGL((decode8_merge_kernel<T, D>), dim3(merge), dim3(64 * kWaves), 0, stream, p);
+  }
 }
 
 template <typename T>
@@ -422,37 +402,42 @@ int heads_a_wave(const Attn8Args& a, int64_t splits) {
 }  // namespace
 
 bool decode8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page) {
-  const int64_t G = hkv > 0 ? hq / hkv : 0;
-  return (d == 64 || d == 128 || d == 256) && page % kUnit == 0 && (G == 1 || G == 2);
+  return (d == 64 || d == 128 || d == 256) && page % kUnit == 0 && hkv > 0 && hq > 0;
 }
 
-int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t d) {
+int split_base(int64_t hq, int64_t hkv) { return hq <= 2 * hkv ? kParts * kUnit : kMfmaSplit; }
+
+int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t hkv, int64_t d) {
   int per, ns;
-  split_plan(max_len, &per, &ns);
+  decode8_split_plan(max_len, split_base(hq, hkv), &per, &ns);
   return ns > 1 ? rows * ns * hq * (d + 2) * 4 : 0;
 }
 
 bool decode8_layout(const Attn8Args& a) {
-  auto rows16 = [](const void* x) { return aligned16(x); };
-  return decode8_shape(a.hq, a.hkv, a.d, a.page) && a.kv_dim == 1 && rows16(a.k) && rows16(a.v) && a.kv_head % 16 == 0 &&
-         a.kv_token % 16 == 0 && a.kv_block % 16 == 0 && a.kv_token < (int64_t(1) << 24) && a.kv_head < (int64_t(1) << 24);
+  auto near = [](int64_t x) { return x >= 0 && x < (int64_t(1) << 24) && x % 16 == 0; };
+  return decode8_shape(a.hq, a.hkv, a.d, a.page) && a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && near(a.kv_head) &&
+         near(a.kv_token) && a.kv_block % 16 == 0;
 }
 
 int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, const char* name) {
   Decode8Args p{};
   p.a = a;
+  p.base = split_base(a.hq, a.hkv);
+  const bool mfma = a.hq > 2 * a.hkv;
   int per;
-  split_plan(a.max_len, &per, &p.splits);
-  p.hpw = heads_a_wave(a, p.splits);
-  const int64_t items = a.rows * (a.hkv / p.hpw);
+  decode8_split_plan(a.max_len, p.base, &per, &p.splits);
+  p.hpw = mfma ? 1 : heads_a_wave(a, p.splits);
+  const int64_t columns = mfma ? (a.hq / a.hkv + 15) / 16 : 1;
+  const int64_t items = a.rows * (a.hkv / p.hpw) * columns;
   p.split_slots = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.splits, kMaxGrid / items)));
-  p.xcd = a.hkv / p.hpw * p.split_slots % kXcds == 0;
+  p.xcd = a.hkv / p.hpw * columns * p.split_slots % kXcds == 0;
   const int es = dtype_size(dtype);
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
   p.ws_acc = static_cast<float*>(ws);
   p.ws_ml = reinterpret_cast<float2*>(p.ws_acc + a.rows * p.splits * a.hq * a.d);
+  if (items * p.split_slots > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const unsigned grid = static_cast<unsigned>(items * p.split_slots);
-
+  if (mfma) launch_decode8_mfma(p, dtype, stream);
   switch (dtype) {
     case RLT_BFLOAT16: launch_type<bf16>(p, grid, stream); break;
     case RLT_FLOAT16: launch_type<f16>(p, grid, stream); break;
