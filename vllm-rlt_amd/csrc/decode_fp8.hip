@@ -364,22 +364,20 @@ void launch_shape(const Decode8Args& p, unsigned grid, hipStream_t stream) {
   }
 }
 
-template <typename T, int D>
-void launch_group(const Decode8Args& p, unsigned grid, hipStream_t stream) {
-  if (p.a.hq == p.a.hkv) launch_shape<T, D, 1>(p, grid, stream);
-  else if (p.a.hq == 2 * p.a.hkv) launch_shape<T, D, 2>(p, grid, stream);
-  if (p.splits > 1) {
-    const unsigned merge = static_cast<unsigned>((p.a.rows * p.a.hq + kWaves - 1) / kWaves);
-    hipLaunchKernelGGL((decode8_merge_kernel<T, D>), dim3(merge), dim3(64 * kWaves), 0, stream, p);
-  }
+template <typename T>
+void launch_type(const Decode8Args& p, unsigned grid, hipStream_t stream) {
+  if (p.a.d == 128) launch_shape<T, 128, 1>(p, grid, stream);
+  else if (p.a.hq == p.a.hkv) launch_shape<T, 64, 1>(p, grid, stream);
+  else launch_shape<T, 64, 2>(p, grid, stream);
 }
 
 template <typename T>
-void launch_type(const Decode8Args& p, unsigned grid, hipStream_t stream) {
+void launch_merge(const Decode8Args& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((p.a.rows * p.a.hq + kWaves - 1) / kWaves)), block(64 * kWaves);
   switch (p.a.d) {
-    case 64: launch_group<T, 64>(p, grid, stream); break;
-    case 128: launch_group<T, 128>(p, grid, stream); break;
-    default: launch_group<T, 256>(p, grid, stream); break;
+    case 64: hipLaunchKernelGGL((decode8_merge_kernel<T, 64>), grid, block, 0, stream, p); break;
+    case 128: hipLaunchKernelGGL((decode8_merge_kernel<T, 128>), grid, block, 0, stream, p); break;
+    default: hipLaunchKernelGGL((decode8_merge_kernel<T, 256>), grid, block, 0, stream, p); break;
   }
 }
 
@@ -405,11 +403,17 @@ bool decode8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page) {
   return (d == 64 || d == 128 || d == 256) && page % kUnit == 0 && hkv > 0 && hq > 0;
 }
 
-int split_base(int64_t hq, int64_t hkv) { return hq <= 2 * hkv ? kParts * kUnit : kMfmaSplit; }
+// Which kernel: two heads on the vector units need twice the registers and products, and
+// pay only where a head's 64-byte rows keep the matrix-core kernel's loads short.  Measured,
+// us, vector units / matrix cores, 64 rows of 512-4096 tokens: 16 + 8 heads x 128 115 / 75,
+// x 64 57 / 66, 8 + 4 x 256 281 / 77; one head a KV head 8 x 256 208 / 129, 16 x 128 126 /
+// 139, 16 x 64 65 / 122.
+bool on_matrix_cores(int64_t hq, int64_t hkv, int64_t d) { return hq > 2 * hkv || d == 256 || (d == 128 && hq > hkv); }
+int split_base(int64_t hq, int64_t hkv, int64_t d) { return on_matrix_cores(hq, hkv, d) ? kMfmaSplit : kParts * kUnit; }
 
 int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t hkv, int64_t d) {
   int per, ns;
-  decode8_split_plan(max_len, split_base(hq, hkv), &per, &ns);
+  decode8_split_plan(max_len, split_base(hq, hkv, d), &per, &ns);
   return ns > 1 ? rows * ns * hq * (d + 2) * 4 : 0;
 }
 
@@ -422,8 +426,8 @@ bool decode8_layout(const Attn8Args& a) {
 int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, const char* name) {
   Decode8Args p{};
   p.a = a;
-  p.base = split_base(a.hq, a.hkv);
-  const bool mfma = a.hq > 2 * a.hkv;
+  p.base = split_base(a.hq, a.hkv, a.d);
+  const bool mfma = on_matrix_cores(a.hq, a.hkv, a.d);
   int per;
   decode8_split_plan(a.max_len, p.base, &per, &p.splits);
   p.hpw = mfma ? 1 : heads_a_wave(a, p.splits);
@@ -437,11 +441,21 @@ int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, 
   p.ws_ml = reinterpret_cast<float2*>(p.ws_acc + a.rows * p.splits * a.hq * a.d);
   if (items * p.split_slots > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const unsigned grid = static_cast<unsigned>(items * p.split_slots);
-  if (mfma) launch_decode8_mfma(p, dtype, stream);
-  switch (dtype) {
-    case RLT_BFLOAT16: launch_type<bf16>(p, grid, stream); break;
-    case RLT_FLOAT16: launch_type<f16>(p, grid, stream); break;
-    default: launch_type<float>(p, grid, stream); break;
+  if (mfma) {
+    launch_decode8_mfma(p, dtype, stream);
+  } else {
+    switch (dtype) {
+      case RLT_BFLOAT16: launch_type<bf16>(p, grid, stream); break;
+      case RLT_FLOAT16: launch_type<f16>(p, grid, stream); break;
+      default: launch_type<float>(p, grid, stream); break;
+    }
+  }
+  if (p.splits > 1) {
+    switch (dtype) {
+      case RLT_BFLOAT16: launch_merge<bf16>(p, stream); break;
+      case RLT_FLOAT16: launch_merge<f16>(p, stream); break;
+      default: launch_merge<float>(p, stream); break;
+    }
   }
   return check_launch(name);
 }

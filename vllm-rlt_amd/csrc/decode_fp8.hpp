@@ -1,6 +1,6 @@
 // Decode over the 8-bit cache, shared between its entry point (attention_fp8.hip)
-// and its kernels (decode_fp8.hip: one or two query heads a KV head on the vector
-// units, and the merge; decode_mfma_fp8.hip: more on the matrix cores).
+// and its kernels (decode_fp8.hip: few and short heads on the vector units, and the
+// merge; decode_mfma_fp8.hip: the others on the matrix cores).
 #pragma once
 
 #include <algorithm>

@@ -100,73 +100,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
   const uint32_t token_bytes = static_cast<uint32_t>(a.kv_token);
   uint8_t* const k_lds = lds[wave];
   uint8_t* const v_lds = lds[wave] + kTile * ROW;
-
-  // q's parts, B operands: lane (col, j) holds dims [128 c + 32 j, + 32) of query head c0 +
-  // col; for bf16, 8 of them a k-step.
-  i32x8 qb[NQ][KS];
-  u32x4 qw[NQ][4 * KS];
-  int q_scale[NQ];
-  {
-    const T* qrow = static_cast<const T*>(a.q) + r * a.q_row + (h * G + c0 + min(col, live - 1)) * a.q_head;
-    float y[KS][32];
-    float amax = 0.f;
-#pragma unroll
-    for (int c = 0; c < KS; ++c) {
-      const int d0 = 128 * c + 32 * j;
-      const bool in = d0 < D;
-      if (p.q_vec) {
-        constexpr int N = Packet<T>::N;
-#pragma unroll
-        for (int i = 0; i < 32 / N; ++i)
-          Packet<T>::unpack(in ? *reinterpret_cast<const u32x4*>(qrow + d0 + i * N) : u32x4{0u, 0u, 0u, 0u}, &y[c][i * N]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) y[c][i] = in ? load_elem(qrow + (d0 + i) * a.q_dim) : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) amax = fmaxf(amax, finite_abs(y[c][i]));
-    }
-    if constexpr (WIDE) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int c = 0; c < KS; ++c)
-#pragma unroll
-          for (int w = 0; w < 16; ++w) {
-            const uint32_t lo = __float_as_uint(y[c][2 * w]), hi = __float_as_uint(y[c][2 * w + 1]);
-            qw[n][4 * c + w / 4][w % 4] = lo >> 16 | (hi & 0xffff0000u);
-            y[c][2 * w] -= __uint_as_float(lo & 0xffff0000u);
-            y[c][2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
-          }
-    } else {
-      amax = strided_max<16>(amax);
-      const uint32_t b = max(scale_byte(amax), 4u * NQ);
-      const float inv = inverse_scale(b);
-#pragma unroll
-      for (int c = 0; c < KS; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          y[c][i] = (__float_as_uint(y[c][i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : y[c][i] * inv;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        q_scale[n] = static_cast<int>(b) - 4 * n;
-#pragma unroll
-        for (int c = 0; c < KS; ++c)
-#pragma unroll
-          for (int w = 0; w < 8; ++w) {
-            float* z = &y[c][4 * w];
-            int word = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-            word = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], word, true);
-            qb[n][c][w] = word;
-            if (n + 1 < NQ) {
-              const f32x2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
-              z[0] = (z[0] - lo[0]) * 16.f, z[1] = (z[1] - lo[1]) * 16.f;
-              z[2] = (z[2] - hi[0]) * 16.f, z[3] = (z[3] - hi[1]) * 16.f;
-            }
-          }
-      }
-    }
-  }
+  static_assert(16 * (D + 4) * 4 <= sizeof(lds), "q as fp32 fits the tiles' rows");
+  float(*const q_lds)[D + 4] = reinterpret_cast<float(*)[D + 4]>(lds[0]);
 
   for (int sp = gi / heads; sp < ns; sp += p.split_slots) {
     const int quarter = split_len / kWaves;
@@ -176,34 +111,114 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
     for (int c = 0; c < DT; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    for (int n0 = 0; n0 < n; n0 += 1024) {  // 64 units of 16 tokens, one a lane
-      const int left = min(n - n0, 1024);
-      const int last_unit = (left - 1) / 16;
+    int left = 0, last_unit = 0;  // of the chunk: 64 units of 16 tokens, one a lane
+    int64_t unit_kv = 0, unit_s = 0;
+    u32x4 k[NI], v[NI];
+    uint32_t kb = 0, vb = 0;
+    auto load_units = [&](int n0) __attribute__((always_inline)) {
+      left = min(n - n0, 1024);
+      last_unit = (left - 1) / 16;
       const int tok = t0 + n0 + 16 * min(lane, last_unit);
       const int page = tok / a.page, slot = tok - page * a.page;
       const int64_t blk = block_of(a, trow[page]);
-      const int64_t unit_kv = blk * a.kv_block + slot * a.kv_token;
-      const int64_t unit_s = blk * a.s_block + slot * a.s_token;
-      u32x4 k[NI], v[NI];
-      uint32_t kb, vb;
-      // Tokens past the end re-read the last one: in bounds, and masked below.
-      auto load_tile = [&](int tile) __attribute__((always_inline)) {
+      unit_kv = blk * a.kv_block + slot * a.kv_token;
+      unit_s = blk * a.s_block + slot * a.s_token;
+    };
+    // Tokens past the end re-read the last one: in bounds, and masked below.
+    auto load_tile = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int first = tile * kTile + i * TPI;  // the instruction's tokens lie in one unit
-          const int at = min(first + st, left - 1);
-          const int64_t off = __shfl(unit_kv, min(first / 16, last_unit), 64) +
-                              __umul24(static_cast<uint32_t>(at - min(first / 16, last_unit) * 16), token_bytes);
-          k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + off));
-          v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + off));
-        }
-        const int at = min(tile * kTile + (lane & (kTile - 1)), left - 1);
-        const int64_t off = __shfl(unit_s, at / 16, 64) + at % 16 * a.s_token;
-        kb = ksh[off];
-        vb = vsh[off];
-      };
-      const int tiles = (left + kTile - 1) / kTile;
+      for (int i = 0; i < NI; ++i) {
+        const int first = tile * kTile + i * TPI;  // the instruction's tokens lie in one unit
+        const int at = min(first + st, left - 1);
+        const int64_t off = __shfl(unit_kv, min(first / 16, last_unit), 64) +
+                            __umul24(static_cast<uint32_t>(at - min(first / 16, last_unit) * 16), token_bytes);
+        k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + off));
+        v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + off));
+      }
+      const int at = min(tile * kTile + (lane & (kTile - 1)), left - 1);
+      const int64_t off = __shfl(unit_s, at / 16, 64) + at % 16 * a.s_token;
+      kb = ksh[off];
+      vb = vsh[off];
+    };
+    if (n > 0) {  // the first tile's loads go out before q is worked on
+      load_units(0);
       load_tile(0);
+    }
+    // q's parts, B operands: lane (col, j) holds dims [128 c + 32 j, + 32) of query head c0 +
+    // col; for bf16, 8 of them a k-step.
+    i32x8 qb[NQ][KS];
+    u32x4 qw[NQ][4 * KS];
+    int q_scale[NQ];
+    {
+      // Through the tiles' LDS as fp32, whatever its strides.
+#pragma unroll 1
+      for (int o = threadIdx.x; o < live * D; o += 64 * kWaves)
+        q_lds[o / D][o % D] = load_elem(static_cast<const T*>(a.q) + r * a.q_row + (h * G + c0 + o / D) * a.q_head + o % D * a.q_dim);
+      __syncthreads();
+      float y[KS][32];
+      float amax = 0.f;
+#pragma unroll
+      for (int c = 0; c < KS; ++c) {
+        const int d0 = 128 * c + 32 * j;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const f32x4 z = *reinterpret_cast<const f32x4*>(&q_lds[min(col, live - 1)][(d0 < D ? d0 : 0) + 4 * i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[c][4 * i + e] = d0 < D ? z[e] : 0.f;
+            amax = fmaxf(amax, finite_abs(y[c][4 * i + e]));
+          }
+        }
+      }
+      __syncthreads();
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int c = 0; c < KS; ++c)
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+              const uint32_t lo = __float_as_uint(y[c][2 * w]), hi = __float_as_uint(y[c][2 * w + 1]);
+              qw[n][4 * c + w / 4][w % 4] = lo >> 16 | (hi & 0xffff0000u);
+              y[c][2 * w] -= __uint_as_float(lo & 0xffff0000u);
+              y[c][2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
+            }
+      } else {
+        amax = strided_max<16>(amax);
+        const uint32_t b = max(scale_byte(amax), 4u * NQ);
+        const float inv = inverse_scale(b);
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            y[c][i] = (__float_as_uint(y[c][i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : y[c][i] * inv;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          q_scale[n] = static_cast<int>(b) - 4 * n;
+#pragma unroll
+          for (int c = 0; c < KS; ++c)
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+              float* z = &y[c][4 * w];
+              int word = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+              word = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], word, true);
+              qb[n][c][w] = word;
+              if (n + 1 < NQ) {
+                const f32x2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
+                z[0] = (z[0] - lo[0]) * 16.f, z[1] = (z[1] - lo[1]) * 16.f;
+                z[2] = (z[2] - hi[0]) * 16.f, z[3] = (z[3] - hi[1]) * 16.f;
+              }
+            }
+        }
+      }
+    }
+
+    for (int n0 = 0; n0 < n; n0 += 1024) {
+      if (n0) {
+        load_units(n0);
+        load_tile(0);
+      }
+      const int tiles = (left + kTile - 1) / kTile;
 #pragma unroll 1
       for (int tile = 0; tile < tiles; ++tile) {
 #pragma unroll
