@@ -112,6 +112,14 @@ def test_a_row_depends_on_itself_only(hq, hkv, d):
     assert torch.equal(many, together.repeat(60, 1, 1))
 
 
+@pytest.mark.parametrize("hq,hkv,d,lengths", [(1, 1, 64, [16384, 16400, 8200, 300]), (4, 1, 64, [32768, 32784, 16500, 16384, 600])])
+def test_rows_cut_into_more_splits_than_the_longest(hq, hkv, d, lengths):
+    # A row just past 64 splits has half as many, twice as long.
+    print(f"[decode8] {lengths}", flush=True)
+    c = Case(lengths, hq, hkv, d, seed=8)
+    c.check(c.decode())
+
+
 def strided(t, how):
     if how == "heads first":
         return torch.empty(t.shape[1], t.shape[0], t.shape[2], dtype=t.dtype, device="cuda").transpose(0, 1).copy_(t)

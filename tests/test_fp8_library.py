@@ -129,3 +129,12 @@ def test_host_tensors_are_refused():
     ):
         with pytest.raises(ValueError, match="ROCm device"):
             call()
+
+
+def test_the_decode_workspace_holds_the_splits_of_shorter_rows():
+    # 64 splits of 256 (512 on the matrix cores) keys in a row of 16384 (32768); a row of one page more has 33.
+    lib, _ = library()
+    for heads, page_keys in (((1, 1), 256), ((4, 1), 512)):
+        for pages in (64 * page_keys // 16, 64 * page_keys // 16 + 1, 64 * page_keys // 16 + 1000):
+            assert lib.rlt_paged_decode_fp8_workspace_bytes(1, pages, *heads, 64, 16) >= 64 * heads[0] * (64 + 2) * 4
+        assert lib.rlt_paged_decode_fp8_workspace_bytes(1, page_keys // 16, *heads, 64, 16) == 0

@@ -412,8 +412,7 @@ bool on_matrix_cores(int64_t hq, int64_t hkv, int64_t d) { return hq > 2 * hkv |
 int split_base(int64_t hq, int64_t hkv, int64_t d) { return on_matrix_cores(hq, hkv, d) ? kMfmaSplit : kParts * kUnit; }
 
 int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t hkv, int64_t d) {
-  int per, ns;
-  decode8_split_plan(max_len, split_base(hq, hkv, d), &per, &ns);
+  const int64_t ns = decode8_most_splits(max_len, split_base(hq, hkv, d));
   return ns > 1 ? rows * ns * hq * (d + 2) * 4 : 0;
 }
 
@@ -428,8 +427,7 @@ int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, 
   p.a = a;
   p.base = split_base(a.hq, a.hkv, a.d);
   const bool mfma = on_matrix_cores(a.hq, a.hkv, a.d);
-  int per;
-  decode8_split_plan(a.max_len, p.base, &per, &p.splits);
+  p.splits = decode8_most_splits(a.max_len, p.base);
   p.hpw = mfma ? 1 : heads_a_wave(a, p.splits);
   const int64_t columns = mfma ? (a.hq / a.hkv + 15) / 16 : 1;
   const int64_t items = a.rows * (a.hkv / p.hpw) * columns;

@@ -19,13 +19,18 @@ __host__ __device__ inline void decode8_split_plan(int64_t len, int base, int* s
   *split_len = static_cast<int>(per);
   *nsplit = static_cast<int>(len > 0 ? (len + per - 1) / per : 1);
 }
+// The most splits that a row of up to max_len keys has: not those of max_len itself, whose
+// splits may be twice as long as a shorter row's.
+inline int decode8_most_splits(int64_t max_len, int base) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kDecode8MaxSplits, (max_len + base - 1) / base)));
+}
 
 struct Decode8Args {
   Attn8Args a;
   float* ws_acc;   // [rows][hkv][splits][G][D]
   float2* ws_ml;   // [rows][hkv][splits][G], max in log2 units and sum
   int base;        // tokens of a split (decode8_split_plan)
-  int splits;      // splits a row of the tables' width has
+  int splits;      // most splits of a row inside the tables' width
   int split_slots; // split-dimension workgroups launched; each walks every split_slots-th split
   int hpw;         // heads a wave
   int xcd;         // workgroups of one (split, head block) of all rows share an XCD
