@@ -374,6 +374,8 @@ def test_refusals():
             (dict(lens=c.lens[:1]), "one entry"),
             (dict(out=c.q.float()), "out must match"),
             (dict(kc=kc.cpu()), "same ROCm device"),
+            (dict(kc=kc[:, :, :0], vc=vc[:, :, :0], ks=ks[:, :, :0], vs=vs[:, :, :0]), "positive multiple"),
+            (dict(kc=kc[:, :0], vc=vc[:, :0], ks=ks[:, :0], vs=vs[:, :0]), "page_size"),
         ]:
             with pytest.raises(ValueError, match=match):
                 call(**kw)

@@ -138,3 +138,10 @@ def test_the_decode_workspace_holds_the_splits_of_shorter_rows():
         for pages in (64 * page_keys // 16, 64 * page_keys // 16 + 1, 64 * page_keys // 16 + 1000):
             assert lib.rlt_paged_decode_fp8_workspace_bytes(1, pages, *heads, 64, 16) >= 64 * heads[0] * (64 + 2) * 4
         assert lib.rlt_paged_decode_fp8_workspace_bytes(1, page_keys // 16, *heads, 64, 16) == 0
+
+
+def test_a_page_of_no_tokens_is_refused():
+    lib, native = library()
+    for page in (0, -16):
+        assert lib.rlt_paged_decode_fp8_workspace_bytes(1, 4, 2, 2, 128, page) == 0
+        assert lib.rlt_paged_prefill_fp8_workspace_bytes(1, 1, 4, 2, 2, 128, page) == 0

@@ -400,7 +400,7 @@ int heads_a_wave(const Attn8Args& a, int64_t splits) {
 }  // namespace
 
 bool decode8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page) {
-  return (d == 64 || d == 128 || d == 256) && page % kUnit == 0 && hkv > 0 && hq > 0;
+  return (d == 64 || d == 128 || d == 256) && page > 0 && page % kUnit == 0 && hkv > 0 && hq > 0;
 }
 
 // Which kernel: two heads on the vector units need twice the registers and products, and

@@ -1168,7 +1168,7 @@ def rope_axes_kv_append(
         raise ValueError(f"the caches must use q's dtype {q.dtype}, or 8 bits with their scales")
     nb, nl, page, hkv, d = key_cache.shape
     rows = q.shape[0]
-    if q.ndim != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % hkv:
+    if q.ndim != 3 or q.shape[2] != d or hkv == 0 or q.shape[1] == 0 or q.shape[1] % hkv:
         raise ValueError(f"q must have shape [batch, heads, {d}] with heads a positive multiple of {hkv}")
     for t, name in ((k, "k"), (v, "v")):
         if t.shape != (rows, hkv, d):
@@ -1215,7 +1215,7 @@ def _fp8_attention_inputs(q, key_cache, value_cache, key_scales, value_scales, b
     hkv, d = key_cache.shape[2:]
     if q.ndim != 3 or q.shape[2] != d:
         raise ValueError(f"q must have shape [rows, heads, {d}]")
-    if q.shape[1] == 0 or q.shape[1] % hkv:
+    if hkv == 0 or q.shape[1] == 0 or q.shape[1] % hkv:
         raise ValueError("query heads must be a positive multiple of KV heads")
     if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.stride(1) != 1:
         raise ValueError("block_tables must be int32 [sequences, width] with contiguous rows")
