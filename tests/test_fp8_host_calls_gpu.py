@@ -121,6 +121,9 @@ def test_errors_are_the_same(path):
         c.decode(out=c.q[:3])
     with pytest.raises(ValueError, match="workspace"):
         c.decode(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    for call in (c.decode, c.prefill):  # numbers one above the other, the memory of one
+        with pytest.raises(ValueError, match="workspace"):
+            call(workspace=torch.empty(1, dtype=torch.uint8, device="cuda").expand(1 << 24))
     c.lens = c.lens.long()
     with pytest.raises(ValueError, match="context_lengths"):
         c.prefill()

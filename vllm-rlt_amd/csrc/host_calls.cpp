@@ -322,14 +322,15 @@ bool attention8(const at::Tensor* const* in) {
          tables.dim() == 2 && tables.stride(1) == 1 && tables.size(0) > 0 && ints(lens, at::kInt) && lens.size(0) == tables.size(0);
 }
 
-// The workspace given in o if it holds need bytes on q's device, a new one for None.
+// The workspace given in o if it holds need contiguous bytes on q's device, a new one for None.
 bool workspace_of(PyObject* o, int64_t need, const at::Tensor& q, at::Tensor* ws) {
   if (o == Py_None) {
     *ws = at::empty({need}, q.options().dtype(at::kByte));
     return true;
   }
   const at::Tensor* w = plain(o);
-  if (!w || w->device() != q.device() || w->numel() * static_cast<int64_t>(w->element_size()) < need) return false;
+  if (!w || w->device() != q.device() || !w->is_contiguous() || w->numel() * static_cast<int64_t>(w->element_size()) < need)
+    return false;
   *ws = *w;
   return true;
 }

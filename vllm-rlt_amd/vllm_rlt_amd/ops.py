@@ -1232,8 +1232,8 @@ def _fp8_attention_inputs(q, key_cache, value_cache, key_scales, value_scales, b
 def _workspace_of(need: int, workspace, device):
     if workspace is None:
         return torch.empty(need, dtype=torch.uint8, device=device)
-    if workspace.numel() * workspace.element_size() < need or workspace.device != device:
-        raise ValueError(f"workspace must hold {need} bytes on {device}")
+    if workspace.numel() * workspace.element_size() < need or workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must hold {need} contiguous bytes on {device}")
     return workspace
 
 
