@@ -586,14 +586,14 @@ int rlt_paged_prefill_fp8(const void* q, const int64_t* q_strides, const void* k
  * takes `tokens` new tokens at positions start, start + 1, ... of
  * tables[slot, depth] (plane 0 when planes is 1):
  *   cu_seqlens [size + 1]  int32, running token counts
- *   lengths [size]         int32, start + tokens
+ *   lengths [size]         int32, start + tokens kept
  *   positions, sequences, blocks, offsets [capacity]  int64, per token
  *   out_tables [size, out_width]  int32
  * Sequences count .. size - 1 are padding: no tokens, length 0, a table row of 0.
  * Tokens behind the last sequence get position 0, sequence -1, block -1 (an append
  * skips them).  A descriptor outside the tables keeps its tokens in the packing but
  * gets length 0, a table row of 0 and block -1, position 0; tokens past `capacity`
- * are dropped from the end, in cu_seqlens as well.
+ * are dropped from the end, in cu_seqlens and lengths as well.
  */
 int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t count, int64_t size, const int32_t* tables,
                              int64_t num_slots, int64_t table_width, int64_t planes, int64_t page_size,

@@ -16,9 +16,9 @@ def expected(desc, count, size, tables, page, capacity, width):
         plane = depth if planes > 1 else 0
         valid = (i < count and 0 <= slot < slots and 0 <= plane < planes and start >= 0 and tokens >= 0
                  and start + tokens <= table_width * page)
-        lengths.append(start + tokens if valid else 0)
         first = cu[-1]
         n = min(max(tokens, 0), capacity - first)
+        lengths.append(start + n if valid else 0)
         cu.append(first + n)
         if valid:
             out[i] = tables[slot, plane, :width]

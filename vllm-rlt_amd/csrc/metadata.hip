@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void chunk_metadata_kernel(ChunkMetaArgs 
   const int32_t* src = a.tables + (valid ? (slot * a.planes + plane) * a.table_width : 0);
   if (part == 0 && tid == 0) {
     a.cu[seq] = static_cast<int32_t>(first);
-    a.lengths[seq] = valid ? static_cast<int32_t>(start + asked) : 0;
+    a.lengths[seq] = valid ? static_cast<int32_t>(start + tokens) : 0;
   }
   int32_t* dst = a.out_tables + seq * a.out_stride;
   for (int64_t c = part * kThreads + tid; c < a.out_width; c += parts * kThreads) dst[c] = valid ? src[c] : 0;

@@ -990,7 +990,7 @@ def build_chunk_metadata(
     of every token.  The token buffers share one length, the capacity: tokens
     behind the last sequence get position 0, sequence -1, block -1 and offset 0, so
     an append of the whole buffer skips them; tokens past it are dropped from the
-    end.  Sequences from count on are padding: no tokens, length 0.
+    end, and lengths count the others.  Sequences from count on are padding: no tokens, length 0.
     """
     host, stream = _host_calls_here(tables)
     if host is not None:
