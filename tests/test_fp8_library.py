@@ -35,6 +35,7 @@ def test_append():
     refused(call(d=513), native, "head_dim", native.RLT_EUNSUPPORTED)
     refused(call(scales=None), native, "NULL")
     refused(call(k=None), native, "NULL")
+    refused(call(rows=1 << 26), native, "too many rows", native.RLT_EUNSUPPORTED)
     refused(call(strides=native.int64_array([1, 1, -1, 1, 1])), native, "negative")
     assert call(rows=0) == native.RLT_OK
 
@@ -82,7 +83,8 @@ def test_attention():
         refused(call(d=0), native, "positive")
         refused(call(d=520), native, "head_dim", native.RLT_EUNSUPPORTED)
         refused(call(width=0), native, "positive")
-        refused(call(width=1 << 28), native, "2^31", native.RLT_EUNSUPPORTED)
+        refused(call(width=(1 << 26) + 1), native, "2^30", native.RLT_EUNSUPPORTED)
+        refused(call(rows=1 << 23), native, "too many rows", native.RLT_EUNSUPPORTED)
         refused(call(q=None), native, "NULL")
         assert call(rows=0) == native.RLT_OK
     refused(prefill(cu=None), native, "NULL")
@@ -90,6 +92,16 @@ def test_attention():
     need = lib.rlt_paged_decode_fp8_workspace_bytes(3, 100, 16, 16, 128, 16)
     if need:
         refused(decode(rows=3, hq=16, hkv=16, d=128, width=100, ws_bytes=need - 1), native, "workspace", native.RLT_EWORKSPACE)
+
+
+def test_launches_past_the_largest_grid():
+    lib, native = library()
+    q, kv, sc = (native.int64_array(x) for x in ([4096, 64, 1], [4096, 256, 64, 1], [64, 4, 1]))
+    rows = (1 << 23) - 1
+    refused(lib.rlt_paged_decode_fp8(16, q, 16, 16, kv, 16, 16, sc, 16, 3, 3, 16, 16, q, rows, 64, 4, 64, 16, 4, 1.0, 2, 16, 1 << 60,
+                                     None), native, "too many rows", native.RLT_EUNSUPPORTED)
+    refused(lib.rlt_paged_prefill_fp8(16, q, 16, 16, kv, 16, 16, sc, 16, 3, 3, 16, 16, 1, rows, rows, 16, q, 512, 4, 64, 16, 4, 1.0, 2,
+                                      None, 0, None), native, "too many rows", native.RLT_EUNSUPPORTED)
 
 
 def test_chunk_metadata():
@@ -109,6 +121,7 @@ def test_chunk_metadata():
     refused(call(width=1 << 28), native, "31 bits", native.RLT_EUNSUPPORTED)
     refused(call(desc=None), native, "NULL")
     refused(call(positions=None), native, "NULL")
+    refused(call(size=(1 << 24) - 1), native, "too many sequences", native.RLT_EUNSUPPORTED)
 
 
 def test_host_tensors_are_refused():

@@ -116,9 +116,9 @@ int attention_args(const char* name, const void* q, const int64_t* q_strides, co
   if (d <= 0 || page <= 0 || num_blocks <= 0 || width <= 0 || table_stride < 0)
     return fail(RLT_EINVAL, "%s: head_dim, page_size, num_blocks and the table width must be positive", name);
   if (d > 64 * kPerLane) return fail(RLT_EUNSUPPORTED, "%s: head_dim above %d", name, 64 * kPerLane);
-  if (rows > 0x7fffffff || num_seqs > 0x7fffffff || hq > 65535 || page > 0x7fffffff || num_blocks > 0x7fffffff)
+  if (rows > kMaxRows || num_seqs > 0x7fffffff || hq > 65535 || page > 0x7fffffff || num_blocks > 0x7fffffff)
     return fail(RLT_EUNSUPPORTED, "%s: too many rows, heads, tokens a page or blocks", name);
-  if (width > 0x7fffffff / page) return fail(RLT_EUNSUPPORTED, "%s: the tables cover more than 2^31 tokens", name);
+  if (width > kMaxKeys / page) return fail(RLT_EUNSUPPORTED, "%s: the tables cover more than 2^30 tokens", name);
   if (rows == 0 || num_seqs == 0) return RLT_OK;
   if (!q || !q_strides || !key_cache || !value_cache || !kv_strides || !key_scales || !value_scales ||
       !scale_strides || !tables || !lens || !out || !out_strides)
@@ -166,7 +166,7 @@ using namespace rlt;
 extern "C" int64_t rlt_paged_decode_fp8_workspace_bytes(int64_t n_rows, int64_t max_table_width, int64_t num_q_heads,
                                                         int64_t num_kv_heads, int64_t head_dim, int64_t page_size) {
   if (n_rows <= 0 || max_table_width <= 0 || !decode8_shape(num_q_heads, num_kv_heads, head_dim, page_size) ||
-      max_table_width > 0x7fffffff / page_size)
+      max_table_width > kMaxKeys / page_size)
     return 0;
   return decode8_workspace(n_rows, max_table_width * page_size, num_q_heads, num_kv_heads, head_dim);
 }
@@ -196,7 +196,7 @@ extern "C" int64_t rlt_paged_prefill_fp8_workspace_bytes(int64_t total_q, int64_
                                                          int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
                                                          int64_t page_size) {
   if (total_q <= 0 || num_seqs <= 0 || max_table_width <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
-      !prefill8_shape(head_dim, page_size) || max_table_width > 0x7fffffff / page_size)
+      !prefill8_shape(head_dim, page_size) || max_table_width > kMaxKeys / page_size)
     return 0;
   return prefill8_workspace(total_q, num_seqs, max_table_width * page_size, num_q_heads, head_dim);
 }

@@ -437,7 +437,7 @@ int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, 
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
   p.ws_acc = static_cast<float*>(ws);
   p.ws_ml = reinterpret_cast<float2*>(p.ws_acc + a.rows * p.splits * a.hq * a.d);
-  if (items * p.split_slots > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  if (items * p.split_slots > kMaxBlocks || a.rows * a.hq > kMaxBlocks * kWaves) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const unsigned grid = static_cast<unsigned>(items * p.split_slots);
   if (mfma) {
     launch_decode8_mfma(p, dtype, stream);

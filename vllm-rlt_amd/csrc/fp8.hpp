@@ -66,6 +66,12 @@ __device__ __forceinline__ float group_max(float x) {
   return x;
 }
 
+// Limits of the attention calls: token counts and what is added to them stay inside 31
+// bits, and the threads of a launch (blocks of up to 512) inside 32.
+constexpr int64_t kMaxKeys = int64_t(1) << 30;
+constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
+constexpr int64_t kMaxRows = (int64_t(1) << 23) - 1;
+
 // Arguments of the attention kernels over an 8-bit cache (strides in elements).
 struct Attn8Args {
   const void* q;

@@ -214,7 +214,7 @@ extern "C" int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t coun
     return fail(RLT_EINVAL, "rlt_build_chunk_metadata: need out_width <= table_width and <= out_table_stride");
   if (capacity < 0 || capacity > 0x7fffffff || table_width > 0x7fffffff / page_size)
     return fail(RLT_EUNSUPPORTED, "rlt_build_chunk_metadata: token counts must fit 31 bits");
-  if (size >= 0x7fffffff) return fail(RLT_EUNSUPPORTED, "rlt_build_chunk_metadata: too many sequences");
+  if (size >= (1 << 24) - 1) return fail(RLT_EUNSUPPORTED, "rlt_build_chunk_metadata: too many sequences");
   if (!tables || !cu_seqlens || (size && (!lengths || (out_width && !out_tables))) || (count && !descriptors) ||
       (capacity && (!positions || !sequences || !blocks || !offsets)))
     return fail(RLT_EINVAL, "rlt_build_chunk_metadata: NULL pointer argument");

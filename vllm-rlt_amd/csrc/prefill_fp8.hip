@@ -39,16 +39,10 @@ constexpr int kBN = 64;   // keys a tile
 constexpr float kRescale = 8.f;
 constexpr int kMaxQExp = 24;
 constexpr int kXcds = 8;
-#ifndef TARGET
-#define TARGET 768
-#endif
-#ifndef MINSEG
-#define MINSEG 4
-#endif
-constexpr int kTargetItems = TARGET;
+constexpr int kTargetItems = 768;
 constexpr int kSlots = 512;  // workgroups that run at once: two a CU
-constexpr int kMinSegTiles = MINSEG;
-constexpr int kPlanSeqs = 64;      // sequences ranked and cut: one a lane
+constexpr int kMinSegTiles = 4;
+constexpr int kPlanSeqs = 64;  // sequences ranked and cut: one a lane
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -715,7 +709,7 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   // Query tiles, and the segments past the first (as many items as partial_slots() has such rows).
   const int64_t tiles = a.rows / kBM + std::min<int64_t>(a.num_seqs, a.rows) + (slots ? (kTargetItems + a.hq - 1) / a.hq + 2 : 0);
   const int64_t merge_rows = (a.rows + 3) / 4;
-  if (tiles * a.hq > 0x7fffffff || merge_rows * a.hq > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  if (tiles * a.hq > kMaxBlocks || (slots && merge_rows * a.hq > kMaxBlocks)) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const dim3 grid(static_cast<unsigned>(tiles * a.hq)), merge(static_cast<unsigned>(merge_rows * a.hq)), block(256);
 #define LAUNCH_D(T, D)                                                                                   \
   do {                                                                                                   \
