@@ -438,3 +438,18 @@ def test_prefill_of_a_row_before_the_keys_of_cut_sequences():
     c = Case([1500, 40], 8, 8, 128, seed=2, chunks=[2000, 300])
     c.check(c.prefill())
     assert (c.prefill()[:500] == 0).all()
+
+
+def test_row_ranges_that_overlap_stay_inside_the_workspace():
+    # cu_seqlens must rise; where they do not, no result is promised, but nothing else is written.
+    from vllm_rlt_amd import ops
+
+    c = Case([4096], 1, 1, 64, seed=6, chunks=[1280])
+    tables, lens = c.tables.repeat(64, 1), c.lens.repeat(64)
+    cu = torch.tensor([0, 1280], dtype=torch.int32, device="cuda").repeat(33)[:65].contiguous()
+    need = ops.prefill_fp8_workspace_bytes(1280, 64, tables.shape[1], 1, 1, 64, 16)
+    memory = torch.full((need + (1 << 24),), 7, dtype=torch.uint8, device="cuda")
+    out = torch.full((1280 + 64, 1, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.paged_prefill_fp8(c.q, *c.cache, tables, lens, cu, 1280, out=out[:1280], scale=c.scale, workspace=memory[:need])
+    torch.cuda.synchronize()
+    assert (memory[need:] == 7).all() and (out[1280:] == 3).all()

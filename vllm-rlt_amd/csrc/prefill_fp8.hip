@@ -71,6 +71,7 @@ struct Prefill8Args {
   float* part_acc;    // [slots][hq][D]
   float2* part_ml;    // [slots][hq], max in log2 units and sum
   SeqPlan* plan;      // [kPlanSeqs], for the merge kernel
+  int slots;
   int out_vec;  // 4 elements of an out row can be stored at once
   int q_vec;    // q rows are 16-byte aligned, dims together
 };
@@ -132,8 +133,10 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
       }
       s.segs = max(1, (keys + target - 1) / target);
       s.seg_tiles = (keys + s.segs - 1) / s.segs;
-      const int slots = s.segs > 1 ? s.nq * s.segs : 0;
+      // cu_seqlens that do not rise ask for more slots than there are: those stay whole.
+      const int slots = s.segs > 1 ? static_cast<int>(min(static_cast<int64_t>(s.nq) * s.segs, static_cast<int64_t>(p.slots) + 1)) : 0;
       s.slot0 = scan_sum(slots) - slots;
+      if (s.slot0 + slots > p.slots) s.segs = 1, s.seg_tiles = keys;
     }
   }
   return s;
@@ -692,7 +695,8 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   Prefill8Args p{};
   p.a = a;
   const int64_t slots = ws ? partial_slots(a.rows, a.num_seqs, a.max_len, a.hq) : 0;
-  if (slots > 0x7fffffff) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  if (slots > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);  // 64 sequences' stay inside 31 bits
+  p.slots = static_cast<int>(slots);
   if (slots) {
     p.part_acc = static_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float2*>(p.part_acc + slots * a.hq * a.d);
