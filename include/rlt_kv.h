@@ -504,7 +504,8 @@ int rlt_expand_prefill(const int64_t* positions, const int64_t* sequences,
 
 /*
  * Quantising KV append of one layer: rlt_kv_append to an 8-bit cache.  `dtype` is
- * the type of k and v.  Slots outside the pool are skipped.
+ * the type of k and v.  Slots outside the pool are skipped; the others are distinct
+ * (two rows of one slot would leave codes of one with the scale of the other).
  */
 int rlt_kv_append_fp8(void* key_cache, void* value_cache, const int64_t* cache_strides, void* key_scales,
                       void* value_scales, const int64_t* scale_strides, const void* k, const int64_t* k_strides,
@@ -523,7 +524,8 @@ int rlt_kv_append_fp8(void* key_cache, void* value_cache, const int64_t* cache_s
  * past 2 * half pass through.  q_out[i] for i < n_rows (q_out may be q); rotated k
  * and v go to slot i for i < n_write: quantised into an 8-bit cache when key_scales
  * is given, into a cache of `dtype` when key_scales and value_scales are NULL.  A
- * row with a position outside [0, max_position) gets q_out = 0 and no append.
+ * row with a position outside [0, max_position) gets q_out = 0 and no append.  Slots
+ * are distinct, as for rlt_kv_append_fp8.
  *   positions: device int64, position_strides[2]: row, axis.
  *   table: device fp32 [max_position, half, 2] (cos, sin), contiguous.
  *   axis_of: HOST bytes [half], each below axes.
@@ -560,7 +562,8 @@ int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, const void* ke
  * rlt_paged_prefill over a layer slice of an 8-bit cache: packed chunks, bottom-
  * right causal.  Query row i of sequence s's n_q sees keys 0 .. context_lengths[s]
  * - n_q + i; one that sees none is written as zeros.  Rows of no sequence (at or
- * past cu_seqlens_q[num_seqs]) are left as they were.  The workspace
+ * past cu_seqlens_q[num_seqs]) are left as they were; cu_seqlens_q rises from 0 to at
+ * most total_q.  The workspace
  * (rlt_paged_prefill_fp8_workspace_bytes, on 16 bytes; calls that overlap need one
  * each) holds the partials of long sequences, whose keys are cut by the launch's
  * shapes: a row's last bits may depend on what shares its launch.  With a NULL

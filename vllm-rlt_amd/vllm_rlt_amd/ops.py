@@ -1080,7 +1080,8 @@ def kv_append_fp8(
     torch.float8_e8m0fnu [blocks, layers, page, kv_heads]: a cached value is its
     code times the scale of its (token, head) row, the smallest power of two with
     amax <= 448 * scale over the row's finite values.  Values that are not finite are
-    stored as NaN.  k and v are float32, float16 or bfloat16.
+    stored as NaN.  k and v are float32, float16 or bfloat16; the slots of a call are
+    distinct (rows of one slot would leave a mix), those outside the cache skipped.
     """
     host, stream = _host_calls_here(key_cache)
     if host is not None:
