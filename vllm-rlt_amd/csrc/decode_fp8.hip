@@ -1,19 +1,19 @@
-// Decode over the 8-bit KV cache: one new token a sequence, split over the
-// cache's length and joined.
+// Decode over the 8-bit KV cache: one new token a sequence, split over the cache's
+// length and joined.  Here: which kernel a call takes, the merge of the splits, and the
+// split pass of head_dim 64 with one query head a KV head, on the vector units.
 //
-// A row's keys are cut into splits (decode8_split_plan) and a split into kParts parts of consecutive tokens, a
-// function of the row's length alone.  A part of one head is worked by D/16 lanes in
-// order, with a running maximum and sum of its own; the parts of a split and then
-// the splits are joined in order.  So a row's bits depend neither on its batch nor
-// on how parts are spread over waves.
+// A row's keys are cut into splits (decode8_split_plan), a function of the row's length
+// alone; a split's parts and then the splits are joined in order.  So a row's bits depend
+// neither on its batch nor on how the parts are spread over waves.
 //
-// Bytes bound it: 2 (D + 1) of them a (token, KV head) against 4 D G flops.  A lane
-// owns 16 dims of a (token, head), LPT = D/16 lanes hold one.  A wave works on HPW
-// neighbouring heads of PPI parts at once: a load instruction moves HPW * D
-// contiguous bytes of PPI tokens.  After LPT instructions (a tile, 64 (token, head)
-// rows) a reduce-scatter leaves one row's score in every lane, which does one row's
-// softmax.  Wide waves read longest runs of memory; narrow ones, of more parts,
-// give a small launch more waves.
+// The split pass here.  A split is kParts parts of consecutive tokens, each worked by 4
+// lanes a head in order, with a running maximum and sum of its own.  Bytes bound it: 2 (D +
+// 1) of them a (token, head) against 4 D flops.  A lane owns 16 dims of a (token, head).  A
+// wave works on HPW neighbouring heads of PPI parts at once: a load instruction moves HPW *
+// 64 contiguous bytes of PPI tokens.  After 4 instructions (a tile, 64 (token, head) rows) a
+// reduce-scatter leaves one row's score in every lane, which does one row's softmax.  Wide
+// waves read the longest runs of memory; narrow ones, of more parts, give a small launch
+// more waves.  Measured (16 heads, bf16): 256 rows of 1024-8192 tokens 434 us, 5.65 TB/s.
 #include <type_traits>
 
 #include "decode_fp8.hpp"
@@ -42,26 +42,9 @@ __device__ __forceinline__ void unpack_codes(const u32x4 w, float* x) {
   }
 }
 
-// Sum over the LPT lanes of a group of LPT values at once: lane s of the group ends
-// with the sum of value s.  Every step halves the values a lane still carries.
-template <int LPT>
-__device__ __forceinline__ float reduce_scatter(float (&x)[LPT], int s) {
-  if constexpr (LPT >= 16) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool up = s & 8;
-      const float keep = up ? x[i + 8] : x[i], send = up ? x[i] : x[i + 8];
-      x[i] = keep + __shfl_xor(send, 8, 64);
-    }
-  }
-  if constexpr (LPT >= 8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool up = s & 4;
-      const float keep = up ? x[i + 4] : x[i], send = up ? x[i] : x[i + 4];
-      x[i] = keep + __shfl_xor(send, 4, 64);
-    }
-  }
+// Sum over the 4 lanes of a group of 4 values at once: lane s of the group ends with the
+// sum of value s.  Every step halves the values a lane still carries.
+__device__ __forceinline__ float reduce_scatter(float (&x)[4], int s) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const bool up = s & 2;
@@ -73,28 +56,29 @@ __device__ __forceinline__ float reduce_scatter(float (&x)[LPT], int s) {
   return keep + dpp<kDppXor1>(send);
 }
 
-template <typename T, int D, int G, int HPW, int W>
+template <typename T, int HPW, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void decode8_split_kernel(Decode8Args p) {
-  constexpr int LPT = D / 16;              // lanes a (token, head), and tokens (load instructions) a tile
+  constexpr int D = 64, LPT = D / 16;      // lanes a (token, head), and tokens (load instructions) a tile
   constexpr int PPI = 64 / (LPT * HPW);    // parts a wave works on at once
   constexpr int PPW = kParts / (W * PPI);  // parts a group of lanes works through
   constexpr int TPU = kUnit / LPT;         // tiles a unit
   static_assert(LPT * HPW * PPI == 64 && PPW * W * PPI == kParts && TPU * LPT == kUnit, "whole groups, parts and tiles");
-  __shared__ __align__(16) float part[kParts][HPW][G][D];
-  __shared__ float2 part_ml[kParts][HPW][G];
+  __shared__ __align__(16) float part[kParts][HPW][D];
+  __shared__ float2 part_ml[kParts][HPW];
 
   const Attn8Args& a = p.a;
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
   const uint32_t rows = static_cast<uint32_t>(a.rows), x = blockIdx.x % kXcds, t = blockIdx.x / kXcds;
-  const uint32_t blocks = a.hkv / HPW, groups = blocks * p.split_slots;
+  const uint32_t blocks = a.hkv / HPW;
   uint32_t gi, r;
-  if (p.xcd) {  // workgroup b runs on XCD b % 8: all rows of a (split, head block) on one XCD, back to back
-    gi = t / rows * kXcds + x;
-    r = t % rows;
+  if (p.xcd) {  // workgroup b runs on XCD b % 8: the heads of a (split, row) on one XCD, back to back
+    const uint32_t item = t / blocks * kXcds + x;
+    gi = item / rows * blocks + t % blocks;
+    r = (item + item / rows) % rows;  // a row's splits on different ones
   } else {
-    gi = blockIdx.x % groups;
-    r = blockIdx.x / groups;
+    gi = blockIdx.x / rows;
+    r = blockIdx.x % rows;
   }
   gi = uniform(gi), r = uniform(r);
   const int h0 = gi % blocks * HPW;
@@ -131,28 +115,24 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
       return sp * split_len + wave_tok + static_cast<int>((step >> unit_shift) * PPI + gp) * part_len +
              static_cast<int>(step & (units - 1)) * kUnit;
     };
-    float q[G][16], acc[G][16], m[G], l[G];
+    float q[16], acc[16], m = -INFINITY, l = 0.f;
     if (!p.q_vec) {  // any strides: through LDS, a few elements a thread
 #pragma unroll 1
-      for (int o = threadIdx.x; o < HPW * G * D; o += 64 * W)
-        (&part[0][0][0][0])[o] = load_elem(static_cast<const T*>(a.q) + r * a.q_row + (h0 * G + o / D) * a.q_head + o % D * a.q_dim);
+      for (int o = threadIdx.x; o < HPW * D; o += 64 * W)
+        (&part[0][0][0])[o] = load_elem(static_cast<const T*>(a.q) + r * a.q_row + (h0 + o / D) * a.q_head + o % D * a.q_dim);
       __syncthreads();
     }
+    if (p.q_vec) {
+      const T* qrow = static_cast<const T*>(a.q) + r * a.q_row + (h0 + gh) * a.q_head + 16 * s;
+      constexpr int N = Packet<T>::N;
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      if (p.q_vec) {
-        const T* qrow = static_cast<const T*>(a.q) + r * a.q_row + ((h0 + gh) * G + j) * a.q_head + 16 * s;
-        constexpr int N = Packet<T>::N;
+      for (int c = 0; c < 16 / N; ++c) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + c * N), &q[c * N]);
+    } else {
 #pragma unroll
-        for (int c = 0; c < 16 / N; ++c) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + c * N), &q[j][c * N]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) q[j][e] = part[0][0][0][(gh * G + j) * D + 16 * s + e];
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) q[j][e] *= a.qscale, acc[j][e] = 0.f;
-      m[j] = -INFINITY, l[j] = 0.f;
+      for (int e = 0; e < 16; ++e) q[e] = part[0][0][gh * D + 16 * s + e];
     }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) q[e] *= a.qscale, acc[e] = 0.f;
     if (!p.q_vec) __syncthreads();
 
     if (tiles > 0) {
@@ -192,18 +172,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
       };
       auto step = [&](uint32_t tile, auto more) __attribute__((always_inline)) {
         constexpr bool MORE = decltype(more)::value;  // another tile follows
-        float score[G][LPT];
+        float score[LPT];
 #pragma unroll
         for (int i = 0; i < LPT; ++i) {
           float y[16];
           unpack_codes(k[i], y);
+          score[i] = q[0] * y[0];
 #pragma unroll
-          for (int j = 0; j < G; ++j) {
-            float dot = q[j][0] * y[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) dot = fmaf(q[j][e], y[e], dot);
-            score[j][i] = dot;
-          }
+          for (int e = 1; e < 16; ++e) score[i] = fmaf(q[e], y[e], score[i]);
           __builtin_amdgcn_sched_barrier(0);
         }
         const float sk = scale_value(kb), sv = scale_value(vb), bias = value_bias(vb);
@@ -214,31 +190,24 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
           issue(tile + 1, kh, k);
           __builtin_amdgcn_sched_barrier(0);
         }
-        float pv[G];  // this lane's row: its probability times its V scale
+        const float sum = reduce_scatter(score, s) * sk;
+        const float dot = in ? sum : -INFINITY;
+        const float top = fmaxf(m, group_max<LPT>(dot + bias));
+        const float base = top == -INFINITY ? 0.f : top;  // only -inf scores so far: they weigh 0
+        const float corr = fast_exp2(m - base);
+        const float w = fast_exp2(dot - base);
+        m = top;
+        l = fmaf(l, corr, w);
+        const float pv = w * sv;  // this lane's row: its probability times its V scale
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-          const float sum = reduce_scatter<LPT>(score[j], s) * sk;
-          const float dot = in ? sum : -INFINITY;
-          const float top = fmaxf(m[j], group_max<LPT>(dot + bias));
-          const float base = top == -INFINITY ? 0.f : top;  // only -inf scores so far: they weigh 0
-          const float corr = fast_exp2(m[j] - base);
-          const float w = fast_exp2(dot - base);
-          m[j] = top;
-          l[j] = fmaf(l[j], corr, w);
-          pv[j] = w * sv;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
-        }
+        for (int e = 0; e < 16; ++e) acc[e] *= corr;
 #pragma unroll
         for (int i = 0; i < LPT; ++i) {
           float y[16];
           unpack_codes(v[i], y);
+          const float wi = __shfl(pv, group0 + i, 64);
 #pragma unroll
-          for (int j = 0; j < G; ++j) {
-            const float w = __shfl(pv[j], group0 + i, 64);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[j][e] = fmaf(w, y[e], acc[j][e]);
-          }
+          for (int e = 0; e < 16; ++e) acc[e] = fmaf(wi, y[e], acc[e]);
           __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (MORE) {
@@ -248,19 +217,16 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
         // The end of a part: its state to LDS.
         if (!MORE || (tile + 1) % (units * TPU) == 0) {
           const int pt = (wave * PPW + static_cast<int>(tile / TPU >> unit_shift)) * PPI + gp;
+          const float sum = group_sum<LPT>(l);
+          if (s == 0) part_ml[pt][gh] = make_float2(m, sum);
 #pragma unroll
-          for (int j = 0; j < G; ++j) {
-            const float sum = group_sum<LPT>(l[j]);
-            if (s == 0) part_ml[pt][gh][j] = make_float2(m[j], sum);
+          for (int c = 0; c < 4; ++c) {
+            u32x4 y;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              u32x4 y;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(acc[j][4 * c + e]), acc[j][4 * c + e] = 0.f;
-              *reinterpret_cast<u32x4*>(&part[pt][gh][j][16 * s + 4 * c]) = y;
-            }
-            m[j] = -INFINITY, l[j] = 0.f;
+            for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(acc[4 * c + e]), acc[4 * c + e] = 0.f;
+            *reinterpret_cast<u32x4*>(&part[pt][gh][16 * s + 4 * c]) = y;
           }
+          m = -INFINITY, l = 0.f;
         }
       };
       find_unit(0);
@@ -275,27 +241,26 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
     // Join the parts that have tokens, in order.
     const int live = (n_split + part_len - 1) / part_len;
 #pragma unroll 1
-    for (int o = threadIdx.x; o < HPW * G * D; o += 64 * W) {
-      const int hd = o / (G * D), j = o / D % G, d = o % D;
+    for (int o = threadIdx.x; o < HPW * D; o += 64 * W) {
+      const int hd = o / D, d = o % D, h = h0 + hd;
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kParts; ++i)
-        if (i < live) top = fmaxf(top, part_ml[i][hd][j].x);
+        if (i < live) top = fmaxf(top, part_ml[i][hd].x);
       const float base = top == -INFINITY ? 0.f : top;
       float sum = 0.f, y = 0.f;
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
         if (i >= live) break;
-        const float2 ml = part_ml[i][hd][j];
+        const float2 ml = part_ml[i][hd];
         const float w = fast_exp2(ml.x - base);
         sum = fmaf(ml.y, w, sum);
-        y = fmaf(part[i][hd][j][d], w, y);
+        y = fmaf(part[i][hd][d], w, y);
       }
-      const int h = h0 + hd;
       if (ns == 1) {
-        store_elem(orow + (h * G + j) * a.o_head + d * a.o_dim, len > 0 ? y * (1.f / sum) : 0.f);
+        store_elem(orow + h * a.o_head + d * a.o_dim, len > 0 ? y * (1.f / sum) : 0.f);
       } else {
-        const int64_t at = ((static_cast<int64_t>(r) * a.hkv + h) * p.splits + sp) * G + j;
+        const int64_t at = (static_cast<int64_t>(r) * a.hkv + h) * p.splits + sp;
         p.ws_acc[at * D + d] = y;
         if (d == 0) p.ws_ml[at] = make_float2(top, sum);
       }
@@ -345,30 +310,14 @@ __global__ __launch_bounds__(64 * kWaves) void decode8_merge_kernel(Decode8Args 
   for (int e = 0; e < E; ++e) store_elem(orow + (lane + 64 * e) * a.o_dim, acc[e] * inv);
 }
 
-template <typename T, int D, int G, int HPW>
-void launch_split(const Decode8Args& p, unsigned grid, hipStream_t stream) {
-  constexpr int PPI = 1024 / (D * HPW);
-  if constexpr (PPI > 0 && HPW * G * D <= 1024) {
-    constexpr int W = PPI * 4 <= kParts ? 4 : kParts / PPI;
-    hipLaunchKernelGGL((decode8_split_kernel<T, D, G, HPW, W>), dim3(grid), dim3(64 * W), 0, stream, p);
-  }
-}
-
-template <typename T, int D, int G>
-void launch_shape(const Decode8Args& p, unsigned grid, hipStream_t stream) {
-  switch (p.hpw) {
-    case 8: launch_split<T, D, G, 8>(p, grid, stream); break;
-    case 4: launch_split<T, D, G, 4>(p, grid, stream); break;
-    case 2: launch_split<T, D, G, 2>(p, grid, stream); break;
-    default: launch_split<T, D, G, 1>(p, grid, stream); break;
-  }
-}
-
 template <typename T>
-void launch_type(const Decode8Args& p, unsigned grid, hipStream_t stream) {
-  if (p.a.d == 128) launch_shape<T, 128, 1>(p, grid, stream);
-  else if (p.a.hq == p.a.hkv) launch_shape<T, 64, 1>(p, grid, stream);
-  else launch_shape<T, 64, 2>(p, grid, stream);
+void launch_split(const Decode8Args& p, unsigned grid, hipStream_t stream) {
+  switch (p.hpw) {
+    case 8: hipLaunchKernelGGL((decode8_split_kernel<T, 8, 4>), dim3(grid), dim3(256), 0, stream, p); break;
+    case 4: hipLaunchKernelGGL((decode8_split_kernel<T, 4, 4>), dim3(grid), dim3(256), 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((decode8_split_kernel<T, 2, 2>), dim3(grid), dim3(128), 0, stream, p); break;
+    default: hipLaunchKernelGGL((decode8_split_kernel<T, 1, 1>), dim3(grid), dim3(64), 0, stream, p); break;
+  }
 }
 
 template <typename T>
@@ -381,17 +330,14 @@ void launch_merge(const Decode8Args& p, hipStream_t stream) {
   }
 }
 
-// Heads a wave: as many neighbours as divide the heads, fit a load instruction and
-// the LDS of two workgroups a CU, and leave a workgroup for three CUs in four.  Measured, us
-// (16 heads x 128, bf16, 1 / 2 / 4 / 8 heads a wave): 4 rows of up to 256 tokens 6.7
-// / 7.1 / 12.3 / 20.4, 16 of up to 512 13.8 / 12.2 / 16.8 / 25.2, 1 of 8000 16.5 /
-// 14.6 / 19.4 / 26.5, 256 of up to 256 45.2 / 42.7 / 46.6 / 41.5, 64 of 512-4096 143
-// / 134 / 143 / 126, 256 of 1024-8192 1055 / 1000 / 1020 / 867, 2 of 16384-32768
-// (244 workgroups at 8) 55.9 / 51.6 / 53.1 / 47.5.
+// Heads a wave: as many neighbours as divide the heads and leave a workgroup for three CUs
+// in four.  Measured, us (16 heads x 64, bf16, 1 / 2 / 4 / 8 heads a wave): 4 rows of up to
+// 256 tokens 6.3 / 6.8 / 7.0 / 11.2, 16 of up to 512 10.9 / 10.8 / 11.0 / 15.4, 1 of 8000
+// 12.6 / 12.5 / 12.7 / 16.6, 256 of up to 256 32.0 / 23.7 / 22.3 / 21.8, 64 of 512-4096 93.9
+// / 63.3 / 61.6 / 62.7, 256 of 1024-8192 751 / 474 / 450 / 434.
 int heads_a_wave(const Attn8Args& a, int64_t splits) {
-  const int G = a.hq / a.hkv;
   int hpw = 1;
-  while (hpw < 8 && a.hkv % (2 * hpw) == 0 && 2 * hpw * G * a.d <= 1024 &&
+  while (hpw < 8 && a.hkv % (2 * hpw) == 0 &&
          a.rows * (a.hkv / (2 * hpw)) * splits >= kCus * 3 / 4)
     hpw *= 2;
   return hpw;
@@ -403,12 +349,12 @@ bool decode8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page) {
   return (d == 64 || d == 128 || d == 256) && page > 0 && page % kUnit == 0 && hkv > 0 && hq > 0;
 }
 
-// Which kernel: two heads on the vector units need twice the registers and products, and
-// pay only where a head's 64-byte rows keep the matrix-core kernel's loads short.  Measured,
-// us, vector units / matrix cores, 64 rows of 512-4096 tokens: 16 + 8 heads x 128 115 / 75,
-// x 64 57 / 66, 8 + 4 x 256 281 / 77; one head a KV head 8 x 256 208 / 129, 16 x 128 126 /
-// 139, 16 x 64 65 / 122.
-bool on_matrix_cores(int64_t hq, int64_t hkv, int64_t d) { return hq > 2 * hkv || d == 256 || (d == 128 && hq > hkv); }
+// Which kernel.  The matrix cores leave 15 columns of 16 empty for one query head a KV head,
+// and pay there only from head_dim 128 on.  Measured, us, vector units / matrix cores: 16
+// heads x 64, 64 rows of 512-4096 tokens 62 / 82; 16 x 128 121 / 115, 256 rows of 1024-8192
+// 850 / 831, 16 of up to 512 11.9 / 9.5, 4 of up to 256 6.5 / 6.6, 1 of 1000 10.3 / 11.8; 16 +
+// 8 heads x 64, 64 rows of 512-4096 54 / 45.
+bool on_matrix_cores(int64_t hq, int64_t hkv, int64_t d) { return hq > hkv || d > 64; }
 int split_base(int64_t hq, int64_t hkv, int64_t d) { return on_matrix_cores(hq, hkv, d) ? kMfmaSplit : kParts * kUnit; }
 
 int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t hkv, int64_t d) {
@@ -432,7 +378,7 @@ int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, 
   const int64_t columns = mfma ? (a.hq / a.hkv + 15) / 16 : 1;
   const int64_t items = a.rows * (a.hkv / p.hpw) * columns;
   p.split_slots = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.splits, kMaxGrid / items)));
-  p.xcd = a.hkv / p.hpw * columns * p.split_slots % kXcds == 0;
+  p.xcd = a.rows * p.split_slots % kXcds == 0;
   const int es = dtype_size(dtype);
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
   p.ws_acc = static_cast<float*>(ws);
@@ -443,9 +389,9 @@ int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, 
     launch_decode8_mfma(p, dtype, stream);
   } else {
     switch (dtype) {
-      case RLT_BFLOAT16: launch_type<bf16>(p, grid, stream); break;
-      case RLT_FLOAT16: launch_type<f16>(p, grid, stream); break;
-      default: launch_type<float>(p, grid, stream); break;
+      case RLT_BFLOAT16: launch_split<bf16>(p, grid, stream); break;
+      case RLT_FLOAT16: launch_split<f16>(p, grid, stream); break;
+      default: launch_split<float>(p, grid, stream); break;
     }
   }
   if (p.splits > 1) {

@@ -1,6 +1,6 @@
 // Decode over the 8-bit cache, shared between its entry point (attention_fp8.hip)
-// and its kernels (decode_fp8.hip: few and short heads on the vector units, and the
-// merge; decode_mfma_fp8.hip: the others on the matrix cores).
+// and its kernels (decode_fp8.hip: head_dim 64 with one query head a KV head on the vector
+// units, and the merge; decode_mfma_fp8.hip: the others on the matrix cores).
 #pragma once
 
 #include <algorithm>
@@ -33,7 +33,7 @@ struct Decode8Args {
   int splits;      // most splits of a row inside the tables' width
   int split_slots; // split-dimension workgroups launched; each walks every split_slots-th split
   int hpw;         // heads a wave
-  int xcd;         // workgroups of one (split, head block) of all rows share an XCD
+  int xcd;         // the heads of a (split, row) share an XCD
   int q_vec;       // q rows are 16-byte aligned, dims together
 };
 
