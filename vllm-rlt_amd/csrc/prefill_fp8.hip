@@ -18,6 +18,12 @@
 //   bf16 parts for fp16 and fp32 ones.
 // The running maximum moves only when a tile's exceeds it by 2^kRescale.
 //
+// The products' rate and the exponentials beside them bound it (a tile of
+// a wave is 1024 cycles of MFMA and about 1100 of vector work; two waves a SIMD).  In bf16 a wave issues the next
+// tile's products of K between its own softmax.  Measured, 16 chunks of 512 rows at the end of
+// 8192 keys, 16 heads x 128: bf16 622 us, 911 TFLOP/s (657 without the overlap), fp16 881 us,
+// fp32 448 us for four chunks.
+//
 // Key segments.  Items of one launch differ by two orders of magnitude (a new prompt's
 // 128 rows beside a chunk at the end of 16000 keys), and a launch of few rows has too
 // few of them.  So the keys of long sequences are cut into segments of about the
@@ -240,6 +246,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   constexpr int DT = D / 32;       // output tiles of 32 dims
   constexpr int CH = D / 16;       // 16-byte chunks of a code row
   constexpr int TPP = 256 / CH;    // tokens a staging pass
+  // With registers for two tiles' scores a wave issues the next tile's products of K before
+  // this one's softmax: the first half between its maximum, the others before its weights; K is then staged two tiles ahead, else one.
+  constexpr bool PIPE = NQ == 2;
+  constexpr int AHEAD = PIPE ? 2 : 1;
   constexpr int PASSES = kBN / TPP;
   // Padded rows: 8 lanes' 16-byte reads of 8 K rows fall into distinct bank groups
   // (the stride is an odd multiple of 16 bytes modulo 128), and so do the
@@ -360,37 +370,49 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const uint32_t block_bytes = static_cast<uint32_t>(a.kv_block), token_bytes = static_cast<uint32_t>(a.kv_token);
   const uint32_t s_block = static_cast<uint32_t>(a.s_block), s_token = static_cast<uint32_t>(a.s_token);
   const uint32_t page_mask = a.page - 1, last_key = max(wg_keys, 1) - 1, num_blocks = static_cast<uint32_t>(a.num_blocks);
-  uint32_t ids[PASSES], ks_id;
+  uint32_t ids[PASSES] = {}, v_ids[PASSES], ks_id = 0;  // of the K tile loaded next, and of the one before it
   u32x4 kreg[PASSES], vreg[PASSES];
   uint32_t vsreg[PASSES], ksreg;
   auto token = [&](int tile, int t) { return min(static_cast<uint32_t>(tile * kBN + t), last_key); };
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
+    for (int i = 0; i < PASSES; ++i) {
+      v_ids[i] = ids[i];
+      ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
+    }
     if (wave == 0) ks_id = trow[token(tile, lane) >> p.page_shift];
   };
-  auto load_tile = [&](int tile) __attribute__((always_inline)) {
+  auto load_k = [&](int tile, const uint32_t (&of)[PASSES], uint32_t ks_of, u32x4 (&k)[PASSES], uint32_t& ks) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const uint32_t slot = token(tile, i * TPP + st) & page_mask;
-      const uint64_t id = ids[i] < num_blocks ? ids[i] : 0;
-      const uint64_t at = id * block_bytes + __umul24(slot, token_bytes);
-      kreg[i] = *reinterpret_cast<const u32x4*>(kbase + at);
-      vreg[i] = *reinterpret_cast<const u32x4*>(vbase + at);
-      vsreg[i] = vsbase[id * s_block + __umul24(slot, s_token)];
+      const uint64_t id = of[i] < num_blocks ? of[i] : 0;
+      k[i] = *reinterpret_cast<const u32x4*>(kbase + (id * block_bytes + __umul24(token(tile, i * TPP + st) & page_mask, token_bytes)));
     }
     if (wave == 0)
-      ksreg = ksbase[static_cast<uint64_t>(ks_id < num_blocks ? ks_id : 0) * s_block + __umul24(token(tile, lane) & page_mask, s_token)];
+      ks = ksbase[static_cast<uint64_t>(ks_of < num_blocks ? ks_of : 0) * s_block + __umul24(token(tile, lane) & page_mask, s_token)];
+  };
+  auto load_v = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const uint32_t slot = token(tile, i * TPP + st) & page_mask, of = PIPE ? v_ids[i] : ids[i];
+      const uint64_t id = of < num_blocks ? of : 0;
+      vreg[i] = *reinterpret_cast<const u32x4*>(vbase + (id * block_bytes + __umul24(slot, token_bytes)));
+      vsreg[i] = vsbase[id * s_block + __umul24(slot, s_token)];
+    }
+  };
+  auto store_k = [&](int buf, const u32x4 (&k)[PASSES], uint32_t ks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(&k_lds[buf][(i * TPP + st) * KROW + sc * 16]) = k[i];
+    if (wave == 0) ks_lds[buf][lane] = static_cast<uint8_t>(ks);
   };
   // A V that is NaN must not reach the rows that do not see it through a product with 0:
   // in tiles that some row sees part of, it is stored as 0, and noted (see the end).
   bool nan = false;
-  auto store_tile = [&](int buf, bool masked) __attribute__((always_inline)) {
+  auto store_v = [&](int buf, bool masked) __attribute__((always_inline)) {
     uint32_t top = 0;  // largest V scale
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int t = i * TPP + st;
-      *reinterpret_cast<u32x4*>(&k_lds[buf][t * KROW + sc * 16]) = kreg[i];
       if (masked) {
         bool here = vsreg[i] == 255u;
 #pragma unroll
@@ -413,7 +435,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
       *reinterpret_cast<u32x4*>(dst + 8) = w[1];
       top = max(top, vsreg[i]);
     }
-    if (wave == 0) ks_lds[buf][lane] = static_cast<uint8_t>(ksreg);
     float bias = 0.f;
     if (__builtin_amdgcn_ballot_w64(top > 191u)) bias = group_max<64>(value_bias(top == 255u ? 0u : top));
     if (lane == 0) bias_lds[buf][wave] = bias;
@@ -431,57 +452,60 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const int grp = lane >> 4, gl = lane & 15;
   const int tr_off = (4 * (grp >> 1) + (gl >> 2)) * VROW + 16 * (grp & 1) + 4 * (gl & 3);
 
-  if (ntiles > first_tile) {
-    load_ids(first_tile);
-    load_tile(first_tile);
-    load_ids(first_tile + 1);
-    store_tile(first_tile & 1, tile_masked(first_tile));
-  }
-  __syncthreads();
-  for (int j = first_tile; j < ntiles; ++j) {
+  // S^T of tile j: steps [from, to) over the dims, with between(i) after the i-th product.
+  auto scores = [&](int j, f32x16 (&s)[2], int from, int to, auto between) __attribute__((always_inline)) {
     const int buf = j & 1;
-    if (j + 1 < ntiles) {
-      load_tile(j + 1);
-      load_ids(j + 2);
-    }
-    if (wave_live && j * kBN <= wave_last) {
-      f32x16 s[2] = {{}, {}};
-      if constexpr (WIDE) {
+    if (from == 0) s[0] = s[1] = f32x16{};
+    if constexpr (WIDE) {
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const uint32_t ksc = ks_lds[buf][hh * 32 + col];
+      for (int hh = 0; hh < 2; ++hh) {
+        const uint32_t ksc = ks_lds[buf][hh * 32 + col];
 #pragma unroll
-          for (int c = 0; c < DT; ++c) {
-            const u32x4 codes = *reinterpret_cast<const u32x4*>(&k_lds[buf][(hh * 32 + col) * KROW + 32 * c + 16 * half]);
+        for (int c = 0; c < DT; ++c) {
+          const u32x4 codes = *reinterpret_cast<const u32x4*>(&k_lds[buf][(hh * 32 + col) * KROW + 32 * c + 16 * half]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              u32x4 ka;
+          for (int u = 0; u < 2; ++u) {
+            u32x4 ka;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) ka[e] = scaled_bf16(codes[2 * u + e / 2], ksc, e % 2);
+            for (int e = 0; e < 4; ++e) ka[e] = scaled_bf16(codes[2 * u + e / 2], ksc, e % 2);
 #pragma unroll
-              for (int n = 0; n < NQ; ++n) s[hh] = Ops::mma(as_v8<bf16x8>(ka), as_v8<bf16x8>(qw[n][2 * c + u]), s[hh]);
-            }
+            for (int n = 0; n < NQ; ++n) s[hh] = Ops::mma(as_v8<bf16x8>(ka), as_v8<bf16x8>(qw[n][2 * c + u]), s[hh]);
           }
-        }
-      } else {
-        const int ksc[2] = {ks_lds[buf][col], ks_lds[buf][32 + col]};
-#pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          i32x8 ka[2];
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const uint8_t* row = &k_lds[buf][(hh * 32 + col) * KROW + 64 * c + 32 * half];
-            const u32x4 lo = *reinterpret_cast<const u32x4*>(row), hi = *reinterpret_cast<const u32x4*>(row + 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ka[hh][e] = static_cast<int>(lo[e]), ka[hh][4 + e] = static_cast<int>(hi[e]);
-          }
-#pragma unroll
-          for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh)
-              s[hh] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[hh], qb[n][c], s[hh], 0, 0, 0, ksc[hh], 0, q_scale[n]);
         }
       }
+    } else {
+      const int ksc[2] = {ks_lds[buf][col], ks_lds[buf][32 + col]};
+#pragma unroll
+      for (int c = 0; c < KS; ++c) {
+        if (c < from || c >= to) continue;
+        i32x8 ka[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const uint8_t* row = &k_lds[buf][(hh * 32 + col) * KROW + 64 * c + 32 * half];
+          const u32x4 lo = *reinterpret_cast<const u32x4*>(row), hi = *reinterpret_cast<const u32x4*>(row + 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ka[hh][e] = static_cast<int>(lo[e]), ka[hh][4 + e] = static_cast<int>(hi[e]);
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            s[hh] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[hh], qb[n][c], s[hh], 0, 0, 0, ksc[hh], 0, q_scale[n]);
+            between(n * 2 + hh);
+          }
+      }
+    }
+  };
+  auto nothing = [](int) {};
+  auto step = [&](int j, f32x16 (&s)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
+    const int buf = j & 1;
+    if (j + AHEAD < ntiles) load_k(j + AHEAD, ids, ks_id, kreg, ksreg);
+    if (j + 1 < ntiles) {
+      load_v(j + 1);
+      load_ids(j + AHEAD + 1);
+    }
+    if (wave_live && j * kBN <= wave_last) {
+      if constexpr (!PIPE) scores(j, s, 0, KS, nothing);
       // Element r of half hh is key key0 + 32 hh + 8 (r / 4) + 4 half + r % 4.
       const int key0 = j * kBN;
       const bool masked = uniform(key0 + kBN - 1 > prefix + wave_row0 || wave_row0 + 31 >= nq);
@@ -493,10 +517,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
           for (int r = 0; r < 16; ++r) s[hh][r] = hh * 32 + (r / 4) * 8 + r % 4 > lim ? -INFINITY : s[hh][r];
       }
       float tmax = -INFINITY;
+      auto max8 = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
+        for (int r = 0; r < 8; ++r) tmax = fmaxf(tmax, s[i / 2][i % 2 * 8 + r]);
+        // (In this order: the compiler would put the products in one block, 870 TFLOP/s against 911.)
+        if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+      };
+      if constexpr (PIPE) {
+        __builtin_amdgcn_sched_barrier(0);
+        scores(j + 1, next, 0, 1, max8);
+      } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
+        for (int i = 0; i < 4; ++i) max8(i);
+      }
       const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias_lds[buf]);
       tmax = max_across_halves(tmax) * p.qscale + fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
       const bool rescale = __builtin_amdgcn_ballot_w64(tmax > m + kRescale) != 0;
@@ -544,6 +577,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
       }
+      if constexpr (PIPE) {
+        __builtin_amdgcn_sched_barrier(0);
+        scores(j + 1, next, 1, KS, nothing);
+      }
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         u32x4 pb[NP];
@@ -556,8 +593,42 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         }
       }
     }
-    if (j + 1 < ntiles) store_tile(buf ^ 1, tile_masked(j + 1));
+    if (j + AHEAD < ntiles) store_k(j + AHEAD & 1, kreg, ksreg);
+    if (j + 1 < ntiles) store_v(buf ^ 1, tile_masked(j + 1));
     __syncthreads();
+  };
+
+  f32x16 sa[2], sb[2];
+  if (ntiles > first_tile) {
+    const int buf = first_tile & 1;
+    load_ids(first_tile);
+    if constexpr (PIPE) {
+      const uint32_t ks_first = ks_id;
+      u32x4 k1[PASSES];
+      uint32_t ks1;
+      load_ids(first_tile + 1);
+      load_k(first_tile, v_ids, ks_first, kreg, ksreg);
+      load_v(first_tile);
+      load_k(first_tile + 1, ids, ks_id, k1, ks1);
+      load_ids(first_tile + 2);
+      store_k(buf, kreg, ksreg);
+      store_v(buf, tile_masked(first_tile));
+      store_k(buf ^ 1, k1, ks1);
+      __syncthreads();
+      scores(first_tile, sa, 0, KS, nothing);
+      __syncthreads();  // the tile after the next takes its place
+    } else {
+      load_k(first_tile, ids, ks_id, kreg, ksreg);
+      load_v(first_tile);
+      load_ids(first_tile + 1);
+      store_k(buf, kreg, ksreg);
+      store_v(buf, tile_masked(first_tile));
+      __syncthreads();
+    }
+  }
+  for (int j = first_tile; j < ntiles; j += 2) {
+    step(j, sa, sb);
+    if (j + 1 < ntiles) step(j + 1, sb, sa);
   }
 
   // V that was NaN in tiles that some row sees part of: it is NaN in the rows that see it.
