@@ -13,7 +13,8 @@ namespace {
 // Any head size up to 64 * kPerLane, page size, grouping and strides: one
 // workgroup a (row, query head), wave w takes tokens w, w + kGenericWaves, ...
 // with the head's dims over its lanes and a running maximum and sum of its own;
-// the waves are joined through LDS in wave order.
+// the waves are joined through LDS in wave order.  Every query head reads its keys itself, a
+// byte a lane: latency bounds it (64 rows of 512-4096 tokens, 16 heads x 80: 1117 us).
 constexpr int kPerLane = 8;
 constexpr int kGenericWaves = 8;
 
