@@ -115,11 +115,23 @@ def test_empty_batches():
         check(none, 0, size, tables, 16, capacity, 4)
 
 
-def test_graph_replays_read_the_descriptors_again():
+@pytest.mark.parametrize("n,longest", [(1, 9000), (3, 9000), (300, 9000), (1100, 40)])
+def test_long_chunks_and_many_sequences(n, longest):
+    # One round of workgroups for any number of sequences, whichever of them holds the tokens.
+    g = torch.Generator().manual_seed(n)
+    tables = torch.randint(0, 5000, (4, 2, 600), generator=g, dtype=torch.int32)
+    desc = torch.stack([torch.randint(0, 4, (n,), generator=g), torch.randint(0, 2, (n,), generator=g),
+                        torch.randint(0, 300, (n,), generator=g), torch.randint(0, 30, (n,), generator=g)], 1)
+    desc[n // 2, 3] = longest
+    check(desc, n, n + 1, tables, 16, int(desc[:, 3].sum()) + 700, 600)
+
+
+@pytest.mark.parametrize("pinned", [False, True])
+def test_graph_replays_read_the_descriptors_again(pinned):
     from vllm_rlt_amd import ops
 
     desc, tables = batch(9, 12, 4, 30, 16, 50, 3)
-    capacity, dev, tab = 9 * 50, desc.cuda(), tables.cuda()
+    capacity, dev, tab = 9 * 50, desc.pin_memory() if pinned else desc.cuda(), tables.cuda()
     outs = buffers(9, capacity, 30, spare=0)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):

@@ -112,6 +112,15 @@ def test_a_row_depends_on_itself_only(hq, hkv, d):
     assert torch.equal(many, together.repeat(60, 1, 1))
 
 
+@pytest.mark.parametrize("hq,hkv,d,page,lengths", [(4, 1, 64, 16, [300000]), (1, 1, 64, 16, [300000]), (8, 2, 128, 48, [47, 48, 600, 1025]),
+                                                  (2, 2, 128, 128, [1, 129, 1500]), (3, 3, 256, 32, [33, 700]), (16, 1, 64, 64, [63, 513])])
+def test_decode_of_the_longest_rows_and_other_pages(hq, hkv, d, page, lengths):
+    # Past 262144 keys a wave's part of a split is more than one look-up of its units.
+    print(f"[decode8] {hq}/{hkv} x {d} page {page} {lengths}", flush=True)
+    c = Case(lengths, hq, hkv, d, page=page, seed=13)
+    c.check(c.decode())
+
+
 @pytest.mark.parametrize("hq,hkv,d,lengths", [(1, 1, 64, [16384, 16400, 8200, 300]), (4, 1, 64, [32768, 32784, 16500, 16384, 600])])
 def test_rows_cut_into_more_splits_than_the_longest(hq, hkv, d, lengths):
     # A row just past 64 splits has half as many, twice as long.
@@ -332,6 +341,41 @@ def test_streams_graphs_and_given_buffers():
         # Bits, not values: a row that has come to read a slot of nobody is NaN either way.
         assert torch.equal(out.view(torch.int16), c.decode().view(torch.int16))
         assert torch.equal(out_p.view(torch.int16), p.prefill().view(torch.int16))
+
+
+def test_a_captured_prefill_follows_the_lengths_of_each_replay():
+    # The cut of the keys is worked out on the device: long and short sequences in turn, one of them cut, all, none.
+    p = Case([6000, 500, 40], 8, 2, 128, seed=4, chunks=[70, 300, 40])
+    out = torch.empty_like(p.q)
+    graph = torch.cuda.CUDAGraph()
+    p.prefill()
+    with torch.cuda.graph(graph):
+        p.prefill(out=out)
+    for lengths, chunks in [([6000, 500, 40], [70, 300, 40]), ([70, 300, 40], [70, 300, 40]), ([6000, 500, 40], [400, 10, 0]),
+                            ([900, 500, 40], [1, 1, 1]), ([6000, 0, 0], [410, 0, 0])]:
+        p.lengths, p.chunks = lengths, chunks
+        p.lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        p.cu.copy_(torch.tensor([0, *chunks], dtype=torch.int32).cumsum(0))
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        n = sum(chunks)
+        p.check(out[:n])
+        assert (out[n:] == 7).all()
+
+
+def test_two_calls_at_once():
+    c = Case([4000, 90, 700, 2500], 8, 8, 128, seed=1)
+    p = Case([5000, 90], 8, 4, 128, seed=1, chunks=[200, 60])
+    want, want_p = c.decode(), p.prefill()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append((c.decode(), p.prefill()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, want_p) for a, b in got)
 
 
 def test_repeated_calls_give_the_same_bits():
