@@ -497,3 +497,24 @@ def test_row_ranges_that_overlap_stay_inside_the_workspace():
     ops.paged_prefill_fp8(c.q, *c.cache, tables, lens, cu, 1280, out=out[:1280], scale=c.scale, workspace=memory[:need])
     torch.cuda.synchronize()
     assert (memory[need:] == 7).all() and (out[1280:] == 3).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 64), (4, 2, 64), (2, 2, 128), (2, 2, 80)])
+def test_offsets_past_32_bits(hq, hkv, d):
+    from vllm_rlt_amd import ops
+
+    c = Case([70, 600, 5], hq, hkv, d, seed=3, chunks=[30, 140, 5])
+    layers, n = 256, c.cache[0].shape[0]
+    blocks = (1 << 32) // (layers * 16 * hkv * d) + n + 1  # the cache's blocks begin past element 2^32
+    big = []
+    for t in c.cache:
+        shape = (blocks, layers, *t.shape[1:])
+        whole = torch.empty(shape, dtype=torch.uint8, device="cuda").view(t.dtype)
+        whole[blocks - n :, layers - 1].view(torch.uint8).copy_(t.view(torch.uint8))
+        big.append(whole[:, layers - 1])
+    tables = torch.where(c.tables >= 0, c.tables + blocks - n, -1)
+    q = c.q[:3].contiguous()
+    got = ops.paged_decode_fp8(q, *big, tables, c.lens, scale=c.scale)
+    assert torch.equal(got, ops.paged_decode_fp8(q, *c.cache, c.tables, c.lens, scale=c.scale))
+    got = ops.paged_prefill_fp8(c.q, *big, tables, c.lens, c.cu, 140, scale=c.scale)
+    assert torch.equal(got, c.prefill())
