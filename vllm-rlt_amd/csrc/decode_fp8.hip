@@ -283,21 +283,24 @@ __global__ __launch_bounds__(64 * kWaves) void decode8_merge_kernel(Decode8Args 
   decode8_split_plan(sequence_length(a, r), p.base, &split_len, &ns);
   if (ns < 2) return;
   const int64_t base = (static_cast<int64_t>(r) * a.hkv + h) * p.splits * G + j;
-  const float2 ml = lane < ns ? p.ws_ml[base + static_cast<int64_t>(lane) * G] : make_float2(-INFINITY, 0.f);
-  const float top = group_max<64>(ml.x);
-  const float off = top == -INFINITY ? 0.f : top;
-  const float w = lane < ns ? fast_exp2(ml.x - off) : 0.f;
-  const float inv = 1.f / group_sum<64>(ml.y * w);
   constexpr int E = D / 64;
-  float acc[E] = {};
-  const float* src = p.ws_acc + base * D + lane;
   constexpr int BATCH = 8;
-  for (int s0 = 0; s0 < ns; s0 += BATCH) {
-    float x[BATCH][E];
+  const float* src = p.ws_acc + base * D + lane;
+  float x[BATCH][E], acc[E] = {};
+  auto load = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < BATCH; ++i)
 #pragma unroll
       for (int e = 0; e < E; ++e) x[i][e] = src[static_cast<int64_t>(min(s0 + i, ns - 1)) * G * D + 64 * e];
+  };
+  const float2 ml = lane < ns ? p.ws_ml[base + static_cast<int64_t>(lane) * G] : make_float2(-INFINITY, 0.f);
+  load(0);  // on its way while the weights are worked out
+  const float top = group_max<64>(ml.x);
+  const float off = top == -INFINITY ? 0.f : top;
+  const float w = lane < ns ? fast_exp2(ml.x - off) : 0.f;
+  const float inv = 1.f / group_sum<64>(ml.y * w);
+  for (int s0 = 0; s0 < ns; s0 += BATCH) {
+    if (s0) load(s0);
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
       const float wi = s0 + i < ns ? __shfl(w, s0 + i, 64) : 0.f;
