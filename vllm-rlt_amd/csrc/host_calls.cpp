@@ -16,6 +16,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -290,12 +291,18 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // ----------------------------------------------------------- 8-bit KV cache
-// All of args[at[0]], args[at[1]], ... plain device tensors of one device.
+// Whether t is on the current device, which a launch goes to.
+bool here(const at::Tensor& t) {
+  static const c10::impl::VirtualGuardImpl device(c10::DeviceType::CUDA);
+  return t.device().index() == device.getDevice().index();
+}
+
+// All of args[at[0]], args[at[1]], ... plain tensors of the current device.
 template <int N>
 bool all_plain(PyObject* const* args, const int (&at)[N], const at::Tensor* (&out)[N]) {
   for (int i = 0; i < N; ++i)
     if (!(out[i] = plain(args[at[i]])) || out[i]->device() != out[0]->device()) return false;
-  return true;
+  return here(*out[0]);
 }
 
 // An int64 argument; false where it is none (a subclass, or past 64 bits).
@@ -495,6 +502,7 @@ PyObject* chunk_metadata(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!desc.defined() || desc.layout() != at::kStrided || at::isTensorSubclassLike(desc)) Py_RETURN_NONE;
   for (int i = 1; i < 9; ++i)
     if (!(in[i] = plain(args[kAt[i]])) || in[i]->device() != in[1]->device()) Py_RETURN_NONE;
+  if (!here(*in[1])) Py_RETURN_NONE;
   const at::Tensor &tables = *in[1], &cu = *in[2], &lens = *in[3], &out = *in[8];
   if (desc.is_cuda() ? desc.device() != tables.device() : !desc.device().is_cpu() || !desc.is_pinned()) Py_RETURN_NONE;
   if (desc.scalar_type() != at::kLong || desc.dim() != 2 || desc.size(1) != 4 || !desc.is_contiguous() ||

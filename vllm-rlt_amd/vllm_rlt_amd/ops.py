@@ -42,13 +42,6 @@ def _host_calls(t: torch.Tensor):
     return _native.host, stream_handle(t.device)
 
 
-def _host_calls_here(t: torch.Tensor):
-    """_host_calls for launches on the current device; (None, 0) where t is on another."""
-    if not t.is_cuda or torch.cuda.current_device() != t.device.index:
-        return None, 0
-    return _host_calls(t)
-
-
 def _finish(result, name: str) -> torch.Tensor:
     if type(result) is int:
         check(result, name)
@@ -992,7 +985,7 @@ def build_chunk_metadata(
     an append of the whole buffer skips them; tokens past it are dropped from the
     end, and lengths count the others.  Sequences from count on are padding: no tokens, length 0.
     """
-    host, stream = _host_calls_here(tables)
+    host, stream = _host_calls(tables)
     if host is not None:
         result = host.chunk_metadata(
             descriptors, count, size, tables, page_size, cu_seqlens, lengths, positions, sequences, blocks, offsets,
@@ -1083,7 +1076,7 @@ def kv_append_fp8(
     stored as NaN.  k and v are float32, float16 or bfloat16; the slots of a call are
     distinct (rows of one slot would leave a mix), those outside the cache skipped.
     """
-    host, stream = _host_calls_here(key_cache)
+    host, stream = _host_calls(key_cache)
     if host is not None:
         result = host.append8(
             key_cache, value_cache, key_scales, value_scales, layer, write_blocks, write_offsets, k, v, n_rows, stream
@@ -1147,7 +1140,7 @@ def rope_axes_kv_append(
     is rotated for every row.  A row with a position outside the table gets zeros
     and is not written.  `out` may be q itself.
     """
-    host, stream = _host_calls_here(q)
+    host, stream = _host_calls(q)
     if host is not None:
         result = host.rope_axes(
             key_cache, value_cache, layer, write_blocks, write_offsets, q, k, v, positions, table, axes, key_scales,
@@ -1270,7 +1263,7 @@ def paged_decode_fp8(
     rows and is allocated here unless given.  A row's output bits depend on its own
     q, pages and length only.
     """
-    host, stream = _host_calls_here(q)
+    host, stream = _host_calls(q)
     if host is not None:
         result = host.decode8(
             q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out, workspace, scale, stream
@@ -1338,7 +1331,7 @@ def paged_prefill_fp8(
     are cut, by the launch's shapes, and is allocated here unless given.  With
     `batch_invariant` none is cut: a row's bits depend on its own sequence only.
     """
-    host, stream = _host_calls_here(q)
+    host, stream = _host_calls(q)
     if host is not None:
         result = host.prefill8(
             q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, cu_seqlens_q, max_seqlen_q,
