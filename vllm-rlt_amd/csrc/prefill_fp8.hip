@@ -45,9 +45,13 @@ constexpr int kBN = 64;   // keys a tile
 constexpr float kRescale = 8.f;
 constexpr int kMaxQExp = 24;
 constexpr int kXcds = 8;
-constexpr int kTargetItems = 768;
-constexpr int kSlots = 512;  // workgroups that run at once: two a CU
-constexpr int kMinSegTiles = 4;
+constexpr int kRound = 512;  // workgroups that run at once: two a CU (fp32 at head_dim 128: one)
+constexpr int kTargetItems = kRound * 3 / 2;
+// Shorter segments are not worth an item (about 9 us of plan, first loads and merge beside
+// 1.5 a tile).  Measured, us, in 4 / 3 / 2 / 1: one chunk of 40 rows over 340 keys 15.4 / 15.4 /
+// 14.0 / 13.6, of 128 over 4128 31.4 / 30.2 / 30.2 / 30.2, two of 20-100 over 200-1200 18.3 /
+// 18.7 / 18.5 / 23.3.
+constexpr int kMinSegTiles = 2;
 constexpr int kPlanSeqs = 64;  // sequences ranked and cut: one a lane
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -78,6 +82,7 @@ struct Prefill8Args {
   float2* part_ml;    // [slots][hq], max in log2 units and sum
   SeqPlan* plan;      // [kPlanSeqs], for the merge kernel
   int slots;
+  int round;  // workgroups that run at once
   int out_vec;  // 4 elements of an out row can be stored at once
   int q_vec;    // q rows are 16-byte aligned, dims together
 };
@@ -126,16 +131,16 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
     const int longest = __builtin_amdgcn_readlane(wave_scan(keys, [](int a, int b) { return max(a, b); }), 63);
     // Cut where the longest item would outlast the others by half: 24 chunks of 100-170 rows
     // over up to 1000 keys (768 items of up to 18 tiles) took 66 us whole, 90 cut.
-    if (longest * (2.f * kSlots) > 3.f * work) {
+    if (longest * (2.f * p.round) > 3.f * work) {
       // Few items: cut into one round of workgroups.  Many, of different lengths: into half as
       // many again, so that the short ones fill the gaps (eight chunks 444 us in 512, 392
       // in 768, 431 in 1024; one chunk of 64 items 112, 134, 129).
-      const bool few = __builtin_amdgcn_readlane(scan_sum(s.tiles), 63) * p.a.hq <= kSlots / 2;
-      int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few ? kSlots : kTargetItems)), 1e9f)));
+      const bool few = __builtin_amdgcn_readlane(scan_sum(s.tiles), 63) * p.a.hq <= p.round / 2;
+      int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few ? p.round : p.round * 3 / 2)), 1e9f)));
       for (int i = 0; few && i < 4; ++i) {  // as rounding up makes more items, towards the round
         const int items = __builtin_amdgcn_readlane(scan_sum(s.tiles * max(1, (keys + target - 1) / target)), 63) * p.a.hq;
-        if (items <= kSlots) break;
-        target = max(target + 1, static_cast<int>(static_cast<float>(target) * items * (1.f / kSlots)));
+        if (items <= p.round) break;
+        target = max(target + 1, static_cast<int>(static_cast<float>(target) * items / p.round));
       }
       s.segs = max(1, (keys + target - 1) / target);
       s.seg_tiles = (keys + s.segs - 1) / s.segs;
@@ -770,6 +775,7 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   const int64_t slots = ws ? partial_slots(a.rows, a.num_seqs, a.max_len, a.hq) : 0;
   if (slots > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);  // 64 sequences' stay inside 31 bits
   p.slots = static_cast<int>(slots);
+  p.round = dtype == RLT_FLOAT32 && a.d == 128 ? kRound / 2 : kRound;
   if (slots) {
     p.part_acc = static_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float2*>(p.part_acc + slots * a.hq * a.d);
