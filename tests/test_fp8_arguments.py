@@ -1,0 +1,48 @@
+"""What the 8-bit cache's calls hand to the library, and what it refuses at the limits (CPU only)."""
+
+import contextlib
+
+import pytest
+import torch
+
+
+class Library:
+    """Stands for the loaded library: keeps the arguments of every call, launches nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return call
+
+
+@pytest.fixture
+def library(monkeypatch):
+    from vllm_rlt_amd import _native, ops
+
+    lib = Library()
+    monkeypatch.setattr(_native, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_require_rocm", lambda *t: t[0].device)
+    monkeypatch.setattr(ops, "_current", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(ops, "stream_handle", lambda device: None)
+    monkeypatch.setattr(torch.Tensor, "is_pinned", lambda t: True)
+    return lib
+
+
+@pytest.mark.parametrize("size", [1, 3])
+def test_the_stride_of_out_tables_goes_to_the_library_as_it_is(library, size):
+    # Rows that share their memory have stride 0, which the library refuses: it writes size rows of out_width entries.
+    from vllm_rlt_amd import ops
+
+    long = lambda: torch.empty(9, dtype=torch.int64)  # noqa: E731
+    short = lambda *n: torch.empty(n, dtype=torch.int32)  # noqa: E731
+    for out in (short(size, 8), short(1, 8).expand(size, 8), short(size, 12)[:, :8]):
+        ops.build_chunk_metadata(torch.zeros(size, 4, dtype=torch.int64), size, size, short(4, 1, 8), 16, short(size + 1), short(size),
+                                 long(), long(), long(), long(), out, 8)
+        name, args = library.calls.pop()
+        assert name == "rlt_build_chunk_metadata" and args[-2] == 8
+        assert args[-3] == out.stride(0) or size == 1 and args[-3] >= 8

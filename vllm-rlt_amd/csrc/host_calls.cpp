@@ -521,7 +521,7 @@ PyObject* chunk_metadata(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   rc = g_chunk_metadata(desc.data_ptr<int64_t>(), count, size, tables.data_ptr<int32_t>(), tables.size(0), tables.size(2),
                         tables.size(1), page, cu.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), in[4]->data_ptr<int64_t>(),
                         in[5]->data_ptr<int64_t>(), in[6]->data_ptr<int64_t>(), in[7]->data_ptr<int64_t>(), capacity,
-                        out.data_ptr<int32_t>(), std::max(out.stride(0), width), width, stream);
+                        out.data_ptr<int32_t>(), size > 1 ? out.stride(0) : width, width, stream);  // one row's stride is nobody's
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);
   END_HANDLE_TH_ERRORS

@@ -1024,7 +1024,8 @@ def build_chunk_metadata(
         rc = _native.load().rlt_build_chunk_metadata(
             descriptors.data_ptr(), count, size, tables.data_ptr(), tables.shape[0], tables.shape[2], tables.shape[1],
             page_size, cu_seqlens.data_ptr(), lengths.data_ptr(), positions.data_ptr(), sequences.data_ptr(),
-            blocks.data_ptr(), offsets.data_ptr(), capacity, out_tables.data_ptr(), max(out_tables.stride(0), out_width),
+            blocks.data_ptr(), offsets.data_ptr(), capacity, out_tables.data_ptr(),
+            out_tables.stride(0) if size > 1 else out_width,  # (one row's stride is nobody's)
             out_width, stream_handle(device),
         )
     check(rc, "rlt_build_chunk_metadata")
