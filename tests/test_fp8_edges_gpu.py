@@ -2,8 +2,10 @@
 
 import pytest
 import torch
+from test_fp8_attention_gpu import DTYPES, Case
 
 pytestmark = pytest.mark.gpu
+SHAPES = [(4, 4, 128), (8, 2, 128), (4, 4, 64), (2, 2, 80)]
 
 
 @pytest.mark.parametrize("python", [False, True])
@@ -23,3 +25,16 @@ def test_chunk_tables_whose_rows_share_memory_are_refused(python, monkeypatch):
     one = torch.empty(1, 5, dtype=torch.int32, device="cuda").as_strided((1, 5), (0, 1))
     ops.build_chunk_metadata(desc[:1].cuda(), 1, 1, tables.cuda(), 16, *outs[:6], one, 5)
     assert torch.equal(one.cpu(), expected(desc, 1, 1, tables, 16, 40, 5)[-1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-40, -1e-44])
+def test_softmax_scales_of_zero_and_below_the_smallest_normal(dtype, hq, hkv, d, scale):
+    # Every visible key weighs alike, masked ones nothing.
+    c = Case([150, 3000, 30], hq, hkv, d, dtype=dtype, seed=8, chunks=[100, 90, 40])
+    c.scale = scale
+    c.check(c.prefill())
+    c.check(c.prefill(batch_invariant=True))
+    c.q, c.chunks = c.q[:3], None
+    c.check(c.decode())

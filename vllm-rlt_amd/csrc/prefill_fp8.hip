@@ -33,6 +33,7 @@
 #include "prefill_fp8.hpp"
 
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "mfma.hpp"
@@ -783,8 +784,10 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   }
   p.page_shift = __builtin_ctz(a.page);
   p.qscale = std::fabs(a.qscale);
-  p.q_exp = std::isnormal(p.qscale) ? std::min(std::max(std::ilogb(p.qscale), -kMaxQExp), kMaxQExp) : 0;
-  p.qscale = std::ldexp(p.qscale, -p.q_exp);
+  // A scale of 0 stands as 2^-126 2^-kMaxQExp: a finite score ends below 2^-22, a masked one stays -inf.
+  const bool none = p.qscale == 0.f;
+  p.q_exp = none ? -kMaxQExp : std::isfinite(p.qscale) ? std::min(std::max(std::ilogb(p.qscale), -kMaxQExp), kMaxQExp) : 0;
+  p.qscale = none ? std::numeric_limits<float>::min() : std::ldexp(p.qscale, -p.q_exp);
   p.q_sign = a.qscale < 0.f ? 0x80000000u : 0u;
   const int es = dtype_size(dtype);
   p.q_vec = a.q_dim == 1 && aligned16(a.q) && a.q_row * es % 16 == 0 && a.q_head * es % 16 == 0;
