@@ -38,3 +38,28 @@ def test_softmax_scales_of_zero_and_below_the_smallest_normal(dtype, hq, hkv, d,
     c.check(c.prefill(batch_invariant=True))
     c.q, c.chunks = c.q[:3], None
     c.check(c.decode())
+
+
+def channels(c, seed, high=6.0):
+    """Channels of very different sizes: q and K of the case times powers of two over 2^-high .. 2^high that undo each other on
+    the whole, then a softmax scale that puts the largest sums of a score's magnitudes at 100."""
+    d = c.q.shape[-1]
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(-int(high), int(high) + 1, (d,), generator=g)
+    c.q.mul_(torch.ldexp(torch.ones(d), e).to(c.q.dtype).cuda())
+    codes = c.cache[0].float()
+    owned = codes.isfinite()
+    big = torch.randint(-3, 4, (d,), generator=g)
+    codes = torch.where(owned, codes * torch.ldexp(torch.ones(d), big).cuda() / 16, codes)
+    c.cache[0].view(torch.uint8).copy_(codes.to(torch.float8_e4m3fn).view(torch.uint8))
+    k = (codes.nan_to_num(0.0) * torch.where(c.cache[2].float().isfinite(), c.cache[2].float(), 0.0)[..., None]).flatten(0, 1)
+    k = k.abs().transpose(0, 1).repeat_interleave(c.q.shape[1] // k.shape[1], 0)  # [hq, tokens, d]
+    c.scale = 100.0 / float((c.q.float().abs().transpose(0, 1) @ k.transpose(1, 2)).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [*SHAPES, (2, 2, 256)])
+def test_decode_scores_of_channels_of_very_different_sizes_are_sums_in_32_bits(dtype, hq, hkv, d):
+    c = Case([40, 300, 700, 1200, 100, 90, 80, 70], hq, hkv, d, dtype=dtype, seed=31)
+    channels(c, 3)
+    c.check(c.decode())

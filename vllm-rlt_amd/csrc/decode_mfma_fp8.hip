@@ -4,10 +4,10 @@
 //
 // A workgroup takes one (row, KV head, 16 query heads, split); its four waves take every
 // fourth 32 tokens of the split each, through LDS of their own (no barrier):
-// - S^T = K Q^T on the scaled 8-bit MFMA (16x16x128), codes and scales as they are, q in
-//   parts of 4 significant bits (two hold a bf16, three an fp16); an fp32 q in three bf16
-//   parts on the bf16 MFMA against K converted with its scale (prefill_fp8.hip has the
-//   reasons).
+// - S^T = K Q^T on the 16-bit MFMA of q's type (16x16x32; an fp32 q in three bf16 parts): a
+//   code is a bf16 or an fp16 exactly, and its token's scale multiplies the fp32 sum.  (The
+//   scaled 8-bit MFMA would take codes and scales as they are, but drops what lies 2^-11
+//   below the largest product of its 128; the 16-bit ones keep fp32's bits.)
 // - O^T += V^T P^T on the bf16 MFMA (16x16x32): P stays in the registers S^T left it in,
 //   times its token's V scale, in one, two or three bf16 parts for bf16, fp16 and fp32; V's
 //   codes come from transposing 8-bit LDS reads and become bf16 exactly.
@@ -31,26 +31,31 @@ constexpr int kXcds = 8;
 constexpr int kTile = 32;
 constexpr float kRescale = 8.f;  // the running maximum moves when a tile's exceeds it by 2^kRescale
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
+// Parts of q and of P, and the type of the scores' operands.
 template <typename T> struct Parts;
-template <> struct Parts<bf16> { static constexpr int Q = 2, P = 1; };
-template <> struct Parts<f16> { static constexpr int Q = 3, P = 2; };
-template <> struct Parts<float> { static constexpr int Q = 3, P = 3; };
+template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf16; };
+template <> struct Parts<f16> { static constexpr int Q = 1, P = 2; using S = f16; };
+template <> struct Parts<float> { static constexpr int Q = 3, P = 3; using S = bf16; };
 
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) { return MfmaOps<bf16>::pack2(x, y); }
 
-// Two codes of a word (its low or high half) times a power of two, as bf16.
-__device__ __forceinline__ uint32_t scaled_bf16(uint32_t word, float scale, bool high) {
-  const bf16x2 r = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(word), scale, true)
-                        : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(word), scale, false);
-  return __builtin_bit_cast(uint32_t, r);
+// Two codes of a word (its low or high half) as bf16 or fp16, both exact.
+template <typename S>
+__device__ __forceinline__ uint32_t code_pair(uint32_t word, bool high) {
+  const int w = static_cast<int>(word);
+  if constexpr (std::is_same_v<S, f16>)
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+  else
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
 }
 
+template <typename S>
 __device__ __forceinline__ f32x4 mma16(u32x4 x, u32x4 y, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_v8<bf16x8>(x), as_v8<bf16x8>(y), c, 0, 0, 0);
+  if constexpr (std::is_same_v<S, f16>) return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8<f16x8>(x), as_v8<f16x8>(y), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_v8<bf16x8>(x), as_v8<bf16x8>(y), c, 0, 0, 0);
 }
 
 // Direct global -> LDS loads, as assembly so that the compiler's wait analysis, which cannot
@@ -93,20 +98,19 @@ constexpr int kWavesPerEu = D == 256 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4
 
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<T, D>))) void decode8_mfma_kernel(Decode8Args p) {
-  constexpr bool WIDE = sizeof(T) == 4;
+  using S = typename Parts<T>::S;
   constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P;
-  constexpr int KS = (D + 127) / 128;  // 8-bit MFMA steps over the dims
+  constexpr int KS = (D + 127) / 128;  // 128 dims each: four MFMA steps
   constexpr int DT = D / 16;           // output tiles of 16 dims
   constexpr int CH = D / 16;           // 16-byte chunks of a code row
   constexpr int TPI = 64 / CH;         // tokens a load instruction
   constexpr int NI = kTile / TPI;      // loads a tile, of K and of V
   constexpr int kScales = 2 * kTile * D, kWaveBytes = kScales + 512;  // K rows, V rows, two sets of K and V scale bytes (a dword each)
   constexpr int JROW = D + 4;
-  constexpr int QE = D / 16, QROW = D * (WIDE ? 2 : 1);
+  constexpr int QE = D / 16, QROW = 2 * D;
   static_assert(16 * JROW * 4 <= kWaveBytes, "a wave's accumulators fit its tile");
   __shared__ __align__(16) uint8_t lds[kWaves][kWaveBytes];
   __shared__ __align__(16) uint8_t q_lds[NQ][16][QROW];
-  uint8_t* const q_scales = lds[0] + kScales + 256;  // of the second tile, until then free
   float2(*const ml_lds)[16] = reinterpret_cast<float2(*)[16]>(q_lds);
 
   const Attn8Args& a = p.a;
@@ -203,69 +207,45 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
       load_v(0);
     }
     // q's parts, B operands: lane (col, j) holds dims [128 c + 32 j, + 32) of query head c0 +
-    // col; for bf16, 8 of them a k-step.
-    i32x8 qb[NQ][KS];
+    // col, 8 of them a step.
     u32x4 qw[NQ][4 * KS];
-    int q_scale[NQ];
     {
       uint32_t thread = threadIdx.x;
       opaque(thread);
       const int qh = thread / 16, qd = thread % 16 * QE;
-      if constexpr (WIDE) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
+      for (int e = 0; e < QE; ++e)  // infinities as NaN, which no other head's maximum takes up
+        if ((__float_as_uint(y[e]) & 0x7f800000u) == 0x7f800000u) y[e] = __uint_as_float(0x7fc00000u);
 #pragma unroll
-          for (int e = 0; e < QE; e += 2) {
+      for (int i = 0; i < NQ; ++i)
+#pragma unroll
+        for (int e = 0; e < QE; e += 2) {
+          uint32_t word;
+          if constexpr (NQ > 1) {  // the top 16 bits: the rest is exact, and the third part holds all of it
             const uint32_t lo = __float_as_uint(y[e]), hi = __float_as_uint(y[e + 1]);
-            *reinterpret_cast<uint32_t*>(q_lds[i][qh] + 2 * (qd + e)) = lo >> 16 | (hi & 0xffff0000u);
+            word = lo >> 16 | (hi & 0xffff0000u);
             y[e] -= __uint_as_float(lo & 0xffff0000u);
             y[e + 1] -= __uint_as_float(hi & 0xffff0000u);
+          } else {
+            word = MfmaOps<S>::pack2(y[e], y[e + 1]);
           }
-      } else {
-        float amax = 0.f;
-#pragma unroll
-        for (int e = 0; e < QE; ++e) amax = fmaxf(amax, finite_abs(y[e]));
-        const uint32_t b = max(scale_byte(group_max<16>(amax)), 4u * NQ);
-        const float inv = inverse_scale(b);
-        if (qd == 0) q_scales[qh] = static_cast<uint8_t>(b);
-#pragma unroll
-        for (int e = 0; e < QE; ++e)
-          y[e] = (__float_as_uint(y[e]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : y[e] * inv;
-#pragma unroll
-        for (int i = 0; i < NQ; ++i)
-#pragma unroll
-          for (int e = 0; e < QE; e += 4) {
-            int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[e], y[e + 1], 0, false);
-            word = __builtin_amdgcn_cvt_pk_fp8_f32(y[e + 2], y[e + 3], word, true);
-            *reinterpret_cast<int*>(q_lds[i][qh] + qd + e) = word;
-            const f32x2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
-            y[e] = (y[e] - lo[0]) * 16.f, y[e + 1] = (y[e + 1] - lo[1]) * 16.f;
-            y[e + 2] = (y[e + 2] - hi[0]) * 16.f, y[e + 3] = (y[e + 3] - hi[1]) * 16.f;
-          }
-      }
+          *reinterpret_cast<uint32_t*>(q_lds[i][qh] + 2 * (qd + e)) = word;
+        }
       wait_lds();
       asm volatile("s_barrier" ::: "memory");  // (__syncthreads() would wait for the tile)
       const u32x4 zero = {0u, 0u, 0u, 0u};
-      const bool in = D >= 128 || j < 2;  // head_dim 64: the upper half of the step is 0
+      const bool in = D >= 128 || j < 2;  // head_dim 64: the upper half of the 128 is 0
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        if constexpr (!WIDE) q_scale[i] = static_cast<int>(q_scales[col]) - 4 * i;
+      for (int i = 0; i < NQ; ++i)
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
           const int d0 = in ? 128 * c + 32 * j : 0;
-          if constexpr (WIDE) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const u32x4 w = *reinterpret_cast<const u32x4*>(q_lds[i][col] + 2 * (d0 + 8 * e));
-              qw[i][4 * c + e] = in ? w : zero;
-            }
-          } else {
-            const u32x4 lo = *reinterpret_cast<const u32x4*>(q_lds[i][col] + d0), hi = *reinterpret_cast<const u32x4*>(q_lds[i][col] + d0 + 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) qb[i][c][e] = static_cast<int>(in ? lo[e] : 0u), qb[i][c][4 + e] = static_cast<int>(in ? hi[e] : 0u);
+          for (int e = 0; e < 4; ++e) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(q_lds[i][col] + 2 * (d0 + 8 * e));
+            qw[i][4 * c + e] = in ? w : zero;
           }
         }
-      }
       wait_lds();
       asm volatile("s_barrier" ::: "memory");
     }
@@ -280,12 +260,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
       opaque(k_read), opaque(v_read), opaque(k_chunk), opaque(v_chunk), opaque(load_row);
       const uint32_t* scales = reinterpret_cast<const uint32_t*>(lds[wave] + kScales + tile % 2 * 256);  // K's, then V's
       wait_loads<NI>();  // V may still be on its way
-      u32x4 ka[2][KS][2];
-      uint32_t ksc[2];
+      u32x4 ka[2][KS][2], kb[2];
       const bool in = D >= 128 || j < 2;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        ksc[u] = scales[16 * u + col] & 255u;
+        kb[u] = *reinterpret_cast<const u32x4*>(scales + 16 * u + 4 * j);
 #pragma unroll
         for (int c = 0; c < KS; ++c)
 #pragma unroll
@@ -302,34 +281,23 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          if constexpr (WIDE) {
-            const float scale = scale_value(ksc[u]);
+        for (int c = 0; c < KS; ++c)
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              u32x4 kw;
+          for (int q4 = 0; q4 < 4; ++q4) {
+            u32x4 kw;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) kw[e] = scaled_bf16(ka[u][c][q4 / 2][q4 % 2 * 2 + e / 2], scale, e % 2);
+            for (int e = 0; e < 4; ++e) kw[e] = code_pair<S>(ka[u][c][q4 / 2][q4 % 2 * 2 + e / 2], e % 2);
 #pragma unroll
-              for (int i = 0; i < NQ; ++i) s[u] = mma16(kw, qw[i][4 * c + q4], s[u]);
-            }
-          } else {
-            i32x8 kc;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) kc[e] = static_cast<int>(ka[u][c][0][e]), kc[4 + e] = static_cast<int>(ka[u][c][1][e]);
-#pragma unroll
-            for (int i = 0; i < NQ; ++i)
-              s[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kc, qb[i][c], s[u], 0, 0, 0, static_cast<int>(ksc[u]), 0,
-                                                                      q_scale[i]);
+            for (int i = 0; i < NQ; ++i) s[u] = mma16<S>(kw, qw[i][4 * c + q4], s[u]);
           }
-        }
       }
       float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[u][e] = t0 + tile * (kWaves * kTile) + 16 * u + 4 * j + e < end ? s[u][e] * a.qscale : -INFINITY;
+          const float x = s[u][e] * scale_value(kb[u][e] & 255u) * a.qscale;
+          s[u][e] = t0 + tile * (kWaves * kTile) + 16 * u + 4 * j + e < end ? x : -INFINITY;
           top = fmaxf(top, s[u][e]);
         }
       f32x4 sv[2];
@@ -387,9 +355,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
       for (int c = 0; c < DT; ++c) {
         u32x4 va;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) va[e] = scaled_bf16(static_cast<uint32_t>(codes[c][e / 2]), 1.f, e % 2);
+        for (int e = 0; e < 4; ++e) va[e] = code_pair<bf16>(static_cast<uint32_t>(codes[c][e / 2]), e % 2);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) acc[c] = mma16(va, pb[i], acc[c]);
+        for (int i = 0; i < NP; ++i) acc[c] = mma16<bf16>(va, pb[i], acc[c]);
       }
     }
     // Join the waves, in order.
