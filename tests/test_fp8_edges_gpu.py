@@ -63,3 +63,29 @@ def test_decode_scores_of_channels_of_very_different_sizes_are_sums_in_32_bits(d
     c = Case([40, 300, 700, 1200, 100, 90, 80, 70], hq, hkv, d, dtype=dtype, seed=31)
     channels(c, 3)
     c.check(c.decode())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_prefill_scores_of_channels_of_very_different_sizes_are_sums_in_32_bits(dtype, hq, hkv, d):
+    c = Case([140, 300, 700], hq, hkv, d, dtype=dtype, seed=31, chunks=[100, 33, 200])
+    channels(c, 3)
+    c.check(c.prefill())
+    c.check(c.prefill(batch_invariant=True))
+
+
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_prefill_keys_of_two_to_the_128_take_all_the_weight(hq, hkv, d):
+    # Key 60 is what the append makes of the largest finite number in one dim where the queries are 1, and of 0 elsewhere.
+    c = Case([150], hq, hkv, d, dtype=torch.bfloat16, seed=8, chunks=[100])
+    at = (int(c.tables[0, 3]), 60 % 16)
+    c.cache[0].view(torch.uint8)[at] = 0
+    c.cache[0].view(torch.uint8)[at][:, 5] = 0x78
+    c.cache[2].view(torch.uint8)[at] = 247
+    c.q[..., 5] = 1.0
+    c.q[..., 6] = 0.0
+    c.scale = 0.5
+    out = c.prefill()
+    v = (c.cache[1].float() * c.cache[3].float()[..., None])[at].repeat_interleave(hq // hkv, 0)
+    assert torch.equal(out[10:].float(), v.bfloat16().float().expand(90, -1, -1))
+    assert out.isfinite().all()

@@ -3,26 +3,22 @@
 //
 // A workgroup of 4 waves takes 128 query rows of one (sequence, query head) over a
 // segment of its keys, a wave 32 rows, 64 keys a tile:
-// - S^T = K Q^T on the scaled 8-bit MFMA (32x32x64): K's codes go from LDS into it as
-//   they are, and its scale operand takes a key's e8m0 byte, so nothing of K is
-//   converted.  q becomes rows of codes, each the rest of the one before with a scale 16
-//   times smaller: 4 significant bits each, so two hold a bf16 and three an fp16 (the
-//   last bits of values 2^13 below their row's largest aside).  The 8-bit MFMA has twice
-//   the rate of the 16-bit one: two parts cost what a bf16 q would.  Its sums carry about
-//   18 bits, too few for an fp32 q, which is split in three bf16 parts for the bf16
-//   MFMA against K converted with its scale (exact: a code has 4 bits).
-// - O^T += V^T P^T on the bf16 MFMA (32x32x16).  V becomes bf16, its scale included
-//   (exact: a code has 4 bits), once a workgroup, on its way into LDS; V^T comes from
-//   transposing LDS reads, P from the registers S^T left it in.  P is rounded to bf16
+// - S^T = K Q^T on the 16-bit MFMA (32x32x16).  K becomes bf16, its scale included (exact: a
+//   code has 4 bits), once a workgroup, on its way into LDS, for q in bf16, or fp32 in three bf16
+//   parts.  For an fp16 q codes become fp16, and their scales multiply the sums (two bf16 parts
+//   of q instead: 980 us for 877 below).  (The scaled 8-bit MFMA would take K's codes and scales
+//   as they are, but drops what lies 2^-11 below the largest product of its 64; the 16-bit
+//   ones keep fp32's bits.)
+// - O^T += V^T P^T likewise.  V becomes bf16 as K does; V^T comes from transposing LDS reads, P
+//   from the registers S^T left it in.  P is rounded to bf16
 //   (its sum is taken over the rounded values) for bf16 outputs, and split in two or three
 //   bf16 parts for fp16 and fp32 ones.
 // The running maximum moves only when a tile's exceeds it by 2^kRescale.
 //
-// The products' rate and the exponentials beside them bound it (a tile of
-// a wave is 1024 cycles of MFMA and about 1100 of vector work; two waves a SIMD).  In bf16 a wave issues the next
-// tile's products of K between its own softmax.  Measured, 16 chunks of 512 rows at the end of
-// 8192 keys, 16 heads x 128: bf16 622 us, 911 TFLOP/s (657 without the overlap), fp16 881 us,
-// fp32 448 us for four chunks.
+// The products' rate and the vector work beside them bound it (a tile of a wave is 1024 cycles of
+// MFMA and some 1100 of vector work in bf16; two waves a SIMD).  Measured, 16 chunks of 512 rows at
+// the end of 8192 keys, 16 heads x 128: bf16 655 us, 865 TFLOP/s, fp16 877 us, fp32 406 us for four
+// chunks.
 //
 // Key segments.  Items of one launch differ by two orders of magnitude (a new prompt's
 // 128 rows beside a chunk at the end of 16000 keys), and a launch of few rows has too
@@ -55,12 +51,10 @@ constexpr int kTargetItems = kRound * 3 / 2;
 constexpr int kMinSegTiles = 2;
 constexpr int kPlanSeqs = 64;  // sequences ranked and cut: one a lane
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 template <typename T> struct Parts;
-template <> struct Parts<bf16> { static constexpr int Q = 2, P = 1; };
-template <> struct Parts<f16> { static constexpr int Q = 3, P = 2; };
-template <> struct Parts<float> { static constexpr int Q = 3, P = 3; };
+template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf16; };
+template <> struct Parts<f16> { static constexpr int Q = 1, P = 2; using S = f16; };
+template <> struct Parts<float> { static constexpr int Q = 3, P = 3; using S = bf16; };
 
 // One sequence a lane: its rows, keys and cut.
 struct SeqPlan {
@@ -73,8 +67,8 @@ struct SeqPlan {
 struct Prefill8Args {
   Attn8Args a;
   int page_shift;
-  // |softmax scale| * log2(e) = qscale * 2^q_exp: the power of two goes into q, so that
-  // a score overflows only where the scaled one does.
+  // |softmax scale| * log2(e) = qscale * 2^q_exp, q_exp in [-kMaxQExp, 0]: the power of two goes
+  // into q, so that a score overflows only where the scaled one does.
   float qscale;
   int q_exp;
   uint32_t q_sign;  // 0x80000000 negates q (a negative scale), else 0
@@ -232,6 +226,13 @@ __device__ __forceinline__ uint32_t scaled_bf16(uint32_t word, uint32_t b, bool 
   return __builtin_bit_cast(uint32_t, r);
 }
 
+// Two codes of a word (its low or high half) as fp16, exact.
+__device__ __forceinline__ uint32_t f16_codes(uint32_t word, bool high) {
+  const f16x2 r = high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(word), 1.f, true)
+                       : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(word), 1.f, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
 // Elements d .. d + 3 of an out row.
 template <typename T>
 __device__ __forceinline__ void store4(T* orow, int d, const float (&x)[4], int64_t stride, bool vec) {
@@ -247,23 +248,21 @@ __device__ __forceinline__ void store4(T* orow, int d, const float (&x)[4], int6
 template <typename T, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void prefill8_kernel(Prefill8Args p) {
   using Ops = MfmaOps<bf16>;
+  using S = typename Parts<T>::S;  // of the scores' operands
+  constexpr bool LATE = std::is_same_v<S, f16>;  // K's scales multiply the sums
   constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P;
-  constexpr int KS = D / 64;       // MFMA steps over the dims
+  constexpr int KS = D / 16;       // MFMA steps over the dims
   constexpr int DT = D / 32;       // output tiles of 32 dims
   constexpr int CH = D / 16;       // 16-byte chunks of a code row
   constexpr int TPP = 256 / CH;    // tokens a staging pass
-  // With registers for two tiles' scores a wave issues the next tile's products of K before
-  // this one's softmax: the first half between its maximum, the others before its weights; K is then staged two tiles ahead, else one.
-  constexpr bool PIPE = NQ == 2;
-  constexpr int AHEAD = PIPE ? 2 : 1;
   constexpr int PASSES = kBN / TPP;
   // Padded rows: 8 lanes' 16-byte reads of 8 K rows fall into distinct bank groups
   // (the stride is an odd multiple of 16 bytes modulo 128), and so do the
   // transposing V reads (64 modulo 256).
-  constexpr int KROW = D + 16, VROW = D + 32;  // bytes, bf16 elements
-  __shared__ __align__(16) uint8_t k_lds[2][kBN * KROW];
+  constexpr int KROW = D + 8, VROW = D + 32;
+  __shared__ __align__(16) uint16_t k_lds[2][kBN * KROW];
   __shared__ __align__(16) uint16_t v_lds[2][kBN * VROW];
-  __shared__ uint8_t ks_lds[2][kBN];
+  __shared__ __align__(16) float ks_lds[2][LATE ? kBN : 4];  // K's scales times 2^q_exp
   __shared__ __align__(16) float bias_lds[2][4];  // of each wave's staged V scales (value_bias)
 
   const Attn8Args& a = p.a;
@@ -288,80 +287,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const int wave_last = prefix + min(wave_row0 + 31, nq - 1);
   const bool wave_live = wave_row0 < nq;
 
-  // q's parts, B operands.  8-bit: lane (col, half) holds dims [64c + 32 half, + 32) of
-  // row col; bf16: of the 32 dims of a pair of k-steps, [16 half, + 8) for the first and
-  // the next 8 for the second.
-  constexpr bool WIDE = sizeof(T) == 4;
-  i32x8 qb[NQ][KS];
-  u32x4 qw[NQ][2 * DT];
-  int q_scale[NQ];
+  // q's parts, B operands: lane (col, half) holds dims [16 c + 8 half, + 8) of row col for step c.
+  u32x4 qw[NQ][KS];
   {
     const T* qrow = static_cast<const T*>(a.q) + (row0 + min(my_row, nq - 1)) * a.q_row + h * a.q_head;
-    constexpr int RUN = WIDE ? 16 : 32, RUNS = D / 2 / RUN;  // a lane's dims: RUNS runs of RUN
-    float x[RUNS][RUN];
-    float amax = 0.f;
+    const float power = __uint_as_float(static_cast<uint32_t>(127 + (LATE ? 0 : p.q_exp)) << 23 | p.q_sign);
 #pragma unroll
-    for (int c = 0; c < RUNS; ++c) {
-      const int d0 = 2 * RUN * c + RUN * half;
+    for (int c = 0; c < KS; ++c) {
+      const int d0 = 16 * c + 8 * half;
+      float x[8];
       if (p.q_vec) {
         constexpr int N = Packet<T>::N;
 #pragma unroll
-        for (int i = 0; i < RUN / N; ++i) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + d0 + i * N), &x[c][i * N]);
+        for (int i = 0; i < 8 / N; ++i) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + d0 + i * N), &x[i * N]);
       } else {
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) x[c][i] = load_elem(qrow + (d0 + i) * a.q_dim);
+        for (int i = 0; i < 8; ++i) x[i] = load_elem(qrow + (d0 + i) * a.q_dim);
       }
 #pragma unroll
-      for (int i = 0; i < RUN; ++i) {
-        x[c][i] = __uint_as_float(__float_as_uint(x[c][i]) ^ p.q_sign);
-        amax = fmaxf(amax, finite_abs(x[c][i]));
-      }
-    }
-    if constexpr (WIDE) {
-      const float power = __uint_as_float(static_cast<uint32_t>(127 + p.q_exp) << 23);
-#pragma unroll
-      for (int c = 0; c < RUNS; ++c)
-#pragma unroll
-        for (int i = 0; i < RUN; ++i) x[c][i] *= power;
+      for (int i = 0; i < 8; ++i)  // infinities as NaN, which no other row's maximum takes up
+        x[i] = (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : x[i] * power;
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int c = 0; c < RUNS; ++c)
-#pragma unroll
-          for (int w = 0; w < 8; ++w) {
-            // The top 16 bits: the rest is exact, and the third part holds all of it.
-            const uint32_t lo = __float_as_uint(x[c][2 * w]), hi = __float_as_uint(x[c][2 * w + 1]);
-            qw[n][2 * c + w / 4][w % 4] = lo >> 16 | (hi & 0xffff0000u);
-            x[c][2 * w] -= __uint_as_float(lo & 0xffff0000u);
-            x[c][2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (NQ > 1) {  // the top 16 bits: the rest is exact, and the last part holds all of it
+            const uint32_t lo = __float_as_uint(x[2 * w]), hi = __float_as_uint(x[2 * w + 1]);
+            qw[n][c][w] = lo >> 16 | (hi & 0xffff0000u);
+            x[2 * w] -= __uint_as_float(lo & 0xffff0000u);
+            x[2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
+          } else {
+            qw[n][c][w] = MfmaOps<S>::pack2(x[2 * w], x[2 * w + 1]);
           }
-    } else {
-      amax = max_across_halves(amax);
-      const uint32_t b = max(scale_byte(amax), 4u * NQ + kMaxQExp);
-      const float inv = inverse_scale(b);
-#pragma unroll
-      for (int c = 0; c < KS; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          x[c][i] = (__float_as_uint(x[c][i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : x[c][i] * inv;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        q_scale[n] = min(static_cast<int>(b) + p.q_exp, 254) - 4 * n;
-#pragma unroll
-        for (int c = 0; c < KS; ++c)
-#pragma unroll
-          for (int w = 0; w < 8; ++w) {
-            float* y = &x[c][4 * w];
-            int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-            word = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], word, true);
-            qb[n][c][w] = word;
-            if (n + 1 < NQ) {
-              const f32x2v lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
-              y[0] = (y[0] - lo[0]) * 16.f, y[1] = (y[1] - lo[1]) * 16.f;
-              y[2] = (y[2] - hi[0]) * 16.f, y[3] = (y[3] - hi[1]) * 16.f;
-            }
-          }
-      }
+        }
     }
   }
 
@@ -376,40 +334,47 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const uint32_t block_bytes = static_cast<uint32_t>(a.kv_block), token_bytes = static_cast<uint32_t>(a.kv_token);
   const uint32_t s_block = static_cast<uint32_t>(a.s_block), s_token = static_cast<uint32_t>(a.s_token);
   const uint32_t page_mask = a.page - 1, last_key = max(wg_keys, 1) - 1, num_blocks = static_cast<uint32_t>(a.num_blocks);
-  uint32_t ids[PASSES] = {}, v_ids[PASSES], ks_id = 0;  // of the K tile loaded next, and of the one before it
+  uint32_t ids[PASSES];  // of the tile loaded next
   u32x4 kreg[PASSES], vreg[PASSES];
-  uint32_t vsreg[PASSES], ksreg;
+  uint32_t ksreg[PASSES], vsreg[PASSES];
   auto token = [&](int tile, int t) { return min(static_cast<uint32_t>(tile * kBN + t), last_key); };
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      v_ids[i] = ids[i];
-      ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
-    }
-    if (wave == 0) ks_id = trow[token(tile, lane) >> p.page_shift];
+    for (int i = 0; i < PASSES; ++i) ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
   };
-  auto load_k = [&](int tile, const uint32_t (&of)[PASSES], uint32_t ks_of, u32x4 (&k)[PASSES], uint32_t& ks) __attribute__((always_inline)) {
+  auto load_tile = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const uint64_t id = of[i] < num_blocks ? of[i] : 0;
-      k[i] = *reinterpret_cast<const u32x4*>(kbase + (id * block_bytes + __umul24(token(tile, i * TPP + st) & page_mask, token_bytes)));
+      const uint32_t slot = token(tile, i * TPP + st) & page_mask;
+      const uint64_t id = ids[i] < num_blocks ? ids[i] : 0;
+      const uint64_t at = id * block_bytes + __umul24(slot, token_bytes), s_at = id * s_block + __umul24(slot, s_token);
+      kreg[i] = *reinterpret_cast<const u32x4*>(kbase + at);
+      ksreg[i] = ksbase[s_at];
+      vreg[i] = *reinterpret_cast<const u32x4*>(vbase + at);
+      vsreg[i] = vsbase[s_at];
     }
-    if (wave == 0)
-      ks = ksbase[static_cast<uint64_t>(ks_of < num_blocks ? ks_of : 0) * s_block + __umul24(token(tile, lane) & page_mask, s_token)];
   };
-  auto load_v = [&](int tile) __attribute__((always_inline)) {
+  // Keys of 2^128 and more become the largest finite bf16: a score then is as large as fp32
+  // holds, and not NaN where q is 0.
+  auto store_k = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const uint32_t slot = token(tile, i * TPP + st) & page_mask, of = PIPE ? v_ids[i] : ids[i];
-      const uint64_t id = of < num_blocks ? of : 0;
-      vreg[i] = *reinterpret_cast<const u32x4*>(vbase + (id * block_bytes + __umul24(slot, token_bytes)));
-      vsreg[i] = vsbase[id * s_block + __umul24(slot, s_token)];
-    }
-  };
-  auto store_k = [&](int buf, const u32x4 (&k)[PASSES], uint32_t ks) __attribute__((always_inline)) {
+      u32x4 w[2];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(&k_lds[buf][(i * TPP + st) * KROW + sc * 16]) = k[i];
-    if (wave == 0) ks_lds[buf][lane] = static_cast<uint8_t>(ks);
+      for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = LATE ? f16_codes(kreg[i][e / 2], e % 2) : scaled_bf16(kreg[i][e / 2], ksreg[i], e % 2);
+      if constexpr (LATE) {
+        if (sc == 0) ks_lds[buf][i * TPP + st] = scale_value(ksreg[i]) * __uint_as_float(static_cast<uint32_t>(127 + p.q_exp) << 23);
+      } else if (__builtin_amdgcn_ballot_w64(ksreg[i] > 246u)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t x = w[e / 4][e % 4];
+          w[e / 4][e % 4] = x - ((x & 0x7fffu) == 0x7f80u ? 1u : 0u) - ((x >> 16 & 0x7fffu) == 0x7f80u ? 0x10000u : 0u);
+        }
+      }
+      uint16_t* dst = &k_lds[buf][(i * TPP + st) * KROW + sc * 16];
+      *reinterpret_cast<u32x4*>(dst) = w[0];
+      *reinterpret_cast<u32x4*>(dst + 8) = w[1];
+    }
   };
   // A V that is NaN must not reach the rows that do not see it through a product with 0:
   // in tiles that some row sees part of, it is stored as 0, and noted (see the end).
@@ -458,60 +423,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const int grp = lane >> 4, gl = lane & 15;
   const int tr_off = (4 * (grp >> 1) + (gl >> 2)) * VROW + 16 * (grp & 1) + 4 * (gl & 3);
 
-  // S^T of tile j: steps [from, to) over the dims, with between(i) after the i-th product.
-  auto scores = [&](int j, f32x16 (&s)[2], int from, int to, auto between) __attribute__((always_inline)) {
-    const int buf = j & 1;
-    if (from == 0) s[0] = s[1] = f32x16{};
-    if constexpr (WIDE) {
+  // S^T of tile j.
+  auto scores = [&](int buf, f32x16 (&s)[2]) __attribute__((always_inline)) {
+    s[0] = s[1] = f32x16{};
+#pragma unroll
+    for (int c = 0; c < KS; ++c)
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        const uint32_t ksc = ks_lds[buf][hh * 32 + col];
+        const u32x4 ka = *reinterpret_cast<const u32x4*>(&k_lds[buf][(hh * 32 + col) * KROW + 16 * c + 8 * half]);
 #pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          const u32x4 codes = *reinterpret_cast<const u32x4*>(&k_lds[buf][(hh * 32 + col) * KROW + 32 * c + 16 * half]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            u32x4 ka;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ka[e] = scaled_bf16(codes[2 * u + e / 2], ksc, e % 2);
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) s[hh] = Ops::mma(as_v8<bf16x8>(ka), as_v8<bf16x8>(qw[n][2 * c + u]), s[hh]);
-          }
-        }
+        for (int n = 0; n < NQ; ++n) s[hh] = MfmaOps<S>::mma(as_v8<typename MfmaOps<S>::V8>(ka), as_v8<typename MfmaOps<S>::V8>(qw[n][c]), s[hh]);
       }
-    } else {
-      const int ksc[2] = {ks_lds[buf][col], ks_lds[buf][32 + col]};
+    if constexpr (LATE) {
 #pragma unroll
-      for (int c = 0; c < KS; ++c) {
-        if (c < from || c >= to) continue;
-        i32x8 ka[2];
+      for (int g = 0; g < 8; ++g) {
+        const f32x4 k4 = *reinterpret_cast<const f32x4*>(&ks_lds[buf][8 * g + 4 * half]);
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const uint8_t* row = &k_lds[buf][(hh * 32 + col) * KROW + 64 * c + 32 * half];
-          const u32x4 lo = *reinterpret_cast<const u32x4*>(row), hi = *reinterpret_cast<const u32x4*>(row + 16);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) ka[hh][e] = static_cast<int>(lo[e]), ka[hh][4 + e] = static_cast<int>(hi[e]);
-        }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            s[hh] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[hh], qb[n][c], s[hh], 0, 0, 0, ksc[hh], 0, q_scale[n]);
-            between(n * 2 + hh);
-          }
+        for (int e = 0; e < 4; ++e) s[g / 4][g % 4 * 4 + e] *= k4[e];
       }
     }
   };
-  auto nothing = [](int) {};
-  auto step = [&](int j, f32x16 (&s)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
+  auto step = [&](int j) __attribute__((always_inline)) {
     const int buf = j & 1;
-    if (j + AHEAD < ntiles) load_k(j + AHEAD, ids, ks_id, kreg, ksreg);
     if (j + 1 < ntiles) {
-      load_v(j + 1);
-      load_ids(j + AHEAD + 1);
+      load_tile(j + 1);
+      load_ids(j + 2);
     }
     if (wave_live && j * kBN <= wave_last) {
-      if constexpr (!PIPE) scores(j, s, 0, KS, nothing);
+      f32x16 s[2];
+      scores(buf, s);
       // Element r of half hh is key key0 + 32 hh + 8 (r / 4) + 4 half + r % 4.
       const int key0 = j * kBN;
       const bool masked = uniform(key0 + kBN - 1 > prefix + wave_row0 || wave_row0 + 31 >= nq);
@@ -523,19 +463,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
           for (int r = 0; r < 16; ++r) s[hh][r] = hh * 32 + (r / 4) * 8 + r % 4 > lim ? -INFINITY : s[hh][r];
       }
       float tmax = -INFINITY;
-      auto max8 = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) tmax = fmaxf(tmax, s[i / 2][i % 2 * 8 + r]);
-        // (In this order: the compiler would put the products in one block, 870 TFLOP/s against 911.)
-        if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
-      };
-      if constexpr (PIPE) {
-        __builtin_amdgcn_sched_barrier(0);
-        scores(j + 1, next, 0, 1, max8);
-      } else {
+      for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) max8(i);
-      }
+        for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
       const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias_lds[buf]);
       tmax = max_across_halves(tmax) * p.qscale + fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
       const bool rescale = __builtin_amdgcn_ballot_w64(tmax > m + kRescale) != 0;
@@ -583,10 +514,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
       }
-      if constexpr (PIPE) {
-        __builtin_amdgcn_sched_barrier(0);
-        scores(j + 1, next, 1, KS, nothing);
-      }
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         u32x4 pb[NP];
@@ -599,43 +526,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         }
       }
     }
-    if (j + AHEAD < ntiles) store_k(j + AHEAD & 1, kreg, ksreg);
-    if (j + 1 < ntiles) store_v(buf ^ 1, tile_masked(j + 1));
+    if (j + 1 < ntiles) {
+      store_k(buf ^ 1);
+      store_v(buf ^ 1, tile_masked(j + 1));
+    }
     __syncthreads();
   };
 
-  f32x16 sa[2], sb[2];
   if (ntiles > first_tile) {
-    const int buf = first_tile & 1;
     load_ids(first_tile);
-    if constexpr (PIPE) {
-      const uint32_t ks_first = ks_id;
-      u32x4 k1[PASSES];
-      uint32_t ks1;
-      load_ids(first_tile + 1);
-      load_k(first_tile, v_ids, ks_first, kreg, ksreg);
-      load_v(first_tile);
-      load_k(first_tile + 1, ids, ks_id, k1, ks1);
-      load_ids(first_tile + 2);
-      store_k(buf, kreg, ksreg);
-      store_v(buf, tile_masked(first_tile));
-      store_k(buf ^ 1, k1, ks1);
-      __syncthreads();
-      scores(first_tile, sa, 0, KS, nothing);
-      __syncthreads();  // the tile after the next takes its place
-    } else {
-      load_k(first_tile, ids, ks_id, kreg, ksreg);
-      load_v(first_tile);
-      load_ids(first_tile + 1);
-      store_k(buf, kreg, ksreg);
-      store_v(buf, tile_masked(first_tile));
-      __syncthreads();
-    }
+    load_tile(first_tile);
+    load_ids(first_tile + 1);
+    store_k(first_tile & 1);
+    store_v(first_tile & 1, tile_masked(first_tile));
+    __syncthreads();
   }
-  for (int j = first_tile; j < ntiles; j += 2) {
-    step(j, sa, sb);
-    if (j + 1 < ntiles) step(j + 1, sb, sa);
-  }
+  for (int j = first_tile; j < ntiles; ++j) step(j);
 
   // V that was NaN in tiles that some row sees part of: it is NaN in the rows that see it.
   if (__syncthreads_or(nan)) {
@@ -786,7 +692,7 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   p.qscale = std::fabs(a.qscale);
   // A scale of 0 stands as 2^-126 2^-kMaxQExp: a finite score ends below 2^-22, a masked one stays -inf.
   const bool none = p.qscale == 0.f;
-  p.q_exp = none ? -kMaxQExp : std::isfinite(p.qscale) ? std::min(std::max(std::ilogb(p.qscale), -kMaxQExp), kMaxQExp) : 0;
+  p.q_exp = none ? -kMaxQExp : std::isfinite(p.qscale) ? std::min(std::max(std::ilogb(p.qscale), -kMaxQExp), 0) : 0;
   p.qscale = none ? std::numeric_limits<float>::min() : std::ldexp(p.qscale, -p.q_exp);
   p.q_sign = a.qscale < 0.f ? 0x80000000u : 0u;
   const int es = dtype_size(dtype);
