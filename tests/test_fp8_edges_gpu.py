@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+from fp8_cases import assert_within, attention
 from test_fp8_attention_gpu import DTYPES, Case
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +90,28 @@ def test_prefill_keys_of_two_to_the_128_take_all_the_weight(hq, hkv, d):
     v = (c.cache[1].float() * c.cache[3].float()[..., None])[at].repeat_interleave(hq // hkv, 0)
     assert torch.equal(out[10:].float(), v.bfloat16().float().expand(90, -1, -1))
     assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 128), (16, 2, 128), (4, 4, 64), (8, 2, 64), (2, 2, 256), (2, 2, 80)])
+def test_decode_keeps_its_probabilities_in_16_bits_or_more(dtype, hq, hkv, d):
+    # The bound of attention() with 2^-16 in place of half a step of q's type for a probability.
+    c = Case([1, 40, 700, 3000], hq, hkv, d, dtype=dtype, seed=21)
+    out = c.decode()
+    for r, n in enumerate(c.lengths):
+        assert_within(out[r : r + 1], *attention(c.q[r : r + 1], c.cache, c.tables[r], [n], c.scale, 2.0**-16))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 128), (16, 2, 128), (4, 4, 64)])
+@pytest.mark.parametrize("ahead", [0.3, 2.7, 5.1, 5.5])
+def test_a_key_that_dominates_late_weighs_what_it_should(hq, hkv, d, ahead):
+    # Key 300 scores `ahead` (natural units) above all others, which agree: the running maximum may still be theirs.
+    c = Case([400], hq, hkv, d, dtype=torch.bfloat16, seed=2)
+    kc, vc, ks, vs = (t.view(torch.uint8) for t in c.cache)
+    kc.zero_(), ks.fill_(127), vs.fill_(127), vc.copy_(torch.randint_like(vc, 0x30, 0x40))
+    at = (int(c.tables[0, 300 // 16]), 300 % 16)
+    kc[at] = torch.tensor(0x38, dtype=torch.uint8)  # ones
+    c.q = torch.full_like(c.q, 1.0)
+    c.scale = ahead / d
+    want, bound = attention(c.q, c.cache, c.tables[0], [400], c.scale, 2.0**-16)
+    assert_within(c.decode(), want, bound)

@@ -9,8 +9,10 @@
 //   scaled 8-bit MFMA would take codes and scales as they are, but drops what lies 2^-11
 //   below the largest product of its 128; the 16-bit ones keep fp32's bits.)
 // - O^T += V^T P^T on the bf16 MFMA (16x16x32): P stays in the registers S^T left it in,
-//   times its token's V scale, in one, two or three bf16 parts for bf16, fp16 and fp32; V's
-//   codes come from transposing 8-bit LDS reads and become bf16 exactly.
+//   times its token's V scale, in two bf16 parts (16 bits) for bf16 and fp16, three for fp32 (one
+//   part for bf16 would save 1% of a large call and 4% of a small one, and lose half a step of
+//   the output's type again); its sum is taken before that.  V's codes come from transposing
+//   8-bit LDS reads and become bf16 exactly.
 // Bytes bound it.  Tiles go from memory into LDS directly: K of the next one as soon as this
 // one's K is in registers, V likewise, one buffer each, so that a wave needs 8 KiB of LDS and
 // no registers for what is on its way, and sixteen waves a CU (twelve for fp32, eight at
@@ -36,7 +38,7 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
 // Parts of q and of P, and the type of the scores' operands.
 template <typename T> struct Parts;
-template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf16; };
+template <> struct Parts<bf16> { static constexpr int Q = 1, P = 2; using S = bf16; };
 template <> struct Parts<f16> { static constexpr int Q = 1, P = 2; using S = f16; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 3; using S = bf16; };
 
