@@ -115,3 +115,27 @@ def test_a_key_that_dominates_late_weighs_what_it_should(hq, hkv, d, ahead):
     c.scale = ahead / d
     want, bound = attention(c.q, c.cache, c.tables[0], [400], c.scale, 2.0**-16)
     assert_within(c.decode(), want, bound)
+
+
+SMALL = [(torch.bfloat16, -112), (torch.float32, -100), (torch.float32, -60)]
+
+
+def same_bits_of_small_values(c, call, dtype, shift):
+    """V times 2^shift: outputs times 2^shift, bit for bit, as far as they are normal numbers."""
+    vs = c.cache[3].view(torch.uint8)
+    usual = vs.clone()
+    big = call()
+    vs.copy_(torch.where(usual == 255, 255, usual + shift))
+    small = call()
+    assert big.isfinite().all()
+    want = big.double() * 2.0**shift
+    normal = want.abs() >= torch.finfo(dtype).smallest_normal
+    assert normal.float().mean() > 0.9
+    assert torch.equal(small[normal].double(), want[normal])
+
+
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("dtype,shift", SMALL)
+def test_decode_of_values_of_any_small_size_gives_the_same_bits(dtype, hq, hkv, d, shift):
+    c = Case([150, 1500, 30], hq, hkv, d, dtype=dtype, seed=5)
+    same_bits_of_small_values(c, c.decode, dtype, shift)

@@ -70,10 +70,11 @@ __global__ __launch_bounds__(64 * kGenericWaves) void attn8_generic_kernel(Attn8
     const float corr = fast_exp2(m - off);
     const float p = fast_exp2(dot - off);
     l = l * corr + p;
+    const float pv = p * kLift * sv;
 #pragma unroll
     for (int c = 0; c < kPerLane; ++c) {
       const int d = lane + 64 * c;
-      if (d < a.d) acc[c] = fmaf(p, code_value(a.v[base + d * a.kv_dim]) * sv, acc[c] * corr);
+      if (d < a.d) acc[c] = fmaf(pv, code_value(a.v[base + d * a.kv_dim]), acc[c] * corr);
     }
     m = mn;
   }
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(64 * kGenericWaves) void attn8_generic_kernel(Attn8
     weight[w] = fast_exp2(ms[w] - off);
     sum += ls[w] * weight[w];
   }
-  const float inv = 1.f / sum;
+  const float inv = 1.f / kLift / sum;
   for (int d = threadIdx.x; d < a.d; d += 64 * kGenericWaves) {
     float x = 0.f;
 #pragma unroll

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
         const float w = fast_exp2(dot - base);
         m = top;
         l = fmaf(l, corr, w);
-        const float pv = w * sv;  // this lane's row: its probability times its V scale
+        const float pv = w * kLift * sv;  // this lane's row: its probability times its V scale
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[e] *= corr;
 #pragma unroll
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
         y = fmaf(part[i][hd][d], w, y);
       }
       if (ns == 1) {
-        store_elem(orow + h * a.o_head + d * a.o_dim, len > 0 ? y * (1.f / sum) : 0.f);
+        store_elem(orow + h * a.o_head + d * a.o_dim, len > 0 ? y * (1.f / kLift / sum) : 0.f);
       } else {
         const int64_t at = (static_cast<int64_t>(r) * a.hkv + h) * p.splits + sp;
         p.ws_acc[at * D + d] = y;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(64 * kWaves) void decode8_merge_kernel(Decode8Args 
   const float top = group_max<64>(ml.x);
   const float off = top == -INFINITY ? 0.f : top;
   const float w = lane < ns ? fast_exp2(ml.x - off) : 0.f;
-  const float inv = 1.f / group_sum<64>(ml.y * w);
+  const float inv = 1.f / kLift / group_sum<64>(ml.y * w);
   for (int s0 = 0; s0 < ns; s0 += BATCH) {
     if (s0) load(s0);
 #pragma unroll

@@ -310,7 +310,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         for (int e = 0; e < 4; ++e) sv[u][e] = scale_value(b[e] & 255u);
       }
       float bias = 0.f;
-      if (__builtin_amdgcn_ballot_w64(vb > 191u)) bias = group_max<64>(value_bias(vb == 255u ? 0u : vb));
+      if (__builtin_amdgcn_ballot_w64(vb > kFreeScale)) bias = group_max<64>(value_bias(vb == 255u ? 0u : vb));
       top = strided_max<16>(top) + bias;
       if (__builtin_amdgcn_ballot_w64(top > m + kRescale) != 0) {
         const float mn = fmaxf(m, top);
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         for (int e = 0; e < 4; ++e) {
           w[e] = fast_exp2(s[u][e] - off);
           l += w[e];
-          w[e] *= sv[u][e];
+          w[e] = w[e] * kLift * sv[u][e];
         }
 #pragma unroll
         for (int i = 0; i < NP; ++i)
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
       }
       const int q = c0 + hd;  // of the KV head's
       if (ns == 1) {
-        store_elem(static_cast<T*>(a.out) + r * a.o_row + (h * G + q) * a.o_head + d * a.o_dim, len > 0 ? y * (1.f / sum) : 0.f);
+        store_elem(static_cast<T*>(a.out) + r * a.o_row + (h * G + q) * a.o_head + d * a.o_dim, len > 0 ? y * (1.f / kLift / sum) : 0.f);
       } else {
         const int64_t at = ((static_cast<int64_t>(r) * a.hkv + h) * p.splits + sp) * G + q;
         p.ws_acc[at * D + d] = y;

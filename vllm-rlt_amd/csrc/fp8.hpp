@@ -30,11 +30,15 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
   return __uint_as_float(b == 255u ? 0x7fc00000u : u);
 }
 
-// What a key whose V scale has byte b adds to its candidate for the running
-// maximum (log2 units): sums of p V stay below 2^72 a key, so a row of values
-// near the end of fp32 does not overflow before the division by sum p.  0 up to
-// a scale of 2^64.
-__device__ __forceinline__ float value_bias(uint32_t b) { return static_cast<float>(max(static_cast<int>(b) - 191, 0)); }
+// Sums of p V are kept kLift times as large, so that products with the smallest scales are
+// normal numbers (in bf16, too).  What a key whose V scale has byte b adds to its candidate for
+// the running maximum (log2 units): p V, lifted, stays below 2^81 a key, so a row of values near
+// the end of fp32 does not overflow before the division by sum p.  0 up to kFreeScale, 2^32.
+constexpr float kLift = 0x1p32f;
+constexpr uint32_t kFreeScale = 159;
+__device__ __forceinline__ float value_bias(uint32_t b) {
+  return static_cast<float>(max(static_cast<int>(b) - static_cast<int>(kFreeScale), 0));
+}
 
 // |x| where x is finite, 0 elsewhere: what a row's scale is taken over.
 __device__ __forceinline__ float finite_abs(float x) {
