@@ -139,3 +139,51 @@ def same_bits_of_small_values(c, call, dtype, shift):
 def test_decode_of_values_of_any_small_size_gives_the_same_bits(dtype, hq, hkv, d, shift):
     c = Case([150, 1500, 30], hq, hkv, d, dtype=dtype, seed=5)
     same_bits_of_small_values(c, c.decode, dtype, shift)
+
+
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("dtype,shift", SMALL)
+def test_prefill_of_values_of_any_small_size_gives_the_same_bits(dtype, hq, hkv, d, shift):
+    c = Case([150, 1500, 30], hq, hkv, d, dtype=dtype, seed=5, chunks=[100, 90, 30])
+    same_bits_of_small_values(c, c.prefill, dtype, shift)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("invariant", [False, True])
+def test_a_value_of_two_to_the_128_is_weighed_and_stays_with_the_rows_that_see_it(dtype, hq, hkv, d, invariant):
+    # What the append makes of the largest finite numbers: code 256, scale 2^120.  Key 120 of sequence 0 is seen by its
+    # rows from 70 on, key 2000 of sequence 1 by all but its first 10 rows, both in a head's last dim.
+    c = Case([150, 2080], hq, hkv, d, dtype=dtype, seed=8, chunks=[100, 90])
+    clean = c.prefill(batch_invariant=invariant)
+    for s, t, sign in ((0, 120, 0x78), (1, 2000, 0xF8)):
+        at = (int(c.tables[s, t // 16]), t % 16, hkv - 1)
+        c.cache[1].view(torch.uint8)[at] = 0
+        c.cache[1].view(torch.uint8)[at][d - 1] = sign
+        c.cache[3].view(torch.uint8)[at] = 247
+    out = c.prefill(batch_invariant=invariant)
+    heads = slice((hkv - 1) * (hq // hkv), hq)
+    sees = torch.zeros(out.shape[:2], dtype=torch.bool, device="cuda")
+    sees[70:100, heads] = True
+    sees[110:, heads] = True
+    others = [h for h in range(hq) if h // (hq // hkv) != hkv - 1]
+    assert torch.equal(out[:, others], clean[:, others]) and out[~sees].isfinite().all()
+    limits = [50 + i + 1 for i in range(100)], [1990 + i + 1 for i in range(90)]
+    for s, rows in ((0, slice(0, 100)), (1, slice(100, 190))):
+        want, bound = attention(c.q[rows], c.cache, c.tables[s], limits[s], c.scale, torch.finfo(dtype).eps / 2)
+        fits = want.abs() + bound < torch.finfo(dtype).max
+        assert fits[..., : d - 1].all()
+        assert not ((out[rows].double() - want).abs() > bound)[fits].any() and not out[rows].isnan().any()
+        past = want.abs() - bound > torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps)
+        assert out[rows][past].isinf().all()
+        if dtype != torch.float16:
+            assert fits.all()
+    # Decode: the last row of sequence 0 at a length that sees the key, and at one that does not.
+    from vllm_rlt_amd import ops
+
+    lens = torch.tensor([121, 120], dtype=torch.int32, device="cuda")
+    q = c.q[:1].repeat(2, 1, 1)
+    got = ops.paged_decode_fp8(q, *c.cache, c.tables[[0, 0]].contiguous(), lens, scale=c.scale)
+    want, bound = attention(q, c.cache, c.tables[0], [121, 120], c.scale, torch.finfo(dtype).eps / 2)
+    fits = want.abs() + bound < torch.finfo(dtype).max
+    assert not ((got.double() - want).abs() > bound)[fits].any() and not got.isnan().any() and fits[1].all()

@@ -9,8 +9,9 @@
 //   of q instead: 980 us for 877 below).  (The scaled 8-bit MFMA would take K's codes and scales
 //   as they are, but drops what lies 2^-11 below the largest product of its 64; the 16-bit
 //   ones keep fp32's bits.)
-// - O^T += V^T P^T likewise.  V becomes bf16 as K does; V^T comes from transposing LDS reads, P
-//   from the registers S^T left it in.  P is split in two or three bf16 parts for fp16 and fp32
+// - O^T += V^T P^T likewise.  V becomes bf16 as K does, kLift times as large (keys whose scale
+//   leaves no room for that get a larger weight instead, on a path of their own); V^T comes from
+//   transposing LDS reads, P from the registers S^T left it in.  P is split in two or three bf16 parts for fp16 and fp32
 //   outputs.  For bf16 ones it is rounded to bf16, as rlt_paged_prefill does, and its sum taken
 //   over the rounded values: outputs are off by 0.0023 of their rms, 0.0017 of it their own
 //   rounding, which is what two parts would leave for 27% more time (835 us for 655 below).
@@ -50,6 +51,9 @@ constexpr int kTargetItems = kRound * 3 / 2;
 // 14.0 / 13.6, of 128 over 4128 31.4 / 30.2 / 30.2 / 30.2, two of 20-100 over 200-1200 18.3 /
 // 18.7 / 18.5 / 23.3.
 constexpr int kMinSegTiles = 2;
+constexpr uint32_t kLargestScale = 246;  // the largest scale byte whose codes are all finite in bf16
+constexpr uint32_t kLiftExp = 32;        // kLift = 2^kLiftExp
+static_assert(kLift == static_cast<float>(uint64_t(1) << kLiftExp) && kLargestScale - kLiftExp > kFreeScale);
 constexpr int kPlanSeqs = 64;  // sequences ranked and cut: one a lane
 
 template <typename T> struct Parts;
@@ -234,6 +238,12 @@ __device__ __forceinline__ uint32_t f16_codes(uint32_t word, bool high) {
   return __builtin_bit_cast(uint32_t, r);
 }
 
+// x y, rounded also where the product is added to something.
+__device__ __forceinline__ float rounded_product(float x, float y) {
+#pragma clang fp contract(off)
+  return x * y;
+}
+
 // Elements d .. d + 3 of an out row.
 template <typename T>
 __device__ __forceinline__ void store4(T* orow, int d, const float (&x)[4], int64_t stride, bool vec) {
@@ -265,6 +275,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   __shared__ __align__(16) uint16_t v_lds[2][kBN * VROW];
   __shared__ __align__(16) float ks_lds[2][LATE ? kBN : 4];  // K's scales times 2^q_exp
   __shared__ __align__(16) float bias_lds[2][4];  // of each wave's staged V scales (value_bias)
+  __shared__ uint8_t vs_lds[2][kBN];              // and those scales' bytes, where that is not 0
 
   const Attn8Args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -365,7 +376,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
       for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = LATE ? f16_codes(kreg[i][e / 2], e % 2) : scaled_bf16(kreg[i][e / 2], ksreg[i], e % 2);
       if constexpr (LATE) {
         if (sc == 0) ks_lds[buf][i * TPP + st] = scale_value(ksreg[i]) * __uint_as_float(static_cast<uint32_t>(127 + p.q_exp) << 23);
-      } else if (__builtin_amdgcn_ballot_w64(ksreg[i] > 246u)) {
+      } else if (__builtin_amdgcn_ballot_w64(ksreg[i] > kLargestScale)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t x = w[e / 4][e % 4];
@@ -400,15 +411,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         }
       }
       u32x4 w[2];
+      const uint32_t lifted = vsreg[i] == 255u ? 255u : min(vsreg[i] + kLiftExp, kLargestScale);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = scaled_bf16(vreg[i][e / 2], vsreg[i], e % 2);
+      for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = scaled_bf16(vreg[i][e / 2], lifted, e % 2);
       uint16_t* dst = &v_lds[buf][t * VROW + sc * 16];
       *reinterpret_cast<u32x4*>(dst) = w[0];
       *reinterpret_cast<u32x4*>(dst + 8) = w[1];
       top = max(top, vsreg[i]);
     }
     float bias = 0.f;
-    if (__builtin_amdgcn_ballot_w64(top > kFreeScale)) bias = group_max<64>(value_bias(top == 255u ? 0u : top));
+    if (__builtin_amdgcn_ballot_w64(top > kFreeScale)) {
+      bias = group_max<64>(value_bias(top == 255u ? 0u : top));
+      if (sc == 0) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) vs_lds[buf][i * TPP + st] = static_cast<uint8_t>(vsreg[i]);
+      }
+    }
     if (lane == 0) bias_lds[buf][wave] = bias;
   };
   // Whether some row of the workgroup does not see all of a tile's keys.
@@ -469,7 +487,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 #pragma unroll
         for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
       const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias_lds[buf]);
-      tmax = max_across_halves(tmax) * p.qscale + fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+      const float bias = fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+      tmax = max_across_halves(tmax) * p.qscale + bias;
       const bool rescale = __builtin_amdgcn_ballot_w64(tmax > m + kRescale) != 0;
       float corr = 1.f;
       if (rescale) {
@@ -479,14 +498,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         lsum *= corr;
       }
       const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
-      // exp2(s * qscale - m) in one rounding, unless m's own is no longer small.
-      float qs = p.qscale;
-      if (__builtin_amdgcn_ballot_w64(fabsf(mb) > 4096.f) != 0) {
+      // exp2(s * qscale - m) in one rounding, unless m's own is no longer small.  Keys whose V is
+      // stored less than kLift as large weigh the more; the sum of the weights is taken before that.
+      float qs = p.qscale, whole = -1.f;  // that sum
+      if (__builtin_amdgcn_ballot_w64(fabsf(mb) > 4096.f || bias > value_bias(kLargestScale - kLiftExp)) != 0) {
         qs = 1.f;
+        whole = lsum;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[hh][r] *= p.qscale;
+          for (int r = 0; r < 16; ++r) {
+            s[hh][r] = rounded_product(s[hh][r], p.qscale);  // the same in both sums
+            const float x = fast_exp2(s[hh][r] - mb);
+            whole += NP == 1 ? bf16_lo(bf16_pair(x, x)) : x;
+            const int key = hh * 32 + r / 4 * 8 + 4 * half + r % 4;
+            const uint32_t b = b4[key % TPP / (TPP / 4)] > 0.f ? vs_lds[buf][key] : 0u;  // (of the wave that staged it)
+            s[hh][r] += static_cast<float>(max(b, kLargestScale - kLiftExp) - (kLargestScale - kLiftExp));
+          }
       }
       // P of k-step ks, in parts; its sum is taken over what the products see.
       auto weights = [&](int ks, u32x4 (&pb)[NP]) __attribute__((always_inline)) {
@@ -526,6 +554,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
           for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<bf16x8>(va), as_v8<bf16x8>(pb[n]), acc[c]);
         }
       }
+      if (whole >= 0.f) lsum = whole;
     }
     if (j + 1 < ntiles) {
       store_k(buf ^ 1);
@@ -579,7 +608,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     return;
   }
   // A row that sees no key is zeros.
-  const float inv = limit < 0 ? 0.f : 1.f / lsum;
+  const float inv = limit < 0 ? 0.f : 1.f / kLift / lsum;
   T* orow = static_cast<T*>(a.out) + (row0 + my_row) * a.o_row + h * a.o_head;
 #pragma unroll
   for (int c = 0; c < DT; ++c)
@@ -644,7 +673,7 @@ __global__ __launch_bounds__(256) void prefill8_merge_kernel(Prefill8Args p, int
     }
   }
   const bool blind = s.len - s.nq + i < 0;  // a row that sees no key
-  const float inv = 1.f / sum;
+  const float inv = 1.f / kLift / sum;
   float y[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = blind ? 0.f : acc[e] * inv;
