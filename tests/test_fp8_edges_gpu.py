@@ -187,3 +187,16 @@ def test_a_value_of_two_to_the_128_is_weighed_and_stays_with_the_rows_that_see_i
     want, bound = attention(q, c.cache, c.tables[0], [121, 120], c.scale, torch.finfo(dtype).eps / 2)
     fits = want.abs() + bound < torch.finfo(dtype).max
     assert not ((got.double() - want).abs() > bound)[fits].any() and not got.isnan().any() and fits[1].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_sequence_without_rows_does_not_change_how_the_others_are_cut(dtype):
+    # Balanced chunks beside one idle sequence of a long context: the bits of the batch without it.
+    lengths, chunks = [600] * 24, [128] * 24
+    c = Case([*lengths, 16000], 16, 4, 128, dtype=dtype, seed=4, chunks=[*chunks, 0])
+    from vllm_rlt_amd import ops
+
+    alone = ops.paged_prefill_fp8(c.q, *c.cache, c.tables[:24], c.lens[:24], c.cu[:25], 128, scale=c.scale)
+    beside = c.prefill()
+    assert torch.equal(alone, beside)
+    c.check(beside)

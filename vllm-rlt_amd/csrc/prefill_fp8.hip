@@ -128,7 +128,7 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
     // partial_slots() and of the grid.
     const float work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(
         static_cast<float>(s.tiles) * static_cast<float>(keys), [](float a, float b) { return a + b; })), 63)) * p.a.hq;
-    const int longest = __builtin_amdgcn_readlane(wave_scan(keys, [](int a, int b) { return max(a, b); }), 63);
+    const int longest = __builtin_amdgcn_readlane(wave_scan(s.tiles ? keys : 0, [](int a, int b) { return max(a, b); }), 63);
     // Cut where the longest item would outlast the others by half: 24 chunks of 100-170 rows
     // over up to 1000 keys (768 items of up to 18 tiles) took 66 us whole, 90 cut.
     if (longest * (2.f * p.round) > 3.f * work) {
