@@ -46,3 +46,17 @@ def test_the_stride_of_out_tables_goes_to_the_library_as_it_is(library, size):
         name, args = library.calls.pop()
         assert name == "rlt_build_chunk_metadata" and args[-2] == 8
         assert args[-3] == out.stride(0) or size == 1 and args[-3] >= 8
+
+
+@pytest.mark.parametrize("rows", [4 * ((1 << 24) - 1) + 1, (1 << 26) - 1])
+def test_appends_of_more_rows_than_a_grid_holds_are_refused(rows):
+    # Four rows a workgroup of 256 threads, of which a launch has fewer than 2^24.
+    from test_fp8_library import library, refused
+
+    lib, native = library()
+    s = native.int64_array([1 << 20, 1 << 18, 256, 64, 1])
+    x = native.int64_array([128, 64, 1])
+    refused(lib.rlt_kv_append_fp8(16, 16, s, 16, 16, s, 16, x, 16, x, 16, 16, rows, 0, 1, 4, 16, 2, 64, 2, None), native, "too many rows",
+            native.RLT_EUNSUPPORTED)
+    refused(lib.rlt_rope_axes_kv_append(16, 16, s, 16, 16, s, 16, x, 16, x, 16, x, 16, x, 16, x, 1, 16, 10, bytes(32), 32, 16, 16, rows,
+                                        rows, 0, 1, 4, 16, 2, 2, 64, 2, None), native, "too many rows", native.RLT_EUNSUPPORTED)

@@ -293,7 +293,8 @@ int append_args(const char* name, void* key_cache, void* value_cache, const int6
   if (d > 2 * kMaxHalf) return fail(RLT_EUNSUPPORTED, "%s: head_dim above %d", name, 2 * kMaxHalf);
   if (num_blocks <= 0 || num_layers <= 0 || page_size <= 0) return fail(RLT_EINVAL, "%s: pool dimensions must be positive", name);
   if (layer < 0 || layer >= num_layers) return fail(RLT_EINVAL, "%s: layer %lld out of range", name, (long long)layer);
-  if (n_rows >= int64_t(1) << 26 || hkv > 16384) return fail(RLT_EUNSUPPORTED, "%s: too many rows or heads", name);
+  // (A wave a row in workgroups of four, and one a row and head: threads of a launch inside 32 bits.)
+  if (n_rows > 4 * kMaxBlocks || hkv > 16384) return fail(RLT_EUNSUPPORTED, "%s: too many rows or heads", name);
   if (n_rows == 0) return RLT_OK;
   if (!key_cache || !value_cache || !cache_strides || !k || !k_strides || !v || !v_strides ||
       (n_write > 0 && (!write_blocks || !write_offsets)) || !key_scales != !value_scales || (key_scales && !scale_strides))
