@@ -2,6 +2,7 @@
 
 import contextlib
 
+import numpy as np
 import pytest
 import torch
 
@@ -46,6 +47,24 @@ def test_the_stride_of_out_tables_goes_to_the_library_as_it_is(library, size):
         name, args = library.calls.pop()
         assert name == "rlt_build_chunk_metadata" and args[-2] == 8
         assert args[-3] == out.stride(0) or size == 1 and args[-3] >= 8
+
+
+@pytest.mark.parametrize("kind", [tuple, list, bytes, torch.tensor, np.array, lambda x: np.array(x, dtype=np.int32)])
+def test_axes_of_any_sequence_go_to_the_library_as_one_byte_each(library, kind):
+    # An array's own bytes would be eight or four an axis.
+    from vllm_rlt_amd import ops
+
+    cache = torch.zeros(2, 1, 16, 1, 8)
+    x, one = torch.zeros(1, 1, 8), torch.zeros(1, dtype=torch.int64)
+
+    def rope(axes):
+        ops.rope_axes_kv_append(cache, cache.clone(), 0, one, one, x, x, x, one[:, None].expand(1, 3), torch.zeros(5, 4, 2), axes)
+        return next(a for a in library.calls.pop()[1] if isinstance(a, bytes))
+
+    assert rope(kind((0, 1, 2, 1))) == bytes([0, 1, 2, 1])
+    for bad in ([0, 1, 2, -1], [0, 1, 2, 256], np.array([0, 1, 2, 300])):
+        with pytest.raises(ValueError):
+            rope(bad)
 
 
 @pytest.mark.parametrize("rows", [4 * ((1 << 24) - 1) + 1, (1 << 26) - 1])

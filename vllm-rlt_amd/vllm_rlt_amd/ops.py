@@ -1194,7 +1194,7 @@ def rope_axes_kv_append(
             None if key_scales is None else int64_array(key_scales.stride()),
             q.data_ptr(), int64_array(q.stride()), k.data_ptr(), int64_array(k.stride()), v.data_ptr(),
             int64_array(v.stride()), out.data_ptr(), int64_array(out.stride()), positions.data_ptr(),
-            int64_array(positions.stride()), positions.shape[1], table.data_ptr(), table.shape[0], bytes(axes), half,
+            int64_array(positions.stride()), positions.shape[1], table.data_ptr(), table.shape[0], bytes(list(axes)), half,
             write_blocks.data_ptr(), write_offsets.data_ptr(), rows, n, layer, nl, nb, page, q.shape[1], hkv, d,
             dtype_code(q.dtype), stream_handle(device),
         )
