@@ -79,3 +79,12 @@ def test_appends_of_more_rows_than_a_grid_holds_are_refused(rows):
             native.RLT_EUNSUPPORTED)
     refused(lib.rlt_rope_axes_kv_append(16, 16, s, 16, 16, s, 16, x, 16, x, 16, x, 16, x, 16, x, 1, 16, 10, bytes(32), 32, 16, 16, rows,
                                         rows, 0, 1, 4, 16, 2, 2, 64, 2, None), native, "too many rows", native.RLT_EUNSUPPORTED)
+
+
+@pytest.mark.parametrize("rows,seqs,width,heads,d,most", [(32768, 32, 256, 32, 128, 100), (4096, 8, 1056, 16, 128, 82), (1 << 18, 64, 4096, 16, 64, 52)])
+def test_the_prefill_workspace_holds_cut_sequences_only(rows, seqs, width, heads, d, most):
+    # MiB, whatever the rows: 2 * 128 * 768 / heads rows of partials of 4 (d + 2) bytes a head.
+    from test_fp8_library import library
+
+    lib, _ = library()
+    assert 0 < lib.rlt_paged_prefill_fp8_workspace_bytes(rows, seqs, width, heads, heads, d, 16) <= most << 20

@@ -680,13 +680,16 @@ __global__ __launch_bounds__(256) void prefill8_merge_kernel(Prefill8Args p, int
   store4(static_cast<T*>(a.out) + row * a.o_row + h * a.o_head, d, y, a.o_dim, p.out_vec);
 }
 
-// Partial rows that a launch can need: a sequence's rows once a segment.  Segments
-// are at least (all work) / kTargetItems, so those past each sequence's first cover at
-// most 128 kTargetItems / hq rows; and no sequence has more than its table's keys.
+// Partial rows that a launch can need: a cut sequence's rows once a segment.  It has more keys
+// than a segment, which is at least (all work) / kTargetItems: so its segments are fewer than
+// twice its keys over a segment's, and those of all sequences, times their query tiles, fewer
+// than 2 kTargetItems / hq; those past each sequence's first, fewer than half as many.  No
+// sequence has more segments than its table's keys allow.
 int64_t partial_slots(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq) {
   const int64_t most = ((max_len + kBN - 1) / kBN + kMinSegTiles - 1) / kMinSegTiles;
   if (num_seqs > kPlanSeqs || most < 2) return 0;
-  return std::min(rows * most, rows + (kBM * kTargetItems + hq - 1) / hq + 64);
+  constexpr int64_t cut = kBM * kTargetItems;
+  return std::min({rows * most, rows + (cut + hq - 1) / hq + 64, (2 * cut + hq - 1) / hq + 64});
 }
 
 }  // namespace
