@@ -47,13 +47,14 @@ constexpr int kXcds = 8;
 constexpr int kRound = 512;  // workgroups that run at once: two a CU (fp32 at head_dim 128: one)
 constexpr int kTargetItems = kRound * 3 / 2;
 // Shorter segments are not worth an item (about 9 us of plan, first loads and merge beside
-// 1.5 a tile).  Measured, us, in 4 / 3 / 2 / 1: one chunk of 40 rows over 340 keys 15.4 / 15.4 /
-// 14.0 / 13.6, of 128 over 4128 31.4 / 30.2 / 30.2 / 30.2, two of 20-100 over 200-1200 18.3 /
-// 18.7 / 18.5 / 23.3.
+// 1.5 a tile).  Measured, us, in 4 / 3 / 2 / 1: one chunk of 40 rows over 340 keys 14.8 / 14.9 /
+// 13.2 / 12.5, of 128 over 4128 30.3 / 28.0 / 28.1 / 28.0, two of 20-100 over 200-1200 17.9 /
+// 17.8 / 17.2 / 21.0.
 constexpr int kMinSegTiles = 2;
 constexpr uint32_t kLargestScale = 246;  // the largest scale byte whose codes are all finite in bf16
 constexpr uint32_t kLiftExp = 32;        // kLift = 2^kLiftExp
 static_assert(kLift == static_cast<float>(uint64_t(1) << kLiftExp) && kLargestScale - kLiftExp > kFreeScale);
+constexpr int64_t kMergeRound = 2048;  // workgroups of the merge that run at once
 constexpr int kPlanSeqs = 64;  // sequences ranked and cut: one a lane
 
 template <typename T> struct Parts;
@@ -130,11 +131,11 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
         static_cast<float>(s.tiles) * static_cast<float>(keys), [](float a, float b) { return a + b; })), 63)) * p.a.hq;
     const int longest = __builtin_amdgcn_readlane(wave_scan(s.tiles ? keys : 0, [](int a, int b) { return max(a, b); }), 63);
     // Cut where the longest item would outlast the others by half: 24 chunks of 100-170 rows
-    // over up to 1000 keys (768 items of up to 18 tiles) took 66 us whole, 90 cut.
+    // over up to 1000 keys (768 items of up to 18 tiles) take 55 us whole, 69 cut.
     if (longest * (2.f * p.round) > 3.f * work) {
       // Few items: cut into one round of workgroups.  Many, of different lengths: into half as
-      // many again, so that the short ones fill the gaps (eight chunks 444 us in 512, 392
-      // in 768, 431 in 1024; one chunk of 64 items 112, 134, 129).
+      // many again, so that the short ones fill the gaps (eight chunks 402 us in 512, 353
+      // in 768, 369 in 1024; one chunk of 64 items 96, 119, 109).
       const bool few = __builtin_amdgcn_readlane(scan_sum(s.tiles), 63) * p.a.hq <= p.round / 2;
       int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few ? p.round : p.round * 3 / 2)), 1e9f)));
       for (int i = 0; few && i < 4; ++i) {  // as rounding up makes more items, towards the round
@@ -622,62 +623,68 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     }
 }
 
-// Joins the segments of cut sequences: a workgroup takes 1024 neighbouring elements of a
-// row, 4 a thread, and adds the segments in order under a running maximum, BATCH of them on
-// their way at once.  Bytes and latency bound it: eight chunks of 512 rows over 0-16384 keys
-// x 16 heads 13.9 us (20.8 with a wave a row and head).
+// Joins the segments of cut sequences: a workgroup takes 1024 neighbouring elements of a row
+// at a time, 4 a thread, and adds the segments in order under a running maximum, BATCH of them
+// on their way at once.  Bytes and latency bound it: eight chunks of 512 rows over 0-16384 keys
+// x 16 heads 12.9 us.  The grid is one round at most and walks the rows of cut sequences only:
+// 16 chunks of 512 rows, none of them cut, take 64 us, 67 with workgroups for every row.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefill8_merge_kernel(Prefill8Args p, int parts) {
   constexpr int BATCH = 4;
   const Attn8Args& a = p.a;
   const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x / parts, e0 = (blockIdx.x % parts * 256 + static_cast<int>(threadIdx.x)) * 4;
-  int first = 0, n = 0;
-  if (lane < a.num_seqs) first = p.plan[lane].row0, n = p.plan[lane].nq;
-  const uint64_t hit = __builtin_amdgcn_ballot_w64(row >= first && row < first + n);
-  if (!hit) return;
-  const SeqPlan s = p.plan[__builtin_ctzll(hit)];
-  const int h = e0 / D, d = e0 % D, i = row - s.row0;
-  if (s.segs < 2 || h >= a.hq) return;
-  // Segments past the last key of the row's query tile were not computed.
-  const int keys = max(s.len - s.nq + min(i / kBM * kBM + kBM, s.nq), 0);
-  const int seg_keys = s.seg_tiles * kBN;
-  const int live = min(s.segs, max(1, (keys + seg_keys - 1) / seg_keys));
-  const int64_t step = static_cast<int64_t>(s.nq) * a.hq;  // slots from one segment to the next
-  const int64_t base = (static_cast<int64_t>(s.slot0) + i) * a.hq + h;
-  float m = -INFINITY, sum = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int g0 = 0; g0 < live; g0 += BATCH) {
-    float2 ml[BATCH];
-    f32x4 x[BATCH];
+  SeqPlan s{};
+  if (lane < a.num_seqs) s = p.plan[lane];
+  const int rows = s.segs > 1 ? s.nq : 0, last = scan_sum(rows), first = last - rows;
+  const int64_t items = static_cast<int64_t>(__builtin_amdgcn_readlane(last, 63)) * parts;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int r = static_cast<int>(item / parts), e0 = (static_cast<int>(item % parts) * 256 + static_cast<int>(threadIdx.x)) * 4;
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(r >= first && r < last));
+    const int nq = __builtin_amdgcn_readlane(s.nq, at), len = __builtin_amdgcn_readlane(s.len, at);
+    const int segs = __builtin_amdgcn_readlane(s.segs, at), slot0 = __builtin_amdgcn_readlane(s.slot0, at);
+    const int seg_keys = __builtin_amdgcn_readlane(s.seg_tiles, at) * kBN;
+    const int i = r - __builtin_amdgcn_readlane(first, at), row = __builtin_amdgcn_readlane(s.row0, at) + i;
+    const int h = e0 / D, d = e0 % D;
+    if (h >= a.hq) continue;
+    // Segments past the last key of the row's query tile were not computed.
+    const int keys = max(len - nq + min(i / kBM * kBM + kBM, nq), 0);
+    const int live = min(segs, max(1, (keys + seg_keys - 1) / seg_keys));
+    const int64_t step = static_cast<int64_t>(nq) * a.hq;  // slots from one segment to the next
+    const int64_t base = (static_cast<int64_t>(slot0) + i) * a.hq + h;
+    float m = -INFINITY, sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int g0 = 0; g0 < live; g0 += BATCH) {
+      float2 ml[BATCH];
+      f32x4 x[BATCH];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int64_t slot = base + min(g0 + u, live - 1) * step;
-      ml[u] = p.part_ml[slot];
-      x[u] = *reinterpret_cast<const f32x4*>(p.part_acc + slot * D + d);
+      for (int u = 0; u < BATCH; ++u) {
+        const int64_t slot = base + min(g0 + u, live - 1) * step;
+        ml[u] = p.part_ml[slot];
+        x[u] = *reinterpret_cast<const f32x4*>(p.part_acc + slot * D + d);
+      }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) top = fmaxf(top, ml[u].x);
+      const float off = top == -INFINITY ? 0.f : top;
+      const float corr = fast_exp2(m - off);
+      m = top;
+      sum *= corr;
+      acc *= corr;
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const float w = g0 + u < live ? fast_exp2(ml[u].x - off) : 0.f;
+        sum = fmaf(ml[u].y, w, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = g0 + u < live ? fmaf(x[u][e], w, acc[e]) : acc[e];
+      }
     }
-    float top = m;
+    const bool blind = len - nq + i < 0;  // a row that sees no key
+    const float inv = 1.f / kLift / sum;
+    float y[4];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) top = fmaxf(top, ml[u].x);
-    const float off = top == -INFINITY ? 0.f : top;
-    const float corr = fast_exp2(m - off);
-    m = top;
-    sum *= corr;
-    acc *= corr;
-#pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const float w = g0 + u < live ? fast_exp2(ml[u].x - off) : 0.f;
-      sum = fmaf(ml[u].y, w, sum);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = g0 + u < live ? fmaf(x[u][e], w, acc[e]) : acc[e];
-    }
+    for (int e = 0; e < 4; ++e) y[e] = blind ? 0.f : acc[e] * inv;
+    store4(static_cast<T*>(a.out) + row * a.o_row + h * a.o_head, d, y, a.o_dim, p.out_vec);
   }
-  const bool blind = s.len - s.nq + i < 0;  // a row that sees no key
-  const float inv = 1.f / kLift / sum;
-  float y[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = blind ? 0.f : acc[e] * inv;
-  store4(static_cast<T*>(a.out) + row * a.o_row + h * a.o_head, d, y, a.o_dim, p.out_vec);
 }
 
 // Partial rows that a launch can need: a cut sequence's rows once a segment.  It has more keys
@@ -734,8 +741,9 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   // Query tiles, and the segments past the first (as many items as partial_slots() has such rows).
   const int64_t tiles = a.rows / kBM + std::min<int64_t>(a.num_seqs, a.rows) + (slots ? (kTargetItems + a.hq - 1) / a.hq + 2 : 0);
   const int parts = static_cast<int>((static_cast<int64_t>(a.hq) * a.d + 1023) / 1024);
-  if (tiles * a.hq > kMaxBlocks || (slots && a.rows * parts > kMaxBlocks)) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
-  const dim3 grid(static_cast<unsigned>(tiles * a.hq)), merge(static_cast<unsigned>(a.rows * parts)), block(256);
+  if (tiles * a.hq > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  const dim3 grid(static_cast<unsigned>(tiles * a.hq)), block(256);
+  const dim3 merge(static_cast<unsigned>(std::min<int64_t>(a.rows * parts, kMergeRound)));
 #define LAUNCH_D(T, D)                                                                                   \
   do {                                                                                                   \
     hipLaunchKernelGGL((prefill8_kernel<T, D>), grid, block, 0, stream, p);                              \
