@@ -200,3 +200,10 @@ def test_a_sequence_without_rows_does_not_change_how_the_others_are_cut(dtype):
     beside = c.prefill()
     assert torch.equal(alone, beside)
     c.check(beside)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(3, 1, 64), (9, 9, 128)])
+def test_a_merge_of_more_rows_than_its_grid_holds(hq, hkv, d):
+    # Heads that do not fill the merge's 1024 elements, two cut sequences with an uncut one between.
+    c = Case([5000, 30, 4000], hq, hkv, d, seed=14, chunks=[2000, 30, 500])
+    c.check(c.prefill())
