@@ -545,6 +545,7 @@ int rlt_rope_axes_kv_append(void* key_cache, void* value_cache, const int64_t* c
  * rlt_paged_decode over a layer slice of an 8-bit cache; q and out are of `dtype`.
  * A row of length 0 (or less) is written as zeros; lengths are clamped to what the
  * table covers.  A row's output bits depend on its own q, pages and length only.
+ * Scores and sums are fp32; a probability has 16 bits or more (24 for an fp32 q).
  * The workspace (rlt_paged_decode_fp8_workspace_bytes, a function of the shape)
  * holds the partials of cut rows; calls that overlap need one each.
  */
@@ -563,11 +564,19 @@ int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, const void* ke
  * right causal.  Query row i of sequence s's n_q sees keys 0 .. context_lengths[s]
  * - n_q + i; one that sees none is written as zeros.  Rows of no sequence (at or
  * past cu_seqlens_q[num_seqs]) are left as they were; cu_seqlens_q rises from 0 to at
- * most total_q.  The workspace
- * (rlt_paged_prefill_fp8_workspace_bytes, on 16 bytes; calls that overlap need one
- * each) holds the partials of long sequences, whose keys are cut by the launch's
- * shapes: a row's last bits may depend on what shares its launch.  With a NULL
- * workspace none is cut, and they depend on its own sequence only.
+ * most total_q.  Lengths are clamped to what the table covers, and the rows' limits
+ * move with them.  max_seqlen_q is rlt_paged_prefill's: it must not be negative, and
+ * nothing else depends on it.
+ * Scores and sums are fp32; a probability is held in 16 bits for an fp16 q and 24 for
+ * an fp32 one, and rounded to bf16 for a bf16 one, as in rlt_paged_prefill.  Keys of
+ * 2^128 and more (the append makes that of the largest finite numbers) count as bf16's
+ * largest number where q is bf16 or fp32.
+ * The workspace (rlt_paged_prefill_fp8_workspace_bytes, on 16 bytes; calls that
+ * overlap need one each) holds the partials of long sequences, whose keys are cut by
+ * the launch's shapes: a row's last bits may depend on what shares its launch.  It is
+ * at most 768 KiB * (head_dim + 2) whatever the rows (98 MiB at head_dim 128), and 64
+ * rows of it more.  With a NULL workspace none is cut, and the bits depend on the row's
+ * own sequence only.
  */
 int64_t rlt_paged_prefill_fp8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
                                               int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
@@ -594,7 +603,9 @@ int rlt_paged_prefill_fp8(const void* q, const int64_t* q_strides, const void* k
  *   out_tables [size, out_width]  int32
  * Sequences count .. size - 1 are padding: no tokens, length 0, a table row of 0.
  * Tokens behind the last sequence get position 0, sequence -1, block -1 (an append
- * skips them).  A descriptor outside the tables keeps its tokens in the packing but
+ * skips them).  out_width has to cover the longest sequence (start + tokens, in
+ * pages): lengths do not shrink with it, and attention over rows that are too short
+ * for them clamps them.  A descriptor outside the tables keeps its tokens in the packing but
  * gets length 0, a table row of 0 and block -1, position 0; tokens past `capacity`
  * are dropped from the end, in cu_seqlens and lengths as well.
  */

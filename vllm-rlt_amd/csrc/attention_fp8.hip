@@ -1,8 +1,9 @@
 // Attention over the 8-bit paged KV cache (codes and scales: fp8.hpp):
 //   s_j = scale * q . (K_j 2^ek_j),  out = sum_j softmax(s)_j (V_j 2^ev_j)
 // over a sequence's keys, for one new token a sequence (decode) and for packed
-// chunks, bottom-right causal (prefill).  Scores, softmax sums and outputs are
-// fp32; the scales multiply the score and the probability of their token.
+// chunks, bottom-right causal (prefill).  Scores, softmax sums and the sums of p V are
+// fp32, outputs of q's type; the scales multiply the score and the probability of their
+// token, or become part of a bf16 that holds their code exactly.
 #include "decode_fp8.hpp"
 #include "fp8.hpp"
 #include "prefill_fp8.hpp"
@@ -14,7 +15,7 @@ namespace {
 // workgroup a (row, query head), wave w takes tokens w, w + kGenericWaves, ...
 // with the head's dims over its lanes and a running maximum and sum of its own;
 // the waves are joined through LDS in wave order.  Every query head reads its keys itself, a
-// byte a lane: latency bounds it (64 rows of 512-4096 tokens, 16 heads x 80: 1117 us).
+// byte a lane: latency bounds it (64 rows of 512-4096 tokens, 16 heads x 80: 1112 us).
 constexpr int kPerLane = 8;
 constexpr int kGenericWaves = 8;
 

@@ -353,10 +353,11 @@ bool decode8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page) {
 }
 
 // Which kernel.  The matrix cores leave 15 columns of 16 empty for one query head a KV head,
-// and pay there only from head_dim 128 on.  Measured, us, vector units / matrix cores: 16
-// heads x 64, 64 rows of 512-4096 tokens 62 / 82; 16 x 128 121 / 115, 256 rows of 1024-8192
-// 850 / 831, 16 of up to 512 11.9 / 9.5, 4 of up to 256 6.5 / 6.6, 1 of 1000 10.3 / 11.8; 16 +
-// 8 heads x 64, 64 rows of 512-4096 54 / 45.
+// and pay there only from head_dim 128 on, where all but the smallest launches gain and a
+// single row loses.  Measured, us, vector units / matrix cores: 16 heads x 64, 64 rows of
+// 512-4096 tokens 64 / 90; 16 x 128 121 / 116, 256 rows of 1024-8192 850 / 821, 16 of up to 512
+// 11.9 / 10.3, 4 of up to 256 6.5 / 6.9, 1 of 1000 10.3 / 12.4; 16 + 8 heads x 64, 64 rows of
+// 512-4096 54 / 48.
 bool on_matrix_cores(int64_t hq, int64_t hkv, int64_t d) { return hq > hkv || d > 64; }
 int split_base(int64_t hq, int64_t hkv, int64_t d) { return on_matrix_cores(hq, hkv, d) ? kMfmaSplit : kParts * kUnit; }
 

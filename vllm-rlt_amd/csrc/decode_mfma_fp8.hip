@@ -18,8 +18,8 @@
 // no registers for what is on its way, and sixteen waves a CU (twelve for fp32, eight at
 // head_dim 256) keep 128 KiB in flight.  The heads of a row's split run on one XCD at the
 // same time, which reads whole token rows of the cache: 256 rows of 1024-8192 tokens, 16 + 8
-// heads x 128, took 471 us with a head an XCD, 418 (5.8 TB/s) so.  24 rows of 512-4096, 32 + 8
-// heads, fp16, 114 MB, take 30 us and the merge 5.
+// heads x 128, take 468 us with a head an XCD, 440 (5.5 TB/s) so.  24 rows of 512-4096, 32 + 8
+// heads, fp16, 114 MB, take 32 us, 4.6 of them the merge.
 #include <type_traits>
 
 #include "decode_fp8.hpp"

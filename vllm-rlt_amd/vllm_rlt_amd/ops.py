@@ -984,6 +984,7 @@ def build_chunk_metadata(
     behind the last sequence get position 0, sequence -1, block -1 and offset 0, so
     an append of the whole buffer skips them; tokens past it are dropped from the
     end, and lengths count the others.  Sequences from count on are padding: no tokens, length 0.
+    out_width has to cover the longest sequence in pages: lengths do not shrink with it.
     """
     host, stream = _host_calls(tables)
     if host is not None:
@@ -1131,7 +1132,7 @@ def rope_axes_kv_append(
     [max_position, half, 2] of (cos, sin), computed once from the angles
     position * inv_freq in float64.  axes: for each of the `half` frequencies the
     axis whose position turns it, e.g. (0,) * 24 + (1,) * 20 + (2,) * 20, or
-    interleaved.  Frequency j turns the dims j and j + half of a head; dims past
+    interleaved; any sequence of whole numbers, a tuple is the quickest.  Frequency j turns the dims j and j + half of a head; dims past
     2 * half pass through.  Products and sums are rounded to float32, results once to
     the type they are stored in (rope_kv_append rounds to the storage type after
     each step).
@@ -1260,7 +1261,8 @@ def paged_decode_fp8(
     Codes torch.float8_e4m3fn [blocks, page, kv_heads, head_dim], scales
     torch.float8_e8m0fnu [blocks, page, kv_heads] (kv_append_fp8); q float32, float16
     or bfloat16.  Returns a new tensor like q unless out is given; a row of length 0
-    is zeros.  `workspace` (decode_fp8_workspace_bytes) holds the partials of long
+    is zeros.  Scores and sums are float32, a probability has 16 bits or more (24 for
+    float32 q).  `workspace` (decode_fp8_workspace_bytes) holds the partials of long
     rows and is allocated here unless given.  A row's output bits depend on its own
     q, pages and length only.
     """
@@ -1326,11 +1328,15 @@ def paged_prefill_fp8(
     The cache is paged_decode_fp8's; the new tokens' keys are in it already.  Query row
     i of a sequence's n sees its keys up to context_length - n + i; one that sees
     none is zeros.  Rows of no sequence (from cu_seqlens_q[-1] on) are left as they
-    are in `out`.  max_seqlen_q is at least the longest chunk.
+    are in `out`.  max_seqlen_q is paged_prefill's: not negative, and without effect.
 
-    `workspace` (prefill_fp8_workspace_bytes) holds the partials of sequences whose keys
-    are cut, by the launch's shapes, and is allocated here unless given.  With
-    `batch_invariant` none is cut: a row's bits depend on its own sequence only.
+    Scores and sums are float32; a probability is held in 16 bits for float16 q, 24 for
+    float32, and rounded to bfloat16 for bfloat16, as in paged_prefill.
+
+    `workspace` (prefill_fp8_workspace_bytes, at most about 98 MiB at head_dim 128) holds
+    the partials of sequences whose keys are cut, by the launch's shapes, and is
+    allocated here unless given.  With `batch_invariant` none is cut: a row's bits
+    depend on its own sequence only.
     """
     host, stream = _host_calls(q)
     if host is not None:
