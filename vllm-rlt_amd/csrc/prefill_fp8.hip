@@ -11,10 +11,11 @@
 //   ones keep fp32's bits.)
 // - O^T += V^T P^T likewise.  V becomes bf16 as K does, kLift times as large (keys whose scale
 //   leaves no room for that get a larger weight instead, on a path of their own); V^T comes from
-//   transposing LDS reads, P from the registers S^T left it in.  P is split in two or three bf16 parts for fp16 and fp32
-//   outputs.  For bf16 ones it is rounded to bf16, as rlt_paged_prefill does, and its sum taken
-//   over the rounded values: outputs are off by 0.0023 of their rms, 0.0017 of it their own
-//   rounding, which is what two parts would leave for 27% more time (835 us for 655 below).
+//   transposing LDS reads, P from the registers S^T left it in.  P is split in two or three bf16
+//   parts for fp16 and fp32 outputs.  For bf16 ones it is rounded to bf16, as rlt_paged_prefill
+//   does, and its sum taken over the rounded values: outputs are off by 0.0023 of their rms.
+//   Their own rounding is 0.0017 of it, which two parts would come down to for 27% more time (835
+//   us for 655 below).
 // The running maximum moves only when a tile's exceeds it by 2^kRescale.
 //
 // The products' rate and the vector work beside them bound it (a tile of a wave is 1024 cycles of

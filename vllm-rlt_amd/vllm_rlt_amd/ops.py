@@ -1132,10 +1132,10 @@ def rope_axes_kv_append(
     [max_position, half, 2] of (cos, sin), computed once from the angles
     position * inv_freq in float64.  axes: for each of the `half` frequencies the
     axis whose position turns it, e.g. (0,) * 24 + (1,) * 20 + (2,) * 20, or
-    interleaved; any sequence of whole numbers, a tuple is the quickest.  Frequency j turns the dims j and j + half of a head; dims past
-    2 * half pass through.  Products and sums are rounded to float32, results once to
-    the type they are stored in (rope_kv_append rounds to the storage type after
-    each step).
+    interleaved; any sequence of whole numbers, a tuple is the quickest.  Frequency j
+    turns the dims j and j + half of a head; dims past 2 * half pass through.  Products
+    and sums are rounded to float32, results once to the type they are stored in
+    (rope_kv_append rounds to the storage type after each step).
 
     The cache is one of q's dtype, or an 8-bit one when its scales are given
     (kv_append_fp8).  Rows below n_rows (default: all of write_blocks) are written; q
