@@ -207,3 +207,23 @@ def test_a_merge_of_more_rows_than_its_grid_holds(hq, hkv, d):
     # Heads that do not fill the merge's 1024 elements, two cut sequences with an uncut one between.
     c = Case([5000, 30, 4000], hq, hkv, d, seed=14, chunks=[2000, 30, 500])
     c.check(c.prefill())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("byte", [220, 235, 247])
+def test_small_weights_of_the_largest_values_count(dtype, hq, hkv, d, byte):
+    # Key 30 scores 40 binary orders below key 3, whose value is 1; its own, of 256 and a scale up to 2^120, rules the sum.
+    c = Case([40], hq, hkv, d, dtype=dtype, seed=2, chunks=[5])
+    kc, vc, ks, vs = (t.view(torch.uint8) for t in c.cache)
+    kc.zero_(), ks.fill_(127), vs.fill_(127), vc.zero_()
+    for t, key, value, scale in ((3, 0x38, 0x38, 127), (30, 0xB8, 0x78, byte)):  # keys of 1 and -1 in every dim
+        at = (int(c.tables[0, t // 16]), t % 16)
+        kc[at], vc[at], vs[at] = key, value, scale
+    c.q = torch.full_like(c.q, 1.0)
+    c.scale = 20 * 0.6931471805599453 / d  # scores of +-20 in binary orders, the others 0
+    c.check(c.prefill())
+    assert (c.prefill().float() > 2.0 ** (byte - 127 + 8 - 41)).all()
+    c.q, c.chunks = c.q[:1], None
+    c.check(c.decode())
+    assert (c.decode().float() > 2.0 ** (byte - 127 + 8 - 41)).all()

@@ -32,10 +32,11 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
 
 // Sums of p V are kept kLift times as large, so that products with the smallest scales are
 // normal numbers (in bf16, too).  What a key whose V scale has byte b adds to its candidate for
-// the running maximum (log2 units): p V, lifted, stays below 2^81 a key, so a row of values near
-// the end of fp32 does not overflow before the division by sum p.  0 up to kFreeScale, 2^32.
-constexpr float kLift = 0x1p32f;
-constexpr uint32_t kFreeScale = 159;
+// the running maximum (log2 units): with p at most 2^8, p V stays below 2^96 a key, lifted, and
+// its sum over 2^30 keys inside fp32.  0 up to kFreeScale, 2^55; no more than that, for beside a
+// bias of x weights of 2^(x - 126) become 0.
+constexpr float kLift = 0x1p24f;
+constexpr uint32_t kFreeScale = 182;
 __device__ __forceinline__ float value_bias(uint32_t b) {
   return static_cast<float>(max(static_cast<int>(b) - static_cast<int>(kFreeScale), 0));
 }

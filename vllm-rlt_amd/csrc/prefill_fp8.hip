@@ -53,7 +53,7 @@ constexpr int kTargetItems = kRound * 3 / 2;
 // 17.8 / 17.2 / 21.0.
 constexpr int kMinSegTiles = 2;
 constexpr uint32_t kLargestScale = 246;  // the largest scale byte whose codes are all finite in bf16
-constexpr uint32_t kLiftExp = 32;        // kLift = 2^kLiftExp
+constexpr uint32_t kLiftExp = 24;        // kLift = 2^kLiftExp
 static_assert(kLift == static_cast<float>(uint64_t(1) << kLiftExp) && kLargestScale - kLiftExp > kFreeScale);
 constexpr int64_t kMergeRound = 2048;  // workgroups of the merge that run at once
 constexpr int kPlanSeqs = 64;  // sequences ranked and cut: one a lane
