@@ -615,6 +615,82 @@ int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t count, int64_t 
                              int64_t* blocks, int64_t* offsets, int64_t capacity, int32_t* out_tables,
                              int64_t out_table_stride, int64_t out_width, void* stream);
 
+/*
+ * Block-scaled 8-bit KV cache.  Key and value caches of signed 8-bit codes, -127 to
+ * 127, and one fp32 scale for each (block, head): a cached value is code * scale.
+ * Caches are [num_blocks, num_layers, page_size, num_kv_heads, head_dim] (a layer
+ * slice without num_layers), scales [num_blocks, num_layers, num_kv_heads] (a slice
+ * without num_layers), on 4 bytes; strides in elements, shared by K and V.  Scales are
+ * not negative; one that is not finite makes its whole block NaN to attention.
+ */
+
+/*
+ * Quantising KV append of one layer: rlt_kv_append to a block-scaled cache.  `dtype`
+ * is the type of k and v.  For every block and head that gets rows, with s0 its scale,
+ * or 0 where a row goes to its offset 0, which begins the block:
+ *   s = max(s0, largest |x| of the rows / 127, 2^-126), the block's new scale
+ *   codes the block holds: rint(code * (s0 / s)) where s is not s0, unless it begins
+ *   codes of the rows: rint(x * (1 / s))
+ * every operation rounded to fp32, rint to even.  Rows that hold what is not finite
+ * make s NaN, and a scale that is NaN stays so until the block begins again.
+ * Rows of one block stand together in the call (as the tokens of a packed prompt do,
+ * and those of a decode batch, which have a block each); their slots are distinct.
+ * Rows of a block outside the pool, or of an offset outside its page, are skipped.
+ */
+int rlt_kv_append_int8(void* key_cache, void* value_cache, const int64_t* cache_strides, void* key_scales,
+                       void* value_scales, const int64_t* scale_strides, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, const int64_t* write_blocks,
+                       const int64_t* write_offsets, int64_t n_rows, int64_t layer, int64_t num_layers,
+                       int64_t num_blocks, int64_t page_size, int64_t num_kv_heads, int64_t head_dim, int dtype,
+                       void* stream);
+
+/*
+ * Read slots of one layer of a block-scaled cache back as values of `dtype`:
+ *   out_k[i] = codes[blocks[i], layer, offsets[i]] * scales[blocks[i], layer]  (and V)
+ * rounded to fp32, then to `dtype`; out_k and out_v contiguous [n_rows, num_kv_heads,
+ * head_dim].  Slots in any order, repeated or not; one outside the pool gives zeros.
+ */
+int rlt_kv_gather_int8(const void* key_cache, const void* value_cache, const int64_t* cache_strides,
+                       const void* key_scales, const void* value_scales, const int64_t* scale_strides,
+                       const int64_t* blocks, const int64_t* offsets, int64_t n_rows, void* out_k, void* out_v,
+                       int64_t layer, int64_t num_layers, int64_t num_blocks, int64_t page_size,
+                       int64_t num_kv_heads, int64_t head_dim, int dtype, void* stream);
+
+/*
+ * rlt_paged_decode over a layer slice of a block-scaled cache; q and out are of
+ * `dtype`, scale_strides[2]: block, head.  A row of length 0 (or less) is written as
+ * zeros; lengths are clamped to what the table covers.  A row's output bits depend on
+ * its own q, blocks and length only.
+ * The workspace (rlt_paged_decode_int8_workspace_bytes, a function of the shape, on 16
+ * bytes) holds the partials of cut rows; calls that overlap need one each.
+ */
+int64_t rlt_paged_decode_int8_workspace_bytes(int64_t n_rows, int64_t max_table_width, int64_t num_q_heads,
+                                              int64_t num_kv_heads, int64_t head_dim, int64_t page_size);
+int rlt_paged_decode_int8(const void* q, const int64_t* q_strides, const void* key_cache, const void* value_cache,
+                          const int64_t* kv_strides, const void* key_scales, const void* value_scales,
+                          const int64_t* scale_strides, const int32_t* block_tables, int64_t table_row_stride,
+                          int64_t max_table_width, const int32_t* context_lengths, void* out,
+                          const int64_t* out_strides, int64_t n_rows, int64_t num_q_heads, int64_t num_kv_heads,
+                          int64_t head_dim, int64_t page_size, int64_t num_blocks, float scale, int dtype,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * rlt_paged_prefill over a layer slice of a block-scaled cache: packed chunks, bottom-
+ * right causal, with the rows, lengths, max_seqlen_q and workspace of
+ * rlt_paged_prefill_fp8 (its workspace by rlt_paged_prefill_int8_workspace_bytes).
+ */
+int64_t rlt_paged_prefill_int8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
+                                               int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                               int64_t page_size);
+int rlt_paged_prefill_int8(const void* q, const int64_t* q_strides, const void* key_cache, const void* value_cache,
+                           const int64_t* kv_strides, const void* key_scales, const void* value_scales,
+                           const int64_t* scale_strides, const int32_t* block_tables, int64_t table_row_stride,
+                           int64_t max_table_width, const int32_t* context_lengths, const int32_t* cu_seqlens_q,
+                           int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, void* out,
+                           const int64_t* out_strides, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                           int64_t page_size, int64_t num_blocks, float scale, int dtype, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

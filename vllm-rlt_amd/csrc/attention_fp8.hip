@@ -16,30 +16,14 @@ namespace {
 // with the head's dims over its lanes and a running maximum and sum of its own;
 // the waves are joined through LDS in wave order.  Every query head reads its keys itself, a
 // byte a lane: latency bounds it (64 rows of 512-4096 tokens, 16 heads x 80: 1112 us).
-constexpr int kPerLane = 8;
-constexpr int kGenericWaves = 8;
-
 template <typename T>
 __global__ __launch_bounds__(64 * kGenericWaves) void attn8_generic_kernel(Attn8Args a) {
   const int64_t row = blockIdx.x;
   const int h = blockIdx.y;
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
-  int seq = static_cast<int>(row), len;
-  if (a.cu) {
-    int lo = 0, hi = a.num_seqs;  // the last sequence that begins at or before row
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= row) lo = mid;
-      else hi = mid;
-    }
-    if (row < a.cu[lo] || row >= a.cu[lo + 1]) return;  // a row of no sequence is left as it was
-    seq = lo;
-    const int64_t n = sequence_length(a, seq) - (a.cu[lo + 1] - 1 - row);
-    len = static_cast<int>(n < 0 ? 0 : n);
-  } else {
-    len = sequence_length(a, seq);
-  }
+  int seq, len;
+  if (!row_keys(a, row, &seq, &len)) return;
   T* orow = static_cast<T*>(a.out) + row * a.o_row + h * a.o_head;
   const T* qrow = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
   const int kvh = h / (a.hq / a.hkv);
@@ -106,13 +90,13 @@ __global__ __launch_bounds__(64 * kGenericWaves) void attn8_generic_kernel(Attn8
   }
 }
 
-// Checks what both calls share and fills the arguments.
-int attention_args(const char* name, const void* q, const int64_t* q_strides, const void* key_cache,
-                   const void* value_cache, const int64_t* kv_strides, const void* key_scales,
-                   const void* value_scales, const int64_t* scale_strides, const int32_t* tables,
-                   int64_t table_stride, int64_t width, const int32_t* lens, int64_t num_seqs, void* out,
-                   const int64_t* out_strides, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int64_t page,
-                   int64_t num_blocks, float scale, int dtype, Attn8Args* a) {
+}  // namespace
+
+int attn8_args(const char* name, const void* q, const int64_t* q_strides, const void* key_cache, const void* value_cache,
+               const int64_t* kv_strides, const void* key_scales, const void* value_scales, const int64_t* scale_strides,
+               const int32_t* tables, int64_t table_stride, int64_t width, const int32_t* lens, int64_t num_seqs, void* out,
+               const int64_t* out_strides, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int64_t page,
+               int64_t num_blocks, float scale, int dtype, Attn8Args* a) {
   if (!dtype_size(dtype)) return fail(RLT_EINVAL, "%s: unknown dtype %d", name, dtype);
   if (rows < 0 || num_seqs < 0) return fail(RLT_EINVAL, "%s: negative row count", name);
   if (hkv <= 0 || hq <= 0 || hq % hkv) return fail(RLT_EINVAL, "%s: query heads must be a positive multiple of KV heads", name);
@@ -150,8 +134,6 @@ int attention_args(const char* name, const void* q, const int64_t* q_strides, co
   return RLT_OK;
 }
 
-}  // namespace
-
 int launch_attn8_generic(const Attn8Args& a, int dtype, hipStream_t stream, const char* name) {
   const dim3 grid(static_cast<unsigned>(a.rows), static_cast<unsigned>(a.hq)), block(64 * kGenericWaves);
   switch (dtype) {
@@ -182,7 +164,7 @@ extern "C" int rlt_paged_decode_fp8(const void* q, const int64_t* q_strides, con
                                     int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t num_blocks,
                                     float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   Attn8Args a;
-  if (int rc = attention_args("rlt_paged_decode_fp8", q, q_strides, key_cache, value_cache, kv_strides, key_scales,
+  if (int rc = attn8_args("rlt_paged_decode_fp8", q, q_strides, key_cache, value_cache, kv_strides, key_scales,
                               value_scales, scale_strides, block_tables, table_row_stride, max_table_width,
                               context_lengths, n_rows, out, out_strides, n_rows, num_q_heads, num_kv_heads, head_dim,
                               page_size, num_blocks, scale, dtype, &a))
@@ -214,7 +196,7 @@ extern "C" int rlt_paged_prefill_fp8(const void* q, const int64_t* q_strides, co
                                      int64_t num_blocks, float scale, int dtype, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
   Attn8Args a;
-  if (int rc = attention_args("rlt_paged_prefill_fp8", q, q_strides, key_cache, value_cache, kv_strides, key_scales,
+  if (int rc = attn8_args("rlt_paged_prefill_fp8", q, q_strides, key_cache, value_cache, kv_strides, key_scales,
                               value_scales, scale_strides, block_tables, table_row_stride, max_table_width,
                               context_lengths, num_seqs, out, out_strides, total_q, num_q_heads, num_kv_heads,
                               head_dim, page_size, num_blocks, scale, dtype, &a))

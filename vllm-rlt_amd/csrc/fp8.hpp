@@ -7,7 +7,7 @@
 // same relative step at every magnitude.)
 #pragma once
 
-#include "common.hpp"
+#include "attn8.hpp"
 
 namespace rlt {
 
@@ -58,57 +58,6 @@ __device__ __forceinline__ uint32_t codes2(float x, float y, float inv) {
 }
 
 __device__ __forceinline__ float code_value(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8(c, 0); }
-
-// Largest over aligned groups of W lanes (group_sum's butterfly).
-template <int W>
-__device__ __forceinline__ float group_max(float x) {
-  if constexpr (W >= 2) x = fmaxf(x, dpp<kDppXor1>(x));
-  if constexpr (W >= 4) x = fmaxf(x, dpp<kDppXor2>(x));
-  if constexpr (W >= 8) x = fmaxf(x, dpp<kDppHalfMirror>(x));
-  if constexpr (W >= 16) x = fmaxf(x, dpp<kDppMirror>(x));
-  if constexpr (W >= 32) x = fmaxf(x, xor_lane(x, 16));
-  if constexpr (W >= 64) x = fmaxf(x, xor_lane(x, 32));
-  return x;
-}
-
-// Limits of the attention calls: token counts and what is added to them stay inside 31
-// bits, and the threads of a launch (blocks of up to 512) inside 32.
-constexpr int64_t kMaxKeys = int64_t(1) << 30;
-constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
-constexpr int64_t kMaxRows = (int64_t(1) << 23) - 1;
-
-// Arguments of the attention kernels over an 8-bit cache (strides in elements).
-struct Attn8Args {
-  const void* q;
-  int64_t q_row, q_head, q_dim;
-  const uint8_t* k;
-  const uint8_t* v;
-  int64_t kv_block, kv_token, kv_head, kv_dim;
-  const uint8_t* ks;
-  const uint8_t* vs;
-  int64_t s_block, s_token, s_head;
-  const int32_t* tables;
-  int64_t table_stride;
-  const int32_t* lens;
-  const int32_t* cu;  // packed rows of several sequences; null: row r is sequence r's only one
-  void* out;
-  int64_t o_row, o_head, o_dim;
-  int64_t rows;  // packed query rows
-  int num_seqs, hq, hkv, d, page;
-  int64_t num_blocks, max_len;  // max_len: table width * page, lengths are clamped to it
-  float qscale;                 // softmax scale * log2(e)
-};
-
-// The block of table entry id: one outside the pool reads block 0, in bounds.
-__device__ __forceinline__ int64_t block_of(const Attn8Args& a, int32_t id) {
-  return id >= 0 && id < a.num_blocks ? id : 0;
-}
-
-// A sequence's key count, never past what its table covers.
-__device__ __forceinline__ int sequence_length(const Attn8Args& a, int s) {
-  const int64_t n = a.lens[s];
-  return static_cast<int>(n < 0 ? 0 : n < a.max_len ? n : a.max_len);
-}
 
 // Attention of every row by the kernel for any shape (attention_fp8.hip).
 int launch_attn8_generic(const Attn8Args& a, int dtype, hipStream_t stream, const char* name);

@@ -42,6 +42,12 @@ decltype(&rlt_paged_prefill_fp8_workspace_bytes) g_prefill8_bytes = nullptr;
 decltype(&rlt_kv_append_fp8) g_append8 = nullptr;
 decltype(&rlt_rope_axes_kv_append) g_rope_axes = nullptr;
 decltype(&rlt_build_chunk_metadata) g_chunk_metadata = nullptr;
+decltype(&rlt_paged_decode_int8) g_decode_i8 = nullptr;
+decltype(&rlt_paged_decode_int8_workspace_bytes) g_decode_i8_bytes = nullptr;
+decltype(&rlt_paged_prefill_int8) g_prefill_i8 = nullptr;
+decltype(&rlt_paged_prefill_int8_workspace_bytes) g_prefill_i8_bytes = nullptr;
+decltype(&rlt_kv_append_int8) g_append_i8 = nullptr;
+decltype(&rlt_kv_gather_int8) g_gather_i8 = nullptr;
 
 // A plain device tensor of torch.Tensor itself, or null.  (Parameters and other
 // subclasses, wrappers of vmap / grad and fake tensors take the Python path.)
@@ -290,7 +296,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// ----------------------------------------------------------- 8-bit KV cache
+// ---------------------------------------------------------- 8-bit KV caches
 // Whether t is on the current device, which a launch goes to.
 bool here(const at::Tensor& t) {
   static const c10::impl::VirtualGuardImpl device(c10::DeviceType::CUDA);
@@ -321,10 +327,33 @@ bool cache8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, cons
          vs.strides() == ks.strides();
 }
 
+// Signed codes of dims dims with fp32 scales, one a block (and layer) and head.
+bool cache_i8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, int64_t dims) {
+  if (k.dim() != dims || k.scalar_type() != at::kChar || v.scalar_type() != at::kChar || ks.scalar_type() != at::kFloat ||
+      vs.scalar_type() != at::kFloat || k.sizes() != v.sizes() || k.strides() != v.strides() || ks.dim() != dims - 2 ||
+      vs.sizes() != ks.sizes() || vs.strides() != ks.strides())
+    return false;
+  for (int64_t i = 0; i < dims - 3; ++i)
+    if (ks.size(i) != k.size(i)) return false;
+  return ks.size(dims - 3) == k.size(dims - 2);
+}
+
+// Which of the two caches a call is over, its check and its entry points.
+struct Form8 {
+  bool (*cache)(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t);
+  decltype(g_decode8)*decode;
+  decltype(g_decode8_bytes)*decode_bytes;
+  decltype(g_prefill8)*prefill;
+  decltype(g_prefill8_bytes)*prefill_bytes;
+  decltype(g_append8)*append;
+};
+const Form8 kFp8 = {cache8, &g_decode8, &g_decode8_bytes, &g_prefill8, &g_prefill8_bytes, &g_append8};
+const Form8 kInt8 = {cache_i8, &g_decode_i8, &g_decode_i8_bytes, &g_prefill_i8, &g_prefill_i8_bytes, &g_append_i8};
+
 // What decode and prefill share: q, cache, tables and lengths in args[0 .. 6].
-bool attention8(const at::Tensor* const* in) {
+bool attention8(const Form8& form, const at::Tensor* const* in) {
   const at::Tensor &q = *in[0], &k = *in[1], &tables = *in[5], &lens = *in[6];
-  return cache8(k, *in[2], *in[3], *in[4], 4) && q.dim() == 3 && q.size(2) == k.size(3) && code_of(q.scalar_type()) >= 0 &&
+  return form.cache(k, *in[2], *in[3], *in[4], 4) && q.dim() == 3 && q.size(2) == k.size(3) && code_of(q.scalar_type()) >= 0 &&
          k.size(2) > 0 && q.size(1) > 0 && q.size(1) % k.size(2) == 0 && q.size(0) > 0 && tables.scalar_type() == at::kInt &&
          tables.dim() == 2 && tables.stride(1) == 1 && tables.size(0) > 0 && ints(lens, at::kInt) && lens.size(0) == tables.size(0);
 }
@@ -343,22 +372,22 @@ bool workspace_of(PyObject* o, int64_t need, const at::Tensor& q, at::Tensor* ws
 }
 
 // decode8(q, key, value, key_scales, value_scales, tables, lengths, out, workspace, scale, stream)
-PyObject* decode8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+PyObject* decode8(const Form8& form, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   static constexpr int kAt[7] = {0, 1, 2, 3, 4, 5, 6};
   const at::Tensor* in[7];
-  if (nargs != 11 || modes_active() || !all_plain(args, kAt, in) || !attention8(in) || !scale_ok(args[9])) Py_RETURN_NONE;
+  if (nargs != 11 || modes_active() || !all_plain(args, kAt, in) || !attention8(form, in) || !scale_ok(args[9])) Py_RETURN_NONE;
   const at::Tensor &q = *in[0], &k = *in[1], &tables = *in[5];
   const int64_t rows = q.size(0), hq = q.size(1), d = q.size(2), hkv = k.size(2), width = tables.size(1);
   if (tables.size(0) != rows) Py_RETURN_NONE;
   at::Tensor out, ws;
-  if (!workspace_of(args[8], g_decode8_bytes(rows, width, hq, hkv, d, k.size(1)), q, &ws) || !result_like(args[7], q, &out))
+  if (!workspace_of(args[8], (*form.decode_bytes)(rows, width, hq, hkv, d, k.size(1)), q, &ws) || !result_like(args[7], q, &out))
     Py_RETURN_NONE;
   void* const stream = PyLong_AsVoidPtr(args[10]);
   const float scale = scale_of(args[9], d);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_decode8(q.data_ptr(), q.strides().data(), k.data_ptr(), in[2]->data_ptr(), k.strides().data(), in[3]->data_ptr(),
+  rc = (*form.decode)(q.data_ptr(), q.strides().data(), k.data_ptr(), in[2]->data_ptr(), k.strides().data(), in[3]->data_ptr(),
                  in[4]->data_ptr(), in[3]->strides().data(), tables.data_ptr<int32_t>(), tables.stride(0), width,
                  in[6]->data_ptr<int32_t>(), out.data_ptr(), out.strides().data(), rows, hq, hkv, d, k.size(1), k.size(0),
                  scale, code_of(q.scalar_type()), ws.data_ptr(), ws.numel() * static_cast<int64_t>(ws.element_size()), stream);
@@ -369,25 +398,25 @@ PyObject* decode8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // prefill8(q, key, value, key_scales, value_scales, tables, lengths, cu, max_seqlen_q, out, workspace,
 //          scale, batch_invariant, stream)
-PyObject* prefill8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+PyObject* prefill8(const Form8& form, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   static constexpr int kAt[8] = {0, 1, 2, 3, 4, 5, 6, 7};
   const at::Tensor* in[8];
   int64_t longest;
-  if (nargs != 14 || modes_active() || !all_plain(args, kAt, in) || !attention8(in) || !scale_ok(args[11]) ||
+  if (nargs != 14 || modes_active() || !all_plain(args, kAt, in) || !attention8(form, in) || !scale_ok(args[11]) ||
       !PyBool_Check(args[12]) || !int_of(args[8], &longest))
     Py_RETURN_NONE;
   const at::Tensor &q = *in[0], &k = *in[1], &tables = *in[5], &cu = *in[7];
   const int64_t total = q.size(0), hq = q.size(1), d = q.size(2), hkv = k.size(2), n = tables.size(0), width = tables.size(1);
   if (!ints(cu, at::kInt) || cu.size(0) != n + 1) Py_RETURN_NONE;
-  const int64_t need = args[12] == Py_True ? 0 : g_prefill8_bytes(total, n, width, hq, hkv, d, k.size(1));
+  const int64_t need = args[12] == Py_True ? 0 : (*form.prefill_bytes)(total, n, width, hq, hkv, d, k.size(1));
   at::Tensor out, ws;
   if (!workspace_of(args[10], need, q, &ws) || !result_like(args[9], q, &out)) Py_RETURN_NONE;
   void* const stream = PyLong_AsVoidPtr(args[13]);
   const float scale = scale_of(args[11], d);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_prefill8(q.data_ptr(), q.strides().data(), k.data_ptr(), in[2]->data_ptr(), k.strides().data(), in[3]->data_ptr(),
+  rc = (*form.prefill)(q.data_ptr(), q.strides().data(), k.data_ptr(), in[2]->data_ptr(), k.strides().data(), in[3]->data_ptr(),
                   in[4]->data_ptr(), in[3]->strides().data(), tables.data_ptr<int32_t>(), tables.stride(0), width,
                   in[6]->data_ptr<int32_t>(), cu.data_ptr<int32_t>(), n, total, longest, out.data_ptr(), out.strides().data(),
                   hq, hkv, d, k.size(1), k.size(0), scale, code_of(q.scalar_type()), need ? ws.data_ptr() : nullptr,
@@ -405,14 +434,14 @@ bool rows_of(PyObject* o, const at::Tensor& wb, const at::Tensor& wo, int64_t ro
 
 // append8(key_cache, value_cache, key_scales, value_scales, layer, write_blocks, write_offsets, k, v, n_rows,
 //         stream): an int, the library's status.
-PyObject* append8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+PyObject* append8(const Form8& form, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   static constexpr int kAt[8] = {0, 1, 2, 3, 5, 6, 7, 8};
   const at::Tensor* in[8];
   int64_t layer, n;
   if (nargs != 11 || modes_active() || !all_plain(args, kAt, in) || !int_of(args[4], &layer)) Py_RETURN_NONE;
   const at::Tensor &kc = *in[0], &wb = *in[4], &wo = *in[5], &k = *in[6], &v = *in[7];
-  if (!cache8(kc, *in[1], *in[2], *in[3], 5) || !ints(wb, at::kLong) || !ints(wo, at::kLong) || k.dim() != 3 || v.dim() != 3 ||
+  if (!form.cache(kc, *in[1], *in[2], *in[3], 5) || !ints(wb, at::kLong) || !ints(wo, at::kLong) || k.dim() != 3 || v.dim() != 3 ||
       code_of(k.scalar_type()) < 0 || v.scalar_type() != k.scalar_type())
     Py_RETURN_NONE;
   const int64_t hkv = kc.size(3), d = kc.size(4);
@@ -422,13 +451,46 @@ PyObject* append8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* const stream = PyLong_AsVoidPtr(args[10]);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_append8(kc.data_ptr(), in[1]->data_ptr(), kc.strides().data(), in[2]->data_ptr(), in[3]->data_ptr(),
+  rc = (*form.append)(kc.data_ptr(), in[1]->data_ptr(), kc.strides().data(), in[2]->data_ptr(), in[3]->data_ptr(),
                  in[2]->strides().data(), k.data_ptr(), k.strides().data(), v.data_ptr(), v.strides().data(),
                  wb.data_ptr<int64_t>(), wo.data_ptr<int64_t>(), n, layer, kc.size(1), kc.size(0), kc.size(2), hkv, d,
                  code_of(k.scalar_type()), stream);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);
   END_HANDLE_TH_ERRORS
+}
+
+// gather_i8(key_cache, value_cache, key_scales, value_scales, layer, blocks, offsets, dtype code, n_rows, stream): (k, v)
+PyObject* gather_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  static constexpr int kAt[6] = {0, 1, 2, 3, 5, 6};
+  const at::Tensor* in[6];
+  int64_t layer, code, n;
+  if (nargs != 10 || modes_active() || !all_plain(args, kAt, in) || !int_of(args[4], &layer) || !int_of(args[7], &code)) Py_RETURN_NONE;
+  const at::Tensor &kc = *in[0], &blocks = *in[4], &offsets = *in[5];
+  if (!cache_i8(kc, *in[1], *in[2], *in[3], 5) || !ints(blocks, at::kLong) || !ints(offsets, at::kLong)) Py_RETURN_NONE;
+  if (!rows_of(args[8], blocks, offsets, blocks.size(0), &n)) Py_RETURN_NONE;
+  const at::ScalarType type = code == RLT_FLOAT32 ? at::kFloat : code == RLT_FLOAT16 ? at::kHalf : at::kBFloat16;
+  const at::Tensor k = at::empty({n, kc.size(3), kc.size(4)}, kc.options().dtype(type)), v = at::empty_like(k);
+  void* const stream = PyLong_AsVoidPtr(args[9]);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_gather_i8(kc.data_ptr(), in[1]->data_ptr(), kc.strides().data(), in[2]->data_ptr(), in[3]->data_ptr(),
+                   in[2]->strides().data(), blocks.data_ptr<int64_t>(), offsets.data_ptr<int64_t>(), n, k.data_ptr(), v.data_ptr(),
+                   layer, kc.size(1), kc.size(0), kc.size(2), kc.size(3), kc.size(4), static_cast<int>(code), stream);
+  Py_END_ALLOW_THREADS
+  if (rc != RLT_OK) return PyLong_FromLong(rc);
+  PyObject* const pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(k));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(v));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+template <PyObject* (*F)(const Form8&, PyObject* const*, Py_ssize_t), const Form8& FORM>
+PyObject* of_form(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return F(FORM, args, nargs);
 }
 
 // rope_axes(key_cache, value_cache, layer, write_blocks, write_offsets, q, k, v, positions, table, axes,
@@ -536,15 +598,17 @@ bool bind_one(PyObject* o, F* f) {
   return true;
 }
 PyObject* bind(PyObject*, PyObject* args) {
-  PyObject* a[13];
-  if (!PyArg_ParseTuple(args, "OOOOOOOOOOOOO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10],
-                        &a[11], &a[12]))
+  PyObject* a[19];
+  if (!PyArg_ParseTuple(args, "OOOOOOOOOOOOOOOOOOO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10],
+                        &a[11], &a[12], &a[13], &a[14], &a[15], &a[16], &a[17], &a[18]))
     return nullptr;
   if (!bind_one(a[0], &g_decode) || !bind_one(a[1], &g_decode_append) || !bind_one(a[2], &g_decode_bytes) ||
       !bind_one(a[3], &g_prefill) || !bind_one(a[4], &g_prefill_bytes) || !bind_one(a[5], &g_rope) ||
       !bind_one(a[6], &g_decode8) || !bind_one(a[7], &g_decode8_bytes) || !bind_one(a[8], &g_prefill8) ||
       !bind_one(a[9], &g_prefill8_bytes) || !bind_one(a[10], &g_append8) || !bind_one(a[11], &g_rope_axes) ||
-      !bind_one(a[12], &g_chunk_metadata))
+      !bind_one(a[12], &g_chunk_metadata) || !bind_one(a[13], &g_decode_i8) || !bind_one(a[14], &g_decode_i8_bytes) ||
+      !bind_one(a[15], &g_prefill_i8) || !bind_one(a[16], &g_prefill_i8_bytes) || !bind_one(a[17], &g_append_i8) ||
+      !bind_one(a[18], &g_gather_i8))
     return nullptr;
   Py_RETURN_NONE;
 }
@@ -555,11 +619,15 @@ PyMethodDef kMethods[] = {
     {"prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill)), METH_FASTCALL, nullptr},
     {"prefill_bytes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill_bytes)), METH_FASTCALL, nullptr},
     {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope)), METH_FASTCALL, nullptr},
-    {"decode8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode8)), METH_FASTCALL, nullptr},
-    {"prefill8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill8)), METH_FASTCALL, nullptr},
-    {"append8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append8)), METH_FASTCALL, nullptr},
+    {"decode8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(of_form<decode8, kFp8>)), METH_FASTCALL, nullptr},
+    {"decode_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(of_form<decode8, kInt8>)), METH_FASTCALL, nullptr},
+    {"prefill8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(of_form<prefill8, kFp8>)), METH_FASTCALL, nullptr},
+    {"prefill_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(of_form<prefill8, kInt8>)), METH_FASTCALL, nullptr},
+    {"append8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(of_form<append8, kFp8>)), METH_FASTCALL, nullptr},
+    {"append_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(of_form<append8, kInt8>)), METH_FASTCALL, nullptr},
     {"rope_axes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope_axes)), METH_FASTCALL, nullptr},
     {"chunk_metadata", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(chunk_metadata)), METH_FASTCALL, nullptr},
+    {"gather_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gather_i8)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, kMethods};

@@ -175,6 +175,35 @@ SIGNATURES = {
         [c_void_p, c_int64, c_int64, c_void_p] + [c_int64] * 4 + [c_void_p] * 6
         + [c_int64, c_void_p, c_int64, c_int64, c_void_p],
     ),
+    "rlt_kv_append_int8": (
+        c_int,
+        [c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, _i64p, c_void_p, _i64p, c_void_p, c_void_p]
+        + [c_int64] * 7
+        + [c_int, c_void_p],
+    ),
+    "rlt_kv_gather_int8": (
+        c_int,
+        [c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]
+        + [c_int64] * 6
+        + [c_int, c_void_p],
+    ),
+    "rlt_paged_decode_int8_workspace_bytes": (c_int64, [c_int64] * 6),
+    "rlt_paged_decode_int8": (
+        c_int,
+        [c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_int64, c_int64, c_void_p]
+        + [c_void_p, _i64p]
+        + [c_int64] * 6
+        + [c_float, c_int, c_void_p, c_int64, c_void_p],
+    ),
+    "rlt_paged_prefill_int8_workspace_bytes": (c_int64, [c_int64] * 7),
+    "rlt_paged_prefill_int8": (
+        c_int,
+        [c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_void_p, _i64p, c_void_p, c_int64, c_int64, c_void_p]
+        + [c_void_p] + [c_int64] * 3
+        + [c_void_p, _i64p]
+        + [c_int64] * 5
+        + [c_float, c_int, c_void_p, c_int64, c_void_p],
+    ),
 }
 
 _lib = None
@@ -199,6 +228,12 @@ HOST_CALLED = (
     "rlt_kv_append_fp8",
     "rlt_rope_axes_kv_append",
     "rlt_build_chunk_metadata",
+    "rlt_paged_decode_int8",
+    "rlt_paged_decode_int8_workspace_bytes",
+    "rlt_paged_prefill_int8",
+    "rlt_paged_prefill_int8_workspace_bytes",
+    "rlt_kv_append_int8",
+    "rlt_kv_gather_int8",
 )
 
 

@@ -1203,10 +1203,10 @@ def rope_axes_kv_append(
     return out
 
 
-def _fp8_attention_inputs(q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out):
-    """Validated arguments that decode and prefill over an 8-bit cache share, and the output."""
+def _attention8_inputs(require, q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out):
+    """Validated arguments that decode and prefill over an 8-bit cache (checked by `require`) share, and the output."""
     device = _require_rocm(q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths)
-    _require_fp8(key_cache, value_cache, key_scales, value_scales, 4)
+    require(key_cache, value_cache, key_scales, value_scales, 4)
     dtype_code(q.dtype)
     hkv, d = key_cache.shape[2:]
     if q.ndim != 3 or q.shape[2] != d:
@@ -1273,8 +1273,8 @@ def paged_decode_fp8(
         )
         if result is not None:
             return _finish(result, "rlt_paged_decode_fp8")
-    device, out = _fp8_attention_inputs(
-        q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
+    device, out = _attention8_inputs(
+        _require_fp8, q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
     )
     rows, hq, d = q.shape
     nb, page, hkv, _ = key_cache.shape
@@ -1346,8 +1346,8 @@ def paged_prefill_fp8(
         )
         if result is not None:
             return _finish(result, "rlt_paged_prefill_fp8")
-    device, out = _fp8_attention_inputs(
-        q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
+    device, out = _attention8_inputs(
+        _require_fp8, q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
     )
     _require_rocm(q, cu_seqlens_q)
     _require_int(cu_seqlens_q, torch.int32, "cu_seqlens_q")
@@ -1371,4 +1371,257 @@ def paged_prefill_fp8(
             workspace.numel() * workspace.element_size(), stream_handle(device),
         )
     check(rc, "rlt_paged_prefill_fp8")
+    return out
+
+
+def _require_int8(key_cache, value_cache, key_scales, value_scales, ndim: int):
+    """Checks a block-scaled cache: int8 codes with ndim dims and float32 scales a block (and layer) and head."""
+    if key_cache.dtype != torch.int8 or value_cache.dtype != torch.int8:
+        raise ValueError("a block-scaled cache holds torch.int8 codes")
+    if key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32:
+        raise ValueError("key_scales and value_scales must be torch.float32")
+    layers = "layers, " if ndim == 5 else ""
+    if key_cache.ndim != ndim:
+        raise ValueError(f"caches must be [blocks, {layers}page, kv_heads, head_dim]")
+    if key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride():
+        raise ValueError("key_cache and value_cache must share shape and strides")
+    for t in (key_scales, value_scales):
+        if t.shape != (*key_cache.shape[: ndim - 3], key_cache.shape[-2]) or t.stride() != key_scales.stride():
+            raise ValueError(f"scales must be [blocks, {layers}kv_heads] as the caches are, with equal strides")
+
+
+def kv_append_int8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    write_blocks: torch.Tensor,
+    write_offsets: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    n_rows: int | None = None,
+) -> None:
+    """kv_append to a block-scaled cache: k[i] and v[i] quantised into slot i for i < n_rows (rlt_kv_append_int8).
+
+    Caches are torch.int8 [blocks, layers, page, kv_heads, head_dim], scales torch.float32
+    [blocks, layers, kv_heads]: a cached value is code * scale, its code from -127 to 127.
+    A block's scale is its largest magnitude / 127 (at least 2^-126); where new rows are
+    larger it grows, and the codes that the block holds are rounded anew.  A row at
+    offset 0 begins its block: what was in it counts no more.  Rows that hold what is
+    not finite make their blocks' scales NaN, until the block begins again.
+
+    k and v are float32, float16 or bfloat16.  Rows of one block stand together in the
+    call, in any order of their offsets; the slots of a call are distinct, those outside
+    the cache skipped.
+    """
+    host, stream = _host_calls(key_cache)
+    if host is not None:
+        result = host.append_i8(
+            key_cache, value_cache, key_scales, value_scales, layer, write_blocks, write_offsets, k, v, n_rows, stream
+        )
+        if result is not None:
+            return check(result, "rlt_kv_append_int8")
+    device = _require_rocm(key_cache, value_cache, key_scales, value_scales, write_blocks, write_offsets, k, v)
+    _require_int8(key_cache, value_cache, key_scales, value_scales, 5)
+    nb, nl, page, hkv, d = key_cache.shape
+    for t, name in ((k, "k"), (v, "v")):
+        if t.ndim != 3 or t.shape[1:] != (hkv, d):
+            raise ValueError(f"{name} must have shape [batch, {hkv}, {d}]")
+    if k.dtype != v.dtype:
+        raise ValueError("k and v must share a dtype")
+    _require_int(write_blocks, torch.int64, "write_blocks")
+    _require_int(write_offsets, torch.int64, "write_offsets")
+    n = len(write_blocks) if n_rows is None else n_rows
+    if n > min(len(write_blocks), len(write_offsets), k.shape[0], v.shape[0]):
+        raise ValueError("n_rows exceeds the provided rows")
+    with _current(device):
+        rc = _native.load().rlt_kv_append_int8(
+            key_cache.data_ptr(), value_cache.data_ptr(), int64_array(key_cache.stride()), key_scales.data_ptr(),
+            value_scales.data_ptr(), int64_array(key_scales.stride()), k.data_ptr(), int64_array(k.stride()),
+            v.data_ptr(), int64_array(v.stride()), write_blocks.data_ptr(), write_offsets.data_ptr(), n, layer, nl, nb,
+            page, hkv, d, dtype_code(k.dtype), stream_handle(device),
+        )
+    check(rc, "rlt_kv_append_int8")
+
+
+def kv_gather_int8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    blocks: torch.Tensor,
+    offsets: torch.Tensor,
+    dtype: torch.dtype = torch.float32,
+    n_rows: int | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Slots of a block-scaled cache as values: new k and v [n_rows, kv_heads, head_dim] of `dtype` (rlt_kv_gather_int8).
+
+    Row i is slot (blocks[i], offsets[i]) of the layer, code * scale rounded to float32,
+    float16 or bfloat16; a slot outside the cache gives zeros.  With kv_append_int8 it
+    moves tokens between blocks, whose scales differ (exit copies, re-packing).
+    """
+    host, stream = _host_calls(key_cache)
+    if host is not None:
+        result = host.gather_i8(
+            key_cache, value_cache, key_scales, value_scales, layer, blocks, offsets, dtype_code(dtype), n_rows, stream
+        )
+        if result is not None:
+            return _finish(result, "rlt_kv_gather_int8")
+    device = _require_rocm(key_cache, value_cache, key_scales, value_scales, blocks, offsets)
+    _require_int8(key_cache, value_cache, key_scales, value_scales, 5)
+    code = dtype_code(dtype)
+    nb, nl, page, hkv, d = key_cache.shape
+    _require_int(blocks, torch.int64, "blocks")
+    _require_int(offsets, torch.int64, "offsets")
+    n = len(blocks) if n_rows is None else n_rows
+    if n < 0 or n > min(len(blocks), len(offsets)):
+        raise ValueError("n_rows exceeds the provided slots")
+    k = torch.empty((n, hkv, d), dtype=dtype, device=device)
+    v = torch.empty_like(k)
+    with _current(device):
+        rc = _native.load().rlt_kv_gather_int8(
+            key_cache.data_ptr(), value_cache.data_ptr(), int64_array(key_cache.stride()), key_scales.data_ptr(),
+            value_scales.data_ptr(), int64_array(key_scales.stride()), blocks.data_ptr(), offsets.data_ptr(), n,
+            k.data_ptr(), v.data_ptr(), layer, nl, nb, page, hkv, d, code, stream_handle(device),
+        )
+    check(rc, "rlt_kv_gather_int8")
+    return k, v
+
+
+def decode_int8_workspace_bytes(
+    n_rows: int, table_width: int, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int
+) -> int:
+    """Bytes of partials rlt_paged_decode_int8 needs (shape only)."""
+    return int(
+        _native.load().rlt_paged_decode_int8_workspace_bytes(
+            n_rows, table_width, num_q_heads, num_kv_heads, head_dim, page_size
+        )
+    )
+
+
+def paged_decode_int8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lengths: torch.Tensor,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """paged_decode over layer slices of a block-scaled cache (rlt_paged_decode_int8).
+
+    Codes torch.int8 [blocks, page, kv_heads, head_dim], scales torch.float32
+    [blocks, kv_heads] (kv_append_int8); q float32, float16 or bfloat16.  Returns a new
+    tensor like q unless out is given; a row of length 0 is zeros.  `workspace`
+    (decode_int8_workspace_bytes, on 16 bytes) holds the partials of long rows and is
+    allocated here unless given.  A row's output bits depend on its own q, blocks and
+    length only.
+    """
+    host, stream = _host_calls(q)
+    if host is not None:
+        result = host.decode_i8(
+            q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out, workspace, scale, stream
+        )
+        if result is not None:
+            return _finish(result, "rlt_paged_decode_int8")
+    device, out = _attention8_inputs(
+        _require_int8, q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
+    )
+    rows, hq, d = q.shape
+    nb, page, hkv, _ = key_cache.shape
+    if block_tables.shape[0] != rows:
+        raise ValueError("block_tables and context_lengths must have one entry per row")
+    if rows == 0:
+        return out
+    width = block_tables.shape[1]
+    workspace = _workspace_of(decode_int8_workspace_bytes(rows, width, hq, hkv, d, page), workspace, device)
+    with _current(device):
+        rc = _native.load().rlt_paged_decode_int8(
+            q.data_ptr(), int64_array(q.stride()), key_cache.data_ptr(), value_cache.data_ptr(),
+            int64_array(key_cache.stride()), key_scales.data_ptr(), value_scales.data_ptr(),
+            int64_array(key_scales.stride()), block_tables.data_ptr(), block_tables.stride(0), width,
+            context_lengths.data_ptr(), out.data_ptr(), int64_array(out.stride()), rows, hq, hkv, d, page, nb,
+            1.0 / math.sqrt(d) if scale is None else scale, dtype_code(q.dtype), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), stream_handle(device),
+        )
+    check(rc, "rlt_paged_decode_int8")
+    return out
+
+
+def prefill_int8_workspace_bytes(
+    total_q: int, num_seqs: int, table_width: int, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int
+) -> int:
+    """Bytes rlt_paged_prefill_int8 needs (shape only)."""
+    return int(
+        _native.load().rlt_paged_prefill_int8_workspace_bytes(
+            total_q, num_seqs, table_width, num_q_heads, num_kv_heads, head_dim, page_size
+        )
+    )
+
+
+def paged_prefill_int8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lengths: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_seqlen_q: int,
+    out: torch.Tensor | None = None,
+    scale: float | None = None,
+    workspace: torch.Tensor | None = None,
+    batch_invariant: bool = False,
+) -> torch.Tensor:
+    """paged_prefill over layer slices of a block-scaled cache: packed chunks, bottom-right causal (rlt_paged_prefill_int8).
+
+    The cache is paged_decode_int8's; the new tokens' keys are in it already.  Query row
+    i of a sequence's n sees its keys up to context_length - n + i; one that sees
+    none is zeros.  Rows of no sequence (from cu_seqlens_q[-1] on) are left as they
+    are in `out`.  max_seqlen_q is paged_prefill's: not negative, and without effect.
+
+    `workspace` (prefill_int8_workspace_bytes, on 16 bytes) holds the partials of
+    sequences whose keys are cut, by the launch's shapes, and is allocated here unless
+    given.  With `batch_invariant` none is cut: a row's bits depend on its own sequence
+    only.
+    """
+    host, stream = _host_calls(q)
+    if host is not None:
+        result = host.prefill_i8(
+            q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, cu_seqlens_q, max_seqlen_q,
+            out, workspace, scale, batch_invariant, stream,
+        )
+        if result is not None:
+            return _finish(result, "rlt_paged_prefill_int8")
+    device, out = _attention8_inputs(
+        _require_int8, q, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths, out
+    )
+    _require_rocm(q, cu_seqlens_q)
+    _require_int(cu_seqlens_q, torch.int32, "cu_seqlens_q")
+    total, hq, d = q.shape
+    nb, page, hkv, _ = key_cache.shape
+    nseq, width = block_tables.shape
+    if cu_seqlens_q.shape != (nseq + 1,):
+        raise ValueError("context_lengths and cu_seqlens_q must describe one entry per sequence")
+    if total == 0 or nseq == 0:
+        return out
+    need = 0 if batch_invariant else prefill_int8_workspace_bytes(total, nseq, width, hq, hkv, d, page)
+    workspace = _workspace_of(need, workspace, device)
+    with _current(device):
+        rc = _native.load().rlt_paged_prefill_int8(
+            q.data_ptr(), int64_array(q.stride()), key_cache.data_ptr(), value_cache.data_ptr(),
+            int64_array(key_cache.stride()), key_scales.data_ptr(), value_scales.data_ptr(),
+            int64_array(key_scales.stride()), block_tables.data_ptr(), block_tables.stride(0), width,
+            context_lengths.data_ptr(), cu_seqlens_q.data_ptr(), nseq, total, max_seqlen_q, out.data_ptr(),
+            int64_array(out.stride()), hq, hkv, d, page, nb, 1.0 / math.sqrt(d) if scale is None else scale,
+            dtype_code(q.dtype), workspace.data_ptr() if need else None,
+            workspace.numel() * workspace.element_size(), stream_handle(device),
+        )
+    check(rc, "rlt_paged_prefill_int8")
     return out
