@@ -628,7 +628,7 @@ int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t count, int64_t 
  * Quantising KV append of one layer: rlt_kv_append to a block-scaled cache.  `dtype`
  * is the type of k and v.  For every block and head that gets rows, with s0 its scale,
  * or 0 where a row goes to its offset 0, which begins the block:
- *   s = max(s0, largest |x| of the rows / 127, 2^-126), the block's new scale
+ *   s = max(s0, largest |x| of the rows * (1 / 127), 2^-126), the block's new scale
  *   codes the block holds: rint(code * (s0 / s)) where s is not s0, unless it begins
  *   codes of the rows: rint(x * (1 / s))
  * every operation rounded to fp32, rint to even.  Rows that hold what is not finite

@@ -7,6 +7,7 @@ import math
 import torch
 
 SMALLEST = 2.0**-126
+INVERSE_127 = torch.tensor(1.0) / 127  # in 32 bits
 
 
 def append(cache, layer, blocks, offsets, k, v):
@@ -27,7 +28,7 @@ def append(cache, layer, blocks, offsets, k, v):
                 if not new.isfinite().all() or s0.isnan():
                     s = torch.tensor(math.nan)
                 else:
-                    s = torch.maximum(torch.maximum(s0, new.abs().max() / 127), torch.tensor(SMALLEST))
+                    s = torch.maximum(torch.maximum(s0, new.abs().max() * INVERSE_127), torch.tensor(SMALLEST))
                     if s != s0 and not begins:
                         codes[b, layer, :, h] = torch.round(codes[b, layer, :, h].float() * (s0 / s)).to(torch.int8)
                 scales[b, layer, h] = s

@@ -9,7 +9,7 @@
 
 namespace rlt {
 
-constexpr float kLargestCode = 127.f;
+constexpr float kInverseLargest = 1.f / 127.f;  // of the largest code
 constexpr float kSmallestScale = 0x1p-126f;  // the smallest normal number, whose inverse is finite as well
 
 // The attention calls' arguments: a.s_block and a.s_head are the scales' strides, a.ks and a.vs unused.
