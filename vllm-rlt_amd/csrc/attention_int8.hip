@@ -3,6 +3,7 @@
 // over a sequence's keys, K_j and V_j codes and b(j) the block of key j; for one new
 // token a sequence (decode) and for packed chunks, bottom-right causal (prefill).
 // Scores, softmax sums and the sums of weighted values are fp32, outputs of q's type.
+#include "decode_int8.hpp"
 #include "int8.hpp"
 
 namespace rlt {
@@ -125,7 +126,10 @@ using namespace rlt;
 
 extern "C" int64_t rlt_paged_decode_int8_workspace_bytes(int64_t n_rows, int64_t max_table_width, int64_t num_q_heads,
                                                          int64_t num_kv_heads, int64_t head_dim, int64_t page_size) {
-  return 0;
+  if (n_rows <= 0 || max_table_width <= 0 || !decode8_shape(num_q_heads, num_kv_heads, head_dim, page_size) ||
+      max_table_width > kMaxKeys / page_size)
+    return 0;
+  return decode_i8_workspace(n_rows, max_table_width * page_size, num_q_heads, head_dim);
 }
 
 extern "C" int rlt_paged_decode_int8(const void* q, const int64_t* q_strides, const void* key_cache,
@@ -145,6 +149,7 @@ extern "C" int rlt_paged_decode_int8(const void* q, const int64_t* q_strides, co
   const int64_t need = rlt_paged_decode_int8_workspace_bytes(n_rows, max_table_width, num_q_heads, num_kv_heads, head_dim, page_size);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(RLT_EWORKSPACE, "%s: workspace must be %lld bytes on 16", name, (long long)need);
+  if (decode8_layout(p.a)) return launch_decode_i8(p, dtype, workspace, as_stream(stream), name);
   return launch_attn_i8_generic(p, dtype, as_stream(stream), name);
 }
 

@@ -5,6 +5,8 @@
 // sixteenth of the scales.  A scale that is not finite makes its whole block NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "attn8.hpp"
 
 namespace rlt {
@@ -43,6 +45,35 @@ __device__ __forceinline__ float weight_scale(float scale, float e) {
 }
 
 constexpr float kNoExponent = -1024.f;  // e before any key
+
+// Of weights in fp16: e puts the largest between 2^5 and 2^7 when it moves, and moves when one
+// could pass 2^15.  So weights down to 2^-19 of the largest are normal numbers of the type.
+constexpr float kUsualExponent = 7.f, kMostExponent = 15.f;
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float f16_value(uint32_t bits) {
+  return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(bits)));
+}
+
+// The four codes of a word as two words of bf16 or fp16 pairs, exact.  For fp16 a code plus 128 becomes
+// the low bits of 1024 plus that, of which 1152 is taken away.
+template <typename S>
+__device__ __forceinline__ uint2 code_pairs(uint32_t word) {
+  if constexpr (std::is_same_v<S, f16>) {
+    const uint32_t x = word ^ 0x80808080u;
+    const half2v shift = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    const half2v lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + shift;
+    const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + shift;
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+  } else {
+    uint32_t f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __float_as_uint(static_cast<float>(static_cast<int8_t>(word >> (8 * i))));
+    // Their upper halves: the lower ones are 0.
+    return make_uint2(__builtin_amdgcn_perm(f[1], f[0], 0x07060302u), __builtin_amdgcn_perm(f[3], f[2], 0x07060302u));
+  }
+}
 
 // Bytes of a partial's state: m, l and e, and a place that keeps them on 16 bytes.
 struct __align__(16) PartState {
