@@ -5,6 +5,7 @@
 // Scores, softmax sums and the sums of weighted values are fp32, outputs of q's type.
 #include "decode_int8.hpp"
 #include "int8.hpp"
+#include "prefill_int8.hpp"
 
 namespace rlt {
 namespace {
@@ -156,7 +157,10 @@ extern "C" int rlt_paged_decode_int8(const void* q, const int64_t* q_strides, co
 extern "C" int64_t rlt_paged_prefill_int8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
                                                           int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
                                                           int64_t page_size) {
-  return 0;
+  if (total_q <= 0 || num_seqs <= 0 || max_table_width <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      !prefill8_shape(head_dim, page_size) || max_table_width > kMaxKeys / page_size)
+    return 0;
+  return prefill_i8_workspace(total_q, num_seqs, max_table_width * page_size, num_q_heads, head_dim);
 }
 
 extern "C" int rlt_paged_prefill_int8(const void* q, const int64_t* q_strides, const void* key_cache,
@@ -182,5 +186,6 @@ extern "C" int rlt_paged_prefill_int8(const void* q, const int64_t* q_strides, c
                                                               head_dim, page_size);
   if (workspace && need > 0 && (workspace_bytes < need || !aligned16(workspace)))
     return fail(RLT_EWORKSPACE, "%s: workspace must be %lld bytes on 16", name, (long long)need);
+  if (prefill8_layout(p.a)) return launch_prefill_i8(p, dtype, workspace, as_stream(stream), name);
   return launch_attn_i8_generic(p, dtype, as_stream(stream), name);
 }

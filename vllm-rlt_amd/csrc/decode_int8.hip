@@ -292,6 +292,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
           w[i] = fast_exp2(s[u][i] - off);
           l += w[i];
           w[i] *= g;
+          if constexpr (NP > 1) asm("" : "+v"(w[i]));  // the parts are of one product, rounded to fp32
         }
 #pragma unroll
         for (int n = 0; n < NP; ++n)
