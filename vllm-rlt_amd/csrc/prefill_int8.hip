@@ -27,6 +27,16 @@ struct PrefillI8Args {
 
 constexpr int kUnits = kBN / 16;
 
+// f(0), f(1), ..., f(N - 1) of constants.
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  unrolled_of(f, std::make_integer_sequence<int, N>{});
+}
+
 // Parts of q and of the weights, and the type of the scores' operands.
 template <typename T> struct Parts;
 template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf16; };
@@ -113,51 +123,69 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     }
   }
 
-  // Staging: thread (token, chunk), PASSES tokens TPP apart.  Tokens past the last key
-  // re-read it (in bounds; they are masked).  Thread u (kUnits + u) has unit u's scale of K (V).
+  // Staging: thread (token, chunk), PASSES tokens TPP apart.  A wave's tokens of a pass are of one unit,
+  // so of one block, and their addresses are the wave's but for an offset that stays.  Units past
+  // the last key are read from its block (in bounds; they are masked).  Lane l looks up the
+  // block of unit l % 4, and has its scale of K, or of V from lane l % 8 = 4 on.
   const int32_t* trow = a.tables + seq * a.table_stride;
   const int st = tid / CH, sc = tid % CH;
-  const uint8_t* kbase = a.k + kvh * a.kv_head + sc * 16;
-  const uint8_t* vbase = a.v + kvh * a.kv_head + sc * 16;
-  const float* sbase = (tid < kUnits ? args.ks : args.vs) + kvh * a.s_head;
-  const float f_scale = tid < kUnits ? p.qscale * __uint_as_float(static_cast<uint32_t>(127 + (LATE ? p.q_exp : 0)) << 23) : 1.f;
+  const uint8_t* kbase = a.k + kvh * a.kv_head;
+  const uint8_t* vbase = a.v + kvh * a.kv_head;
+  const int unit = lane % kUnits;
+  const bool of_k = lane % (2 * kUnits) < kUnits;
+  const float* sbase = (of_k ? args.ks : args.vs) + kvh * a.s_head;
+  const float f_scale = of_k ? p.qscale * __uint_as_float(static_cast<uint32_t>(127 + (LATE ? p.q_exp : 0)) << 23) : 1.f;
   const uint32_t block_bytes = static_cast<uint32_t>(a.kv_block), token_bytes = static_cast<uint32_t>(a.kv_token);
   const uint32_t s_block = static_cast<uint32_t>(a.s_block);
   const uint32_t page_mask = a.page - 1, last_key = max(wg_keys, 1) - 1, num_blocks = static_cast<uint32_t>(a.num_blocks);
-  uint32_t ids[PASSES], unit_id = 0;  // of the tile loaded next
+  uint32_t offset[PASSES];  // of this thread's codes in a block, but for the tile's first token in it
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) offset[i] = ((i * TPP + st) & page_mask) * token_bytes + sc * 16;
+  uint32_t id, v_id;  // the unit's block, of the tile whose K is loaded next and the one whose V is
   u32x4 kreg[PASSES], vreg[PASSES];
-  float sreg = 0.f;
-  auto token = [&](int tile, int t) { return min(static_cast<uint32_t>(tile * kBN + t), last_key); };
-  auto load_ids = [&](int tile) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) ids[i] = trow[token(tile, i * TPP + st) >> p.page_shift];
-    if (tid < 2 * kUnits) unit_id = trow[token(tile, tid % kUnits * 16) >> p.page_shift];
+  float sreg;
+  auto load_id = [&](int tile) __attribute__((always_inline)) {
+    id = trow[min(static_cast<uint32_t>(tile * kBN + unit * 16), last_key) >> p.page_shift];
   };
-  auto load_tile = [&](int tile) __attribute__((always_inline)) {
+  auto load_codes = [&](u32x4 (&reg)[PASSES], const uint8_t* base, uint32_t blocks, int tile) __attribute__((always_inline)) {
+    blocks = blocks < num_blocks ? blocks : 0;
+    const uint64_t first = static_cast<uint64_t>((static_cast<uint32_t>(tile) * kBN) & page_mask) * token_bytes;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const uint32_t slot = token(tile, i * TPP + st) & page_mask;
-      const uint64_t id = ids[i] < num_blocks ? ids[i] : 0;
-      const uint64_t at = id * block_bytes + __umul24(slot, token_bytes);
-      kreg[i] = *reinterpret_cast<const u32x4*>(kbase + at);
-      vreg[i] = *reinterpret_cast<const u32x4*>(vbase + at);
-    }
-    if (tid < 2 * kUnits) sreg = sbase[static_cast<uint64_t>(unit_id < num_blocks ? unit_id : 0) * s_block];
-  };
-  auto store_codes = [&](auto type, const u32x4& codes, uint16_t* dst) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint2 lo = code_pairs<decltype(type)>(codes[2 * i]), hi = code_pairs<decltype(type)>(codes[2 * i + 1]);
-      *reinterpret_cast<u32x4*>(dst + 8 * i) = u32x4{lo.x, lo.y, hi.x, hi.y};
+      const uint32_t of_pass = __builtin_amdgcn_readlane(blocks, (i * TPP + wave * (64 / CH)) / 16);
+      reg[i] = *reinterpret_cast<const u32x4*>(base + (static_cast<uint64_t>(of_pass) * block_bytes + first) + offset[i]);
     }
   };
-  auto store_tile = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      store_codes(S{}, kreg[i], &k_lds[buf][(i * TPP + st) * KROW + sc * 16]);
-      store_codes(f16{}, vreg[i], &v_lds[buf][(i * TPP + st) * VROW + sc * 16]);
+  auto load_k = [&](int tile) __attribute__((always_inline)) { load_codes(kreg, kbase, id, tile); };
+  auto load_v = [&](int tile) __attribute__((always_inline)) {
+    load_codes(vreg, vbase, v_id, tile);
+    sreg = sbase[static_cast<uint64_t>(v_id < num_blocks ? v_id : 0) * s_block];
+  };
+  // Eight codes of one of this thread's rows, of K (the first 2 PASSES chunks) or V, to their place in LDS.
+  constexpr int CHUNKS = 4 * PASSES;
+  auto store_chunk = [&](int chunk, int k_buf, int v_buf) __attribute__((always_inline)) {
+    const int i = chunk % (2 * PASSES) / 2, w = chunk % 2;
+    const int at = i * TPP + st;
+    uint32_t x = chunk < 2 * PASSES ? kreg[i][2 * w] : vreg[i][2 * w], y = chunk < 2 * PASSES ? kreg[i][2 * w + 1] : vreg[i][2 * w + 1];
+    asm volatile("" : "+v"(x), "+v"(y));  // here: not all of them as soon as they have arrived
+    if (chunk < 2 * PASSES) {
+      const uint2 lo = code_pairs<S>(x), hi = code_pairs<S>(y);
+      *reinterpret_cast<u32x4*>(&k_lds[k_buf][at * KROW + sc * 16 + 8 * w]) = u32x4{lo.x, lo.y, hi.x, hi.y};
+    } else {
+      const uint2 lo = code_pairs<f16>(x), hi = code_pairs<f16>(y);
+      *reinterpret_cast<u32x4*>(&v_lds[v_buf][at * VROW + sc * 16 + 8 * w]) = u32x4{lo.x, lo.y, hi.x, hi.y};
     }
-    if (tid < 2 * kUnits) f_lds[buf][tid / kUnits][tid % kUnits] = block_scale(sreg) * f_scale;
+  };
+  auto store_k = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS / 2; ++i) store_chunk(i, buf, 0);
+  };
+  auto store_v = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = CHUNKS / 2; i < CHUNKS; ++i) store_chunk(i, 0, buf);
+  };
+  auto store_scales = [&](int buf) __attribute__((always_inline)) {
+    if (tid < 2 * kUnits) f_lds[buf][tid / kUnits][unit] = block_scale(sreg) * f_scale;
   };
 
   f32x16 acc[DT];
@@ -170,23 +198,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const int grp = lane >> 4, gl = lane & 15;
   const int tr_off = (4 * (grp >> 1) + (gl >> 2)) * VROW + 16 * (grp & 1) + 4 * (gl & 3);
 
+  // S^T of half hh of a tile, step c of its products: element r is key key0 + 32 hh + 8 (r / 4) + 4 half +
+  // r % 4, of unit 2 hh + r / 8.
+  auto scores = [&](int buf, int c, int hh, f32x16& s) __attribute__((always_inline)) {
+    const u32x4 ka = *reinterpret_cast<const u32x4*>(&k_lds[buf][(hh * 32 + col) * KROW + 16 * c + 8 * half]);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) s = SOps::mma(as_v8<typename SOps::V8>(ka), as_v8<typename SOps::V8>(qw[n][c]), s);
+  };
+  f32x16 s[2] = {f32x16{}, f32x16{}};
+  // Loads of the tiles after those whose codes were just stored.  All of them go out, past the last
+  // tile too (the last key again), and in this order: a wait for one is a wait for all before it.
+  auto load_next = [&](int j) __attribute__((always_inline)) {
+    load_v(j + 2);
+    load_k(j + 3);
+    v_id = id;
+  };
+  // Tile j, whose scores s holds.  Its weights and the codes of the tiles after it are worked out
+  // between the products: of its own values, and of the next tile's scores, which take the
+  // registers of its own as they are used up.
   auto step = [&](int j) __attribute__((always_inline)) {
     const int buf = j & 1;
-    if (j + 1 < ntiles) {
-      load_tile(j + 1);
-      load_ids(j + 2);
-    }
-    if (wave_live && j * kBN <= wave_last) {
-      // S^T: element r of half hh is key key0 + 32 hh + 8 (r / 4) + 4 half + r % 4, of unit 2 hh + r / 8.
-      f32x16 s[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-      for (int c = 0; c < KS; ++c)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const u32x4 ka = *reinterpret_cast<const u32x4*>(&k_lds[buf][(hh * 32 + col) * KROW + 16 * c + 8 * half]);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) s[hh] = SOps::mma(as_v8<typename SOps::V8>(ka), as_v8<typename SOps::V8>(qw[n][c]), s[hh]);
-        }
+    load_id(j + 3);
+    {
       f32x4 f = *reinterpret_cast<const f32x4*>(f_lds[buf][0]);
       const f32x4 vs = *reinterpret_cast<const f32x4*>(f_lds[buf][1]);
       const int key0 = j * kBN;
@@ -215,68 +248,125 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
       const float top = max_across_halves(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
       const float highest = scale_exponent(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
       // No weight is above 2^(top - m + highest - e); it may be 2^15.
-      const bool rescale = __builtin_amdgcn_ballot_w64(top > m + kRescale || top - m + highest > e + kMostExponent) != 0;
-      float corr = 1.f;
-      if (rescale) {
+      if (__builtin_amdgcn_ballot_w64(top > m + kRescale || top - m + highest > e + kMostExponent) != 0) {
         const float mn = fmaxf(m, ceilf(top));
         const float down = mn - m;  // +inf at the first key, NaN before it
         float en = e - down;
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) en = fmaxf(en, ceilf(max_across_halves(x[u]) - mn) + scale_exponent(vs[u]) - kUsualExponent);
         const bool none = mn == -INFINITY;
-        corr = none ? 0.f : fast_exp2(e - down - en);
+        const float corr = none ? 0.f : fast_exp2(e - down - en);
         lsum = none ? 0.f : lsum * fast_exp2(-down);
         m = mn;
         e = none ? kNoExponent : en;
-      }
-      const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
-      // One site for all products: accumulators changed on two paths get two register sets.
-      if (rescale) {
 #pragma unroll
         for (int c = 0; c < DT; ++c)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
       }
+      const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
+      u32x4 pb[kUnits][NP];
+      float g[kUnits];  // a unit that this lane sees nothing of counts 0, whatever its scale
 #pragma unroll
-      for (int ks = 0; ks < kUnits; ++ks) {
-        // The weights of unit ks, in parts; one that this lane sees nothing of counts 0, whatever its scale.
-        const float g = x[ks] == -INFINITY ? 0.f : weight_scale(vs[ks], e);
-        u32x4 pb[NP];
+      for (int u = 0; u < kUnits; ++u) g[u] = x[u] == -INFINITY ? 0.f : weight_scale(vs[u], e);
+      // Two weights, in parts: elements 2 i and 2 i + 1 of unit u.
+      auto pair = [&](int k) __attribute__((always_inline)) {
+        const int u = k / 4, i = k % 4, r = u % 2 * 8 + 2 * i;
+        float y = fast_exp2(fmaf(s[u / 2][r], f[u], -mb)), z = fast_exp2(fmaf(s[u / 2][r + 1], f[u], -mb));
+        lsum += y + z;
+        asm volatile("" : "+v"(lsum));  // here: left to the end, the sums would keep 32 probabilities
+        y *= g[u], z *= g[u];
+        if constexpr (NP > 1) asm("" : "+v"(y), "+v"(z));  // the parts are of one product, rounded to fp32
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = (ks % 2) * 8 + 2 * i;
-          float y = fast_exp2(fmaf(s[ks / 2][r], f[ks], -mb)), z = fast_exp2(fmaf(s[ks / 2][r + 1], f[ks], -mb));
-          lsum += y + z;
-          y *= g, z *= g;
-          if constexpr (NP > 1) asm("" : "+v"(y), "+v"(z));  // the parts are of one product, rounded to fp32
-#pragma unroll
-          for (int n = 0; n < NP; ++n) {
-            pb[n][i] = Ops::pack2(y, z);
-            if (n + 1 < NP) y -= f16_value(pb[n][i]), z -= f16_value(pb[n][i] >> 16);
-          }
+        for (int n = 0; n < NP; ++n) {
+          pb[u][n][i] = Ops::pack2(y, z);
+          if (n + 1 < NP) y -= f16_value(pb[u][n][i]), z -= f16_value(pb[u][n][i] >> 16);
         }
+      };
+      // The products, in this order: values of unit 0, scores of half 0, values of units 1 and 2, scores of
+      // half 1, values of unit 3.  `values` of slot i: whether, of which unit; the step or output tile.
+      constexpr int SLOTS = 4 * DT + 2 * KS;
+      auto unit_of = [](int i) { return i < DT ? 0 : i < DT + KS ? -1 : i < 2 * DT + KS ? 1 : i < 3 * DT + KS ? 2 : i < 3 * DT + 2 * KS ? -2 : 3; };
+      auto part_of = [](int i) { return i < DT ? i : i < DT + KS ? i - DT : i < 3 * DT + KS ? (i - KS) % DT : i < 3 * DT + 2 * KS ? i - 3 * DT - KS : i - 3 * DT - 2 * KS; };
+      auto operand = [&](int i) __attribute__((always_inline)) {
+        const int u = unit_of(i), c = part_of(i);
+        if (u < 0) return *reinterpret_cast<const u32x4*>(&k_lds[buf ^ 1][((-u - 1) * 32 + col) * KROW + 16 * c + 8 * half]);
+        const uint16_t* vlo = &v_lds[buf][tr_off + u * 16 * VROW + c * 32];
+        const u32x2 lo = lds_read_tr(vlo), hi = lds_read_tr(vlo + 8 * VROW);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      };
+      auto product = [&](int i, const u32x4& x) __attribute__((always_inline)) {
+        const int u = unit_of(i), c = part_of(i);
+        if (u < 0) {
+          const int hh = -u - 1;
+          if (c == 0) s[hh] = f32x16{};
 #pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          const uint16_t* vlo = &v_lds[buf][tr_off + ks * 16 * VROW + c * 32];
-          const u32x2 lo = lds_read_tr(vlo), hi = lds_read_tr(vlo + 8 * VROW);
-          const u32x4 va = {lo[0], lo[1], hi[0], hi[1]};
+          for (int n = 0; n < NQ; ++n) s[hh] = SOps::mma(as_v8<typename SOps::V8>(x), as_v8<typename SOps::V8>(qw[n][c]), s[hh]);
+        } else {
 #pragma unroll
-          for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<f16x8>(va), as_v8<f16x8>(pb[n]), acc[c]);
+          for (int n = 0; n < NP; ++n) acc[c] = Ops::mma(as_v8<f16x8>(x), as_v8<f16x8>(pb[u][n]), acc[c]);
         }
-      }
+      };
+      constexpr int AHEAD = 4;
+      u32x4 ring[AHEAD];
+      unrolled<AHEAD>([&](auto at) __attribute__((always_inline)) { ring[at] = operand(at); });
+      unrolled<4>([&](auto k) __attribute__((always_inline)) { pair(k); });
+      __builtin_amdgcn_sched_barrier(0);
+      unrolled<SLOTS>([&](auto at) __attribute__((always_inline)) {
+        constexpr int i = decltype(at)::value;
+        product(i, ring[i % AHEAD]);
+        if constexpr (i + AHEAD < SLOTS) ring[i % AHEAD] = operand(i + AHEAD);
+        unrolled<12>([&](auto of) __attribute__((always_inline)) {
+          constexpr int k = 4 + decltype(of)::value;
+          if constexpr (i == (k < 8 ? (k - 4) * DT / 4 : k < 14 ? DT + (k - 8) * (KS + DT) / 6 : 2 * DT + KS + (k - 14) * DT / 2)) pair(k);
+        });
+        unrolled<CHUNKS>([&](auto of) __attribute__((always_inline)) {
+          constexpr int k = decltype(of)::value;
+          if constexpr (i == 3 * DT + KS + k * (KS + DT) / CHUNKS) store_chunk(k, buf, buf ^ 1);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
     }
-    if (j + 1 < ntiles) store_tile(buf ^ 1);
+    store_scales(buf ^ 1);
+    load_next(j);
     __syncthreads();
   };
 
   if (ntiles > first_tile) {
-    load_ids(first_tile);
-    load_tile(first_tile);
-    load_ids(first_tile + 1);
-    store_tile(first_tile & 1);
+    load_id(first_tile);
+    load_k(first_tile);
+    v_id = id;
+    load_v(first_tile);
+    load_id(first_tile + 1);
+    store_k(first_tile & 1);
+    load_k(first_tile + 1);
+    v_id = id;
+    load_id(first_tile + 2);
+    store_v(first_tile & 1);
+    store_scales(first_tile & 1);
+    load_v(first_tile + 1);
+    store_k(first_tile & 1 ^ 1);
+    load_k(first_tile + 2);
+    v_id = id;
     __syncthreads();
+#pragma unroll
+    for (int c = 0; c < KS; ++c)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) scores(first_tile & 1, c, hh, s[hh]);
+    __syncthreads();
+    // Tiles that some row of the wave sees, and those that it only helps to stage.
+    const int seen = wave_live && wave_last >= 0 ? min(ntiles, wave_last / kBN + 1) : first_tile;
+    int j = first_tile;
+    for (; j < seen; ++j) step(j);
+    for (; j < ntiles; ++j) {
+      load_id(j + 3);
+      store_k(j & 1);
+      store_v(j & 1 ^ 1);
+      store_scales(j & 1 ^ 1);
+      load_next(j);
+      __syncthreads();
+    }
   }
-  for (int j = first_tile; j < ntiles; ++j) step(j);
 
   lsum += __shfl_xor(lsum, 32, 64);
   if (!row_valid) return;
