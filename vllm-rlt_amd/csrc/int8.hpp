@@ -56,16 +56,16 @@ __device__ __forceinline__ float f16_value(uint32_t bits) {
   return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(bits)));
 }
 
-// The four codes of a word as two words of bf16 or fp16 pairs, exact.
+// The four codes of a word as two words of bf16 or fp16 pairs, exact.  For fp16 a code plus 128 becomes
+// the low bits of 1024 plus that, of which 1152 is taken away.
 template <typename S>
 __device__ __forceinline__ uint2 code_pairs(uint32_t word) {
   if constexpr (std::is_same_v<S, f16>) {
-    uint32_t lo, hi;  // one conversion a code, into its half of the word
-    asm("v_cvt_f16_i16_sdwa %0, sext(%1) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(lo) : "v"(word));
-    asm("v_cvt_f16_i16_sdwa %0, sext(%1) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1" : "+v"(lo) : "v"(word));
-    asm("v_cvt_f16_i16_sdwa %0, sext(%1) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(hi) : "v"(word));
-    asm("v_cvt_f16_i16_sdwa %0, sext(%1) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3" : "+v"(hi) : "v"(word));
-    return make_uint2(lo, hi);
+    const uint32_t x = word ^ 0x80808080u;
+    const half2v shift = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    const half2v lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + shift;
+    const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + shift;
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
   } else {
     uint32_t f[4];
 #pragma unroll
