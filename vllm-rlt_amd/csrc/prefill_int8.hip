@@ -89,39 +89,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   // An fp16 q goes in as it is, the others times 2^q_exp.
   constexpr bool LATE = std::is_same_v<S, f16>;
   u32x4 qw[NQ][KS];
-  {
-    const T* qrow = static_cast<const T*>(a.q) + (row0 + min(my_row, nq - 1)) * a.q_row + h * a.q_head;
-    const float power = __uint_as_float(static_cast<uint32_t>(127 + (LATE ? 0 : p.q_exp)) << 23 | p.q_sign);
-#pragma unroll
-    for (int c = 0; c < KS; ++c) {
-      const int d0 = 16 * c + 8 * half;
-      float x[8];
-      if (p.q_vec) {
-        constexpr int N = Packet<T>::N;
-#pragma unroll
-        for (int i = 0; i < 8 / N; ++i) Packet<T>::unpack(*reinterpret_cast<const u32x4*>(qrow + d0 + i * N), &x[i * N]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = load_elem(qrow + (d0 + i) * a.q_dim);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)  // infinities as NaN, which no other row's maximum takes up
-        x[i] = (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : x[i] * power;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          if constexpr (NQ > 1) {  // the top 16 bits: the rest is exact, and the last part holds all of it
-            const uint32_t lo = __float_as_uint(x[2 * w]), hi = __float_as_uint(x[2 * w + 1]);
-            qw[n][c][w] = lo >> 16 | (hi & 0xffff0000u);
-            x[2 * w] -= __uint_as_float(lo & 0xffff0000u);
-            x[2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
-          } else {
-            qw[n][c][w] = SOps::pack2(x[2 * w], x[2 * w + 1]);
-          }
-        }
-    }
-  }
 
   // Staging: thread (token, chunk), PASSES tokens TPP apart.  A wave's tokens of a pass are of one unit,
   // so of one block, and their addresses are the wave's but for an offset that stays.  Units past
@@ -337,19 +304,67 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   };
 
   if (ntiles > first_tile) {
+    // What the first products wait for is on its way at once: the blocks of three tiles; then q and the
+    // codes of two (each in turn: 6.9 us to the first step, so 6.2).
     load_id(first_tile);
-    load_k(first_tile);
     v_id = id;
-    load_v(first_tile);
     load_id(first_tile + 1);
-    store_k(first_tile & 1);
-    load_k(first_tile + 1);
-    v_id = id;
+    const uint32_t next_id = id;
     load_id(first_tile + 2);
+    constexpr int N = Packet<T>::N;
+    const T* const qrow = static_cast<const T*>(a.q) + (row0 + min(my_row, nq - 1)) * a.q_row + h * a.q_head;
+    u32x4 raw[KS][8 / N];
+    if (p.q_vec) {
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) raw[c][i] = *reinterpret_cast<const u32x4*>(qrow + 16 * c + 8 * half + i * N);
+    } else {
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) {
+          T x[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[e] = qrow[(16 * c + 8 * half + i * N + e) * a.q_dim];
+          raw[c][i] = __builtin_bit_cast(u32x4, x);
+        }
+    }
+    u32x4 knext[PASSES];
+    load_codes(kreg, kbase, v_id, first_tile);
+    load_v(first_tile);
+    load_codes(knext, kbase, next_id, first_tile + 1);
+    const float power = __uint_as_float(static_cast<uint32_t>(127 + (LATE ? 0 : p.q_exp)) << 23 | p.q_sign);
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8 / N; ++i) Packet<T>::unpack(raw[c][i], &x[i * N]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)  // infinities as NaN, which no other row's maximum takes up
+        x[i] = (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : x[i] * power;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (NQ > 1) {  // the top 16 bits: the rest is exact, and the last part holds all of it
+            const uint32_t lo = __float_as_uint(x[2 * w]), hi = __float_as_uint(x[2 * w + 1]);
+            qw[n][c][w] = lo >> 16 | (hi & 0xffff0000u);
+            x[2 * w] -= __uint_as_float(lo & 0xffff0000u);
+            x[2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
+          } else {
+            qw[n][c][w] = SOps::pack2(x[2 * w], x[2 * w + 1]);
+          }
+        }
+    }
+    store_k(first_tile & 1);
     store_v(first_tile & 1);
     store_scales(first_tile & 1);
-    load_v(first_tile + 1);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) kreg[i] = knext[i];
     store_k(first_tile & 1 ^ 1);
+    v_id = next_id;
+    load_v(first_tile + 1);
     load_k(first_tile + 2);
     v_id = id;
     __syncthreads();
