@@ -97,6 +97,32 @@ def test_attention():
         assert lib.rlt_paged_prefill_int8_workspace_bytes(1, 1, 4, 2, 2, 128, page) == 0
 
 
+def test_launches_past_the_largest_grid():
+    lib, native = library()
+    q, kv, sc = (native.int64_array(x) for x in ([4096, 64, 1], [4096, 256, 64, 1], [4, 1]))
+    rows = (1 << 23) - 1
+    refused(lib.rlt_paged_decode_int8(16, q, 16, 16, kv, 16, 16, sc, 16, 3, 3, 16, 16, q, rows, 64, 4, 64, 16, 4, 1.0, 2, 16, 1 << 60,
+                                      None), native, "too many rows", native.RLT_EUNSUPPORTED)
+    refused(lib.rlt_paged_prefill_int8(16, q, 16, 16, kv, 16, 16, sc, 16, 3, 3, 16, 16, 1, rows, rows, 16, q, 512, 4, 64, 16, 4, 1.0, 2,
+                                       None, 0, None), native, "too many rows", native.RLT_EUNSUPPORTED)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_workspaces_are_bounded(d):
+    """A decode's: rows, splits of 512 keys, 64 at most; a prefill's: 768 KiB (head_dim + 4) and 65 rows, a plan of 64 sequences."""
+    lib, _ = library()
+    for rows, hq, hkv, width in [(1, 16, 16, 64), (7, 32, 8, 100), (256, 16, 2, 1 << 20)]:
+        splits = min(-(-width * 16 // 512), 64)
+        assert lib.rlt_paged_decode_int8_workspace_bytes(rows, width, hq, hkv, d, 16) == rows * splits * hq * (d + 4) * 4
+    assert lib.rlt_paged_decode_int8_workspace_bytes(5, 32, 16, 16, d, 16) == 0  # one split: no partials
+    for rows in (1, 300, 4096, 1 << 20):
+        for seqs in (1, 7, 64):
+            for hq, hkv in [(16, 16), (32, 8), (5, 5)]:
+                need = lib.rlt_paged_prefill_int8_workspace_bytes(rows, seqs, 1 << 14, hq, hkv, d, 16)
+                assert 0 < need <= (768 * 1024 + 65 * hq * 4) * (d + 4) + 64 * 28
+    assert lib.rlt_paged_prefill_int8_workspace_bytes(4096, 65, 1 << 14, 16, 16, d, 16) == 0
+
+
 def cache(ndim):
     codes = torch.zeros((2, 1, 16, 2, 64)[5 - ndim :], dtype=torch.int8)
     return [codes, codes.clone(), *(torch.zeros(*codes.shape[: ndim - 3], 2) for _ in "kv")]
