@@ -621,7 +621,9 @@ int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t count, int64_t 
  * Caches are [num_blocks, num_layers, page_size, num_kv_heads, head_dim] (a layer
  * slice without num_layers), scales [num_blocks, num_layers, num_kv_heads] (a slice
  * without num_layers), on 4 bytes; strides in elements, shared by K and V.  Scales are
- * not negative; one that is not finite makes its whole block NaN to attention.
+ * not negative; one that is not finite makes its whole block NaN to attention.  Nothing
+ * has to be initialised: a block begins when its offset 0 is written, so that one goes
+ * first, or with the others of its call.
  */
 
 /*
@@ -636,6 +638,8 @@ int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t count, int64_t 
  * Rows of one block stand together in the call (as the tokens of a packed prompt do,
  * and those of a decode batch, which have a block each); their slots are distinct.
  * Rows of a block outside the pool, or of an offset outside its page, are skipped.
+ * Moving a token to another block is a read back and an append (its scale changes);
+ * whole blocks move as bytes, with their scales.
  */
 int rlt_kv_append_int8(void* key_cache, void* value_cache, const int64_t* cache_strides, void* key_scales,
                        void* value_scales, const int64_t* scale_strides, const void* k, const int64_t* k_strides,
@@ -659,8 +663,10 @@ int rlt_kv_gather_int8(const void* key_cache, const void* value_cache, const int
 /*
  * rlt_paged_decode over a layer slice of a block-scaled cache; q and out are of
  * `dtype`, scale_strides[2]: block, head.  A row of length 0 (or less) is written as
- * zeros; lengths are clamped to what the table covers.  A row's output bits depend on
- * its own q, blocks and length only.
+ * zeros; lengths are clamped to what the table covers; a table entry outside the pool
+ * reads block 0.  A row's output bits depend on its own q, blocks and length only.
+ * Scores, sums and accumulators are fp32; a probability times its block's scale goes into
+ * the products with 11 bits for bf16 and 22 for fp16 and fp32.
  * The workspace (rlt_paged_decode_int8_workspace_bytes, a function of the shape, on 16
  * bytes) holds the partials of cut rows; calls that overlap need one each.
  */
@@ -677,7 +683,9 @@ int rlt_paged_decode_int8(const void* q, const int64_t* q_strides, const void* k
 /*
  * rlt_paged_prefill over a layer slice of a block-scaled cache: packed chunks, bottom-
  * right causal, with the rows, lengths, max_seqlen_q and workspace of
- * rlt_paged_prefill_fp8 (its workspace by rlt_paged_prefill_int8_workspace_bytes).
+ * rlt_paged_prefill_fp8 (its bytes by rlt_paged_prefill_int8_workspace_bytes: at most
+ * 768 KiB * (head_dim + 4) and 65 rows of partials).  A probability times its block's
+ * scale goes into the products with 11 bits for bf16 and fp16 and 22 for fp32.
  */
 int64_t rlt_paged_prefill_int8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
                                                int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,

@@ -22,6 +22,7 @@ def test_append():
     refused(call(heads=0), native, "positive")
     refused(call(d=513), native, "head_dim", native.RLT_EUNSUPPORTED)
     refused(call(rows=1 << 24), native, "too many rows", native.RLT_EUNSUPPORTED)
+    refused(call(page=(1 << 30) + 1), native, "tokens a page", native.RLT_EUNSUPPORTED)
     refused(call(scales=None), native, "NULL")
     refused(call(k=None), native, "NULL")
     refused(call(at=None), native, "NULL")

@@ -8,7 +8,7 @@
 //   new codes: rint(x * (1 / s))
 // each operation rounded to fp32 on its own, ties to even.  A code that is kept is rounded
 // again each time s grows, by at most half a step of the new scale.  New rows with a value that
-// is not finite make s NaN and their codes 0; s0 NaN stays.
+// is not finite make s NaN, and their codes say nothing then; s0 NaN stays.
 #include <algorithm>
 #include <type_traits>
 
@@ -399,8 +399,9 @@ int cache_args(const char* name, const void* key_cache, const void* value_cache,
   if (num_blocks <= 0 || num_layers <= 0 || page_size <= 0) return fail(RLT_EINVAL, "%s: pool dimensions must be positive", name);
   if (layer < 0 || layer >= num_layers) return fail(RLT_EINVAL, "%s: layer %lld out of range", name, (long long)layer);
   if (d > 64 * kPerLane) return fail(RLT_EUNSUPPORTED, "%s: head_dim above %d", name, 64 * kPerLane);
-  // (A wave a row, K or V and head at worst, four a workgroup: threads of a launch inside 32 bits.)
-  if (n_rows > kMaxBlocks || hkv > 16384 || n_rows * hkv > 2 * kMaxBlocks || num_blocks > 0x7fffffff || page_size > 0x7fffffff)
+  // (A wave a row, K or V and head at worst, four a workgroup: threads of a launch inside 32 bits.  A
+  // page's tokens and what a wave's steps add to them stay inside 31.)
+  if (n_rows > kMaxBlocks || hkv > 16384 || n_rows * hkv > 2 * kMaxBlocks || num_blocks > 0x7fffffff || page_size > kMaxKeys)
     return fail(RLT_EUNSUPPORTED, "%s: too many rows, heads, blocks or tokens a page", name);
   if (n_rows == 0) return RLT_OK;
   if (!key_cache || !value_cache || !cache_strides || !key_scales || !value_scales || !scale_strides || !blocks || !offsets)
