@@ -477,6 +477,21 @@ def test_prefill_of_cut_keys_and_the_batch_invariant_form(dtype, prefixes, chunk
         at += n
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(6, 2, 128), (5, 1, 64), (28, 4, 128), (40, 1, 128), (24, 8, 64), (200, 1, 64)])
+def test_prefill_of_groups_of_any_size(dtype, hq, hkv, d):
+    """Tiles hold the query heads of a row together: groups that do not divide them, and ones larger than a wave's rows or a tile."""
+    for prefixes, chunks in [([0, 300, 77, 1500], [1, 9, 43, 130]), ([2000], [3]), ([5, -3] * 35, [2, 4] * 35)]:
+        lengths = [max(p + c, 0) for p, c in zip(prefixes, chunks)]
+        c = Case(lengths, hq, hkv, d, dtype=dtype, seed=hq, chunks=chunks)
+        out = c.prefill()
+        c.check(out)
+        whole = c.prefill(batch_invariant=True)
+        c.check(whole)
+        if len(chunks) > 64:
+            assert torch.equal(out, whole)
+
+
 @pytest.mark.parametrize("hq,hkv,d", [(3, 1, 64), (9, 9, 128)])
 def test_cut_sequences_of_many_rows(hq, hkv, d):
     # Heads that do not fill a merge's workgroup, two cut sequences with an uncut one between, rows that see no key.

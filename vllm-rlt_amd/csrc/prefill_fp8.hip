@@ -512,6 +512,7 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
   const int64_t slots = ws ? partial_slots(a.rows, a.num_seqs, a.max_len, a.hq) : 0;
   if (slots > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);  // 64 sequences' stay inside 31 bits
   p.slots = static_cast<int>(slots);
+  p.group = 1;
   p.round = dtype == RLT_FLOAT32 && a.d == 128 ? kRound / 2 : kRound;
   if (slots) {
     p.part_acc = static_cast<float*>(ws);

@@ -2,15 +2,18 @@
 // matrix cores (head_dim 64 / 128, pages of a power of two of at least 16 tokens; int8.hpp has
 // the softmax, prefill_plan.hpp the launch's plan).
 //
-// A workgroup of 4 waves takes 128 query rows of one (sequence, query head) over a
-// segment of its keys, a wave 32 rows, 64 keys a tile, four units of 16 keys that have one
-// scale of K and one of V each:
+// A workgroup of 4 waves takes 128 (query row, query head) pairs of one (sequence, KV head), a
+// row's heads together, over a segment of its keys, a wave 32 of them, 64 keys a tile, four units
+// of 16 keys that have one scale of K and one of V each.  (A tile of one head's rows only: four
+// chunks of 740-983 rows over up to 4400 keys, 16 + 4 heads, 125.8 us, so 118.2; sixteen of 8 rows
+// over 4000, 32 + 8 heads, 123 and 44.)
 // - S^T = K Q^T on the 16-bit MFMA of q's type (32x32x16; an fp32 q in three bf16 parts).  Codes
 //   become bf16 or fp16, exactly, once a workgroup, on their way into LDS; their unit's scale
 //   multiplies the sums, in the instruction that takes the running maximum off.
 // - O^T += V^T W^T on the fp16 MFMA, codes as fp16 likewise; V^T comes from transposing LDS
 //   reads, W, the probabilities times their unit's V scale, from the registers S^T left it
-//   in: in one part, 11 bits, for bf16 and fp16, in two for fp32.
+//   in: in one part, 11 bits, for bf16 and fp16, in two for fp32.  (Two for fp16 would bring its outputs
+//   from 2.9e-4 to 2.1e-4 of their rms, which is their own rounding, and cost 21 to 27%.)
 #include "prefill_int8.hpp"
 
 #include "prefill_plan.hpp"
@@ -67,12 +70,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Item it;
   if (!find_item(p, &it)) return;
-  const int seq = uniform(it.seq), h = uniform(it.head), row0 = uniform(it.row0), nq = uniform(it.nq);
+  const int seq = uniform(it.seq), kvh = uniform(it.head), row0 = uniform(it.row0), nq = uniform(it.nq);
+  const int group = p.group, rows = nq * group;  // row i of the tiles is row i / group of query head i % group
   const int len = uniform(it.len);
   const int prefix = len - nq;  // query row i sees keys up to prefix + i
   const int qt0 = uniform(it.tile) * kBM;
-  const int kvh = h / (a.hq / a.hkv);
-  const int wg_keys = min(prefix + min(qt0 + kBM, nq), len);  // keys that some row of the workgroup sees
+  const int wg_keys = min(prefix + min((qt0 + kBM - 1) / group + 1, nq), len);  // keys that some row of the workgroup sees
   const int first_tile = uniform(it.seg * it.seg_tiles);
   const int ntiles = min(first_tile + uniform(it.seg_tiles), (max(wg_keys, 0) + kBN - 1) / kBN);
   if (it.segs > 1 && it.seg > 0 && ntiles <= first_tile) return;  // the merge skips such a segment
@@ -80,10 +83,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const int half = lane >> 5, col = lane & 31;
   const int wave_row0 = qt0 + wave * 32;
   const int my_row = wave_row0 + col;
-  const bool row_valid = my_row < nq;
-  const int limit = row_valid ? prefix + my_row : -1;  // last key this lane's query sees
-  const int wave_last = prefix + min(wave_row0 + 31, nq - 1);
-  const bool wave_live = wave_row0 < nq;
+  const bool row_valid = my_row < rows;
+  const int at_row = min(my_row, rows - 1) / group, h = kvh * group + min(my_row, rows - 1) - at_row * group;
+  const int limit = row_valid ? prefix + at_row : -1;  // last key this lane's query sees
+  const int wave_first = prefix + wave_row0 / group, wave_last = prefix + min((wave_row0 + 31) / group, nq - 1);
+  const bool wave_live = wave_row0 < rows;
 
   // q's parts, B operands: lane (col, half) holds dims [16 c + 8 half, + 8) of row col for step c.
   // An fp16 q goes in as it is, the others times 2^q_exp.
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
       const int key0 = j * kBN;
       // Scores are scaled ahead where some are masked (a scale of 0 or NaN times -inf would not
       // be) and where they are so large that the scaled maximum's own rounding counts.
-      const bool masked = uniform(key0 + kBN - 1 > prefix + wave_row0 || wave_row0 + 31 >= nq);
+      const bool masked = uniform(key0 + kBN - 1 > wave_first || wave_row0 + 31 >= rows);
       if (masked || __builtin_amdgcn_ballot_w64(fabsf(m) > 4096.f && m != -INFINITY) != 0) {
         const int lim = limit - key0 - 4 * half;
 #pragma unroll
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     const uint32_t next_id = id;
     load_id(first_tile + 2);
     constexpr int N = Packet<T>::N;
-    const T* const qrow = static_cast<const T*>(a.q) + (row0 + min(my_row, nq - 1)) * a.q_row + h * a.q_head;
+    const T* const qrow = static_cast<const T*>(a.q) + (row0 + at_row) * a.q_row + h * a.q_head;
     u32x4 raw[KS][8 / N];
     if (p.q_vec) {
 #pragma unroll
@@ -390,7 +394,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   lsum += __shfl_xor(lsum, 32, 64);
   if (!row_valid) return;
   if (uniform(it.segs) > 1) {
-    const int64_t slot = (static_cast<int64_t>(it.slot0) + static_cast<int64_t>(it.seg) * nq + my_row) * a.hq + h;
+    const int64_t slot = (static_cast<int64_t>(it.slot0) + static_cast<int64_t>(it.seg) * nq + at_row) * a.hq + h;
     float* dst = p.part_acc + slot * D + 4 * half;
 #pragma unroll
     for (int c = 0; c < DT; ++c)
@@ -403,7 +407,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   // A row that sees no key is zeros.
   const float inv = 1.f / lsum;
   const int exponent = static_cast<int>(e);
-  T* orow = static_cast<T*>(a.out) + (row0 + my_row) * a.o_row + h * a.o_head;
+  T* orow = static_cast<T*>(a.out) + (row0 + at_row) * a.o_row + h * a.o_head;
 #pragma unroll
   for (int c = 0; c < DT; ++c)
 #pragma unroll
@@ -439,7 +443,8 @@ __global__ __launch_bounds__(256) void prefill_i8_merge_kernel(PrefillI8Args arg
     const int h = e0 / D, d = e0 % D;
     if (h >= a.hq) continue;
     // Segments past the last key of the row's query tile were not computed.
-    const int keys = max(len - nq + min(i / kBM * kBM + kBM, nq), 0);
+    const int tile_end = (i * p.group + h % p.group) / kBM * kBM + kBM;
+    const int keys = max(len - nq + min((tile_end - 1) / p.group + 1, nq), 0);
     const int live = min(segs, max(1, (keys + seg_keys - 1) / seg_keys));
     const int64_t step = static_cast<int64_t>(nq) * a.hq;  // slots from one segment to the next
     const int64_t base = (static_cast<int64_t>(slot0) + i) * a.hq + h;
@@ -515,6 +520,7 @@ int launch_prefill_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t stre
   const int64_t slots = ws ? partial_slots(a.rows, a.num_seqs, a.max_len, a.hq) : 0;
   if (slots > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);  // 64 sequences' stay inside 31 bits
   p.slots = static_cast<int>(slots);
+  p.group = a.hq / a.hkv;
   p.round = dtype == RLT_FLOAT32 && a.d == 128 ? kRound / 2 : kRound;
   if (slots) {
     p.part_acc = static_cast<float*>(ws);
@@ -523,8 +529,9 @@ int launch_prefill_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t stre
   }
   fill_prefill8(&p, dtype);
   const int64_t tiles = prefill8_tiles(p);
-  if (tiles * a.hq > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
-  const unsigned grid = static_cast<unsigned>(tiles * a.hq);
+  // (So that rows of a tile, a row and head each, stay inside 31 bits as well.)
+  if (tiles * a.hkv > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
+  const unsigned grid = static_cast<unsigned>(tiles * a.hkv);
   switch (dtype) {
     case RLT_BFLOAT16: launch_type<bf16>(args, grid, stream); break;
     case RLT_FLOAT16: launch_type<f16>(args, grid, stream); break;

@@ -21,7 +21,6 @@ constexpr int kBM = 128;  // query rows a workgroup
 constexpr int kBN = 64;   // keys a tile
 constexpr float kRescale = 8.f;
 constexpr int kMaxQExp = 24;
-constexpr int kXcds = 8;
 constexpr int kRound = 512;  // workgroups that run at once: two a CU (fp32 at head_dim 128: one)
 constexpr int kTargetItems = kRound * 3 / 2;
 // Shorter segments are not worth an item (about 9 us of plan, first loads and merge beside
@@ -54,6 +53,7 @@ struct Prefill8Args {
   SeqPlan* plan;      // [kPlanSeqs], for the merge kernel
   int slots;
   int round;  // workgroups that run at once
+  int group;  // query heads whose rows stand together in a query tile: row i of head g of them is its row i * group + g
   int out_vec;  // 4 elements of an out row can be stored at once
   int q_vec;    // q rows are 16-byte aligned, dims together
 };
@@ -90,7 +90,8 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
     seq_rows(p.a, lane, s.row0, s.nq);
     s.len = sequence_length(p.a, lane);
   }
-  s.tiles = (s.nq + kBM - 1) / kBM;
+  s.tiles = (s.nq * p.group + kBM - 1) / kBM;
+  const int heads = p.a.hq / p.group;
   const int keys = (s.len + kBN - 1) / kBN;
   s.segs = 1;
   s.seg_tiles = keys;
@@ -98,7 +99,7 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
     // In (query tile, key tile) pairs.  The sum's rounding is inside the slack of
     // partial_slots() and of the grid.
     const float work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(
-        static_cast<float>(s.tiles) * static_cast<float>(keys), [](float a, float b) { return a + b; })), 63)) * p.a.hq;
+        static_cast<float>(s.tiles) * static_cast<float>(keys), [](float a, float b) { return a + b; })), 63)) * heads;
     const int longest = __builtin_amdgcn_readlane(wave_scan(s.tiles ? keys : 0, [](int a, int b) { return max(a, b); }), 63);
     // Cut where the longest item would outlast the others by half: 24 chunks of 100-170 rows
     // over up to 1000 keys (768 items of up to 18 tiles) take 55 us whole, 69 cut.
@@ -106,10 +107,10 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
       // Few items: cut into one round of workgroups.  Many, of different lengths: into half as
       // many again, so that the short ones fill the gaps (eight chunks 402 us in 512, 353
       // in 768, 369 in 1024; one chunk of 64 items 96, 119, 109).
-      const bool few = __builtin_amdgcn_readlane(scan_sum(s.tiles), 63) * p.a.hq <= p.round / 2;
+      const bool few = __builtin_amdgcn_readlane(scan_sum(s.tiles), 63) * heads <= p.round / 2;
       int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few ? p.round : p.round * 3 / 2)), 1e9f)));
       for (int i = 0; few && i < 4; ++i) {  // as rounding up makes more items, towards the round
-        const int items = __builtin_amdgcn_readlane(scan_sum(s.tiles * max(1, (keys + target - 1) / target)), 63) * p.a.hq;
+        const int items = __builtin_amdgcn_readlane(scan_sum(s.tiles * max(1, (keys + target - 1) / target)), 63) * heads;
         if (items <= p.round) break;
         target = max(target + 1, static_cast<int>(static_cast<float>(target) * items / p.round));
       }
@@ -125,7 +126,7 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
 }
 
 struct Item {
-  int seq, head, tile, seg;
+  int seq, head, tile, seg;  // head: a group of them
   int row0, nq, len, segs, seg_tiles, slot0;
 };
 
@@ -133,8 +134,9 @@ struct Item {
 __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
   const Attn8Args& a = p.a;
   const int lane = threadIdx.x & 63;
-  // Workgroup b runs on XCD b % 8, which serves the heads h == b (mod 8).
-  const int groups = a.hq % kXcds == 0 ? kXcds : 1, heads = a.hq / groups;
+  // Workgroup b runs on XCD b % 8, which serves the heads h == b (mod 8) (or 4 or 2, where there are so few).
+  const int all_heads = a.hq / p.group;
+  const int groups = all_heads % 8 == 0 ? 8 : all_heads % 4 == 0 ? 4 : all_heads % 2 == 0 ? 2 : 1, heads = all_heads / groups;
   const int x = blockIdx.x % groups;
   int pos = blockIdx.x / groups;
   int unit;
@@ -170,7 +172,7 @@ __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
   for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
     int row0 = 0, nq = 0;
     if (s0 + lane < a.num_seqs) seq_rows(a, s0 + lane, row0, nq);
-    const int tiles = (nq + kBM - 1) / kBM, before = scan_sum(tiles) - tiles;
+    const int tiles = (nq * p.group + kBM - 1) / kBM, before = scan_sum(tiles) - tiles;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(unit >= before && unit < before + tiles);
     if (hit) {
       const int at = __builtin_ctzll(hit);
@@ -234,7 +236,8 @@ inline void fill_prefill8(Prefill8Args* p, int dtype) {
 
 // Query tiles, and the segments past the first (as many items as partial_slots() has such rows).
 inline int64_t prefill8_tiles(const Prefill8Args& p) {
-  return p.a.rows / kBM + std::min<int64_t>(p.a.num_seqs, p.a.rows) + (p.slots ? (kTargetItems + p.a.hq - 1) / p.a.hq + 2 : 0);
+  const int64_t heads = p.a.hq / p.group;
+  return p.a.rows * p.group / kBM + std::min<int64_t>(p.a.num_seqs, p.a.rows) + (p.slots ? (kTargetItems + heads - 1) / heads + 2 : 0);
 }
 
 }  // namespace rlt
