@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const Attn8Args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Item it;
-  if (!find_item(p, &it)) return;
+  if (!find_item<false>(p, &it)) return;
   const int seq = uniform(it.seq), h = uniform(it.head), row0 = uniform(it.row0), nq = uniform(it.nq);
   const int len = uniform(it.len);
   const int prefix = len - nq;  // query row i sees keys up to prefix + i

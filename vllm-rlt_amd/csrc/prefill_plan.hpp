@@ -84,8 +84,12 @@ __device__ __forceinline__ X wave_scan(X x, F join) {
 }
 __device__ __forceinline__ int scan_sum(int x) { return wave_scan(x, [](int a, int b) { return a + b; }); }
 
-__device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
+// TAILS: the sequences of launches of many items are cut into whole segments and a shorter last one,
+// not into equal ones; *tails: whether they are.
+template <bool TAILS>
+__device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane, bool* tails) {
   SeqPlan s{};
+  *tails = false;
   if (lane < p.a.num_seqs) {
     seq_rows(p.a, lane, s.row0, s.nq);
     s.len = sequence_length(p.a, lane);
@@ -108,14 +112,18 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane) {
       // many again, so that the short ones fill the gaps (eight chunks 402 us in 512, 353
       // in 768, 369 in 1024; one chunk of 64 items 96, 119, 109).
       const bool few = __builtin_amdgcn_readlane(scan_sum(s.tiles), 63) * heads <= p.round / 2;
-      int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few ? p.round : p.round * 3 / 2)), 1e9f)));
+      // Or, with tails, into a round of whole segments, longest first, and the shorter last ones of
+      // their sequences, which fill the gaps (four chunks of 740-983 rows over up to 4400 keys, 16 + 4
+      // heads, 119.1 us in equal ones, 113.8).
+      *tails = TAILS && !few;
+      int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few || *tails ? p.round : p.round * 3 / 2)), 1e9f)));
       for (int i = 0; few && i < 4; ++i) {  // as rounding up makes more items, towards the round
         const int items = __builtin_amdgcn_readlane(scan_sum(s.tiles * max(1, (keys + target - 1) / target)), 63) * heads;
         if (items <= p.round) break;
         target = max(target + 1, static_cast<int>(static_cast<float>(target) * items / p.round));
       }
       s.segs = max(1, (keys + target - 1) / target);
-      s.seg_tiles = (keys + s.segs - 1) / s.segs;
+      s.seg_tiles = *tails && s.segs > 1 ? target : (keys + s.segs - 1) / s.segs;
       // cu_seqlens that do not rise ask for more slots than there are: those stay whole.
       const int slots = s.segs > 1 ? static_cast<int>(min(static_cast<int64_t>(s.nq) * s.segs, static_cast<int64_t>(p.slots) + 1)) : 0;
       s.slot0 = scan_sum(slots) - slots;
@@ -131,6 +139,7 @@ struct Item {
 };
 
 // Work item blockIdx.x, worked out by every wave alike; false past the last.
+template <bool TAILS>
 __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
   const Attn8Args& a = p.a;
   const int lane = threadIdx.x & 63;
@@ -141,28 +150,44 @@ __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
   int pos = blockIdx.x / groups;
   int unit;
   if (a.num_seqs <= kPlanSeqs) {
-    const SeqPlan s = plan_of(p, lane);
+    bool tails;
+    const SeqPlan s = plan_of<TAILS>(p, lane, &tails);
     if (p.part_acc && blockIdx.x == 0 && threadIdx.x < a.num_seqs) p.plan[lane] = s;
-    const int units = s.tiles * s.segs, cost = s.seg_tiles;
-    int before = 0;  // units of sequences with longer items (equal ones in order)
-    for (int q = 0; q < a.num_seqs; ++q) {
-      const int c = __builtin_amdgcn_readlane(cost, q), u = __builtin_amdgcn_readlane(units, q);
-      before += c > cost || (c == cost && q < lane) ? u : 0;
-    }
-    const int64_t first = static_cast<int64_t>(before) * heads, end = first + static_cast<int64_t>(units) * heads;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < a.num_seqs && pos >= first && pos < end);
-    if (!hit) return false;
-    const int at = __builtin_ctzll(hit);
+    // A sequence's items: those of its segments, a shorter last one (`tail`) apart.
+    const int last = (s.len + kBN - 1) / kBN - (s.segs - 1) * s.seg_tiles;
+    const int tail_units = tails && s.segs > 1 && last < s.seg_tiles ? s.tiles : 0, units = s.tiles * s.segs - tail_units;
+    // Units of longer items than these: their keys are distinct, equal lengths in the sequences' order.
+    const uint32_t key = static_cast<uint32_t>(s.seg_tiles) << 7 | (127 - lane), tail_key = static_cast<uint32_t>(last) << 7 | (63 - lane);
+    int before = 0, tail_before = 0;
+    auto count = [&](uint32_t of_key, int of_units) __attribute__((always_inline)) {
+#pragma unroll 4
+      for (int q = 0; q < a.num_seqs; ++q) {
+        const uint32_t k = __builtin_amdgcn_readlane(of_key, q);
+        const int u = __builtin_amdgcn_readlane(of_units, q);
+        before += k > key ? u : 0;
+        if (tails) tail_before += k > tail_key ? u : 0;
+      }
+    };
+    count(key, units);
+    if (tails) count(tail_key, tail_units);
+    auto item_of = [&](int b, int n) __attribute__((always_inline)) {  // the lane whose items [b, b + n) hold this one
+      const int64_t first = static_cast<int64_t>(b) * heads, end = first + static_cast<int64_t>(n) * heads;
+      return __builtin_amdgcn_ballot_w64(lane < a.num_seqs && pos >= first && pos < end);
+    };
+    const uint64_t body = item_of(before, units), tail = tails ? item_of(tail_before, tail_units) : 0;
+    if (!(body | tail)) return false;
+    const int at = __builtin_ctzll(body ? body : tail);
     it->seq = at;
-    pos -= __builtin_amdgcn_readlane(before, at) * heads;
+    pos -= __builtin_amdgcn_readlane(body ? before : tail_before, at) * heads;
     it->row0 = __builtin_amdgcn_readlane(s.row0, at), it->nq = __builtin_amdgcn_readlane(s.nq, at);
     it->len = __builtin_amdgcn_readlane(s.len, at), it->segs = __builtin_amdgcn_readlane(s.segs, at);
     it->seg_tiles = __builtin_amdgcn_readlane(s.seg_tiles, at), it->slot0 = __builtin_amdgcn_readlane(s.slot0, at);
-    const int tiles = __builtin_amdgcn_readlane(s.tiles, at), of_head = tiles * it->segs;
+    const int tiles = __builtin_amdgcn_readlane(s.tiles, at), of_head = __builtin_amdgcn_readlane(body ? units : tail_units, at);
     it->head = x + groups * (pos / of_head);
     unit = pos % of_head;
     it->seg = unit / tiles;
     unit -= it->seg * tiles;
+    if (!body) it->seg = it->segs - 1;
     it->tile = tiles - 1 - unit;  // the last rows, which see most keys, first
     return true;
   }
