@@ -50,7 +50,8 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<T, D>))) void decode_i8_kernel(DecodeI8Args p) {
   using S = typename Parts<T>::S;
   constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P;
-  constexpr int KS = (D + 127) / 128;  // 128 dims each: four MFMA steps
+  constexpr int KD = D < 128 ? D : 128, KS = D / KD;  // dims of K at a time, of which a lane has LD: ST MFMA steps
+  constexpr int LD = KD / 4, ST = LD / 8, KC = LD / 16;
   constexpr int DT = D / 16;           // output tiles of 16 dims
   constexpr int CH = D / 16;           // 16-byte chunks of a code row
   constexpr int TPI = 64 / CH;         // tokens a load instruction
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
   uint8_t* const v_lds = lds[wave] + kTile * D;
   // The swizzles are linear in the row's bits, so that a place is a base of the lane's xor a
   // constant; `opaque` keeps the compiler from holding one register for each in the tile loop.
-  uint32_t k_read = col * D + 16 * ((D >= 128 || j < 2 ? 2 * j : 0) ^ k_swizzle<D>(col));
+  uint32_t k_read = col * D + 16 * (KC * j ^ k_swizzle<D>(col));
   const int vt = lane & 15, v_row = 4 * j + vt / 2 % 4 + 16 * (vt / 8);  // of a transposing read
   uint32_t v_read = v_row * D + 16 * v_swizzle<D>(v_row) + 8 * (vt & 1);
   uint32_t k_chunk = 16 * (lane % CH ^ k_swizzle<D>(lane / CH)), v_chunk = 16 * (lane % CH ^ v_swizzle<D>(lane / CH));
@@ -156,9 +157,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
       load_k(0);
       load_v(0);
     }
-    // q's parts, B operands: lane (col, j) holds dims [128 c + 32 j, + 32) of query head c0 +
+    // q's parts, B operands: lane (col, j) holds dims [KD c + LD j, + LD) of query head c0 +
     // col, 8 of them a step.
-    u32x4 qw[NQ][4 * KS];
+    u32x4 qw[NQ][ST * KS];
     {
       uint32_t thread = threadIdx.x;
       opaque(thread);
@@ -183,19 +184,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         }
       wait_lds();
       asm volatile("s_barrier" ::: "memory");  // (__syncthreads() would wait for the tile)
-      const u32x4 zero = {0u, 0u, 0u, 0u};
-      const bool in = D >= 128 || j < 2;  // head_dim 64: the upper half of the 128 is 0
 #pragma unroll
       for (int i = 0; i < NQ; ++i)
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          const int d0 = in ? 128 * c + 32 * j : 0;
+        for (int c = 0; c < KS; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(q_lds[i][col] + 2 * (d0 + 8 * e));
-            qw[i][4 * c + e] = in ? w : zero;
-          }
-        }
+          for (int e = 0; e < ST; ++e)
+            qw[i][ST * c + e] = *reinterpret_cast<const u32x4*>(q_lds[i][col] + 2 * (KD * c + LD * j + 8 * e));
       wait_lds();
       asm volatile("s_barrier" ::: "memory");
     }
@@ -210,19 +205,15 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
       opaque(k_read), opaque(v_read), opaque(k_chunk), opaque(v_chunk), opaque(load_row);
       const float* scales = reinterpret_cast<const float*>(lds[wave] + kScales + tile % 2 * 256);  // K's, then V's
       wait_loads<NI>();  // V may still be on its way
-      u32x4 ka[2][KS][2];
+      u32x4 ka[2][KS][KC];
       float kf[2], vf[2];  // of the two halves: 16 tokens lie in one block
-      const bool in = D >= 128 || j < 2;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         kf[u] = scales[16 * u], vf[u] = scales[kTile + 16 * u];
 #pragma unroll
         for (int c = 0; c < KS; ++c)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(k_lds + (k_read ^ (16 * (8 * c + e))) + 16 * u * D);
-            ka[u][c][e] = in ? w : u32x4{0u, 0u, 0u, 0u};
-          }
+          for (int e = 0; e < KC; ++e) ka[u][c][e] = *reinterpret_cast<const u32x4*>(k_lds + (k_read ^ (16 * (KD / 16 * c + e))) + 16 * u * D);
       }
       wait_lds();
       if (more) load_k(tile + 1);
@@ -233,7 +224,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
 #pragma unroll
         for (int c = 0; c < KS; ++c)
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
+          for (int q4 = 0; q4 < ST; ++q4) {
             u32x4 kw;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -241,7 +232,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
               kw[2 * i] = pairs.x, kw[2 * i + 1] = pairs.y;
             }
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) s[u] = mma16<S>(kw, qw[i][4 * c + q4], s[u]);
+            for (int i = 0; i < NQ; ++i) s[u] = mma16<S>(kw, qw[i][ST * c + q4], s[u]);
           }
       }
       const int first = t0 + tile * (kWaves * kTile);
