@@ -138,13 +138,27 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
     // Tokens past the end re-read the last one: in bounds, and masked below.
     auto load_rows = [&](int tile, const uint8_t* base, uint32_t to, uint32_t chunk, auto swizzle) __attribute__((always_inline)) {
       const int last = min(end - 1 - t0 - tile * (kWaves * kTile), kTile - 1);  // row
+      auto unit_at = [&](int half) __attribute__((always_inline)) {  // an instruction's tokens lie in one
+        const int unit = tile % 32 * 2 + half;
+        return static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(unit_kv >> 32), unit)) << 32 |
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(unit_kv), unit));
+      };
+      if (last == kTile - 1) {
+        const uint32_t row = __umul24(load_row, token_bytes);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint8_t* from = base + unit_at(half);
+#pragma unroll
+          for (int i = half * NI / 2; i < (half + 1) * NI / 2; ++i, from += TPI * token_bytes)
+            dma16(to + i * 1024, row + (chunk ^ (16 * swizzle(i * TPI))), from);
+        }
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int half = min(i * TPI, last) / 16, unit = tile % 32 * 2 + half;  // the instruction's tokens lie in one
-        const int64_t from = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(unit_kv >> 32), unit)) << 32 |
-                             static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(unit_kv), unit));
+        const int half = min(i * TPI, last) / 16;
         const uint32_t tok = min(i * TPI + static_cast<int>(load_row), last) - 16 * half;
-        dma16(to + i * 1024, __umul24(tok, token_bytes) + (chunk ^ (16 * swizzle(i * TPI))), base + from);
+        dma16(to + i * 1024, __umul24(tok, token_bytes) + (chunk ^ (16 * swizzle(i * TPI))), base + unit_at(half));
       }
     };
     auto load_k = [&](int tile) __attribute__((always_inline)) {
@@ -240,13 +254,24 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const float f = block_scale(kf[u]) * a.qscale;
-        vf[u] = first + 16 * u < end ? block_scale(vf[u]) : 0.f;
+        vf[u] = block_scale(vf[u]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][i] *= f;
+      }
+      if (first + kTile > end) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (first + 16 * u >= end) vf[u] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (first + 16 * u + 4 * j + i >= end) s[u][i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
         highest = fmaxf(highest, scale_exponent(vf[u]));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[u][i] = first + 16 * u + 4 * j + i < end ? s[u][i] * f : -INFINITY;
-          top = fmaxf(top, s[u][i]);
-        }
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
       }
       top = strided_max<16>(top);
       // No weight is above 2^(top - m + highest - e); it may be 2^15.
