@@ -32,6 +32,11 @@ __device__ __forceinline__ void dma16(uint32_t lds_byte, uint32_t offset, const 
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_byte), "v"(offset), "s"(base)
                : "memory", "m0");
 }
+// The same, of bytes that stay in the L2: others read the rest of their lines.
+__device__ __forceinline__ void dma16_kept(uint32_t lds_byte, uint32_t offset, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_byte), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
 __device__ __forceinline__ void dma_byte(uint32_t lds_byte, const uint8_t* from) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(lds_byte), "v"(from) : "memory", "m0");
 }
