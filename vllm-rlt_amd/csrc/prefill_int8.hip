@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     load_id(j + 3);
     {
       f32x4 f = *reinterpret_cast<const f32x4*>(f_lds[buf][0]);
-      const f32x4 vs = *reinterpret_cast<const f32x4*>(f_lds[buf][1]);
+      f32x4 vs = *reinterpret_cast<const f32x4*>(f_lds[buf][1]);
       const int key0 = j * kBN;
       // Scores are scaled ahead where some are masked (a scale of 0 or NaN times -inf would not
       // be) and where they are so large that the scaled maximum's own rounding counts.
@@ -206,6 +206,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
             s[hh][r] = rounded_product(s[hh][r], f[2 * hh + r / 8]);
             if (hh * 32 + (r / 4) * 8 + r % 4 > lim) s[hh][r] = -INFINITY;
           }
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)  // a unit that the row sees nothing of counts 0, whatever its scale
+          if (16 * u > limit - key0) vs[u] = 0.f;
         f = f32x4{1.f, 1.f, 1.f, 1.f};
       }
       float x[kUnits];  // the largest score of a unit, of this lane's eight
@@ -237,9 +240,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
       }
       const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
       u32x4 pb[kUnits][NP];
-      float g[kUnits];  // a unit that this lane sees nothing of counts 0, whatever its scale
+      float g[kUnits];
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) g[u] = x[u] == -INFINITY ? 0.f : weight_scale(vs[u], e);
+      for (int u = 0; u < kUnits; ++u) g[u] = weight_scale(vs[u], e);
       // Two weights, in parts: elements 2 i and 2 i + 1 of unit u.
       auto pair = [&](int k) __attribute__((always_inline)) {
         const int u = k / 4, i = k % 4, r = u % 2 * 8 + 2 * i;
