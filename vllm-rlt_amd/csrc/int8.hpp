@@ -38,10 +38,10 @@ __device__ __forceinline__ float scale_exponent(float scale) {
   return static_cast<float>(static_cast<int>(__float_as_uint(scale) >> 23 & 255u) - 126);
 }
 
-// scale * 2^-e.  Past fp32's largest number that number: a weight it multiplies is 0 there.
+// scale * 2^-e, NaN if that is.  Past fp32's largest number that number: a weight it multiplies is 0 there.
 __device__ __forceinline__ float weight_scale(float scale, float e) {
   const float g = ldexpf(scale, -static_cast<int>(e));
-  return g > 3.4028234664e38f ? 3.4028234664e38f : g;
+  return __builtin_elementwise_minimum(g, 3.4028234664e38f);
 }
 
 constexpr float kNoExponent = -1024.f;  // e before any key
