@@ -1,0 +1,79 @@
+"""Attention over the block-scaled 8-bit cache at head sizes between and beyond its kernels' (GPU).
+
+Multiples of 16 up to 128 (decode: 256) run the kernels of the next larger size; the others a kernel for any
+shape, which goes through the tests of the kernels on the matrix cores.
+"""
+
+import pytest
+import test_int8_attention_gpu as attention_tests
+import torch
+from test_int8_attention_gpu import DTYPES, Case
+
+pytestmark = pytest.mark.gpu
+SIZES = [(4, 4, 16), (4, 2, 32), (4, 2, 48), (6, 2, 80), (3, 3, 96), (20, 1, 112), (4, 4, 144), (8, 2, 192), (2, 2, 240)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", SIZES)
+def test_multiples_of_16(dtype, hq, hkv, d):
+    c = Case([0, 1, 15, 16, 17, 33, 64, 65, 129, 513, 1500], hq, hkv, d, dtype=dtype, seed=d)
+    c.check(c.decode())
+    p = Case([3, 270, 69, 1020, 2500], hq, hkv, d, dtype=dtype, seed=d, chunks=[3, 200, 64, 20, 5])
+    p.check(p.prefill())
+    p.check(p.prefill(batch_invariant=True))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 16), (6, 2, 80), (3, 3, 112), (2, 2, 176)])
+def test_nothing_is_stored_past_a_head(dtype, hq, hkv, d):
+    for c in (Case([700, 30], hq, hkv, d, dtype=dtype, seed=1), Case([2000, 30], hq, hkv, d, dtype=dtype, seed=1, chunks=[30, 9])):
+        wide = torch.full((len(c.q), hq, d + 16), 7.0, dtype=dtype, device="cuda")
+        c.check((c.prefill if c.chunks else c.decode)(out=wide[..., :d]))
+        assert (wide[..., d:] == 7.0).all()
+
+
+@pytest.mark.parametrize("how", ["heads first", "dims apart", "off 16 bytes"])
+def test_strides_of_a_padded_head(how):
+    c = Case([70, 300, 2200], 6, 2, 80, seed=5, chunks=[30, 140, 11])
+    out = attention_tests.strided(torch.zeros_like(c.q), how)
+    c.prefill(q=attention_tests.strided(c.q, how), out=out)
+    c.check(out)
+
+
+def test_values_next_to_a_padded_head_do_not_reach_it():
+    """q, K and V of the neighbouring heads change; a head's bits do not, with infinities and NaN among q."""
+    c = Case([900, 40], 3, 3, 80, seed=2, chunks=[40, 20])
+    first = c.prefill()[:, 1].clone()
+    q = c.q.clone()
+    q[:, 0], q[:, 2] = float("inf"), float("nan")
+    for codes in c.cache[:2]:
+        codes[:, :, 0], codes[:, :, 2] = 127, -127
+    assert torch.equal(c.prefill(q=q)[:, 1], first)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(
+    "name,more",
+    [
+        ("test_decode_at_length_edges", ()),
+        ("test_a_block_that_is_not_finite_reaches_only_the_rows_that_see_it", (float("nan"),)),
+        ("test_a_block_that_is_not_finite_reaches_only_the_rows_that_see_it", (float("inf"),)),
+        ("test_queries_that_are_not_finite_or_huge", ()),
+        ("test_softmax_scales_of_zero_and_below", (0.0,)),
+        ("test_softmax_scales_of_zero_and_below", (-0.17,)),
+        ("test_scales_far_apart", ()),
+        ("test_blocks_of_zeros_keep_their_weight", ()),
+        ("test_scores_of_channels_of_very_different_sizes_are_sums_in_32_bits", ()),
+    ],
+)
+def test_the_kernel_for_any_shape(name, more, dtype):
+    getattr(attention_tests, name)(dtype, 2, 2, 72, *more)
+
+
+@pytest.mark.parametrize("name", ["test_table_entries_outside_the_pool_read_block_0", "test_offsets_past_32_bits", "test_a_row_depends_on_itself_only"])
+def test_the_kernel_for_any_shape_and_its_reads(name):
+    getattr(attention_tests, name)(2, 2, 72)
+
+
+def test_rows_of_the_kernel_for_any_shape():
+    attention_tests.test_rows_that_see_no_key_are_zero_and_rows_of_no_sequence_are_left(torch.bfloat16, 72)

@@ -124,6 +124,20 @@ def test_workspaces_are_bounded(d):
     assert lib.rlt_paged_prefill_int8_workspace_bytes(4096, 65, 1 << 14, 16, 16, d, 16) == 0
 
 
+def test_workspaces_of_other_head_sizes():
+    """Multiples of 16 as the next of 64, 128 and (decode) 256; none for what runs the kernel for any shape."""
+    lib, _ = library()
+    decode = lambda d, page=16: lib.rlt_paged_decode_int8_workspace_bytes(3, 1 << 10, 8, 2, d, page)  # noqa: E731
+    prefill = lambda d, page=16: lib.rlt_paged_prefill_int8_workspace_bytes(300, 3, 1 << 10, 8, 2, d, page)  # noqa: E731
+    for d, like in [(16, 64), (48, 64), (80, 128), (112, 128)]:
+        assert decode(d) == decode(like) > 0 and prefill(d) == prefill(like) > 0
+    assert decode(144) == decode(240) == decode(256) > 0
+    for d in (8, 72, 100, 272, 512):
+        assert decode(d) == prefill(d) == 0
+    assert prefill(144) == prefill(256) == 0
+    assert decode(128, 8) == prefill(128, 8) == prefill(128, 48) == 0 and decode(128, 48) > 0
+
+
 def cache(ndim):
     codes = torch.zeros((2, 1, 16, 2, 64)[5 - ndim :], dtype=torch.int8)
     return [codes, codes.clone(), *(torch.zeros(*codes.shape[: ndim - 3], 2) for _ in "kv")]

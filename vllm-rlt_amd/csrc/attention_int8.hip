@@ -127,7 +127,7 @@ using namespace rlt;
 
 extern "C" int64_t rlt_paged_decode_int8_workspace_bytes(int64_t n_rows, int64_t max_table_width, int64_t num_q_heads,
                                                          int64_t num_kv_heads, int64_t head_dim, int64_t page_size) {
-  if (n_rows <= 0 || max_table_width <= 0 || !decode8_shape(num_q_heads, num_kv_heads, head_dim, page_size) ||
+  if (n_rows <= 0 || max_table_width <= 0 || !decode_i8_shape(num_q_heads, num_kv_heads, head_dim, page_size) ||
       max_table_width > kMaxKeys / page_size)
     return 0;
   return decode_i8_workspace(n_rows, max_table_width * page_size, num_q_heads, head_dim);
@@ -150,7 +150,7 @@ extern "C" int rlt_paged_decode_int8(const void* q, const int64_t* q_strides, co
   const int64_t need = rlt_paged_decode_int8_workspace_bytes(n_rows, max_table_width, num_q_heads, num_kv_heads, head_dim, page_size);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(RLT_EWORKSPACE, "%s: workspace must be %lld bytes on 16", name, (long long)need);
-  if (decode8_layout(p.a)) return launch_decode_i8(p, dtype, workspace, as_stream(stream), name);
+  if (decode_i8_shape(p.a.hq, p.a.hkv, p.a.d, p.a.page) && decode8_strides(p.a)) return launch_decode_i8(p, dtype, workspace, as_stream(stream), name);
   return launch_attn_i8_generic(p, dtype, as_stream(stream), name);
 }
 
@@ -158,7 +158,7 @@ extern "C" int64_t rlt_paged_prefill_int8_workspace_bytes(int64_t total_q, int64
                                                           int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
                                                           int64_t page_size) {
   if (total_q <= 0 || num_seqs <= 0 || max_table_width <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
-      !prefill8_shape(head_dim, page_size) || max_table_width > kMaxKeys / page_size)
+      !prefill_i8_shape(head_dim, page_size) || max_table_width > kMaxKeys / page_size)
     return 0;
   return prefill_i8_workspace(total_q, num_seqs, max_table_width * page_size, num_q_heads, head_dim);
 }
@@ -186,6 +186,6 @@ extern "C" int rlt_paged_prefill_int8(const void* q, const int64_t* q_strides, c
                                                               head_dim, page_size);
   if (workspace && need > 0 && (workspace_bytes < need || !aligned16(workspace)))
     return fail(RLT_EWORKSPACE, "%s: workspace must be %lld bytes on 16", name, (long long)need);
-  if (prefill8_layout(p.a)) return launch_prefill_i8(p, dtype, workspace, as_stream(stream), name);
+  if (prefill_i8_shape(p.a.d, p.a.page) && prefill8_strides(p.a)) return launch_prefill_i8(p, dtype, workspace, as_stream(stream), name);
   return launch_attn_i8_generic(p, dtype, as_stream(stream), name);
 }

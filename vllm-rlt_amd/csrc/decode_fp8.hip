@@ -366,9 +366,10 @@ int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t hkv
   return ns > 1 ? rows * ns * hq * (d + 2) * 4 : 0;
 }
 
-bool decode8_layout(const Attn8Args& a) {
+bool decode8_layout(const Attn8Args& a) { return decode8_shape(a.hq, a.hkv, a.d, a.page) && decode8_strides(a); }
+bool decode8_strides(const Attn8Args& a) {
   auto near = [](int64_t x) { return x >= 0 && x < (int64_t(1) << 24) && x % 16 == 0; };
-  return decode8_shape(a.hq, a.hkv, a.d, a.page) && a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && near(a.kv_head) &&
+  return a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && near(a.kv_head) &&
          near(a.kv_token) && a.kv_block % 16 == 0;
 }
 

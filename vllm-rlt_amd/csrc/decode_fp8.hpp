@@ -40,6 +40,7 @@ struct Decode8Args {
 // Whether the split kernels cover the shape, and the layout of a call of it.
 bool decode8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page);
 bool decode8_layout(const Attn8Args& a);
+bool decode8_strides(const Attn8Args& a);  // of the layout all but the shape
 // Bytes of the partials of rows of up to max_len tokens.
 int64_t decode8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t hkv, int64_t d);
 int launch_decode8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream, const char* name);

@@ -46,7 +46,9 @@ template <> struct Parts<float> { static constexpr int Q = 3, P = 2; using S = b
 template <typename T, int D>
 constexpr int kWavesPerEu = D == 256 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4 ? 3 : 4;  // as LDS holds
 
-template <typename T, int D>
+// PAD: heads of fewer than D dims, a multiple of 16.  q is 0 in the others, where K and V are codes of the
+// head's last 16 dims (any codes: they are finite), and nothing of them is stored.
+template <typename T, int D, bool PAD>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<T, D>))) void decode_i8_kernel(DecodeI8Args p) {
   using S = typename Parts<T>::S;
   constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
     const T* src = static_cast<const T*>(a.q) + r * a.q_row + (h * G + c0 + min(static_cast<int>(thread) / 16, live - 1)) * a.q_head +
                    static_cast<int>(thread) % 16 * QE * a.q_dim;
 #pragma unroll
-    for (int e = 0; e < QE; ++e) y[e] = load_elem(src + e * a.q_dim);
+    for (int e = 0; e < QE; ++e) y[e] = !PAD || static_cast<int>(thread) % 16 * QE + e < a.d ? load_elem(src + e * a.q_dim) : 0.f;
   };
   // A wave's tile i of split sp is its (4 i + wave)-th 32 tokens.  Lane l holds where the 16 tokens
   // of half l % 2 of tile first + l / 2 begin (past the row's end anything inside the tables).
@@ -135,6 +137,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
   for (;;) {
     const int t0 = sp * split_len + wave * kTile, end = min(len, (sp + 1) * split_len);  // this wave's first token
     const int tiles = end > t0 ? (end - t0 + kWaves * kTile - 1) / (kWaves * kTile) : 0;
+    auto chunk_of = [&](uint32_t chunk) __attribute__((always_inline)) { return PAD ? min(chunk, static_cast<uint32_t>(a.d - 16)) : chunk; };
     // At head_dim 64 a token's row is half a line of the L2, where it stays for the next head (256 rows
     // of 1024-8192 tokens, 16 + 8 heads, 304 us as other loads, so 268).
     auto load16 = [](uint32_t lds_byte, uint32_t offset, const uint8_t* from) __attribute__((always_inline)) {
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
           const uint8_t* from = base + unit_at(half);
 #pragma unroll
           for (int i = half * NI / 2; i < (half + 1) * NI / 2; ++i, from += TPI * token_bytes)
-            load16(to + i * 1024, row + (chunk ^ (16 * swizzle(i * TPI))), from);
+            load16(to + i * 1024, row + chunk_of(chunk ^ (16 * swizzle(i * TPI))), from);
         }
         return;
       }
@@ -164,7 +167,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
       for (int i = 0; i < NI; ++i) {
         const int half = min(i * TPI, last) / 16;
         const uint32_t tok = min(i * TPI + static_cast<int>(load_row), last) - 16 * half;
-        load16(to + i * 1024, __umul24(tok, token_bytes) + (chunk ^ (16 * swizzle(i * TPI))), base + unit_at(half));
+        load16(to + i * 1024, __umul24(tok, token_bytes) + chunk_of(chunk ^ (16 * swizzle(i * TPI))), base + unit_at(half));
       }
     };
     auto load_k = [&](int tile) __attribute__((always_inline)) {
@@ -373,6 +376,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         y = fmaf(reinterpret_cast<const float*>(lds[w])[hd * JROW + d], fast_exp2(x.e + (x.m - base) - exponent), y);
       }
       const int q = c0 + hd;  // of the KV head's
+      if (PAD && ns == 1 && d >= a.d) continue;
       if (ns == 1) {
         store_elem(static_cast<T*>(a.out) + r * a.o_row + (h * G + q) * a.o_head + d * a.o_dim,
                    len > 0 ? ldexpf(y * (1.f / sum), static_cast<int>(exponent)) : 0.f);
@@ -431,7 +435,7 @@ __global__ __launch_bounds__(64 * kWaves) void decode_i8_merge_kernel(DecodeI8Ar
   for (int e = 0; e < E; ++e) sums[wave][lane + 64 * e] = acc[e];
   __syncthreads();
   T* orow = static_cast<T*>(a.out) + r * a.o_row + hq * a.o_head;
-  for (int d = threadIdx.x; d < D; d += 64 * kWaves) {
+  for (int d = threadIdx.x; d < a.d; d += 64 * kWaves) {
     float y = 0.f;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) y += sums[v][d];
@@ -439,17 +443,21 @@ __global__ __launch_bounds__(64 * kWaves) void decode_i8_merge_kernel(DecodeI8Ar
   }
 }
 
+// The kernel's head size.
+int64_t padded_dims(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
 template <typename T, int D>
 void launch_size(const DecodeI8Args& p, unsigned grid, hipStream_t stream) {
   const Attn8Args& a = p.s.a;
-  hipLaunchKernelGGL((decode_i8_kernel<T, D>), dim3(grid), dim3(64 * kWaves), 0, stream, p);
+  if (a.d == D) hipLaunchKernelGGL((decode_i8_kernel<T, D, false>), dim3(grid), dim3(64 * kWaves), 0, stream, p);
+  else hipLaunchKernelGGL((decode_i8_kernel<T, D, true>), dim3(grid), dim3(64 * kWaves), 0, stream, p);
   if (p.splits < 2) return;
   hipLaunchKernelGGL((decode_i8_merge_kernel<T, D>), dim3(static_cast<unsigned>(a.rows * a.hq)), dim3(64 * kWaves), 0, stream, p);
 }
 
 template <typename T>
 void launch_type(const DecodeI8Args& p, unsigned grid, hipStream_t stream) {
-  switch (p.s.a.d) {
+  switch (padded_dims(p.s.a.d)) {
     case 64: launch_size<T, 64>(p, grid, stream); break;
     case 128: launch_size<T, 128>(p, grid, stream); break;
     default: launch_size<T, 256>(p, grid, stream); break;
@@ -458,9 +466,13 @@ void launch_type(const DecodeI8Args& p, unsigned grid, hipStream_t stream) {
 
 }  // namespace
 
+bool decode_i8_shape(int64_t hq, int64_t hkv, int64_t d, int64_t page) {
+  return d > 0 && d <= 256 && d % 16 == 0 && page > 0 && page % 16 == 0 && hkv > 0 && hq > 0;
+}
+
 int64_t decode_i8_workspace(int64_t rows, int64_t max_len, int64_t hq, int64_t d) {
   const int64_t ns = decode8_most_splits(max_len, kMfmaSplit);
-  return ns > 1 ? rows * ns * hq * (d * 4 + static_cast<int64_t>(sizeof(PartState))) : 0;
+  return ns > 1 ? rows * ns * hq * (padded_dims(d) * 4 + static_cast<int64_t>(sizeof(PartState))) : 0;
 }
 
 int launch_decode_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t stream, const char* name) {
@@ -472,7 +484,7 @@ int launch_decode_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t strea
   p.split_slots = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.splits, kMaxGrid / items)));
   p.xcd = a.rows * p.split_slots % kXcds == 0;
   p.ws_acc = static_cast<float*>(ws);
-  p.ws_state = reinterpret_cast<PartState*>(p.ws_acc + a.rows * p.splits * a.hq * a.d);
+  p.ws_state = reinterpret_cast<PartState*>(p.ws_acc + a.rows * p.splits * a.hq * padded_dims(a.d));
   if (items * p.split_slots > kMaxBlocks || a.rows * a.hq > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const unsigned grid = static_cast<unsigned>(items * p.split_slots);
   switch (dtype) {

@@ -493,10 +493,11 @@ __global__ __launch_bounds__(256) void prefill8_merge_kernel(Prefill8Args p, int
 
 bool prefill8_shape(int64_t d, int64_t page) { return (d == 64 || d == 128) && page >= 16 && (page & (page - 1)) == 0; }
 
-bool prefill8_layout(const Attn8Args& a) {
+bool prefill8_layout(const Attn8Args& a) { return prefill8_shape(a.d, a.page) && prefill8_strides(a); }
+bool prefill8_strides(const Attn8Args& a) {
   auto near = [](int64_t x) { return x >= 0 && x < (int64_t(1) << 24); };
   auto small = [](int64_t x) { return x >= 0 && x < (int64_t(1) << 32); };
-  return prefill8_shape(a.d, a.page) && a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && a.kv_head % 16 == 0 &&
+  return a.kv_dim == 1 && aligned16(a.k) && aligned16(a.v) && a.kv_head % 16 == 0 &&
          a.kv_token % 16 == 0 && a.kv_block % 16 == 0 && small(a.kv_block) && small(a.s_block) &&
          near(a.kv_token) && near(a.s_token) && near(a.page) && small(a.kv_token * a.page) && small(a.s_token * a.page);
 }

@@ -1,6 +1,6 @@
 // Packed chunked prefill over the block-scaled 8-bit KV cache, bottom-right causal, on the
-// matrix cores (head_dim 64 / 128, pages of a power of two of at least 16 tokens; int8.hpp has
-// the softmax, prefill_plan.hpp the launch's plan).
+// matrix cores (head sizes of multiples of 16 up to 128, pages of a power of two of at least 16
+// tokens; int8.hpp has the softmax, prefill_plan.hpp the launch's plan).
 //
 // A workgroup of 4 waves takes 128 (query row, query head) pairs of one (sequence, KV head), a
 // row's heads together, over a segment of its keys, a wave 32 of them, 64 keys a tile, four units
@@ -46,7 +46,9 @@ template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf
 template <> struct Parts<f16> { static constexpr int Q = 1, P = 1; using S = f16; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 2; using S = bf16; };
 
-template <typename T, int D>
+// PAD: heads of fewer than D dims, a multiple of 16.  q is 0 in the others, where K and V are codes of the
+// head's last 16 dims (any codes: they are finite), and nothing of them is stored.
+template <typename T, int D, bool PAD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void prefill_i8_kernel(PrefillI8Args args) {
   using S = typename Parts<T>::S;
   using SOps = MfmaOps<S>;
@@ -109,9 +111,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
   const uint32_t block_bytes = static_cast<uint32_t>(a.kv_block), token_bytes = static_cast<uint32_t>(a.kv_token);
   const uint32_t s_block = static_cast<uint32_t>(a.s_block);
   const uint32_t page_mask = a.page - 1, last_key = max(wg_keys, 1) - 1, num_blocks = static_cast<uint32_t>(a.num_blocks);
+  const int last_chunk = PAD ? a.d / 16 - 1 : CH - 1;
   uint32_t offset[PASSES];  // of this thread's codes in a block, but for the tile's first token in it
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) offset[i] = ((i * TPP + st) & page_mask) * token_bytes + sc * 16;
+  for (int i = 0; i < PASSES; ++i) offset[i] = ((i * TPP + st) & page_mask) * token_bytes + min(sc, last_chunk) * 16;
   uint32_t id, v_id;  // the unit's block, of the tile whose K is loaded next and the one whose V is
   u32x4 kreg[PASSES], vreg[PASSES];
   float sreg;
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 #pragma unroll
       for (int c = 0; c < KS; ++c)
 #pragma unroll
-        for (int i = 0; i < 8 / N; ++i) raw[c][i] = *reinterpret_cast<const u32x4*>(qrow + 16 * c + 8 * half + i * N);
+        for (int i = 0; i < 8 / N; ++i) raw[c][i] = *reinterpret_cast<const u32x4*>(qrow + 16 * min(c, last_chunk) + 8 * half + i * N);
     } else {
 #pragma unroll
       for (int c = 0; c < KS; ++c)
@@ -333,7 +336,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         for (int i = 0; i < 8 / N; ++i) {
           T x[N];
 #pragma unroll
-          for (int e = 0; e < N; ++e) x[e] = qrow[(16 * c + 8 * half + i * N + e) * a.q_dim];
+          for (int e = 0; e < N; ++e) x[e] = qrow[(16 * min(c, last_chunk) + 8 * half + i * N + e) * a.q_dim];
           raw[c][i] = __builtin_bit_cast(u32x4, x);
         }
     }
@@ -356,11 +359,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         for (int w = 0; w < 4; ++w) {
           if constexpr (NQ > 1) {  // the top 16 bits: the rest is exact, and the last part holds all of it
             const uint32_t lo = __float_as_uint(x[2 * w]), hi = __float_as_uint(x[2 * w + 1]);
-            qw[n][c][w] = lo >> 16 | (hi & 0xffff0000u);
+            qw[n][c][w] = c > last_chunk ? 0u : lo >> 16 | (hi & 0xffff0000u);
             x[2 * w] -= __uint_as_float(lo & 0xffff0000u);
             x[2 * w + 1] -= __uint_as_float(hi & 0xffff0000u);
           } else {
-            qw[n][c][w] = SOps::pack2(x[2 * w], x[2 * w + 1]);
+            qw[n][c][w] = c > last_chunk ? 0u : SOps::pack2(x[2 * w], x[2 * w + 1]);
           }
         }
     }
@@ -416,6 +419,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * c + 8 * g + 4 * half;
+      if (2 * c + g / 2 > last_chunk) continue;
       float x[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = limit < 0 ? 0.f : ldexpf(acc[c][4 * g + i] * inv, exponent);
@@ -487,31 +491,39 @@ __global__ __launch_bounds__(256) void prefill_i8_merge_kernel(PrefillI8Args arg
     float y[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] = blind ? 0.f : ldexpf(acc[k] * inv, static_cast<int>(exponent));
-    store4(static_cast<T*>(a.out) + row * a.o_row + h * a.o_head, d, y, a.o_dim, p.out_vec);
+    if (d < a.d) store4(static_cast<T*>(a.out) + row * a.o_row + h * a.o_head, d, y, a.o_dim, p.out_vec);
   }
 }
 
 template <typename T, int D>
 void launch_size(const PrefillI8Args& args, unsigned grid, hipStream_t stream) {
   const Attn8Args& a = args.p.a;
-  hipLaunchKernelGGL((prefill_i8_kernel<T, D>), dim3(grid), dim3(256), 0, stream, args);
+  if (a.d == D) hipLaunchKernelGGL((prefill_i8_kernel<T, D, false>), dim3(grid), dim3(256), 0, stream, args);
+  else hipLaunchKernelGGL((prefill_i8_kernel<T, D, true>), dim3(grid), dim3(256), 0, stream, args);
   if (!args.p.slots) return;
   const int parts = static_cast<int>((static_cast<int64_t>(a.hq) * D + 1023) / 1024);
   const dim3 merge(static_cast<unsigned>(std::min<int64_t>(a.rows * parts, kMergeRound)));
   hipLaunchKernelGGL((prefill_i8_merge_kernel<T, D>), merge, dim3(256), 0, stream, args, parts);
 }
 
+// The kernel's head size.
+int64_t padded_dims(int64_t d) { return d <= 64 ? 64 : 128; }
+
 template <typename T>
 void launch_type(const PrefillI8Args& args, unsigned grid, hipStream_t stream) {
-  if (args.p.a.d == 64) launch_size<T, 64>(args, grid, stream);
+  if (padded_dims(args.p.a.d) == 64) launch_size<T, 64>(args, grid, stream);
   else launch_size<T, 128>(args, grid, stream);
 }
 
 }  // namespace
 
+bool prefill_i8_shape(int64_t d, int64_t page) {
+  return d > 0 && d <= 128 && d % 16 == 0 && page >= 16 && (page & (page - 1)) == 0;
+}
+
 int64_t prefill_i8_workspace(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq, int64_t d) {
   const int64_t slots = partial_slots(rows, num_seqs, max_len, hq);
-  return slots ? slots * hq * (d * 4 + static_cast<int64_t>(sizeof(PartState))) + kPlanSeqs * static_cast<int64_t>(sizeof(SeqPlan)) : 0;
+  return slots ? slots * hq * (padded_dims(d) * 4 + static_cast<int64_t>(sizeof(PartState))) + kPlanSeqs * static_cast<int64_t>(sizeof(SeqPlan)) : 0;
 }
 
 int launch_prefill_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t stream, const char* name) {
@@ -524,10 +536,10 @@ int launch_prefill_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t stre
   if (slots > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);  // 64 sequences' stay inside 31 bits
   p.slots = static_cast<int>(slots);
   p.group = a.hq / a.hkv;
-  p.round = dtype == RLT_FLOAT32 && a.d == 128 ? kRound / 2 : kRound;
+  p.round = dtype == RLT_FLOAT32 && a.d > 64 ? kRound / 2 : kRound;
   if (slots) {
     p.part_acc = static_cast<float*>(ws);
-    args.part_state = reinterpret_cast<PartState*>(p.part_acc + slots * a.hq * a.d);
+    args.part_state = reinterpret_cast<PartState*>(p.part_acc + slots * a.hq * padded_dims(a.d));
     p.plan = reinterpret_cast<SeqPlan*>(args.part_state + slots * a.hq);
   }
   fill_prefill8(&p, dtype);
