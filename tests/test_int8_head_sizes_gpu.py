@@ -1,12 +1,15 @@
-"""Attention over the block-scaled 8-bit cache at head sizes between and beyond its kernels' (GPU).
+"""The block-scaled 8-bit cache at head sizes between and beyond its kernels' (GPU).
 
-Multiples of 16 up to 128 (decode: 256) run the kernels of the next larger size; the others a kernel for any
-shape, which goes through the tests of the kernels on the matrix cores.
+Attention: multiples of 16 up to 128 (decode: 256) run the kernels of the next larger size; the others a kernel
+for any shape, which goes through the tests of the kernels on the matrix cores.  Appends and reads: heads of whole
+16-byte packets have a power of two of lanes, not all of them of use.
 """
 
 import pytest
+import test_int8_append_gpu as append_tests
 import test_int8_attention_gpu as attention_tests
 import torch
+from int8_cases import append, random_cache
 from test_int8_attention_gpu import DTYPES, Case
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +80,27 @@ def test_the_kernel_for_any_shape_and_its_reads(name):
 
 def test_rows_of_the_kernel_for_any_shape():
     attention_tests.test_rows_that_see_no_key_are_zero_and_rows_of_no_sequence_are_left(torch.bfloat16, 72)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv,d,page", [(3, 8, 16), (2, 24, 16), (5, 40, 32), (3, 80, 16), (2, 96, 16), (1, 176, 16), (2, 320, 16), (2, 504, 7), (2, 36, 16), (3, 65, 16)])
+def test_appends_and_reads_of_any_head_size(dtype, hkv, d, page):
+    append_tests.test_runs_of_every_length_and_place(dtype, hkv, d, page)
+    append_tests.test_reading_back(dtype, hkv, d, page)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_append_stores_nothing_past_a_head(dtype):
+    from vllm_rlt_amd import ops
+
+    cache = random_cache(6, 16, 3, 96, seed=5, layers=2)
+    wide = [t.cuda() for t in cache]
+    got = [t[..., :80] for t in wide[:2]] + wide[2:]
+    k, v = append_tests.tokens(40, 3, 80, dtype, 6, spread=3.0)
+    blocks, offsets = append_tests.slots([(9, 30), (0, 1), (5, 9)], 16, 6)
+    ops.kv_append_int8(*got, 1, blocks.cuda(), offsets.cuda(), k.cuda(), v.cuda())
+    want = [t[..., :80].clone() for t in cache[:2]] + [t.clone() for t in cache[2:]]
+    append(want, 1, blocks, offsets, k, v)
+    append_tests.same(got, want)
+    for t, old in zip(wide[:2], cache[:2]):
+        assert torch.equal(t[..., 80:].cpu(), old[..., 80:])

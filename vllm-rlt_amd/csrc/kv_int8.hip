@@ -174,9 +174,9 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const Codes<N>& c) {
 }
 __device__ __forceinline__ int code_at(uint32_t word, int byte) { return static_cast<int8_t>(word >> (8 * byte)); }
 
-// Codes that a block holds, rounded anew: this lane's packets of tokens first, first + step, ...
+// Codes that a block holds, rounded anew: this lane's packets of tokens first, first + step, ...; none where own is false.
 template <int N, int BATCH>
-__device__ __forceinline__ void requantise(uint8_t* codes, int64_t c_token, int page, int first, int step, float ratio) {
+__device__ __forceinline__ void requantise(uint8_t* codes, int64_t c_token, int page, int first, int step, float ratio, bool own) {
   for (int t0 = first; t0 < page; t0 += BATCH * step) {
     Codes<N> c[BATCH];
 #pragma unroll
@@ -190,7 +190,7 @@ __device__ __forceinline__ void requantise(uint8_t* codes, int64_t c_token, int 
         for (int e = 0; e < 4; ++e) y[e] = static_cast<float>(code_at(c[u].w[w], e));
         c[u].w[w] = codes4(y, ratio);
       }
-      if (t0 + u * step < page) store_codes<N>(codes + (t0 + u * step) * c_token, c[u]);
+      if (own && t0 + u * step < page) store_codes<N>(codes + (t0 + u * step) * c_token, c[u]);
     }
   }
 }
@@ -206,7 +206,8 @@ __device__ __forceinline__ void store_packet(uint8_t* to, const u32x4& x, float 
   store_codes<N>(to, c);
 }
 
-// Aligned heads of LPH 16-byte packets.  A wave has K or V of a head of up to kHeld rows, `tile`: it looks
+// Aligned heads of LPH 16-byte packets, or (PAD) of fewer: lanes past the last have it again and store
+// nothing.  A wave has K or V of a head of up to kHeld rows, `tile`: it looks
 // for the blocks that begin there.  Those that get one row (a decode batch's) it takes all at once,
 // LPH lanes a row; the others one after another, 64 / LPH tokens at once, so that a block's
 // largest |x| is over the wave, and its scale is the wave's.  kHeld tokens of a block stay in
@@ -214,7 +215,7 @@ __device__ __forceinline__ void store_packet(uint8_t* to, const u32x4& x, float 
 // of 8 sequences, 16 heads x 128, bf16, move 50 MB in 12.4 us, 4.1 TB/s.  (With the heads, not the
 // tokens, of a wave side by side 15.6: 16 registers a lane for every token, and few waves.)
 constexpr int kHeld = 16;
-template <typename T, int LPH>
+template <typename T, int LPH, bool PAD>
 __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, int tile) {
   constexpr int N = Packet<T>::N, TPI = 64 / LPH, H = TPI < kHeld ? kHeld / TPI : 1;  // packets a lane holds
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + uniform(threadIdx.x >> 6);
@@ -223,12 +224,14 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
   const int of_tile = uniform(static_cast<int>(item % (2 * a.hkv)));
   const int which = of_tile >= a.hkv, head = of_tile - which * a.hkv;
   const int lane = threadIdx.x & 63, i = lane % LPH, sub = lane / LPH, page = static_cast<int>(a.page);
+  const int packets = PAD ? a.d / N : LPH, at_dim = min(i, packets - 1) * N;
+  const bool own = i < packets;
   // Lane l has the block and the offset of row row0 - 1 + l; -1 outside the pool and the page.
   const int64_t at = row0 - 1 + lane;
   const bool there = at >= 0 && at < a.rows;
   const int64_t block_at = there ? a.blocks[at] : -1, offset_at = there ? a.offsets[at] : -1;
   const int64_t x_row = a.x_row[which];
-  const T* const x0 = static_cast<const T*>(a.x[which]) + row0 * x_row + head * a.x_head[which] + i * N;
+  const T* const x0 = static_cast<const T*>(a.x[which]) + row0 * x_row + head * a.x_head[which] + at_dim;
   u32x4 held[H];
   const bool early = tile <= TPI;  // few rows, mostly blocks of one: on their way with the block's number
   const int last = static_cast<int>(min(static_cast<int64_t>(tile), a.rows - row0)) - 1;  // (of the tile; rows past it: it again, of no use)
@@ -239,7 +242,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
   const uint64_t same = __builtin_amdgcn_ballot_w64(lane > 0 && block == previous);  // as the row before
   const uint64_t begin = __builtin_amdgcn_ballot_w64(block >= 0) & ~same & (((uint64_t(1) << tile) - 1) << 1);
   const uint64_t single = begin & ~(same >> 1);
-  uint8_t* const codes0 = a.codes[which] + a.layer * a.c_layer + head * a.c_head + i * N;
+  uint8_t* const codes0 = a.codes[which] + a.layer * a.c_layer + head * a.c_head + at_dim;
   float* const scale0 = a.scales[which] + a.layer * a.s_layer + head * a.s_head;
   if (single) {
     float old[H], inv[H], ratio = 1.f;  // ratio: lane t's is row t's
@@ -266,12 +269,12 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
     for (; grown; grown &= grown - 1) {
       const int t = __builtin_ctzll(grown);
       const float r = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ratio), t));
-      requantise<N, (H < 8 ? H : 8)>(codes0 + __builtin_amdgcn_readlane(block, 1 + t) * a.c_block, a.c_token, page, sub, TPI, r);
+      requantise<N, (H < 8 ? H : 8)>(codes0 + __builtin_amdgcn_readlane(block, 1 + t) * a.c_block, a.c_token, page, sub, TPI, r, own);
       if (!(grown & (grown - 1))) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // before the new rows' codes
     }
 #pragma unroll
     for (int u = 0; u < H; ++u)
-      if (slot[u] >= 0) store_packet<T>(codes0 + blk[u] * a.c_block + slot[u] * a.c_token, held[u], inv[u]);
+      if (own && slot[u] >= 0) store_packet<T>(codes0 + blk[u] * a.c_block + slot[u] * a.c_token, held[u], inv[u]);
   }
   for (uint64_t first = begin & ~single; first; first &= first - 1) {
     const int l0 = __builtin_ctzll(first);
@@ -312,7 +315,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
     const float before = fresh ? 0.f : old, s = grown_scale(before, group_umax<64>(top_bits<T>(top)));
     if (lane == 0) *scale = s;
     if (__builtin_amdgcn_ballot_w64(!fresh && s != before && s == s)) {
-      requantise<N, (H < 8 ? H : 8)>(codes, a.c_token, page, sub, TPI, before / s);
+      requantise<N, (H < 8 ? H : 8)>(codes, a.c_token, page, sub, TPI, before / s, own);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // before the new rows' codes
     }
     const float inv = s == s ? 1.f / s : s;
@@ -320,7 +323,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
       if (n > H * TPI) load(from);
 #pragma unroll
       for (int u = 0; u < H; ++u)
-        if (o[u] >= 0) store_packet<T>(codes + o[u] * a.c_token, held[u], inv);
+        if (own && o[u] >= 0) store_packet<T>(codes + o[u] * a.c_token, held[u], inv);
     }
   }
 }
@@ -350,7 +353,7 @@ __global__ __launch_bounds__(64) void gather_i8_generic_kernel(GatherI8Args a) {
     store_elem(out + d, in ? code_value(static_cast<int8_t>(codes[d * a.c_dim]), s) : 0.f);
 }
 
-// Aligned heads of LPH packets of N codes, 16 bytes of the result: a wave takes K and V of a row.
+// Aligned heads of up to LPH packets of N codes, 16 bytes of the result: a wave takes K and V of a row.
 // Bytes bound it: 8192 rows of 16 heads x 128 to bf16, 101 MB, take 17 to 19 us.
 template <typename T, int LPH>
 __global__ __launch_bounds__(64 * kWaves) void gather_i8_kernel(GatherI8Args a) {
@@ -358,6 +361,7 @@ __global__ __launch_bounds__(64 * kWaves) void gather_i8_kernel(GatherI8Args a) 
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + uniform(threadIdx.x >> 6);
   if (row >= a.rows) return;
   const int lane = threadIdx.x & 63, i = lane % LPH;
+  if (i >= a.d / N) return;
   const int64_t block = a.blocks[row], offset = a.offsets[row];
   const bool in = block >= 0 && block < a.num_blocks && offset >= 0 && offset < a.page;
   const int64_t at = in ? block * a.c_block + a.layer * a.c_layer + offset * a.c_token + i * N : 0;
@@ -421,12 +425,15 @@ bool code_packets(const A& a, int n) {
   return a.c_dim == 1 && a.c_block % n == 0 && a.c_layer % n == 0 && a.c_token % n == 0 && a.c_head % n == 0;
 }
 
-// Lanes of a head, one a 16-byte packet of T; 0 where the packet kernels do not cover the head size.
+// Lanes of a head, one a 16-byte packet of T, a power of two of them; 0 where the packet kernels do not
+// cover the head size.
 template <typename T>
 int lanes_of(int d) {
   constexpr int N = Packet<T>::N;
-  const int lanes = d / N;
-  return d % N == 0 && lanes >= 4 && lanes <= 64 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+  if (d % N || d > 64 * N) return 0;
+  int lanes = 4;
+  while (lanes * N < d) lanes *= 2;
+  return lanes;
 }
 
 #define BY_LANES(LAUNCH)   \
@@ -453,7 +460,10 @@ void launch_append(const AppendI8Args& a, hipStream_t stream) {
     while (tile > std::max(1, 64 / lanes) && (a.rows + tile - 1) / tile * 2 * a.hkv < 4096) tile /= 2;
     const int64_t waves = (a.rows + tile - 1) / tile * 2 * a.hkv;
     const dim3 grid(static_cast<unsigned>((waves + kWaves - 1) / kWaves)), block(64 * kWaves);
-#define LAUNCH(L) hipLaunchKernelGGL((append_i8_kernel<T, L>), grid, block, 0, stream, a, tile); return
+#define LAUNCH(L)                                                                                                    \
+  if (a.d == L * Packet<T>::N) hipLaunchKernelGGL((append_i8_kernel<T, L, false>), grid, block, 0, stream, a, tile); \
+  else hipLaunchKernelGGL((append_i8_kernel<T, L, true>), grid, block, 0, stream, a, tile);                          \
+  return
     BY_LANES(LAUNCH)
 #undef LAUNCH
   }
