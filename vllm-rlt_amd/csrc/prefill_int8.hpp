@@ -1,5 +1,5 @@
 // Prefill over the block-scaled cache, shared between its entry point (attention_int8.hip)
-// and its kernels (prefill_int8.hip), which cover head sizes up to 128 that are multiples of 16, pages
+// and its kernels (prefill_int8.hip), which cover head sizes up to 256 that are multiples of 16, pages
 // of a power of two from 16 tokens on and prefill8_strides' layouts.
 #pragma once
 
