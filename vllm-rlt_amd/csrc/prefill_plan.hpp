@@ -119,7 +119,10 @@ __device__ __forceinline__ SeqPlan plan_of(const Prefill8Args& p, int lane, bool
       int target = max(kMinSegTiles, static_cast<int>(fminf(ceilf(work / (few || *tails ? p.round : p.round * 3 / 2)), 1e9f)));
       for (int i = 0; few && i < 4; ++i) {  // as rounding up makes more items, towards the round
         const int items = __builtin_amdgcn_readlane(scan_sum(s.tiles * max(1, (keys + target - 1) / target)), 63) * heads;
-        if (items <= p.round) break;
+        // Segments of two tiles pay for one workgroup a CU (over the block-scaled cache, in 2 / 3, us: six of
+        // 20-67 rows over up to 1526, 16 + 8 heads, 27.3 / 22.8, one of 306 over 757, 16 heads x 64, 21.5 /
+        // 19.2, three of 6-20 over up to 573, fewer items, 14.3 / 15.4).
+        if (items <= (TAILS && target < 3 ? min(p.round, kRound / 2) : p.round)) break;
         target = max(target + 1, static_cast<int>(static_cast<float>(target) * items / p.round));
       }
       s.segs = max(1, (keys + target - 1) / target);
