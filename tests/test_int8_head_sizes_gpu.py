@@ -59,6 +59,13 @@ def test_heads_of_256_where_it_can_go_wrong(name, more, dtype):
     getattr(attention_tests, name)(dtype, 2, 2, 256, *more)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(2, 1, 64), (1, 1, 128), (1, 1, 48)])
+def test_prefill_of_the_longest_rows(hq, hkv, d):
+    c = Case([200005, 70000, 33], hq, hkv, d, seed=13, chunks=[5, 40, 33])
+    c.check(c.prefill())
+    c.check(c.prefill(batch_invariant=True))
+
+
 @pytest.mark.parametrize("how", ["heads first", "dims apart", "off 16 bytes"])
 def test_strides_of_a_padded_head(how):
     c = Case([70, 300, 2200], 6, 2, 80, seed=5, chunks=[30, 140, 11])
