@@ -521,7 +521,7 @@ int launch_prefill8(const Attn8Args& a, int dtype, void* ws, hipStream_t stream,
     p.plan = reinterpret_cast<SeqPlan*>(p.part_ml + slots * a.hq);
   }
   fill_prefill8(&p, dtype);
-  const int64_t tiles = prefill8_tiles(p);
+  const int64_t tiles = prefill8_tiles(p, kTargetItems);
   const int parts = static_cast<int>((static_cast<int64_t>(a.hq) * a.d + 1023) / 1024);
   if (tiles * a.hq > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const dim3 grid(static_cast<unsigned>(tiles * a.hq)), block(256);

@@ -554,7 +554,7 @@ int launch_prefill_i8(const AttnI8Args& s, int dtype, void* ws, hipStream_t stre
     p.plan = reinterpret_cast<SeqPlan*>(args.part_state + slots * a.hq);
   }
   fill_prefill8(&p, dtype);
-  const int64_t tiles = prefill8_tiles(p);
+  const int64_t tiles = prefill8_tiles(p, p.round);
   // (So that rows of a tile, a row and head each, stay inside 31 bits as well.)
   if (tiles * a.hkv > kMaxBlocks) return fail(RLT_EUNSUPPORTED, "%s: too many rows", name);
   const unsigned grid = static_cast<unsigned>(tiles * a.hkv);

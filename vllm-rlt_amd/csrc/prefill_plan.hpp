@@ -262,10 +262,11 @@ inline void fill_prefill8(Prefill8Args* p, int dtype) {
   p->out_vec = a.o_dim == 1 && aligned16(a.out) && a.o_row * es % 16 == 0 && a.o_head * es % 16 == 0;
 }
 
-// Query tiles, and the segments past the first (as many items as partial_slots() has such rows).
-inline int64_t prefill8_tiles(const Prefill8Args& p) {
+// Query tiles, and the segments past the first: of all heads fewer than `more`, as a segment is at least
+// all work / `more` (which is kTargetItems, or with tails the round).
+inline int64_t prefill8_tiles(const Prefill8Args& p, int64_t more) {
   const int64_t heads = p.a.hq / p.group;
-  return p.a.rows * p.group / kBM + std::min<int64_t>(p.a.num_seqs, p.a.rows) + (p.slots ? (kTargetItems + heads - 1) / heads + 2 : 0);
+  return p.a.rows * p.group / kBM + std::min<int64_t>(p.a.num_seqs, p.a.rows) + (p.slots ? (more + heads - 1) / heads + 2 : 0);
 }
 
 }  // namespace rlt
