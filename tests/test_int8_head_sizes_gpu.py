@@ -59,6 +59,28 @@ def test_heads_of_256_where_it_can_go_wrong(name, more, dtype):
     getattr(attention_tests, name)(dtype, 2, 2, 256, *more)
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 256), (torch.bfloat16, 80), (torch.float16, 176)])
+def test_captured_calls(dtype, d):
+    p = Case([700, 64, 2100], 4, 2, d, dtype=dtype, seed=6, chunks=[70, 64, 33])
+    c = Case([700, 64, 2100], 4, 2, d, dtype=dtype, seed=7)
+    first = p.prefill(), c.decode()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = p.prefill(), c.decode()
+    for shift in (0, 1, 0):
+        for x in (p, c):
+            x.q.add_(shift)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, (p.prefill(), c.decode())):
+            assert torch.equal(a, b)
+        for x in (p, c):
+            x.q.sub_(shift)
+    if dtype == torch.float32:
+        p.check(first[0])
+        c.check(first[1])
+
+
 @pytest.mark.parametrize("hq,hkv,d", [(2, 1, 64), (1, 1, 128), (1, 1, 48)])
 def test_prefill_of_the_longest_rows(hq, hkv, d):
     c = Case([200005, 70000, 33], hq, hkv, d, seed=13, chunks=[5, 40, 33])
