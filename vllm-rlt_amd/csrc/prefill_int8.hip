@@ -174,6 +174,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWorkgroups
 #pragma unroll
   for (int c = 0; c < DT; ++c) acc[c] = f32x16{};
   float m = -INFINITY, lsum = 0.f, e = kNoExponent;
+  bool large = false;  // whether some row's maximum is so large that a scaled score's own rounding counts
 
   // V^T operands: in each 16-lane group lane L addresses key row L / 4 of its four and 4
   // dims; k-step ks, element e of half hf holds key 16 ks + 8 (e / 4) + 4 hf + e % 4.
@@ -205,10 +206,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWorkgroups
       f32x4 f = *reinterpret_cast<const f32x4*>(f_lds[buf][0]);
       f32x4 vs = *reinterpret_cast<const f32x4*>(f_lds[buf][1]);
       const int key0 = j * kBN;
-      // Scores are scaled ahead where some are masked (a scale of 0 or NaN times -inf would not
-      // be) and where they are so large that the scaled maximum's own rounding counts.
+      // Scores are scaled ahead where some are masked (a scale of 0 or NaN times -inf would not be).
       const bool masked = uniform(key0 + kBN - 1 > wave_first || wave_row0 + 31 >= rows);
-      if (masked || __builtin_amdgcn_ballot_w64(fabsf(m) > 4096.f && m != -INFINITY) != 0) {
+      if (masked) {
         const int lim = limit - key0 - 4 * half;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
@@ -244,10 +244,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWorkgroups
         lsum = none ? 0.f : lsum * fast_exp2(-down);
         m = mn;
         e = none ? kNoExponent : en;
+        large = __builtin_amdgcn_ballot_w64(fabsf(m) > 4096.f && m != -INFINITY) != 0;
 #pragma unroll
         for (int c = 0; c < DT; ++c)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[c][r] *= corr;
+      }
+      // m is a rounded score's bound.  One that is left unrounded may pass it by half a step of its own:
+      // nothing for small ones, 2^7 at 2^31, whose weight would be infinite.
+      if (large) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[hh][r] = rounded_product(s[hh][r], f[2 * hh + r / 8]);
+        f = f32x4{1.f, 1.f, 1.f, 1.f};
       }
       const float mb = m == -INFINITY ? 0.f : m;  // only -inf scores so far: they weigh 0
       u32x4 pb[kUnits][NP];
