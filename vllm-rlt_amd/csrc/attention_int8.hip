@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64 * kGenericWaves) void attn_i8_generic_kernel(Att
       const int d = lane + 64 * c;
       if (d < a.d) dot = fmaf(qv[c], static_cast<float>(static_cast<int8_t>(a.k[base + d * a.kv_dim])), dot);
     }
-    const float x = group_sum<64>(dot) * sk;
+    const float x = rounded_product(group_sum<64>(dot), sk);  // as its maximum is: a large one's last bits are whole numbers
     const float mn = fmaxf(m, ceilf(x));
     const float off = mn == -INFINITY ? 0.f : mn;  // only -inf scores so far: they weigh 0
     const float w = fast_exp2(x - off);

@@ -18,6 +18,12 @@ __device__ __forceinline__ float group_max(float x) {
   return x;
 }
 
+// x y, rounded also where the product is added to something.
+__device__ __forceinline__ float rounded_product(float x, float y) {
+#pragma clang fp contract(off)
+  return x * y;
+}
+
 // Limits of the attention calls: token counts and what is added to them stay inside 31
 // bits, and the threads of a launch (blocks of up to 512) inside 32.
 constexpr int64_t kMaxKeys = int64_t(1) << 30;

@@ -267,7 +267,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         const float f = block_scale(kf[u]) * a.qscale;
         vf[u] = block_scale(vf[u]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][i] *= f;
+        for (int i = 0; i < 4; ++i) s[u][i] = rounded_product(s[u][i], f);  // as their maximum is
       }
       if (first + kTile > end) {
 #pragma unroll

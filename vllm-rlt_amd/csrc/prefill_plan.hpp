@@ -217,12 +217,6 @@ __device__ __forceinline__ bool find_item(const Prefill8Args& p, Item* it) {
   return false;
 }
 
-// x y, rounded also where the product is added to something.
-__device__ __forceinline__ float rounded_product(float x, float y) {
-#pragma clang fp contract(off)
-  return x * y;
-}
-
 // Elements d .. d + 3 of an out row.
 template <typename T>
 __device__ __forceinline__ void store4(T* orow, int d, const float (&x)[4], int64_t stride, bool vec) {
