@@ -635,9 +635,11 @@ int rlt_build_chunk_metadata(const int64_t* descriptors, int64_t count, int64_t 
  *   codes of the rows: rint(x * (1 / s))
  * every operation rounded to fp32, rint to even.  Rows that hold what is not finite
  * make s NaN, and a scale that is NaN stays so until the block begins again.
+ * Rows of a block outside the pool, or of an offset outside its page, are skipped.
  * Rows of one block stand together in the call (as the tokens of a packed prompt do,
  * and those of a decode batch, which have a block each); their slots are distinct.
- * Rows of a block outside the pool, or of an offset outside its page, are skipped.
+ * Between two of them up to 32 rows may be skipped, or page_size where that is more:
+ * any tokens of a prompt may be taken out.
  * Moving a token to another block is a read back and an append (its scale changes);
  * whole blocks move as bytes, with their scales.
  */

@@ -1,7 +1,7 @@
 // Appends to the block-scaled 8-bit KV cache, and reading it back (int8.hpp).
 //
-// Append.  The rows of a call that go to one block stand together in it; a wave takes them
-// as one, for a head:
+// Append.  The rows of a call that go to one block stand together in it, but for rows that are
+// skipped; a wave takes them as one, for a head:
 //   s0 = the block's scale, 0 where the call writes its offset 0 (which begins the block)
 //   s  = max(s0, largest |x| of the new rows * (1 / 127), 2^-126)
 //   codes the block holds: rint(code * (s0 / s)), where s is not s0
@@ -35,13 +35,43 @@ struct AppendI8Args {
 __device__ __forceinline__ bool valid_block(const AppendI8Args& a, int64_t b) { return b >= 0 && b < a.num_blocks; }
 __device__ __forceinline__ bool valid_offset(const AppendI8Args& a, int64_t o) { return o >= 0 && o < a.page; }
 
-// Rows from row on that go to the same block.
-__device__ __forceinline__ int64_t run_length(const AppendI8Args& a, int64_t row, int64_t block, int lane) {
-  for (int64_t n = 1;; n += 64) {
-    const int64_t at = row + n + lane;
-    const uint64_t other = __builtin_amdgcn_ballot_w64(!(at < a.rows && a.blocks[at] == block));
-    if (other) return n + __builtin_ctzll(other);
+// The block of row `row`, -1 for one that is skipped: outside the pool, or of an offset outside its page.
+__device__ __forceinline__ int block_of_row(const AppendI8Args& a, int64_t row) {
+  const int64_t block = a.blocks[row], offset = a.offsets[row];
+  return valid_block(a, block) && valid_offset(a, offset) ? static_cast<int>(block) : -1;
+}
+
+// Rows of one block are a run, with up to kGap skipped rows between two of them, or a page's tokens: so many
+// as consecutive tokens of a block can have.  (Any number would have a padded batch searched to its end: 100
+// rows of 4096 12.7 us, so 4.5.)
+constexpr int64_t kGap = 32;
+
+// The last row of the run of `block` that has row `last`, its last one up to row from - 1; *count grows by its
+// rows from `from` on.
+__device__ __forceinline__ int64_t run_last(const AppendI8Args& a, int block, int64_t last, int64_t from, int lane, int64_t* count) {
+  const int64_t gap = std::max(kGap, a.page);
+  for (; from < a.rows && from - last - 1 <= gap; from += 64) {
+    const int64_t at = from + lane;
+    const int b = at < a.rows ? block_of_row(a, at) : -1;
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(b == block), other = __builtin_amdgcn_ballot_w64(b >= 0 && b != block);
+    const uint64_t run = other ? mine & ((other & -other) - 1) : mine;
+    if (run) last = from + 63 - __builtin_clzll(run);
+    *count += __builtin_popcountll(run);
+    if (other) return last;
   }
+  return last;
+}
+
+// The block of the last row before `row` that is not skipped; -1 where the rows that a run can have between two
+// of its own are skipped.
+__device__ __forceinline__ int block_before(const AppendI8Args& a, int64_t row, int lane) {
+  const int64_t stop = row - std::max(kGap, a.page);
+  for (; row > 0 && row > stop; row -= 64) {
+    const int64_t at = row - 64 + lane;
+    const int b = at >= 0 ? block_of_row(a, at) : -1;
+    if (const uint64_t in = __builtin_amdgcn_ballot_w64(b >= 0)) return __builtin_amdgcn_readlane(b, 63 - __builtin_clzll(in));
+  }
+  return -1;
 }
 
 // The new scale, from the old one (0 for a block that begins) and the bits of the largest |x|.
@@ -71,27 +101,33 @@ __device__ __forceinline__ float code_value(int code, float scale) {
 }
 
 // Any strides and head size: a wave a (row, K or V, head); the first row of a block works.  Latency bounds it:
-// 4096 rows of 8 sequences, 16 heads x 65, 62 us.
+// 4096 rows of 8 sequences, 16 heads x 65, 65 us.
 template <typename T>
 __global__ __launch_bounds__(64) void append_i8_generic_kernel(AppendI8Args a) {
   const int lane = threadIdx.x, which = blockIdx.y / a.hkv, head = blockIdx.y % a.hkv;
-  const int64_t row = blockIdx.x, block = a.blocks[row];
-  if (!valid_block(a, block) || (row > 0 && a.blocks[row - 1] == block)) return;
-  const int64_t n = run_length(a, row, block, lane);
+  const int64_t row = blockIdx.x;
+  const int block_at = uniform(block_of_row(a, row));
+  if (block_at < 0) return;
+  if (row > 0) {
+    int previous = uniform(block_of_row(a, row - 1));
+    if (previous < 0) previous = block_before(a, row - 1, lane);
+    if (previous == block_at) return;
+  }
+  int64_t count = 1;
+  const int64_t block = block_at, n = run_last(a, block_at, row, row + 1, lane, &count) - row + 1;
+  const bool dense = count == n;  // no skipped rows between them
   const T* x = static_cast<const T*>(a.x[which]) + row * a.x_row[which] + head * a.x_head[which];
   uint8_t* codes = a.codes[which] + block * a.c_block + a.layer * a.c_layer + head * a.c_head;
   float* scale = a.scales[which] + block * a.s_block + a.layer * a.s_layer + head * a.s_head;
   uint32_t top = 0;
-  bool begins = false, any = false;
+  bool begins = false;
   for (int64_t r = 0; r < n; ++r) {
     const int64_t offset = a.offsets[row + r];
-    if (!valid_offset(a, offset)) continue;
-    any = true;
+    if (!dense && (a.blocks[row + r] != block || !valid_offset(a, offset))) continue;
     begins |= offset == 0;
     for (int d = lane; d < a.d; d += 64)
       top = max(top, __float_as_uint(load_elem(x + r * a.x_row[which] + d * a.x_dim[which])) & 0x7fffffffu);
   }
-  if (!any) return;
 #pragma unroll
   for (int i = 1; i < 64; i <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), i, 64)));
   const float before = begins ? 0.f : *scale, s = grown_scale(before, top);
@@ -108,7 +144,7 @@ __global__ __launch_bounds__(64) void append_i8_generic_kernel(AppendI8Args a) {
   const float inv = s == s ? 1.f / s : s;
   for (int64_t r = 0; r < n; ++r) {
     const int64_t offset = a.offsets[row + r];
-    if (!valid_offset(a, offset)) continue;
+    if (!dense && (a.blocks[row + r] != block || !valid_offset(a, offset))) continue;
     for (int d = lane; d < a.d; d += 64)
       codes[offset * a.c_token + d * a.c_dim] =
           static_cast<uint8_t>(code_of(load_elem(x + r * a.x_row[which] + d * a.x_dim[which]), inv));
@@ -227,7 +263,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
   const int lane = threadIdx.x & 63, i = lane % LPH, sub = lane / LPH, page = static_cast<int>(a.page);
   const int packets = PAD ? a.d / N : LPH, at_dim = min(i, packets - 1) * N;
   const bool own = i < packets;
-  // Lane l has the block and the offset of row row0 - 1 + l; -1 outside the pool and the page.
+  // Lane l has the block and the offset of row row0 - 1 + l, -1 for a row that is skipped.
   const int64_t at = row0 - 1 + lane;
   const bool there = at >= 0 && at < a.rows;
   const int64_t block_at = there ? a.blocks[at] : -1, offset_at = there ? a.offsets[at] : -1;
@@ -237,12 +273,31 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
   const bool early = tile <= TPI;  // few rows, mostly blocks of one: on their way with the block's number
   const int last = static_cast<int>(min(static_cast<int64_t>(tile), a.rows - row0)) - 1;  // (of the tile; rows past it: it again, of no use)
   if (early) held[0] = *reinterpret_cast<const u32x4*>(x0 + min(sub, last) * x_row);
-  const int block = valid_block(a, block_at) ? static_cast<int>(block_at) : -1;
-  const int offset = valid_offset(a, offset_at) ? static_cast<int>(offset_at) : -1;
-  const int previous = __shfl_up(block, 1, 64);
-  const uint64_t same = __builtin_amdgcn_ballot_w64(lane > 0 && block == previous);  // as the row before
-  const uint64_t begin = __builtin_amdgcn_ballot_w64(block >= 0) & ~same & (((uint64_t(1) << tile) - 1) << 1);
-  const uint64_t single = begin & ~(same >> 1);
+  const bool used = valid_block(a, block_at) && valid_offset(a, offset_at);
+  const int block = used ? static_cast<int>(block_at) : -1, offset = used ? static_cast<int>(offset_at) : -1;
+  const uint64_t rows = __builtin_amdgcn_ballot_w64(used), below = rows & ((uint64_t(1) << lane) - 1);
+  const int previous = __shfl(block, below ? 63 - __builtin_clzll(below) : lane, 64);
+  uint64_t same = __builtin_amdgcn_ballot_w64(used && below && block == previous);  // as the row before that is not skipped
+  const uint64_t tile_rows = ((uint64_t(1) << tile) - 1) << 1;
+  if (row0 > 1 && rows & tile_rows && !(rows & 1)) {  // that of the tile's first row is further away
+    const int first = __builtin_ctzll(rows);
+    if (block_before(a, row0 - 1, lane) == __builtin_amdgcn_readlane(block, first)) same |= uint64_t(1) << first;
+  }
+  const uint64_t begins_at = rows & ~same, begin = begins_at & tile_rows;
+  // Runs of more than one row: `same` moved down to the row before, over skipped ones, as a carry is.
+  const uint64_t gaps = __builtin_bitreverse64(~rows);
+  uint64_t followed = __builtin_bitreverse64((gaps + (__builtin_bitreverse64(same) << 1)) & ~gaps);
+  // The last run in sight may go on behind it.
+  int64_t end = -1, behind = 0;
+  const int64_t in_sight = row0 - 1 + 63 - __builtin_clzll(rows | 1);
+  if (begin && row0 + 63 < a.rows && row0 + 62 - in_sight <= std::max(kGap, a.page)) {
+    const int first = 63 - __builtin_clzll(begins_at);
+    if (begin >> first & 1) {
+      end = run_last(a, __builtin_amdgcn_readlane(block, first), in_sight, row0 + 63, lane, &behind);
+      if (end > in_sight) followed |= uint64_t(1) << first;
+    }
+  }
+  const uint64_t single = begin & ~followed;
   uint8_t* const codes0 = a.codes[which] + a.layer * a.c_layer + head * a.c_head + at_dim;
   float* const scale0 = a.scales[which] + a.layer * a.s_layer + head * a.s_head;
   if (single) {
@@ -280,8 +335,11 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
   for (uint64_t first = begin & ~single; first; first &= first - 1) {
     const int l0 = __builtin_ctzll(first);
     const int64_t row = row0 - 1 + l0, blk = __builtin_amdgcn_readlane(block, l0);
-    int n = 1 + __builtin_ctzll(~(same >> l0 >> 1));  // rows of the block (zeros are shifted in)
-    if (l0 + n > 63) n = static_cast<int>(run_length(a, row, blk, lane));
+    const uint64_t after = ~((uint64_t(2) << l0) - 1), next = begins_at & after;
+    const uint64_t run = same & after & (next ? (next & -next) - 1 : ~uint64_t(0));
+    // Rows to the block's last, skipped ones among them.
+    const int n = next || end < 0 ? 64 - __builtin_clzll(run) - l0 : static_cast<int>(end - row + 1);
+    const bool dense = 1 + __builtin_popcountll(run) + (next ? 0 : behind) == n;
     float* const scale = scale0 + blk * a.s_block;
     uint8_t* const codes = codes0 + blk * a.c_block;
     const float old = *scale;
@@ -294,24 +352,24 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
         held[u] = *reinterpret_cast<const u32x4*>(x + min(t, n - 1) * x_row);
         o[u] = __shfl(offset, min(l0 + t, 63), 64);
         if (t < n && l0 + t > 63) {
-          const int64_t wide = a.offsets[row + t];
-          o[u] = valid_offset(a, wide) ? static_cast<int>(wide) : -1;
+          // (Worked out for all lanes: of a condition in branches the compiler, ROCm 7.2's, loses the offset.)
+          int64_t wide = a.offsets[row + t], of_block = blk;
+          if (!dense) of_block = a.blocks[row + t];
+          o[u] = static_cast<int>(wide) | -static_cast<int>((of_block != blk) | (wide < 0) | (wide >= a.page));
         }
         if (t >= n) o[u] = -1;
       }
     };
     uint32_t top = 0;
-    bool any = false, begins = false;
+    bool begins = false;
     for (int from = 0; from < n; from += H * TPI) {
       load(from);
 #pragma unroll
       for (int u = 0; u < H; ++u) {
-        any |= o[u] >= 0;
         begins |= o[u] == 0;
         if (o[u] >= 0) top = packet_max<T>(top, held[u]);
       }
     }
-    if (!__builtin_amdgcn_ballot_w64(any)) continue;
     const bool fresh = __builtin_amdgcn_ballot_w64(begins) != 0;
     const float before = fresh ? 0.f : old, s = grown_scale(before, group_umax<64>(top_bits<T>(top)));
     if (lane == 0) *scale = s;

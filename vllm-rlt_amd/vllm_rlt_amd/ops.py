@@ -1413,7 +1413,8 @@ def kv_append_int8(
 
     k and v are float32, float16 or bfloat16.  Rows of one block stand together in the
     call, in any order of their offsets; the slots of a call are distinct, those outside
-    the cache skipped.
+    the cache skipped.  Up to 32 skipped rows, or a page's where that is more, may stand
+    between two rows of a block.
     """
     host, stream = _host_calls(key_cache)
     if host is not None:
