@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
     for (int u = 0; u < H; ++u) {
       const float before = slot[u] == 0 ? 0.f : old[u], s = grown_scale(before, group_umax<LPH>(top_bits<T>(packet_max<T>(0, held[u]))));
       inv[u] = s == s ? 1.f / s : s;
-      const float of_row = slot[u] > 0 && s == s ? before / s : 1.f;
+      const float of_row = slot[u] > 0 && s == s && s != before ? before / s : 1.f;  // (an infinite one stays)
       if (slot[u] >= 0 && i == 0) scale0[blk[u] * a.s_block] = s;
       const float of_lane = __shfl(of_row, lane % TPI * LPH, 64);
       ratio = lane / TPI == u ? of_lane : ratio;
