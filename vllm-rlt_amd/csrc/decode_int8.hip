@@ -7,9 +7,9 @@
 // - S^T = K Q^T on the 16-bit MFMA of q's type (16x16x32; an fp32 q in three bf16 parts): a
 //   code is a bf16 or an fp16 exactly, and the block's scale multiplies the fp32 sum.
 // - O^T += V^T W^T on the fp16 MFMA (16x16x32), W the probabilities times their block's V scale,
-//   near 1 for the keys that matter: in one part, 11 bits, for bf16 (whose own rounding is eight
-//   times that), in two for fp16 and fp32.  The sum of the probabilities is taken before that.
-// Bytes bound it: 256 rows of 1024-8192 tokens, 16 heads x 128, bf16, 4.84 GB, take 802 us, 6.0 TB/s; few rows
+//   near 1 for the keys that matter, in two parts, 22 bits.  (One for bf16 would save 1%, and round
+//   8% of the outputs the other way.)  The sum of the probabilities is taken before that.
+// Bytes bound it: 256 rows of 1024-8192 tokens, 16 heads x 128, bf16, 4.84 GB, take 807 us, 6.0 TB/s; few rows
 // the latency of length, table, first tile and join (24 rows of 512-4096, 32 + 8 heads, fp16, 114 MB: 31.6 us).
 // Tiles go from memory into LDS directly: K of the next one as soon as this
 // one's K is in registers, V likewise, one buffer each.  The heads of a row's split run on one XCD
@@ -41,7 +41,7 @@ struct DecodeI8Args {
 
 // Parts of q and of the weights, and the type of the scores' operands.
 template <typename T> struct Parts;
-template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf16; };
+template <> struct Parts<bf16> { static constexpr int Q = 1, P = 2; using S = bf16; };
 template <> struct Parts<f16> { static constexpr int Q = 1, P = 2; using S = f16; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 2; using S = bf16; };
 
