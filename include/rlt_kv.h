@@ -687,7 +687,7 @@ int rlt_paged_decode_int8(const void* q, const int64_t* q_strides, const void* k
  * right causal, with the rows, lengths, max_seqlen_q and workspace of
  * rlt_paged_prefill_fp8 (its bytes by rlt_paged_prefill_int8_workspace_bytes: at most
  * 768 KiB * (head_dim, rounded up to 64, 128 or 256, + 4) and 65 rows of partials).  A probability times its block's
- * scale goes into the products with 11 bits for bf16 and fp16 and 22 for fp32.
+ * scale goes into the products with 11 bits for bf16 and 22 for fp16 and fp32.
  */
 int64_t rlt_paged_prefill_int8_workspace_bytes(int64_t total_q, int64_t num_seqs, int64_t max_table_width,
                                                int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,

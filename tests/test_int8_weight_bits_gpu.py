@@ -30,3 +30,11 @@ def check(c, out):
 def test_decode(dtype, hq, hkv, d):
     c = Case([1, 17, 100, 300, 700, 1300], hq, hkv, d, dtype=dtype, seed=d, spread=0.5)
     check(c, c.decode())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_prefill(dtype, hq, hkv, d):
+    c = Case([70, 300, 2000, 33], hq, hkv, d, dtype=dtype, seed=d, spread=0.5, chunks=[30, 130, 40, 33])
+    check(c, c.prefill())
+    check(c, c.prefill(batch_invariant=True))

@@ -12,8 +12,9 @@
 //   multiplies the sums, in the instruction that takes the running maximum off.
 // - O^T += V^T W^T on the fp16 MFMA, codes as fp16 likewise; V^T comes from transposing LDS
 //   reads, W, the probabilities times their unit's V scale, from the registers S^T left it
-//   in: in one part, 11 bits, for bf16 and fp16, in two for fp32.  (Two for fp16 would bring its outputs
-//   from 2.9e-4 to 2.1e-4 of their rms, which is their own rounding, and cost 21 to 27%.)
+//   in: in one part, 11 bits, for bf16, in two for fp16 and fp32.  (An fp16 output is off by 2.1e-4 of the
+//   rms so, its own rounding; with one part by 2.9e-4, for 10 to 21% less time, eight chunks as below 349 us
+//   where two take 445.  A bf16 output is off by 0.00167 with one and 0.00166 with two, for 345 and 440.)
 // Products (42% of a SIMD's cycles) and vector work (69%: conversions, exponentials, sums) bound it: eight
 // 512-token chunks over 1024-15360 keys, 16 heads x 128, bf16, take 353 us with their merge, 802 TFLOP/s,
 // where a large product of matrices reaches 1210.  Short launches are 6 us of plan and first loads, a tile 1.6
@@ -47,7 +48,7 @@ __device__ __forceinline__ void unrolled(F f) {
 // Parts of q and of the weights, and the type of the scores' operands.
 template <typename T> struct Parts;
 template <> struct Parts<bf16> { static constexpr int Q = 1, P = 1; using S = bf16; };
-template <> struct Parts<f16> { static constexpr int Q = 1, P = 1; using S = f16; };
+template <> struct Parts<f16> { static constexpr int Q = 1, P = 2; using S = f16; };
 template <> struct Parts<float> { static constexpr int Q = 3, P = 2; using S = bf16; };
 
 // Workgroups a CU, as LDS and registers hold.
