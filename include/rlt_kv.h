@@ -667,8 +667,9 @@ int rlt_kv_gather_int8(const void* key_cache, const void* value_cache, const int
  * `dtype`, scale_strides[2]: block, head.  A row of length 0 (or less) is written as
  * zeros; lengths are clamped to what the table covers; a table entry outside the pool
  * reads block 0.  A row's output bits depend on its own q, blocks and length only.
- * Scores, sums and accumulators are fp32; a probability times its block's scale goes into
- * the products with 22 bits.
+ * Scores, sums and accumulators are fp32 (a score's the sum of q times codes, so that queries
+ * of 2^112 and more may pass its range); a probability times its block's scale goes into the
+ * products with 22 bits.
  * The workspace (rlt_paged_decode_int8_workspace_bytes, a function of the shape, on 16
  * bytes) holds the partials of cut rows; calls that overlap need one each.
  */

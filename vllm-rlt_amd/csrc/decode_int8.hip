@@ -9,7 +9,7 @@
 // - O^T += V^T W^T on the fp16 MFMA (16x16x32), W the probabilities times their block's V scale,
 //   near 1 for the keys that matter, in two parts, 22 bits.  (One for bf16 would save 1%, and round
 //   8% of the outputs the other way.)  The sum of the probabilities is taken before that.
-// Bytes bound it: 256 rows of 1024-8192 tokens, 16 heads x 128, bf16, 4.84 GB, take 807 us, 6.0 TB/s; few rows
+// Bytes bound it: 256 rows of 1024-8192 tokens, 16 heads x 128, bf16, 4.84 GB, take 811 us, 6.0 TB/s; few rows
 // the latency of length, table, first tile and join (24 rows of 512-4096, 32 + 8 heads, fp16, 114 MB: 31.6 us).
 // Tiles go from memory into LDS directly: K of the next one as soon as this
 // one's K is in registers, V likewise, one buffer each.  The heads of a row's split run on one XCD
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
           w[i] = fast_exp2(s[u][i] - off);
           l += w[i];
           w[i] *= g;
-          if constexpr (NP > 1) asm("" : "+v"(w[i]));  // the parts are of one product, rounded to fp32
+          asm("" : "+v"(w[i]));  // the parts are of one product, rounded to fp32
         }
 #pragma unroll
         for (int n = 0; n < NP; ++n)

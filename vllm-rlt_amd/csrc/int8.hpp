@@ -1,8 +1,13 @@
 // The block-scaled 8-bit KV cache: signed codes, -127 to 127, with one fp32 scale
-// for each block (a page of tokens) and KV head.  A cached value is code * scale,
-// so it is off by at most half a step, 1/254 of its block's largest magnitude: a
-// third of what e4m3 codes lose at the same bytes (rms, normal values), with a
-// sixteenth of the scales.  A scale that is not finite makes its whole block NaN.
+// for each block (a page of tokens) and KV head.  A cached value is code * scale.
+// It is off by at most half a step, 1/254 of its block's largest magnitude, where the
+// block was written in one call; by half a step more of each scale that it was rounded to
+// since, where appends made the block's grow.  Rms of normal values in pages of 16 / 128,
+// of theirs: 0.0083 / 0.0094 in one call, 0.0104 / 0.0122 token by token (up to five half
+// steps), where e4m3 codes at the same bytes, with a scale for each token, lose 0.0265.  But
+// a block's scale is its largest channel's: with four channels of 128 times 4 and
+// tokens of different size it is 0.0230 / 0.0318 and 0.0268 / 0.0386.
+// A scale that is not finite makes its whole block NaN.
 #pragma once
 
 #include <type_traits>

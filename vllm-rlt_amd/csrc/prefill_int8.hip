@@ -16,9 +16,9 @@
 //   rms so, its own rounding; with one part by 2.9e-4, for 10 to 21% less time, eight chunks as below 349 us
 //   where two take 445.  A bf16 output is off by 0.00167 with one and 0.00166 with two, for 345 and 440.)
 // Products (42% of a SIMD's cycles) and vector work (69%: conversions, exponentials, sums) bound it: eight
-// 512-token chunks over 1024-15360 keys, 16 heads x 128, bf16, take 353 us with their merge, 802 TFLOP/s,
-// where a large product of matrices reaches 1210.  Short launches are 6 us of plan and first loads, a tile 1.6
-// to 2.4 us, and 4 us of merge.
+// 512-token chunks over 1024-15360 keys, 16 heads x 128, bf16, take 345 to 363 us by run with their
+// merge, 780 to 820 TFLOP/s, where a large product of matrices reaches 1210.  Short launches are 6 us of plan and
+// first loads, a tile 1.6 to 2.4 us, and 4 us of merge.
 #include "prefill_int8.hpp"
 
 #include "prefill_plan.hpp"
