@@ -355,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_i8_kernel(AppendI8Args a, 
         held[u] = *reinterpret_cast<const u32x4*>(x + min(t, n - 1) * x_row);
         o[u] = __shfl(offset, min(l0 + t, 63), 64);
         if (t < n && l0 + t > 63) {
-          // (Worked out for all lanes: of a condition in branches the compiler, ROCm 7.2's, loses the offset.)
+          // (Without branches: the compiler of ROCm 7.2 lost the offset where the condition was one.)
           int64_t wide = a.offsets[row + t], of_block = blk;
           if (!dense) of_block = a.blocks[row + t];
           o[u] = static_cast<int>(wide) | -static_cast<int>((of_block != blk) | (wide < 0) | (wide >= a.page));
